@@ -23,6 +23,7 @@ INCLUDE = os.path.join(REPO, "include")
 OBJDIR = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "flash_attention_v100", "libfa_gfx950.so")
 HOST_SRC = os.path.join(CSRC, "fa_host.cpp")
+HOST_SRCS = [HOST_SRC, os.path.join(CSRC, "fa_ops_host.cpp")]
 HOST_LIB = os.path.join(HERE, "flash_attention_v100", "fa_host.so")
 ARCH = "gfx950"
 
@@ -34,7 +35,8 @@ SOURCES = ["fa_abi.cpp", "fa_misc.hip", "fa_fwd_fit.hip", "fa_fwd_decode.hip"] +
     for pas, modes in (("bwd", _MODES + (("cols256_", _H),)), ("fwd", _MODES))
     for mode, dts in modes
     for dt in dts
-]
+] + [f"fa_scored_{pas}_{dt}.hip" for pas in ("bwd", "fwd") for dt in _A] + [f"fa_rows_{dt}.hip" for dt in _A] + [
+    "fa_ops_abi.cpp", "fa_scored_misc.hip", "fa_rotary.hip"]
 
 # units whose MFMA accumulators may live in AGPRs (the head-dim-256 backward:
 # its dK / dV and dQ kernels need more than 256 registers a lane; with the
@@ -110,13 +112,13 @@ def build_host() -> str:
            "-I", INCLUDE, "-isystem", sysconfig.get_paths()["include"], "-isystem", "/opt/rocm/include"]
     for d in cpp_extension.include_paths():
         cmd += ["-isystem", d]
-    cmd += ["-o", tmp, HOST_SRC]
+    cmd += ["-o", tmp] + HOST_SRCS
     for d in cpp_extension.library_paths():
         cmd += ["-L", d]
     cmd += ["-lc10", "-ltorch_cpu", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"compile failed: {HOST_SRC}\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+        raise RuntimeError(f"compile failed: {HOST_SRCS}\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, HOST_LIB)
     return HOST_LIB
 

@@ -21,6 +21,7 @@
 #include <mutex>
 
 #include "fa_abi.h"
+#include "fa_ops.h"
 #include "fa_params.hpp"
 
 // Device scratch of fa_bwd_static: the backward workspace for callers that
@@ -347,6 +348,10 @@ const char* fa_strerror(int32_t code) {
         case FA_ERR_SCRATCH:
             return "the backward needs more workspace than the static scratch of fa_bwd_static "
                    "(FA_BWD_STATIC_SCRATCH_BYTES); use fa_bwd with a workspace";
+        case FA_ERR_RULE:
+            return "softcap must be finite and >= 0; slopes, documents and their strides must be consistent";
+        case FA_ERR_ROTARY:
+            return "rotary_dim must be even and at most the head dim, with a table and finite positive base and factor";
         default: return "unknown status code";
     }
 }

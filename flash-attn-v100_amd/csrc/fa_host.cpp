@@ -12,9 +12,15 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include "fa_host_util.hpp"
+
 #include "fa_abi.h"
 
 namespace {
+
+using fa_host::dtype_code;
+using fa_host::prepare;
+using fa_host::put_strides;
 
 decltype(&fa_fwd_workspace_size) p_fwd_ws_size;
 decltype(&fa_fwd_ws) p_fwd_ws;
@@ -22,28 +28,6 @@ decltype(&fa_fwd_cols) p_fwd_cols;
 decltype(&fa_bwd_workspace_size) p_bwd_ws_size;
 decltype(&fa_bwd) p_bwd;
 decltype(&fa_bwd_cols) p_bwd_cols;
-
-int32_t dtype_code(at::ScalarType t) {
-    switch (t) {
-        case at::kHalf: return FA_DTYPE_F16;
-        case at::kBFloat16: return FA_DTYPE_BF16;
-        case at::kFloat: return FA_DTYPE_F32;
-        default: return -1;  // the library refuses it
-    }
-}
-
-// t, or a contiguous copy where the kernels' 16-byte loads need one: d stride
-// 1, other strides non-negative multiples of 16 bytes, base 16-byte aligned
-at::Tensor prepare(const at::Tensor& t) {
-    const int64_t es = t.element_size(), n = t.dim();
-    bool ok = n > 0 && t.stride(n - 1) == 1 && ((uintptr_t)t.data_ptr() & 15) == 0;
-    for (int64_t d = 0; ok && d + 1 < n; ++d) ok = t.stride(d) >= 0 && (t.stride(d) * es) % 16 == 0;
-    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
-}
-
-void put_strides(int64_t (&dst)[4], const at::Tensor& t) {
-    for (int d = 0; d < 4; ++d) dst[d] = t.stride(d);
-}
 
 // a tuple of four element strides
 bool get_strides(PyObject* o, int64_t (&dst)[4]) {
@@ -258,4 +242,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "fa_host", nullptr, -1, methods, nu
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_fa_host(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit_fa_host(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddFunctions(m, fa_host::ops_methods) != 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

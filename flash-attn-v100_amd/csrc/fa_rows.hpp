@@ -1,0 +1,380 @@
+// Attention of a few new tokens a sequence over its cache, and over a prefix
+// that all sequences of the batch share; gfx950.
+//
+// A row is one (sequence, new token, query head).  Rows of one KV head are taken
+// 32 at a time: over the prefix the rows of all sequences together (its K and V
+// are read once a tile of rows, not once a sequence), over a sequence's own keys
+// that sequence's rows.  Each tile of rows has its keys split over workgroups;
+// a workgroup's 4 waves walk its 64-key tiles in turn, each copying its own
+// (direct to LDS, two copies in flight), as fwd_decode_kernel does.  A split
+// leaves its rows' maximum, sum and unnormalised output in float32, and
+// rows_join_kernel puts the parts of a row together:
+//   O = sum_x 2^(m_x - m) O_x / sum_x 2^(m_x - m) l_x,  m = max_x m_x.
+// Query i of a sequence with n keys of its own stands at own position
+// n - Sq + i and sees its keys up to there; in distances the prefix lies before
+// them.  Bound by the K and V bytes.
+#pragma once
+
+#include "fa_common.hpp"
+#include "fa_fwd_decode.hpp"
+#include "fa_ops_params.hpp"
+#include "fa_scored.hpp"
+
+namespace fa {
+
+template <typename T, int D>
+struct RowsCfg {
+    static constexpr bool F32 = Elem<T>::kF32;
+    static constexpr int NW = 4;
+    static constexpr int BN = F32 ? 32 : 64;
+    static constexpr int NB = BN / 32;
+    static constexpr int KW = D + (F32 ? 4 : 8);
+    static constexpr int VW = F32 ? D + 8 : D + (D == 64 || D == 96 ? 8 : 24);
+    static constexpr int KTILE = BN * KW, VTILE = BN * VW;
+    static constexpr int REGION = KTILE + VTILE;
+    static_assert((D / 32) * 16 * 64 * 4 <= REGION * (int)sizeof(T), "a wave's O part fits its region");
+};
+
+// one tile of rows over keys [0, n_keys) of K / V, keys of split `split` of `splits`
+template <typename T, int D>
+__global__ __launch_bounds__(256, (D <= 64 && !Elem<T>::kF32 ? 2 : 1)) void rows_kernel(const RowsParams p) {
+    using C = RowsCfg<T, D>;
+    constexpr int BN = C::BN, NB = C::NB, KW = C::KW, VW = C::VW, NW = C::NW;
+    __shared__ __attribute__((aligned(16))) T smem[NW * C::REGION];
+    __shared__ float stat[NW][2][32];
+
+    const int tid = threadIdx.x;
+    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
+    const bool pre = (int64_t)blockIdx.x < p.p_wgs;
+    const int nwg = (int)(pre ? p.p_wgs : p.o_wgs);
+    const int id = xcd_remap(pre ? (int)blockIdx.x : (int)(blockIdx.x - p.p_wgs), nwg);
+    const int splits = pre ? p.p_splits : p.o_splits, rts = pre ? p.p_rt : p.o_rt;
+    const int split = id % splits, unit = id / splits, rt = unit % rts, bk = unit / rts;
+    const int hk = bk % p.Hkv, bs = bk / p.Hkv;  // bs: the sequence (own keys)
+
+    // ---- this lane's row ----
+    const int row = 32 * rt + l32, per_seq = p.Sq * p.group;
+    const int n_rows = pre ? p.B * per_seq : per_seq;
+    const bool live = row < n_rows;
+    const int rr = live ? row : 0;
+    const int b = pre ? rr / per_seq : bs, ig = pre ? rr % per_seq : rr;
+    const int i = ig / p.group, h = hk * p.group + ig % p.group;
+    const int len = p.lens ? max(0, min(p.Sk, p.lens[b])) : p.Sk;
+    const int off = p.tail ? len - p.Sq : max(-kMaxOffset, min(kMaxOffset, p.offsets ? p.offsets[b] : p.offset0));
+    const int own = off + i;  // the query's position among the sequence's own keys
+    int lim = pre ? p.P : p.causal ? min(len, own + 1) : len;  // keys [0, lim) are seen
+    if (!live || (p.masked_neg && own < 0)) lim = 0;
+    const float qpos = (float)(pre ? p.P + own : own);
+    // keys that some row of the tile sees, and that all do
+    int lim_max = lim, lim_min = live ? lim : INT_MAX;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        lim_max = max(lim_max, __shfl_xor(lim_max, x));
+        lim_min = min(lim_min, __shfl_xor(lim_min, x));
+    }
+    lim_max = __builtin_amdgcn_readfirstlane(lim_max);
+    lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+    const int n_keys = max(lim_max, 0), nt = (n_keys + BN - 1) / BN;
+    const int t0 = (int)((int64_t)nt * split / splits), t1 = (int)((int64_t)nt * (split + 1) / splits);
+
+    const int64_t k_ss = pre ? p.kp_ss : p.k_ss, v_ss = pre ? p.vp_ss : p.v_ss;
+    const T* __restrict__ kbase = pre ? (const T*)p.kp + hk * p.kp_sh : (const T*)p.k + bs * p.k_sb + hk * p.k_sh;
+    const T* __restrict__ vbase = pre ? (const T*)p.vp + hk * p.vp_sh : (const T*)p.v + bs * p.v_sb + hk * p.v_sh;
+    T* Ks = smem + w * C::REGION;
+    T* Vs = Ks + C::KTILE;
+    DmaTile<T, BN, D, KW, 1> kd;
+    kd.init(k_ss, lane, 0, p.cols);
+    DmaTile<T, BN, D, VW, 1> vd;
+    vd.init(v_ss, lane, 0, p.cols);
+    constexpr int NKI = decltype(kd)::NI, NVI = decltype(vd)::NI;
+    // tiles past the split's end read nothing but are issued, so that the vmcnt
+    // counts stay exact (float32 tiles are copied and waited for one by one)
+    auto copy_k = [&](int t) FA_INLINE {
+        const int nv = t < t1 ? n_keys - t * BN : 0;
+        if constexpr (C::F32)
+            kd.load(kbase + (int64_t)(t * BN) * k_ss, k_ss, nv, Ks, lane);
+        else
+            kd.load_untracked(kbase + (int64_t)(t * BN) * k_ss, k_ss, nv, Ks, lane);
+    };
+    auto copy_v = [&](int t) FA_INLINE {
+        const int nv = t < t1 ? n_keys - t * BN : 0;
+        if constexpr (C::F32)
+            vd.load(vbase + (int64_t)(t * BN) * v_ss, v_ss, nv, Vs, lane);
+        else
+            vd.load_untracked(vbase + (int64_t)(t * BN) * v_ss, v_ss, nv, Vs, lane);
+    };
+
+    constexpr int QR = C::F32 ? D / 8 : D / 16;
+    uint4 qreg[QR];
+    {
+        const T* qrow = (const T*)p.q + b * p.q_sb + (int64_t)i * p.q_ss + h * p.q_sh;
+#pragma unroll
+        for (int kk = 0; kk < QR; ++kk) {
+            const int d0 = C::F32 ? hi * (D / 2) + 4 * kk : 16 * kk + 8 * hi;
+            qreg[kk] = live && d0 < p.cols ? *reinterpret_cast<const uint4*>(qrow + d0) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    const bool slope = p.slopes != nullptr;
+    const float slope2 = slope ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
+    wait_vmem();
+    asm volatile("" ::: "memory");
+
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) o[n] = f32x16{};
+    float m_run = -1e30f, l_run = 0.f;
+    Cap<C::F32> cap(p);
+
+    int t = t0 + w;
+    copy_k(t);
+    copy_v(t);
+    for (; t < t1; t += NW) {
+        const int k0 = t * BN;
+        // ---- S^T = K Q^T ----
+        if constexpr (C::F32)
+            wait_vmem();
+        else
+            wait_vmem_below<NVI>();  // K(t); only V(t) may be in flight
+        asm volatile("" ::: "memory");
+        f32x16 s[NB];
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk) {
+            s[blk] = f32x16{};
+            const T* krow = Ks + (32 * blk + l32) * KW;
+#pragma unroll
+            for (int kk = 0; kk < QR; ++kk) {
+                if constexpr (C::F32) {
+                    const f32x4 a = *reinterpret_cast<const f32x4*>(krow + hi * (D / 2) + 4 * kk);
+                    const f32x4 bq = __builtin_bit_cast(f32x4, qreg[kk]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[blk] = mfma_f32(a[e], bq[e], s[blk]);
+                } else {
+                    const s16x8 a = *reinterpret_cast<const s16x8*>(krow + 16 * kk + 8 * hi);
+                    s[blk] = Elem<T>::mfma(a, __builtin_bit_cast(s16x8, qreg[kk]), s[blk]);
+                }
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K(t) read before it is overwritten
+        if constexpr (!C::F32) copy_k(t + NW);
+
+        // ---- scores in log2 units ----
+        if (p.cap > 0.f) {
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[blk][e] = cap.value(s[blk][e]);
+        } else {
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[blk][e] *= p.scale_log2;
+        }
+        if (slope) {
+            const float d0 = qpos - (float)(k0 + 4 * hi);
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    s[blk][e] = __builtin_fmaf(-slope2, __builtin_fabsf(d0 - (float)(32 * blk + 8 * (e >> 2) + (e & 3))),
+                                               s[blk][e]);
+        }
+        if (k0 + BN > lim_min) {
+            const int lm = lim - k0 - 4 * hi;
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (32 * blk + 8 * (e >> 2) + (e & 3) >= lm) s[blk][e] = -INFINITY;
+        }
+        // ---- softmax ----
+        float mx = -INFINITY;
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[blk][e]);
+        mx = pair_max(mx);
+        const float m_new = fmaxf(m_run, mx);
+        if (__ballot(m_new > m_run + 8.0f) != 0ull) {
+            const float alpha = fast_exp2(m_run - m_new);
+            l_run *= alpha;
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[n][e] *= alpha;
+            m_run = m_new;
+        }
+        float psum = 0.f;
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[blk][e] = fast_exp2(s[blk][e] - m_run);
+                psum += s[blk][e];
+            }
+        l_run += psum;
+
+        // ---- O^T += V^T P^T ----
+        if constexpr (C::F32) {
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    const T* vrow = Vs + (32 * blk + 8 * (x >> 2) + 4 * hi + (x & 3)) * VW + l32;
+#pragma unroll
+                    for (int n = 0; n < D / 32; ++n) o[n] = mfma_f32(vrow[32 * n], s[blk][x], o[n]);
+                }
+        } else {
+            wait_vmem_below<NKI>();  // V(t); only K(t + 4) may be in flight
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int ks = 0; ks < BN / 16; ++ks) {
+                float tmp[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) tmp[e] = s[ks >> 1][8 * (ks & 1) + e];
+                const s16x8 pk = pack8<T>(tmp);
+#pragma unroll
+                for (int n = 0; n < D / 32; ++n) {
+                    const T* vp = Vs + (16 * ks + 4 * hi + ((lane & 15) >> 2)) * VW + 32 * n + 16 * ((lane >> 4) & 1) +
+                                  4 * (lane & 3);
+                    const s16x8 a = cat4(lds_read_tr16(vp), lds_read_tr16(vp + 8 * VW));
+                    o[n] = Elem<T>::mfma(a, pk, o[n]);
+                }
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V(t) read before it is overwritten
+        if constexpr (C::F32) copy_k(t + NW);
+        copy_v(t + NW);
+    }
+    wait_vmem();  // no copy in flight when the region takes the O part
+    asm volatile("" ::: "memory");
+
+    // ---- the waves' parts, rescaled to their common maximum ----
+    const float l_w = pair_sum(l_run);
+    float* mine = reinterpret_cast<float*>(Ks);
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mine[(16 * n + e) * 64 + lane] = o[n][e];
+    if (hi == 0) {
+        stat[w][0][l32] = m_run;
+        stat[w][1][l32] = l_w;
+    }
+    lds_barrier();
+    float mm = stat[0][0][l32];
+#pragma unroll
+    for (int x = 1; x < NW; ++x) mm = fmaxf(mm, stat[x][0][l32]);
+    float a[NW], l_tot = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+        a[x] = fast_exp2(stat[x][0][l32] - mm);
+        l_tot = __builtin_fmaf(stat[x][1][l32], a[x], l_tot);
+    }
+    const bool only = p.p_wgs == 0 && splits == 1;  // no other part of these rows
+    const int64_t prow = ((pre ? 0 : p.p_wgs) + id) * 32 + l32;
+    if (!only && w == 0 && hi == 0) p.stat[prow] = make_float2(mm, l_tot);
+    if (only && w == 0 && hi == 0 && live && p.lse)
+        p.lse[(int64_t)(b * p.H + h) * p.Sq + i] =
+            l_tot > 0.f ? (mm + __log2f(l_tot)) * kLn2 : l_tot == 0.f ? -INFINITY : l_tot;
+    const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
+#pragma unroll
+    for (int n0 = 0; n0 < D / 32; n0 += NW) {
+        const int n = n0 + w;
+        if (n >= D / 32) break;
+        f32x16 om = f32x16{};
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+            const float* px = reinterpret_cast<const float*>(smem + x * C::REGION);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) om[e] = __builtin_fmaf(px[(16 * n + e) * 64 + lane], a[x], om[e]);
+        }
+        if (!only) {
+            float* op = p.part + prow * D + 32 * n + 4 * hi;
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+                *reinterpret_cast<f32x4*>(op + 8 * q4) = f32x4{om[4 * q4], om[4 * q4 + 1], om[4 * q4 + 2], om[4 * q4 + 3]};
+        } else if (live) {
+            T* ob = (T*)p.o + b * p.o_sb + (int64_t)i * p.o_ss + h * p.o_sh + 32 * n + 4 * hi;
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                if (32 * n + 8 * q4 + 4 * hi >= p.cols) continue;
+                if constexpr (C::F32) {
+                    f32x4 v4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v4[e] = om[4 * q4 + e] * inv;
+                    *reinterpret_cast<f32x4*>(ob + 8 * q4) = v4;
+                } else {
+                    s16x4 v4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v4[e] = Elem<T>::pack1(om[4 * q4 + e] * inv);
+                    *reinterpret_cast<s16x4*>(ob + 8 * q4) = v4;
+                }
+            }
+        }
+    }
+}
+
+// the parts of every row, rescaled to their common maximum: one thread per 4
+// columns of a row (D / 4 threads share a row)
+template <typename T, int D>
+__global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p, const int64_t n_rows) {
+    constexpr int TPR = D / 4;
+    const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t r = gid / TPR;
+    const int col = (int)(gid % TPR) * 4;
+    if (r >= n_rows) return;
+    // r = (b H + h) Sq + i
+    const int i = (int)(r % p.Sq), h = (int)((r / p.Sq) % p.H), b = (int)(r / ((int64_t)p.Sq * p.H));
+    const int hk = h / p.group, ig = i * p.group + h % p.group, per_seq = p.Sq * p.group;
+    const int64_t gp = (int64_t)b * per_seq + ig;  // row of the prefix units
+    const int64_t pbase = ((int64_t)hk * p.p_rt + (gp >> 5)) * p.p_splits * 32 + (gp & 31);
+    const int64_t obase = (p.p_wgs + (((int64_t)b * p.Hkv + hk) * p.o_rt + (ig >> 5)) * p.o_splits) * 32 + (ig & 31);
+    float mm = -1e30f;
+    for (int x = 0; x < p.p_splits; ++x) mm = fmaxf(mm, p.stat[pbase + 32 * x].x);
+    for (int x = 0; x < p.o_splits; ++x) mm = fmaxf(mm, p.stat[obase + 32 * x].x);
+    float l_tot = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](int64_t pr) FA_INLINE {
+        const float2 st = p.stat[pr];
+        const float a = fast_exp2(st.x - mm);
+        l_tot = __builtin_fmaf(st.y, a, l_tot);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(p.part + pr * D + col);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[e], a, acc[e]);
+    };
+    for (int x = 0; x < p.p_splits; ++x) add(pbase + 32 * x);
+    for (int x = 0; x < p.o_splits; ++x) add(obase + 32 * x);
+    const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
+    if (col == 0 && p.lse) p.lse[r] = l_tot > 0.f ? (mm + __log2f(l_tot)) * kLn2 : l_tot == 0.f ? -INFINITY : l_tot;
+    if (col >= p.cols) return;
+    T* ob = (T*)p.o + b * p.o_sb + (int64_t)i * p.o_ss + h * p.o_sh + col;
+    if constexpr (Elem<T>::kF32) {
+        *reinterpret_cast<f32x4*>(ob) = f32x4{acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+    } else {
+        s16x4 v4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v4[e] = Elem<T>::pack1(acc[e] * inv);
+        *reinterpret_cast<s16x4*>(ob) = v4;
+    }
+}
+
+template <typename T, int D>
+hipError_t launch_rows_t(const RowsParams& p, hipStream_t s) {
+    hipLaunchKernelGGL((rows_kernel<T, D>), dim3((unsigned)(p.p_wgs + p.o_wgs)), dim3(256), 0, s, p);
+    if (p.p_wgs > 0 || p.o_splits > 1) {
+        const int64_t n_rows = (int64_t)p.B * p.H * p.Sq, nt = n_rows * (D / 4);
+        hipLaunchKernelGGL((rows_join_kernel<T, D>), dim3((unsigned)((nt + 255) / 256)), dim3(256), 0, s, p, n_rows);
+    }
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_rows(const RowsParams& p, int D, hipStream_t s) {
+    switch (D) {
+        case 32: return launch_rows_t<T, 32>(p, s);
+        case 64: return launch_rows_t<T, 64>(p, s);
+        case 128: return launch_rows_t<T, 128>(p, s);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace fa

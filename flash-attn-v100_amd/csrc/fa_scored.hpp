@@ -1,0 +1,1119 @@
+// Attention with scored rules for gfx950: scores capped by a tanh, a bias that
+// falls with the distance of query and key, and masks by documents, prefixes
+// and key lengths, none of them held as a (query, key) matrix.
+//
+//   x = scale q.k                       t = cap tanh(x / cap)  (or x)
+//   s = t - slope |i + off - j|         P = softmax over the keys seen
+//   seen: j < lim(i), lim(i) = min(len, causal ? max(i + off + 1, prefix) : len)
+//         and the documents of query and key are equal and not negative
+//
+// off, prefix, len are per sequence.  lim never falls with i, so without
+// documents a block of queries sees one run of keys; with documents a block
+// visits the key tiles whose range of document ids (doc_tiles_kernel) meets its
+// own: 64 tiles are tested at a time, one a lane, and a ballot gives the bit
+// mask that the tile loop walks.  A second ballot marks the tiles that every
+// query of the wave sees whole: only the others run the masking step.
+// tanh x = 1 - 2 r, r = 1 / (1 + e^(2x)): one exp2 and one reciprocal a score,
+// and its derivative 1 - tanh^2 = 4 (r - r^2) comes with two more operations.
+//
+// Tiles, operand layouts and pipelines are those of fa_fwd.hpp and fa_bwd.hpp:
+// one workgroup has 4 waves of 32 queries (forward, dQ) or 32 keys (dK/dV).
+#pragma once
+
+#include <limits.h>
+
+#include <type_traits>
+
+#include "fa_bwd.hpp"
+#include "fa_common.hpp"
+#include "fa_fwd.hpp"
+#include "fa_ops_params.hpp"
+
+namespace fa {
+
+// ---------------------------------------------------------------------------
+// per-sequence rules
+struct SeqRule {
+    int off, prefix, len;
+    bool causal;
+    __device__ FA_INLINE inline SeqRule(const ScoredParams& p, int b) {
+        const int o = p.offsets ? p.offsets[b] : p.offset0;
+        off = max(-kMaxOffset, min(kMaxOffset, o));
+        len = p.lens ? max(0, min(p.Sk, p.lens[b])) : p.Sk;
+        prefix = p.prefix ? max(0, min(p.Sk, p.prefix[b])) : 0;
+        causal = p.causal != 0;
+    }
+    // keys [0, lim(i)) may be seen by query i
+    __device__ FA_INLINE inline int lim(int i) const { return causal ? min(len, max(i + off + 1, prefix)) : len; }
+    // queries from first(j) on may see key j
+    __device__ FA_INLINE inline int first(int j) const {
+        return j >= len ? INT_MAX : (!causal || j < prefix) ? 0 : max(0, j - off);
+    }
+};
+
+// tanh cap.  value(): cap tanh(x / cap) log2 e of a raw score s (x = scale s);
+// slope(): the derivative / 4.
+// 16-bit inputs: 1 - 2 r, whose cancellation near 0 is at most 2^-23 of the cap
+// in the score.  float32: a series there (through x^13: 2e-8 of the value below
+// 0.45), so that small scores keep their digits.
+template <bool F32>
+struct Cap {
+    float k1, k2, top;  // scale / cap; that times 2 log2 e; cap log2 e
+    float r, t;         // of the last score
+    template <typename P>
+    __device__ FA_INLINE inline explicit Cap(const P& p) : k1(p.cap_k1), k2(p.cap_k2), top(p.cap_top) {}
+    __device__ FA_INLINE inline float rcp(float s) { return __builtin_amdgcn_rcpf(1.f + fast_exp2(s * k2)); }
+    __device__ FA_INLINE inline float value(float s) {
+        r = rcp(s);
+        if constexpr (!F32) {
+            return __builtin_fmaf(-2.f * top, r, top);
+        } else {
+            const float x = s * k1, u = x * x;
+            float q = 21844.f / 6081075.f;
+            q = __builtin_fmaf(q, u, -1382.f / 155925.f);
+            q = __builtin_fmaf(q, u, 62.f / 2835.f);
+            q = __builtin_fmaf(q, u, -17.f / 315.f);
+            q = __builtin_fmaf(q, u, 2.f / 15.f);
+            q = __builtin_fmaf(q, u, -1.f / 3.f);
+            q = __builtin_fmaf(q * u, x, x);
+            t = __builtin_fabsf(x) < 0.45f ? q : __builtin_fmaf(-2.f, r, 1.f);
+            return top * t;
+        }
+    }
+    __device__ FA_INLINE inline float slope() const {
+        if constexpr (!F32)
+            return __builtin_fmaf(-r, r, r);
+        else
+            return __builtin_fmaf(-0.25f * t, t, 0.25f);
+    }
+};
+
+// ---------------------------------------------------------------------------
+// whether the id ranges of two blocks meet in an id that is not negative
+__device__ FA_INLINE inline bool docs_meet(int2 a, int2 b) {
+    return a.y >= max(b.x, 0) && b.y >= max(a.x, 0);
+}
+__device__ FA_INLINE inline bool docs_one(int2 a, int2 b) { return a.x == a.y && b.x == b.y && a.x == b.x && a.x >= 0; }
+__device__ FA_INLINE inline int2 docs_join(int2 a, int2 b) { return make_int2(min(a.x, b.x), max(a.y, b.y)); }
+__device__ FA_INLINE inline int2 uniform2(int2 a) {
+    return make_int2(__builtin_amdgcn_readfirstlane(a.x), __builtin_amdgcn_readfirstlane(a.y));
+}
+
+// A tile of a walk: its index (-1 past the last) and flags, wave-uniform.
+// kAct: some row of this wave may see it; kFull: every row sees it whole; kNeg:
+// it holds tokens of no document; kMore: the walk has not ended.
+struct TileRef {
+    int t;
+    unsigned fl;
+};
+constexpr unsigned kAct = 1, kFull = 2, kNeg = 4, kMore = 8;
+
+// zeros into the rows of a tile that belong to no document (their values may be
+// anything, and 0 times a NaN is none).  All threads of the NT; a barrier follows.
+template <typename T, int R, int D, int W, int NT>
+__device__ FA_INLINE inline void clear_rows(T* tile, const int* docs, int tid) {
+    constexpr int EPC = 16 / (int)sizeof(T), CPR = D / EPC;
+    for (int c = tid; c < R * CPR; c += NT) {
+        const int row = c / CPR, col = c % CPR;
+        if (docs[row] < 0) *reinterpret_cast<uint4*>(tile + row * W + col * EPC) = make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+
+// The rows of a wave's 32-row block (lane l holds row l % 32, 16 columns of each
+// 32 in accumulator order), times mul, through LDS as rows of T and to global
+// memory in 16-byte chunks.  Holds a barrier; waves that are not `mine` only pass it.
+template <typename T, int D>
+__device__ FA_INLINE inline void store_rows(T* Os, int OW, const f32x16 (&acc)[D / 32], float mul, T* base, int64_t stride,
+                                           int row0, int n_rows, int cols, int lane, bool mine) {
+    const int l32 = lane & 31, hi = lane >> 5;
+    if (mine) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = 32 * i + 8 * g + 4 * hi;
+                if constexpr (Elem<T>::kF32) {
+                    f32x4 v4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v4[e] = acc[i][4 * g + e] * mul;
+                    *reinterpret_cast<f32x4*>(Os + l32 * OW + d) = v4;
+                } else {
+                    s16x4 v4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v4[e] = Elem<T>::pack1(acc[i][4 * g + e] * mul);
+                    *reinterpret_cast<s16x4*>(Os + l32 * OW + d) = v4;
+                }
+            }
+    }
+    lds_barrier();
+    if (mine) {
+        constexpr int EPC = 16 / (int)sizeof(T), CPR = D / EPC;
+#pragma unroll
+        for (int i = 0; i < 32 * CPR / 64; ++i) {
+            const int cidx = lane + 64 * i, row = cidx / CPR, col = cidx % CPR;
+            if (row0 + row < n_rows && col * EPC < cols)
+                *reinterpret_cast<uint4*>(base + (int64_t)(row0 + row) * stride + col * EPC) =
+                    *reinterpret_cast<const uint4*>(Os + row * OW + col * EPC);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Forward, over the tiles of a walk.  KS = 2: two groups of 4 waves on the same
+// queries, taking the walk's tiles in turn, for grids that leave CUs idle.
+template <typename T, int D, bool CAP, bool SLOPE, int KS>
+__global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) ? 2 : 1)) void scored_fwd_kernel(
+    const ScoredParams p) {
+    using C = FwdCfg<T, D>;
+    constexpr int BN = C::BN, NB = C::NB, KW = C::KW, VW = C::VW, NW = C::NW;
+    constexpr int TPD = 64 / BN;  // tiles per range of document ids
+    __shared__ __attribute__((aligned(16))) T smem[C::SMEM_ELEMS * KS];
+
+    const int tid = threadIdx.x;
+    const int lane = tid & 63, wg = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
+    const int w = KS == 1 ? wg : wg & 3, sp = KS == 1 ? 0 : wg >> 2;
+    const int2 tord = tile_order<32 * (KS == 1 ? 2 : 1), true>(p.n_tiles);
+    const int qt = p.n_tiles - 1 - tord.y;  // longest causal rows first
+    const int h = tord.x % p.H, b = tord.x / p.H;
+    const int hk = h / p.group;
+    const int q0 = qt * C::BM, qw0 = q0 + 32 * w, qi = qw0 + l32;
+    const SeqRule rule(p, b);
+
+    const T* __restrict__ kbase = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
+    const T* __restrict__ vbase = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
+
+    // ---- Q into registers (MFMA B operand) ----
+    constexpr int QR = C::F32 ? D / 8 : D / 16;
+    uint4 qreg[QR];
+    {
+        const T* qrow = (const T*)p.q + b * p.q_sb + (int64_t)qi * p.q_ss + h * p.q_sh;
+#pragma unroll
+        for (int i = 0; i < QR; ++i) {
+            const int d0 = C::F32 ? hi * (D / 2) + 4 * i : 16 * i + 8 * hi;
+            qreg[i] = qi < p.Sq && d0 < p.cols ? *reinterpret_cast<const uint4*>(qrow + d0) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+
+    // ---- the walk over key tiles ----
+    const int lim_hi = rule.lim(min(q0 + C::BM, p.Sq) - 1);
+    const int n_kt = (max(lim_hi, 0) + BN - 1) / BN;
+    const int wlim_lo = rule.lim(qw0), wlim_hi = qw0 < p.Sq ? rule.lim(min(qw0 + 31, p.Sq - 1)) : 0;
+    const int lim_l = rule.lim(qi);
+    const bool docs = p.q_docs != nullptr;
+    const int* kdoc = p.k_docs + (docs ? (int64_t)b * p.k_docs_pad : 0);
+    const int2* krng = p.k_rng + (docs ? (int64_t)b * (p.k_docs_pad / 64) : 0);
+    int2 qr = {0, 0}, wr = {0, 0};
+    int qd = -2;  // no key's id
+    if (docs) {
+        const int2* qrng = p.q_rng + (int64_t)b * (p.q_docs_pad / 64) + q0 / 64;
+        const int2 a = uniform2(qrng[0]), c = q0 + 64 < p.q_docs_pad ? uniform2(qrng[1]) : a;
+        qr = docs_join(a, c);
+        // a wave past the last query may lie past the ranges: it is never active
+        wr = w < 2 ? a : c;
+        const int id = qi < p.Sq ? p.q_docs[(int64_t)b * p.q_docs_pad + qi] : -1;
+        if (id >= 0) qd = id;
+    }
+    uint64_t c_vis = 0, c_act = 0, c_full = 0, c_neg = 0;  // the chunk's tiles
+    int base = -64;
+    auto next = [&]() FA_INLINE -> TileRef {
+        while (c_vis == 0) {
+            base += 64;
+            if (base >= n_kt) {
+                base = n_kt;  // stays past the end
+                return TileRef{-1, 0u};
+            }
+            const int t = base + lane, k0 = t * BN;
+            bool v = t < n_kt, a = v && k0 < wlim_hi, f = k0 + BN <= wlim_lo, n = false;
+            if (docs) {
+                const int2 r = v ? krng[t / TPD] : make_int2(-1, -1);
+                v = v && docs_meet(r, qr);
+                a = a && v && docs_meet(r, wr);
+                f = f && docs_one(r, wr);
+                n = r.x < 0;
+            }
+            c_vis = __ballot(v);
+            c_act = __ballot(a);
+            c_full = __ballot(f);
+            c_neg = __ballot(n);
+        }
+        const int i = (int)__builtin_ctzll(c_vis);
+        c_vis &= c_vis - 1;
+        return TileRef{base + i, kMore | ((c_act >> i) & 1 ? kAct : 0u) | ((c_full >> i) & 1 ? kFull : 0u) |
+                                     ((c_neg >> i) & 1 ? kNeg : 0u)};
+    };
+    // this group's next tile; kMore and kNeg of the groups together (barriers)
+    auto fetch = [&]() FA_INLINE -> TileRef {
+        TileRef r = next();
+        if constexpr (KS == 2) {
+            const TileRef r2 = next();
+            const unsigned both = (r.fl | r2.fl) & (kMore | kNeg);
+            if (sp) r = r2;
+            r.fl |= both;
+        }
+        return r;
+    };
+
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) o[i] = f32x16{};
+    float m_run = -1e30f;  // running max in log2 units
+    float l_run = 0.f;     // lane-partial row sum
+    const float c = p.scale_log2;
+    Cap<C::F32> cap(p);
+    const float slope2 = SLOPE ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
+    const float qpos = (float)(qi + rule.off);
+
+    T* Ks0 = smem + sp * C::SMEM_ELEMS;
+    T* Vs0 = Ks0 + 2 * C::KTILE;
+    DmaTile<T, BN, D, KW, NW> kdma;
+    kdma.init(p.k_ss, lane, w, p.cols);
+    DmaTile<T, BN, D, VW, NW> vdma;
+    vdma.init(p.v_ss, lane, w, p.cols);
+    // keys past the sequence's length land as zeros; no tile: nothing is read
+    auto load_k = [&](const TileRef& r, int slot) FA_INLINE {
+        const int k0 = max(r.t, 0) * BN, nv = r.t < 0 ? 0 : rule.len - k0;
+        if constexpr (C::F32)
+            kdma.load(kbase + (int64_t)k0 * p.k_ss, p.k_ss, nv, Ks0 + slot * C::KTILE, lane);
+        else
+            kdma.load_untracked(kbase + (int64_t)k0 * p.k_ss, p.k_ss, nv, Ks0 + slot * C::KTILE, lane);
+    };
+    auto load_v = [&](const TileRef& r, int slot) FA_INLINE {
+        const int k0 = max(r.t, 0) * BN, nv = r.t < 0 ? 0 : rule.len - k0;
+        if constexpr (C::F32)
+            vdma.load(vbase + (int64_t)k0 * p.v_ss, p.v_ss, nv, Vs0 + slot * C::VTILE, lane);
+        else
+            vdma.load_untracked(vbase + (int64_t)k0 * p.v_ss, p.v_ss, nv, Vs0 + slot * C::VTILE, lane);
+    };
+
+    // ---- S^T = K Q^T of a tile ----
+    auto qk = [&](const T* Ks, f32x16 (&s)[NB]) FA_INLINE {
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk) {
+            s[blk] = f32x16{};
+            const T* krow = Ks + (32 * blk + l32) * KW;
+#pragma unroll
+            for (int i = 0; i < QR; ++i) {
+                if constexpr (C::F32) {
+                    const f32x4 a = *reinterpret_cast<const f32x4*>(krow + hi * (D / 2) + 4 * i);
+                    const f32x4 bq = __builtin_bit_cast(f32x4, qreg[i]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[blk] = mfma_f32(a[e], bq[e], s[blk]);
+                } else {
+                    const s16x8 a = *reinterpret_cast<const s16x8*>(krow + 16 * i + 8 * hi);
+                    s[blk] = Elem<T>::mfma(a, __builtin_bit_cast(s16x8, qreg[i]), s[blk]);
+                }
+            }
+        }
+    };
+    // ---- rules, mask and running max.  A score is held as u, its value in log2
+    // units is ua u + ub: u the raw product, or r of the cap (which falls with
+    // the score), or the value itself ----
+    constexpr bool RCP = CAP && !SLOPE && !C::F32, VALUE = SLOPE || (CAP && C::F32);
+    const float ua = VALUE ? 1.f : RCP ? -2.f * cap.top : c, ub = RCP ? cap.top : 0.f;
+    constexpr float kHidden = RCP ? INFINITY : -INFINITY;
+    auto score = [&](f32x16 (&s)[NB], const TileRef& r) FA_INLINE {
+        const int k0 = r.t * BN;
+        if constexpr (RCP) {
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[blk][e] = cap.rcp(s[blk][e]);
+        } else if constexpr (VALUE) {
+            const float d0 = qpos - (float)(k0 + 4 * hi);
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float t = CAP ? cap.value(s[blk][e]) : s[blk][e] * c;
+                    const float d = d0 - (float)(32 * blk + 8 * (e >> 2) + (e & 3));
+                    s[blk][e] = SLOPE ? __builtin_fmaf(-slope2, __builtin_fabsf(d), t) : t;
+                }
+        }
+        if (!(r.fl & kFull)) {
+            const int lim = lim_l - k0 - 4 * hi;
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (32 * blk + 8 * (e >> 2) + (e & 3) >= lim) s[blk][e] = kHidden;
+            if (docs) {
+#pragma unroll
+                for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int4 kd = *reinterpret_cast<const int4*>(kdoc + k0 + 32 * blk + 8 * g + 4 * hi);
+                        if (kd.x != qd) s[blk][4 * g] = kHidden;
+                        if (kd.y != qd) s[blk][4 * g + 1] = kHidden;
+                        if (kd.z != qd) s[blk][4 * g + 2] = kHidden;
+                        if (kd.w != qd) s[blk][4 * g + 3] = kHidden;
+                    }
+            }
+        }
+        float mx = kHidden;
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mx = RCP ? fminf(mx, s[blk][e]) : fmaxf(mx, s[blk][e]);
+        mx = pair_max(__builtin_fmaf(mx, ua, ub));
+        const float m_new = fmaxf(m_run, mx);
+        if (__ballot(m_new > m_run + 8.0f) != 0ull) {
+            const float alpha = fast_exp2(m_run - m_new);
+            l_run *= alpha;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+            m_run = m_new;
+        }
+    };
+    constexpr int NPK = C::F32 ? 1 : BN / 16;
+    auto softmax = [&](f32x16 (&s)[NB], s16x8 (&pk)[NPK]) FA_INLINE {
+        const float um = ub - m_run;
+        float psum = 0.f;
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[blk][e] = fast_exp2(VALUE ? s[blk][e] + um : __builtin_fmaf(s[blk][e], ua, um));
+                psum += s[blk][e];
+            }
+        l_run += psum;
+        if constexpr (!C::F32) {
+#pragma unroll
+            for (int ks = 0; ks < BN / 16; ++ks) {
+                float tmp[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) tmp[e] = s[ks >> 1][8 * (ks & 1) + e];
+                pk[ks] = pack8<T>(tmp);
+            }
+        }
+    };
+    // ---- O^T += V^T P^T ----
+    auto pv = [&](const T* Vs, const f32x16 (&s)[NB], const s16x8 (&pk)[NPK]) FA_INLINE {
+        if constexpr (C::F32) {
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int t = 0; t < 16; ++t) {
+                    const T* vrow = Vs + (32 * blk + 8 * (t >> 2) + 4 * hi + (t & 3)) * VW + l32;
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) o[i] = mfma_f32(vrow[32 * i], s[blk][t], o[i]);
+                }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < BN / 16; ++ks)
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    const T* vp = Vs + (16 * ks + 4 * hi + ((lane & 15) >> 2)) * VW + 32 * i + 16 * ((lane >> 4) & 1) +
+                                  4 * (lane & 3);
+                    const s16x8 a = cat4(lds_read_tr16(vp), lds_read_tr16(vp + 8 * VW));
+                    o[i] = Elem<T>::mfma(a, pk[ks], o[i]);
+                }
+        }
+    };
+    auto sync_tiles = [&]() FA_INLINE {
+        wait_vmem();
+        lds_barrier();
+    };
+
+    // two slots in turn: tile j is read while tile j + 1 lands in the other,
+    // last read before the barrier that opens the iteration
+    TileRef cur = fetch();
+    int slot = 0;
+    if (cur.fl & kMore) {
+        load_k(cur, 0);
+        load_v(cur, 0);
+    }
+    while (cur.fl & kMore) {
+        sync_tiles();
+        const TileRef nxt = fetch();
+        load_k(nxt, slot ^ 1);
+        load_v(nxt, slot ^ 1);
+        T* const Vs = Vs0 + slot * C::VTILE;
+        if (cur.fl & kNeg) {  // the groups together
+            if (cur.t >= 0) clear_rows<T, BN, D, VW, 256>(Vs, kdoc + cur.t * BN, tid & 255);
+            lds_barrier();
+        }
+        if (cur.fl & kAct) {
+            f32x16 s[NB];
+            s16x8 pk[NPK];
+            qk(Ks0 + slot * C::KTILE, s);
+            score(s, cur);
+            softmax(s, pk);
+            pv(Vs, s, pk);
+        }
+        slot ^= 1;
+        cur = nxt;
+    }
+    sync_tiles();  // all waves done with the tiles, no copy in flight
+
+    if constexpr (KS == 2) {
+        // ---- the second group's part joins the first's (rescaled to the common maximum) ----
+        constexpr int NO = (D / 32) * 16, NF = NO + 2;
+        static_assert(4 * NF * 64 * 4 <= C::SMEM_ELEMS * (int)sizeof(T), "a group's part fits its tile buffers");
+        float* mg = reinterpret_cast<float*>(smem + C::SMEM_ELEMS);
+        auto at = [&](int f) FA_INLINE { return mg + (w * NF + f) * 64 + lane; };
+        if (sp > 0) {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) *at(16 * i + e) = o[i][e];
+            *at(NO) = m_run;
+            *at(NO + 1) = l_run;
+        }
+        lds_barrier();
+        if (sp == 0) {
+            const float m1 = *at(NO), mm = fmaxf(m_run, m1);
+            const float a0 = fast_exp2(m_run - mm), a1 = fast_exp2(m1 - mm);
+            l_run = __builtin_fmaf(*at(NO + 1), a1, l_run * a0);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[i][e] = __builtin_fmaf(*at(16 * i + e), a1, o[i][e] * a0);
+            m_run = mm;
+        }
+    }
+
+    // ---- epilogue: normalise, LSE, O^T through LDS as rows ----
+    const float l_tot = pair_sum(l_run);
+    const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
+    if (sp == 0 && hi == 0 && qi < p.Sq)
+        p.lse[(int64_t)(b * p.H + h) * p.Sq + qi] =
+            l_tot > 0.f ? (m_run + __log2f(l_tot)) * kLn2 : l_tot == 0.f ? -INFINITY : l_tot;
+    store_rows<T, D>(smem + w * 32 * C::OW, C::OW, o, inv, (T*)p.o + b * p.o_sb + h * p.o_sh, p.o_ss,
+                     qw0, p.Sq, p.cols, lane, sp == 0);
+}
+
+// ---------------------------------------------------------------------------
+// dQ, and per query the rows LSE * log2 e and delta = rowsum(dO O) that the
+// dK/dV pass reads after it.  dS goes through the cap's derivative (/ 4, made up
+// for in the final scale).
+// DSLOPE: also -d loss / d slope of each row, sum_j |d| P (dP - delta) with
+// delta summed from P dP here instead of taken from the rounded output: the sum
+// over all rows is returned in float32, whose digits the rounding would cost.
+template <typename T, int D, bool CAP, bool SLOPE, bool DSLOPE, int KS>
+__global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) void scored_dq_kernel(const ScoredParams p) {
+    using C = DqCfg<T, D>;
+    constexpr int BN = C::BN, KW = C::KW;
+    static_assert(BN == 64, "one range of document ids a tile");
+    __shared__ __attribute__((aligned(16))) char smem[C::SMEM_BYTES * KS];
+
+    const int tid = threadIdx.x;
+    const int lane = tid & 63, wg = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
+    const int w = KS == 1 ? wg : wg & 3, sp = KS == 1 ? 0 : wg >> 2;
+    const int2 tord = tile_order<32 * (KS == 1 ? C::MIN_BLOCKS : 1), true>(p.n_tiles);
+    const int qt = p.n_tiles - 1 - tord.y;
+    const int h = tord.x % p.H, b = tord.x / p.H;
+    const int hk = h / p.group;
+    const int q0 = qt * C::BM, qw0 = q0 + 32 * w, qi = qw0 + l32;
+    const SeqRule rule(p, b);
+
+    constexpr int QR = C::F32 ? D / 8 : D / 16;
+    uint4 qreg[QR], doreg[QR];
+    float del = 0.f;
+    {
+        const T* qrow = (const T*)p.q + b * p.q_sb + (int64_t)qi * p.q_ss + h * p.q_sh;
+        const T* drow = (const T*)p.dout + b * p.do_sb + (int64_t)qi * p.do_ss + h * p.do_sh;
+        const T* orow = (const T*)p.o + b * p.o_sb + (int64_t)qi * p.o_ss + h * p.o_sh;
+#pragma unroll
+        for (int i = 0; i < QR; ++i) {
+            const int d0 = C::F32 ? hi * (D / 2) + 4 * i : 16 * i + 8 * hi;
+            const bool ok = qi < p.Sq && d0 < p.cols;
+            qreg[i] = ok ? *reinterpret_cast<const uint4*>(qrow + d0) : make_uint4(0u, 0u, 0u, 0u);
+            doreg[i] = ok ? *reinterpret_cast<const uint4*>(drow + d0) : make_uint4(0u, 0u, 0u, 0u);
+            const uint4 ov = ok ? *reinterpret_cast<const uint4*>(orow + d0) : make_uint4(0u, 0u, 0u, 0u);
+            float part = 0.f;
+            if constexpr (C::F32) {
+                const f32x4 x = __builtin_bit_cast(f32x4, ov), y = __builtin_bit_cast(f32x4, doreg[i]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part = __builtin_fmaf(x[e], y[e], part);
+            } else {
+                const s16x8 x = __builtin_bit_cast(s16x8, ov), y = __builtin_bit_cast(s16x8, doreg[i]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) part = __builtin_fmaf(Elem<T>::unpack1(x[e]), Elem<T>::unpack1(y[e]), part);
+            }
+            del += part;
+        }
+        del = pair_sum(del);
+    }
+    const float lse_in = qi < p.Sq ? p.lse[(int64_t)(b * p.H + h) * p.Sq + qi] : -INFINITY;
+    // a row that sees nothing, and rows past the last: P = exp2(s - inf) = 0
+    const float lse2 = lse_in == -INFINITY ? INFINITY : lse_in * kLog2e;
+    if (sp == 0 && hi == 0) {
+        const int64_t wi = ((int64_t)b * p.H + h) * p.ws_stride + qi;  // qi < sq_pad
+        p.lse2[wi] = lse2;
+        p.lse2[wi + p.sq_pad] = qi < p.Sq ? del : 0.f;
+    }
+
+    const int lim_hi = rule.lim(min(q0 + C::BM, p.Sq) - 1);
+    const int n_kt = (max(lim_hi, 0) + BN - 1) / BN;
+    const int wlim_lo = rule.lim(qw0), wlim_hi = qw0 < p.Sq ? rule.lim(min(qw0 + 31, p.Sq - 1)) : 0;
+    const int lim_l = rule.lim(qi);
+    const bool docs = p.q_docs != nullptr;
+    const int* kdoc = p.k_docs + (docs ? (int64_t)b * p.k_docs_pad : 0);
+    const int2* krng = p.k_rng + (docs ? (int64_t)b * (p.k_docs_pad / 64) : 0);
+    int2 qr = {0, 0}, wr = {0, 0};
+    int qd = -2;
+    if (docs) {
+        const int2* qrng = p.q_rng + (int64_t)b * (p.q_docs_pad / 64) + q0 / 64;
+        const int2 a = uniform2(qrng[0]), c = q0 + 64 < p.q_docs_pad ? uniform2(qrng[1]) : a;
+        qr = docs_join(a, c);
+        wr = w < 2 ? a : c;
+        const int id = qi < p.Sq ? p.q_docs[(int64_t)b * p.q_docs_pad + qi] : -1;
+        if (id >= 0) qd = id;
+    }
+    uint64_t c_vis = 0, c_act = 0, c_full = 0, c_neg = 0;  // the chunk's tiles
+    int base = -64;
+    auto next = [&]() FA_INLINE -> TileRef {
+        while (c_vis == 0) {
+            base += 64;
+            if (base >= n_kt) {
+                base = n_kt;
+                return TileRef{-1, 0u};
+            }
+            const int t = base + lane, k0 = t * BN;
+            bool v = t < n_kt, a = v && k0 < wlim_hi, f = k0 + BN <= wlim_lo, n = false;
+            if (docs) {
+                const int2 r = v ? krng[t] : make_int2(-1, -1);
+                v = v && docs_meet(r, qr);
+                a = a && v && docs_meet(r, wr);
+                f = f && docs_one(r, wr);
+                n = r.x < 0;
+            }
+            c_vis = __ballot(v);
+            c_act = __ballot(a);
+            c_full = __ballot(f);
+            c_neg = __ballot(n);
+        }
+        const int i = (int)__builtin_ctzll(c_vis);
+        c_vis &= c_vis - 1;
+        return TileRef{base + i, kMore | ((c_act >> i) & 1 ? kAct : 0u) | ((c_full >> i) & 1 ? kFull : 0u) |
+                                     ((c_neg >> i) & 1 ? kNeg : 0u)};
+    };
+    auto fetch = [&]() FA_INLINE -> TileRef {
+        TileRef r = next();
+        if constexpr (KS == 2) {
+            const TileRef r2 = next();
+            const unsigned both = (r.fl | r2.fl) & (kMore | kNeg);
+            if (sp) r = r2;
+            r.fl |= both;
+        }
+        return r;
+    };
+
+    f32x16 dq[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) dq[i] = f32x16{};
+    const float c = p.scale_log2;
+    Cap<C::F32> cap(p);
+    const float slope2 = SLOPE ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
+    const float qpos = (float)(qi + rule.off);
+    float sum_dp = 0.f, sum_d = 0.f, sum_ddp = 0.f;  // sums of P dP, |d| P, |d| P dP (DSLOPE)
+
+    const T* kbase = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
+    const T* vbase = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
+    const bool copy_k = w < C::NW / 2;
+    typename C::Rows rows;
+    rows.init(copy_k ? p.k_ss : p.v_ss, lane, w % (C::NW / 2), p.cols);
+    auto buf = [&](int s) FA_INLINE -> char* { return smem + sp * C::SMEM_BYTES + s * C::BUF_BYTES; };
+    auto issue = [&](const TileRef& r, int s) FA_INLINE {
+        const int k0 = max(r.t, 0) * BN, nv = r.t < 0 ? 0 : rule.len - k0;
+        const T* src = copy_k ? kbase + (int64_t)k0 * p.k_ss : vbase + (int64_t)k0 * p.v_ss;
+        // (float32: copies that the compiler tracks; with the others it runs out of
+        // scalar registers for their addresses)
+        if constexpr (C::F32)
+            rows.load(src, copy_k ? p.k_ss : p.v_ss, nv, (T*)(buf(s) + (copy_k ? 0 : C::KALLOC)));
+        else
+            rows.load_untracked(src, copy_k ? p.k_ss : p.v_ss, nv, (const T*)(buf(s) + (copy_k ? 0 : C::KALLOC)));
+    };
+    auto sync_tiles = [&]() FA_INLINE {
+        wait_vmem();
+        lds_barrier();
+    };
+    // ---- S^T = K Q^T, dP^T = V dO^T of 32 keys ----
+    auto sdp = [&](const T* Ks, const T* Vs, f32x16& s, f32x16& dp) FA_INLINE {
+        s = f32x16{};
+        dp = f32x16{};
+        const T* krow = Ks + l32 * KW;
+        const T* vrow = Vs + l32 * KW;
+#pragma unroll
+        for (int i = 0; i < QR; ++i) {
+            if constexpr (C::F32) {
+                const f32x4 ak = *reinterpret_cast<const f32x4*>(krow + hi * (D / 2) + 4 * i);
+                const f32x4 av = *reinterpret_cast<const f32x4*>(vrow + hi * (D / 2) + 4 * i);
+                const f32x4 bq = __builtin_bit_cast(f32x4, qreg[i]), bd = __builtin_bit_cast(f32x4, doreg[i]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s = mfma_f32(ak[e], bq[e], s);
+                    dp = mfma_f32(av[e], bd[e], dp);
+                }
+            } else {
+                const s16x8 ak = *reinterpret_cast<const s16x8*>(krow + 16 * i + 8 * hi);
+                const s16x8 av = *reinterpret_cast<const s16x8*>(vrow + 16 * i + 8 * hi);
+                s = Elem<T>::mfma(ak, __builtin_bit_cast(s16x8, qreg[i]), s);
+                dp = Elem<T>::mfma(av, __builtin_bit_cast(s16x8, doreg[i]), dp);
+            }
+        }
+    };
+    // ---- dX^T = P^T (dP^T - delta) cap', then dQ^T += K^T dX^T ----
+    auto fin = [&](int k0, const T* Ks, f32x16& s, const f32x16& dp, bool full) FA_INLINE {
+        const int lim = lim_l - k0 - 4 * hi;
+        const float d0 = qpos - (float)(k0 + 4 * hi);
+        uint32_t hide = 0;  // bit r: masked
+        if (!full) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (8 * (r >> 2) + (r & 3) >= lim) hide |= 1u << r;
+            if (docs) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int4 kd = *reinterpret_cast<const int4*>(kdoc + k0 + 8 * g + 4 * hi);
+                    hide |= (kd.x != qd ? 1u : 0u) << (4 * g) | (kd.y != qd ? 2u : 0u) << (4 * g) |
+                            (kd.z != qd ? 4u : 0u) << (4 * g) | (kd.w != qd ? 8u : 0u) << (4 * g);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float ad = __builtin_fabsf(d0 - (float)(8 * (r >> 2) + (r & 3)));
+            float pv;
+            if constexpr (CAP) {
+                float t = cap.value(s[r]) - lse2;
+                if (SLOPE) t = __builtin_fmaf(-slope2, ad, t);
+                pv = fast_exp2(t);
+            } else {
+                pv = fast_exp2(__builtin_fmaf(s[r], c, SLOPE ? __builtin_fmaf(-slope2, ad, -lse2) : -lse2));
+            }
+            if constexpr (DSLOPE) {
+                const bool out = !full && ((hide >> r) & 1u);
+                const float pz = out ? 0.f : pv, pdp = out ? 0.f : pv * dp[r];
+                sum_dp += pdp;
+                sum_d = __builtin_fmaf(pz, ad, sum_d);
+                sum_ddp = __builtin_fmaf(pdp, ad, sum_ddp);
+            }
+            float ds = pv * (dp[r] - del);
+            if (CAP) ds *= cap.slope();
+            s[r] = !full && ((hide >> r) & 1u) ? 0.f : ds;
+        }
+        if constexpr (C::F32) {
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+                const T* kr = Ks + (8 * (t >> 2) + 4 * hi + (t & 3)) * KW + l32;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) dq[i] = mfma_f32(kr[32 * i], s[t], dq[i]);
+            }
+        } else {
+            const int trow = 4 * hi + ((lane & 15) >> 2);
+            const int tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                float ts[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ts[e] = s[8 * ks + e];
+                const s16x8 bs8 = pack8<T>(ts);
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    const T* kp = Ks + (16 * ks + trow) * KW + 32 * i + tcol;
+                    const s16x8 a = cat4(lds_read_tr16(kp), lds_read_tr16(kp + 8 * KW));
+                    dq[i] = Elem<T>::mfma(a, bs8, dq[i]);
+                }
+            }
+        }
+    };
+
+    // two buffers in turn: tile j is read while tile j + 1 lands in the other,
+    // last read before the barrier that opens the iteration
+    TileRef cur = fetch();
+    int bc = 0;
+    if (cur.fl & kMore) issue(cur, 0);
+    while (cur.fl & kMore) {
+        sync_tiles();
+        const TileRef nxt = fetch();
+        issue(nxt, bc ^ 1);
+        T* const Ks = (T*)buf(bc);
+        const T* const Vs = (const T*)(buf(bc) + C::KALLOC);
+        if (cur.fl & kNeg) {
+            if (cur.t >= 0) clear_rows<T, BN, D, KW, 256>(Ks, kdoc + cur.t * BN, tid & 255);
+            lds_barrier();
+        }
+        if (cur.fl & kAct) {
+            const int k0 = cur.t * BN;
+            const bool full = (cur.fl & kFull) != 0;
+            f32x16 s0, dp0, s1, dp1;
+            sdp(Ks, Vs, s0, dp0);
+            sdp(Ks + 32 * KW, Vs + 32 * KW, s1, dp1);
+            fin(k0, Ks, s0, dp0, full);
+            fin(k0 + 32, Ks + 32 * KW, s1, dp1, full);
+        }
+        bc ^= 1;
+        cur = nxt;
+    }
+    sync_tiles();
+    if constexpr (DSLOPE) {
+        sum_dp = pair_sum(sum_dp);
+        sum_d = pair_sum(sum_d);
+        sum_ddp = pair_sum(sum_ddp);
+    }
+    if constexpr (KS == 2) {
+        constexpr int NO = (D / 32) * 16, NF = NO + (DSLOPE ? 3 : 0);
+        static_assert(4 * NF * 64 * 4 <= C::SMEM_BYTES, "a group's part fits its tile buffers");
+        float* mg = reinterpret_cast<float*>(smem + C::SMEM_BYTES);
+        auto at = [&](int f) FA_INLINE { return mg + (w * NF + f) * 64 + lane; };
+        if (sp > 0) {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) *at(16 * i + e) = dq[i][e];
+            if (DSLOPE) {
+                *at(NO) = sum_dp;
+                *at(NO + 1) = sum_d;
+                *at(NO + 2) = sum_ddp;
+            }
+        }
+        lds_barrier();
+        if (sp == 0) {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) dq[i][e] += *at(16 * i + e);
+            if (DSLOPE) {
+                sum_dp += *at(NO);
+                sum_d += *at(NO + 1);
+                sum_ddp += *at(NO + 2);
+            }
+        }
+    }
+    if constexpr (DSLOPE) {
+        if (sp == 0 && hi == 0 && qi < p.Sq)
+            p.dslope_rows[((int64_t)b * p.H + h) * p.Sq + qi] = __builtin_fmaf(sum_dp, sum_d, -sum_ddp);
+    }
+    store_rows<T, D>((T*)smem + w * 32 * C::OW, C::OW, dq, p.scale * (CAP ? 4.f : 1.f),
+                     (T*)p.dq + b * p.dq_sb + h * p.dq_sh, p.dq_ss, qw0, p.Sq, p.cols, lane, sp == 0);
+}
+
+// ---------------------------------------------------------------------------
+// dK and dV of 128 keys of one (batch, KV head): the query heads of the group
+// one after the other, each over the 64-query tiles that the keys are seen by,
+// the last first (so that the workgroups of a head read the same tiles at about
+// the same time).  K and V rows in registers, as in dkdv_kernel.
+template <typename T, int D, bool CAP, bool SLOPE>
+__global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void scored_dkdv_kernel(const ScoredParams p) {
+    using C = DkdvCfg<T, D>;
+    constexpr int BQ = C::BQ, RW = C::RW;
+    static_assert(BQ == 64, "one range of document ids a tile; one dword a lane for LSE and delta");
+    __shared__ __attribute__((aligned(16))) char smem[C::SMEM_BYTES];
+
+    const int tid = threadIdx.x;
+    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
+    const int2 tord = tile_order<32 * (!(Elem<T>::kF32 && D == 128) ? 2 : 1), true>(p.n_tiles);
+    const int kt = tord.y;  // the first keys are seen by the most queries
+    const int hk = tord.x % p.Hkv, b = tord.x / p.Hkv;
+    const int k0 = kt * C::BK, kw0 = k0 + 32 * w, kj = kw0 + l32;
+    const SeqRule rule(p, b);
+
+    constexpr int KR = C::F32 ? D / 8 : D / 16;
+    uint4 kreg[KR], vreg[KR];
+    {
+        const T* krow = (const T*)p.k + b * p.k_sb + (int64_t)kj * p.k_ss + hk * p.k_sh;
+        const T* vrow = (const T*)p.v + b * p.v_sb + (int64_t)kj * p.v_ss + hk * p.v_sh;
+#pragma unroll
+        for (int i = 0; i < KR; ++i) {
+            const int d0 = C::F32 ? hi * (D / 2) + 4 * i : 16 * i + 8 * hi;
+            const bool ok = kj < rule.len && d0 < p.cols;
+            kreg[i] = ok ? *reinterpret_cast<const uint4*>(krow + d0) : make_uint4(0u, 0u, 0u, 0u);
+            vreg[i] = ok ? *reinterpret_cast<const uint4*>(vrow + d0) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+
+    // ---- the walk over (query head of the group, query tile), downwards ----
+    const int first0 = rule.first(k0);                 // of the block's keys: none of them sooner
+    const int wfirst_lo = rule.first(kw0), wfirst_hi = rule.first(kw0 + 31);
+    const int first_l = rule.first(kj);
+    const int n_qt = (p.Sq + BQ - 1) / BQ;
+    const int t_lo = first0 == INT_MAX ? n_qt : min(n_qt, first0 / BQ);  // tiles [t_lo, n_qt)
+    const bool docs = p.q_docs != nullptr;
+    const int* qdoc = p.q_docs + (docs ? (int64_t)b * p.q_docs_pad : 0);
+    const int2* qrng = p.q_rng + (docs ? (int64_t)b * (p.q_docs_pad / 64) : 0);
+    int2 kr = {0, 0}, wr = {0, 0};
+    int kd = -2;
+    if (docs) {
+        const int2* krng = p.k_rng + (int64_t)b * (p.k_docs_pad / 64) + k0 / 64;
+        const int2 a = uniform2(krng[0]), c = k0 + 64 < p.k_docs_pad ? uniform2(krng[1]) : a;
+        kr = docs_join(a, c);
+        wr = w < 2 ? a : c;
+        const int id = kj < p.Sk ? p.k_docs[(int64_t)b * p.k_docs_pad + kj] : -1;
+        if (id >= 0) kd = id;
+    }
+    uint64_t c_vis = 0, c_act = 0, c_full = 0, c_neg = 0;  // the chunk's tiles
+    int base = n_qt, g = 0;  // chunk [base, base + 64), head of the group
+    int tile_g = 0;
+    auto next = [&]() FA_INLINE -> TileRef {
+        while (c_vis == 0) {
+            if (base <= t_lo) {
+                if (g + 1 >= p.group || t_lo >= n_qt) {
+                    g = p.group;
+                    return TileRef{-1, 0u};
+                }
+                ++g;
+                base = n_qt;
+            }
+            base -= 64;
+            const int t = base + lane, qa = t * BQ, qz = min(qa + BQ, p.Sq) - 1;  // first and last query
+            bool v = t >= t_lo && t < n_qt, a = v && qz >= wfirst_lo, f = qa >= wfirst_hi, n = false;
+            if (docs) {
+                const int2 r = v ? qrng[t] : make_int2(-1, -1);
+                v = v && docs_meet(r, kr);
+                a = a && v && docs_meet(r, wr);
+                f = f && docs_one(r, wr);
+                n = r.x < 0;
+            }
+            c_vis = __ballot(v);
+            c_act = __ballot(a);
+            c_full = __ballot(f);
+            c_neg = __ballot(n);
+        }
+        const int i = 63 - (int)__builtin_clzll(c_vis);
+        c_vis &= ~(1ull << i);
+        tile_g = g;
+        return TileRef{base + i, kMore | ((c_act >> i) & 1 ? kAct : 0u) | ((c_full >> i) & 1 ? kFull : 0u) |
+                                     ((c_neg >> i) & 1 ? kNeg : 0u)};
+    };
+
+    f32x16 dk[D / 32], dv[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+        dk[i] = f32x16{};
+        dv[i] = f32x16{};
+    }
+    const float c = p.scale_log2;
+    Cap<C::F32> cap(p);
+
+    const bool copy_q = w < C::NW / 2;
+    typename C::Rows rows;
+    rows.init(copy_q ? p.q_ss : p.do_ss, lane, w % (C::NW / 2), p.cols);
+    auto buf = [&](int s) FA_INLINE -> char* { return smem + s * C::BUF_BYTES; };
+    auto issue = [&](const TileRef& r, int hh, int s) FA_INLINE {
+        const int qb0 = max(r.t, 0) * BQ, nv = r.t < 0 ? 0 : p.Sq - qb0;
+        char* bp = buf(s);
+        const T* src = copy_q ? (const T*)p.q + b * p.q_sb + (int64_t)qb0 * p.q_ss + hh * p.q_sh
+                              : (const T*)p.dout + b * p.do_sb + (int64_t)qb0 * p.do_ss + hh * p.do_sh;
+        if constexpr (C::F32)
+            rows.load(src, copy_q ? p.q_ss : p.do_ss, nv, (T*)(bp + (copy_q ? 0 : C::QALLOC)));
+        else
+            rows.load_untracked(src, copy_q ? p.q_ss : p.do_ss, nv, (const T*)(bp + (copy_q ? 0 : C::QALLOC)));
+        const float* wrow = p.lse2 + ((int64_t)b * p.H + hh) * p.ws_stride + qb0;  // qb0 + BQ <= sq_pad
+        const u32x4 rs = buffer_words(wrow, r.t < 0 ? 0 : (p.ws_stride - qb0) * 4);
+        const uint32_t f = lds_addr(bp + 2 * C::QALLOC);
+        dma_load4_untracked(rs, f, 4 * lane);
+        dma_load4_untracked(rs, f + 4 * BQ, 4 * (p.sq_pad + lane));
+    };
+    auto sync_tiles = [&]() FA_INLINE {
+        wait_vmem();
+        lds_barrier();
+    };
+    // ---- S = Q K^T, dP = dO V^T of 32 queries ----
+    auto sdp = [&](int s, int st, f32x16& sc, f32x16& dpc) FA_INLINE {
+        sc = f32x16{};
+        dpc = f32x16{};
+        const T* qrow = (const T*)buf(s) + (32 * st + l32) * RW;
+        const T* drow = (const T*)(buf(s) + C::QALLOC) + (32 * st + l32) * RW;
+#pragma unroll
+        for (int i = 0; i < KR; ++i) {
+            if constexpr (C::F32) {
+                const f32x4 aq = *reinterpret_cast<const f32x4*>(qrow + hi * (D / 2) + 4 * i);
+                const f32x4 ad = *reinterpret_cast<const f32x4*>(drow + hi * (D / 2) + 4 * i);
+                const f32x4 bk = __builtin_bit_cast(f32x4, kreg[i]), bv = __builtin_bit_cast(f32x4, vreg[i]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc = mfma_f32(aq[e], bk[e], sc);
+                    dpc = mfma_f32(ad[e], bv[e], dpc);
+                }
+            } else {
+                const s16x8 aq = *reinterpret_cast<const s16x8*>(qrow + 16 * i + 8 * hi);
+                const s16x8 ad = *reinterpret_cast<const s16x8*>(drow + 16 * i + 8 * hi);
+                sc = Elem<T>::mfma(aq, __builtin_bit_cast(s16x8, kreg[i]), sc);
+                dpc = Elem<T>::mfma(ad, __builtin_bit_cast(s16x8, vreg[i]), dpc);
+            }
+        }
+    };
+    float pd[16], ds[16];
+    // ---- P and dX = P (dP - delta) cap' ----
+    auto probs = [&](int qb0, int s, int st, float slope2, const f32x16& sc, const f32x16& dpc, bool full) FA_INLINE {
+        const float* lse2 = (const float*)(buf(s) + 2 * C::QALLOC) + 32 * st;
+        const float* dels = lse2 + BQ;
+        const float d0 = (float)(qb0 + 4 * hi + rule.off) - (float)kj;
+#pragma unroll
+        for (int gg = 0; gg < 4; ++gg) {
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse2 + 8 * gg + 4 * hi);
+            const f32x4 d4 = *reinterpret_cast<const f32x4*>(dels + 8 * gg + 4 * hi);
+            int4 qd4 = make_int4(0, 0, 0, 0);
+            if (!full && docs) qd4 = *reinterpret_cast<const int4*>(qdoc + qb0 + 8 * gg + 4 * hi);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = 4 * gg + e;
+                const float ad = __builtin_fabsf(d0 + (float)(8 * gg + e));
+                float pv;
+                if constexpr (CAP) {
+                    float t = cap.value(sc[r]) - l4[e];
+                    if (SLOPE) t = __builtin_fmaf(-slope2, ad, t);
+                    pv = fast_exp2(t);
+                } else {
+                    pv = fast_exp2(__builtin_fmaf(sc[r], c, SLOPE ? __builtin_fmaf(-slope2, ad, -l4[e]) : -l4[e]));
+                }
+                float x = pv * (dpc[r] - d4[e]);
+                if (CAP) x *= cap.slope();
+                if (!full) {
+                    const int q = qb0 + 8 * gg + 4 * hi + e;
+                    const int id = e == 0 ? qd4.x : e == 1 ? qd4.y : e == 2 ? qd4.z : qd4.w;
+                    if (q < first_l || (docs && id != kd)) {
+                        pv = 0.f;
+                        x = 0.f;
+                    }
+                }
+                pd[r] = pv;
+                ds[r] = x;
+            }
+        }
+    };
+    // ---- dV^T += dO^T P, dK^T += Q^T dX ----
+    auto acc = [&](int s, int st) FA_INLINE {
+        const T* Qs = (const T*)buf(s) + 32 * st * RW;
+        const T* Ds = (const T*)(buf(s) + C::QALLOC) + 32 * st * RW;
+        if constexpr (C::F32) {
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+                const int qr = 8 * (t >> 2) + 4 * hi + (t & 3);
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    dv[i] = mfma_f32(Ds[qr * RW + 32 * i + l32], pd[t], dv[i]);
+                    dk[i] = mfma_f32(Qs[qr * RW + 32 * i + l32], ds[t], dk[i]);
+                }
+            }
+        } else {
+            const int trow = 4 * hi + ((lane & 15) >> 2);
+            const int tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const s16x8 bp8 = pack8<T>(pd + 8 * ks), bs8 = pack8<T>(ds + 8 * ks);
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    const int off = (16 * ks + trow) * RW + 32 * i + tcol;
+                    const s16x8 ad = cat4(lds_read_tr16(Ds + off), lds_read_tr16(Ds + off + 8 * RW));
+                    const s16x8 aq = cat4(lds_read_tr16(Qs + off), lds_read_tr16(Qs + off + 8 * RW));
+                    dv[i] = Elem<T>::mfma(ad, bp8, dv[i]);
+                    dk[i] = Elem<T>::mfma(aq, bs8, dk[i]);
+                }
+            }
+        }
+    };
+
+    TileRef cur = next();
+    int cur_h = hk * p.group + tile_g;
+    int bc = 0;
+    if (cur.fl & kMore) issue(cur, cur_h, 0);
+    while (cur.fl & kMore) {
+        sync_tiles();
+        const TileRef nxt = next();
+        const int nxt_h = hk * p.group + tile_g;
+        issue(nxt, nxt_h, bc ^ 1);
+        const int q0 = cur.t * BQ;
+        if (cur.fl & kNeg) {
+            clear_rows<T, BQ, D, RW, 256>((T*)buf(bc), qdoc + q0, tid);
+            clear_rows<T, BQ, D, RW, 256>((T*)(buf(bc) + C::QALLOC), qdoc + q0, tid);
+            lds_barrier();
+        }
+        if (cur.fl & kAct) {
+            const float slope2 = SLOPE ? p.slopes[b * p.slopes_sb + cur_h] * kLog2e : 0.f;
+            const bool full = (cur.fl & kFull) != 0;
+#pragma unroll
+            for (int st = 0; st < C::NSUB; ++st) {
+                f32x16 sc, dpc;
+                sdp(bc, st, sc, dpc);
+                probs(q0 + 32 * st, bc, st, slope2, sc, dpc, full);
+                acc(bc, st);
+            }
+        }
+        bc ^= 1;
+        cur = nxt;
+        cur_h = nxt_h;
+    }
+    sync_tiles();
+    T* const Os = (T*)smem + w * 32 * C::OW;
+    store_rows<T, D>(Os, C::OW, dk, p.scale * (CAP ? 4.f : 1.f), (T*)p.dk + b * p.dk_sb + hk * p.dk_sh, p.dk_ss, kw0,
+                     p.Sk, p.cols, lane, true);
+    lds_barrier();
+    store_rows<T, D>(Os, C::OW, dv, 1.f, (T*)p.dv + b * p.dv_sb + hk * p.dv_sh, p.dv_ss, kw0, p.Sk, p.cols, lane, true);
+}
+
+// ---------------------------------------------------------------------------
+// launchers (instantiated in fa_scored_{fwd,bwd}_*.hip)
+template <typename T, int D, bool CAP, bool SLOPE>
+hipError_t launch_scored_fwd_t(ScoredParams p, hipStream_t s) {
+    using C = FwdCfg<T, D>;
+    p.n_tiles = (p.Sq + C::BM - 1) / C::BM;
+    const int64_t nb = (int64_t)p.n_tiles * p.H * p.B;
+    if (nb <= 0) return hipSuccess;
+    // grids of fewer workgroups than CUs: two groups of waves share a block's
+    // keys (fp32 tiles of head dim 128 take the whole LDS)
+    if constexpr (!(C::F32 && D == 128)) {
+        if (nb < 256 && p.Sk > C::BN) {
+            hipLaunchKernelGGL((scored_fwd_kernel<T, D, CAP, SLOPE, 2>), dim3((unsigned)nb), dim3(512), 0, s, p);
+            return hipGetLastError();
+        }
+    }
+    hipLaunchKernelGGL((scored_fwd_kernel<T, D, CAP, SLOPE, 1>), dim3((unsigned)nb), dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+
+template <typename T, int D, bool CAP, bool SLOPE>
+hipError_t launch_scored_bwd_t(ScoredParams p, hipStream_t s) {
+    using CQ = DqCfg<T, D>;
+    using CK = DkdvCfg<T, D>;
+    p.n_tiles = (p.Sq + CQ::BM - 1) / CQ::BM;
+    const int64_t nq = (int64_t)p.n_tiles * p.H * p.B;
+    if (nq > 0) {
+        if constexpr (SLOPE) {
+            if (p.dslope_rows)
+                hipLaunchKernelGGL((scored_dq_kernel<T, D, CAP, true, true, 1>), dim3((unsigned)nq), dim3(256), 0, s, p);
+            else
+                hipLaunchKernelGGL((scored_dq_kernel<T, D, CAP, true, false, 1>), dim3((unsigned)nq), dim3(256), 0, s, p);
+        } else {
+            hipLaunchKernelGGL((scored_dq_kernel<T, D, CAP, false, false, 1>), dim3((unsigned)nq), dim3(256), 0, s, p);
+        }
+    }
+    p.n_tiles = (p.Sk + CK::BK - 1) / CK::BK;
+    const int64_t nk = (int64_t)p.n_tiles * p.Hkv * p.B;
+    if (nk > 0) hipLaunchKernelGGL((scored_dkdv_kernel<T, D, CAP, SLOPE>), dim3((unsigned)nk), dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_scored_fwd(const ScoredParams& p, int D, hipStream_t s) {
+    const bool cap = p.cap > 0.f, slope = p.slopes != nullptr;
+#define FA_CASE(DD)                                                                                    \
+    if (D == DD) {                                                                                     \
+        if (cap) return slope ? launch_scored_fwd_t<T, DD, true, true>(p, s) : launch_scored_fwd_t<T, DD, true, false>(p, s); \
+        return slope ? launch_scored_fwd_t<T, DD, false, true>(p, s) : launch_scored_fwd_t<T, DD, false, false>(p, s);        \
+    }
+    FA_CASE(32)
+    FA_CASE(64)
+    FA_CASE(128)
+#undef FA_CASE
+    return hipErrorInvalidValue;
+}
+template <typename T>
+hipError_t launch_scored_bwd(const ScoredParams& p, int D, hipStream_t s) {
+    const bool cap = p.cap > 0.f, slope = p.slopes != nullptr;
+#define FA_CASE(DD)                                                                                    \
+    if (D == DD) {                                                                                     \
+        if (cap) return slope ? launch_scored_bwd_t<T, DD, true, true>(p, s) : launch_scored_bwd_t<T, DD, true, false>(p, s); \
+        return slope ? launch_scored_bwd_t<T, DD, false, true>(p, s) : launch_scored_bwd_t<T, DD, false, false>(p, s);        \
+    }
+    FA_CASE(32)
+    FA_CASE(64)
+    FA_CASE(128)
+#undef FA_CASE
+    return hipErrorInvalidValue;
+}
+
+}  // namespace fa

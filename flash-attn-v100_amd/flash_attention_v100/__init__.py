@@ -5,7 +5,9 @@ Drop-in for the public surface of mini-kio/flash-attn-v100's hot path:
 ``FlashAttentionV100Function`` (``ops/attention.py:36, 756``) and the kernel
 launchers (``kernels/forward_kernel.py:246, 445``,
 ``kernels/backward_kernel.py:208``), all backed by hand-written HIP kernels in
-``libfa_gfx950.so`` (C ABI: ``include/fa_abi.h``).  Importing the package does
+``libfa_gfx950.so`` (C ABI: ``include/fa_abi.h``), and operators around them (C
+ABI: ``include/fa_ops.h``): attention with scored rules, new tokens after a
+shared prefix, rotary positions.  Importing the package does
 not load the library; the first kernel call does, and raises
 ``FlashAttentionExtensionError`` if it is missing.
 """
@@ -31,6 +33,9 @@ from .ops.attention import (  # noqa: F401
     flash_attention_backward,
     flash_attention_forward,
 )
+from .ops.rotary import rotary_embedding_v100, rotary_table_v100  # noqa: F401
+from .ops.scored import flash_attention_v100_scored  # noqa: F401
+from .ops.shared_prefix import flash_attention_v100_shared_prefix  # noqa: F401
 from .modules import EnhancedMultiHeadAttention  # noqa: F401
 from .config import DebugConfig  # noqa: F401
 from .utils import check_tensor_nan_inf  # noqa: F401
@@ -43,6 +48,10 @@ __all__ = [
     "flash_attention_v100_with_dropout",
     "flash_attention_performance_mode",
     "flash_attention_memory_mode",
+    "flash_attention_v100_scored",
+    "flash_attention_v100_shared_prefix",
+    "rotary_table_v100",
+    "rotary_embedding_v100",
     "EnhancedMultiHeadAttention",
     "FlashAttentionV100Function",
     "EnhancedFlashAttentionV100Function",

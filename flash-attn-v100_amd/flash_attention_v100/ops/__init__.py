@@ -14,8 +14,15 @@ from .attention import (  # noqa: F401
     gradient_checkpointing_mode,
     mixed_precision_mode,
 )
+from .rotary import rotary_embedding_v100, rotary_table_v100  # noqa: F401
+from .scored import flash_attention_v100_scored  # noqa: F401
+from .shared_prefix import flash_attention_v100_shared_prefix  # noqa: F401
 
 __all__ = [
+    "flash_attention_v100_scored",
+    "flash_attention_v100_shared_prefix",
+    "rotary_table_v100",
+    "rotary_embedding_v100",
     "FlashAttentionV100Function",
     "EnhancedFlashAttentionV100Function",
     "flash_attention_forward",
