@@ -100,23 +100,49 @@ __device__ FA_INLINE inline int2 uniform2(int2 a) {
 }
 
 // A tile of a walk: its index (-1 past the last) and flags, wave-uniform.
-// kAct: some row of this wave may see it; kFull: every row sees it whole; kNeg:
-// it holds tokens of no document; kMore: the walk has not ended.
+// kAct: some row of this wave may see it; kLim: the causal mask and the lengths
+// leave it whole to every row, kDoc: so do the documents; kNeg: it holds tokens of
+// no document; kMore: the walk has not ended.
 struct TileRef {
     int t;
     unsigned fl;
 };
-constexpr unsigned kAct = 1, kFull = 2, kNeg = 4, kMore = 8;
+constexpr unsigned kAct = 1, kLim = 2, kDoc = 4, kNeg = 8, kMore = 16, kFull = kLim | kDoc;
+
+// 64 tiles of a walk, a bit each: those that some row of the workgroup sees, and
+// the flags above.
+struct TileChunk {
+    uint64_t vis, act, lim, doc, neg;
+    __device__ FA_INLINE inline TileRef ref(int base, int i) const {
+        return TileRef{base + i, kMore | ((act >> i) & 1 ? kAct : 0u) | ((lim >> i) & 1 ? kLim : 0u) |
+                                     ((doc >> i) & 1 ? kDoc : 0u) | ((neg >> i) & 1 ? kNeg : 0u)};
+    }
+};
+
+// Two workgroups share a CU, so each SIMD has two waves that alternate between
+// matrix products and the arithmetic of the scores.  At equal priority they fall
+// into step, both in the same phase; with the wave in the odd slot ahead, one's
+// products run beside the other's arithmetic.
+__device__ FA_INLINE inline void stagger_waves() {
+    if (__builtin_amdgcn_s_getreg(4 | (0 << 6) | (0 << 11)) & 1)  // HW_ID, bit 0 of the wave's slot
+        __builtin_amdgcn_s_setprio(2);
+}
 
 // zeros into the rows of a tile that belong to no document (their values may be
 // anything, and 0 times a NaN is none).  All threads of the NT; a barrier follows.
 template <typename T, int R, int D, int W, int NT>
 __device__ FA_INLINE inline void clear_rows(T* tile, const int* docs, int tid) {
     constexpr int EPC = 16 / (int)sizeof(T), CPR = D / EPC;
+#pragma unroll 1
     for (int c = tid; c < R * CPR; c += NT) {
         const int row = c / CPR, col = c % CPR;
         if (docs[row] < 0) *reinterpret_cast<uint4*>(tile + row * W + col * EPC) = make_uint4(0u, 0u, 0u, 0u);
     }
+}
+
+// -x for four floats
+__device__ FA_INLINE inline uint4 neg32x4(uint4 v) {
+    return make_uint4(v.x ^ 0x80000000u, v.y ^ 0x80000000u, v.z ^ 0x80000000u, v.w ^ 0x80000000u);
 }
 
 // The rows of a wave's 32-row block (lane l holds row l % 32, 16 columns of each
@@ -168,10 +194,12 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
     constexpr int BN = C::BN, NB = C::NB, KW = C::KW, VW = C::VW, NW = C::NW;
     constexpr int TPD = 64 / BN;  // tiles per range of document ids
     __shared__ __attribute__((aligned(16))) T smem[C::SMEM_ELEMS * KS];
+    __shared__ __attribute__((aligned(16))) int ids[KS][2][64];  // document ids of the tiles
 
     const int tid = threadIdx.x;
     const int lane = tid & 63, wg = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
     const int w = KS == 1 ? wg : wg & 3, sp = KS == 1 ? 0 : wg >> 2;
+    if constexpr (KS == 1) stagger_waves();
     const int2 tord = tile_order<32 * (KS == 1 ? 2 : 1), true>(p.n_tiles);
     const int qt = p.n_tiles - 1 - tord.y;  // longest causal rows first
     const int h = tord.x % p.H, b = tord.x / p.H;
@@ -213,39 +241,37 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
         const int id = qi < p.Sq ? p.q_docs[(int64_t)b * p.q_docs_pad + qi] : -1;
         if (id >= 0) qd = id;
     }
-    uint64_t c_vis = 0, c_act = 0, c_full = 0, c_neg = 0;  // the chunk's tiles
-    int base = -64;
-    auto next = [&]() FA_INLINE -> TileRef {
-        while (c_vis == 0) {
-            base += 64;
-            if (base >= n_kt) {
-                base = n_kt;  // stays past the end
-                return TileRef{-1, 0u};
-            }
-            const int t = base + lane, k0 = t * BN;
-            bool v = t < n_kt, a = v && k0 < wlim_hi, f = k0 + BN <= wlim_lo, n = false;
-            if (docs) {
-                const int2 r = v ? krng[t / TPD] : make_int2(-1, -1);
-                v = v && docs_meet(r, qr);
-                a = a && v && docs_meet(r, wr);
-                f = f && docs_one(r, wr);
-                n = r.x < 0;
-            }
-            c_vis = __ballot(v);
-            c_act = __ballot(a);
-            c_full = __ballot(f);
-            c_neg = __ballot(n);
+    // key tiles [base, base + 64)
+    auto chunk_at = [&](int base) FA_INLINE -> TileChunk {
+        const int t = base + lane, k0 = t * BN;
+        bool v = t < n_kt, a = v && k0 < wlim_hi;
+        TileChunk c;
+        c.lim = __ballot(k0 + BN <= wlim_lo);
+        c.doc = ~0ull;
+        c.neg = 0;
+        if (docs) {
+            const int2 r = v ? krng[t / TPD] : make_int2(-1, -1);
+            v = v && docs_meet(r, qr);
+            a = a && v && docs_meet(r, wr);
+            c.doc = __ballot(docs_one(r, wr));
+            c.neg = __ballot(r.x < 0);
         }
-        const int i = (int)__builtin_ctzll(c_vis);
-        c_vis &= c_vis - 1;
-        return TileRef{base + i, kMore | ((c_act >> i) & 1 ? kAct : 0u) | ((c_full >> i) & 1 ? kFull : 0u) |
-                                     ((c_neg >> i) & 1 ? kNeg : 0u)};
+        c.vis = __ballot(v);
+        c.act = __ballot(a);
+        return c;
     };
-    // this group's next tile; kMore and kNeg of the groups together (barriers)
-    auto fetch = [&]() FA_INLINE -> TileRef {
-        TileRef r = next();
+    // the next tile of a chunk.  KS = 2: of this group, with kMore and kNeg of the
+    // groups together (they share the barriers)
+    auto next = [&](TileChunk& c, int base) FA_INLINE -> TileRef {
+        auto one = [&]() FA_INLINE -> TileRef {
+            if (c.vis == 0) return TileRef{-1, 0u};
+            const int i = (int)__builtin_ctzll(c.vis);
+            c.vis &= c.vis - 1;
+            return c.ref(base, i);
+        };
+        TileRef r = one();
         if constexpr (KS == 2) {
-            const TileRef r2 = next();
+            const TileRef r2 = one();
             const unsigned both = (r.fl | r2.fl) & (kMore | kNeg);
             if (sp) r = r2;
             r.fl |= both;
@@ -285,6 +311,12 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
             vdma.load_untracked(vbase + (int64_t)k0 * p.v_ss, p.v_ss, nv, Vs0 + slot * C::VTILE, lane);
     };
 
+    // (the ids of a 64-token range, of which a float32 tile is one half)
+    auto load_ids = [&](const TileRef& r, int slot) FA_INLINE {
+        if (docs && w == 0 && r.t >= 0)
+            dma_load4_untracked(buffer_words(kdoc + r.t / TPD * 64, 256), lds_addr(ids[sp][slot]), 4 * lane);
+    };
+
     // ---- S^T = K Q^T of a tile ----
     auto qk = [&](const T* Ks, f32x16 (&s)[NB]) FA_INLINE {
 #pragma unroll
@@ -311,7 +343,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
     constexpr bool RCP = CAP && !SLOPE && !C::F32, VALUE = SLOPE || (CAP && C::F32);
     const float ua = VALUE ? 1.f : RCP ? -2.f * cap.top : c, ub = RCP ? cap.top : 0.f;
     constexpr float kHidden = RCP ? INFINITY : -INFINITY;
-    auto score = [&](f32x16 (&s)[NB], const TileRef& r) FA_INLINE {
+    auto score = [&](f32x16 (&s)[NB], const TileRef& r, const int* id) FA_INLINE {
         const int k0 = r.t * BN;
         if constexpr (RCP) {
 #pragma unroll
@@ -329,25 +361,25 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
                     s[blk][e] = SLOPE ? __builtin_fmaf(-slope2, __builtin_fabsf(d), t) : t;
                 }
         }
-        if (!(r.fl & kFull)) {
+        if (!(r.fl & kLim)) {
             const int lim = lim_l - k0 - 4 * hi;
 #pragma unroll
             for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                     if (32 * blk + 8 * (e >> 2) + (e & 3) >= lim) s[blk][e] = kHidden;
-            if (docs) {
+        }
+        if (!(r.fl & kDoc)) {
 #pragma unroll
-                for (int blk = 0; blk < NB; ++blk)
+            for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int4 kd = *reinterpret_cast<const int4*>(kdoc + k0 + 32 * blk + 8 * g + 4 * hi);
-                        if (kd.x != qd) s[blk][4 * g] = kHidden;
-                        if (kd.y != qd) s[blk][4 * g + 1] = kHidden;
-                        if (kd.z != qd) s[blk][4 * g + 2] = kHidden;
-                        if (kd.w != qd) s[blk][4 * g + 3] = kHidden;
-                    }
-            }
+                for (int g = 0; g < 4; ++g) {
+                    const int4 kd = *reinterpret_cast<const int4*>(id + 32 * blk + 8 * g + 4 * hi);
+                    if (kd.x != qd) s[blk][4 * g] = kHidden;
+                    if (kd.y != qd) s[blk][4 * g + 1] = kHidden;
+                    if (kd.z != qd) s[blk][4 * g + 2] = kHidden;
+                    if (kd.w != qd) s[blk][4 * g + 3] = kHidden;
+                }
         }
         float mx = kHidden;
 #pragma unroll
@@ -416,34 +448,40 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
         lds_barrier();
     };
 
-    // two slots in turn: tile j is read while tile j + 1 lands in the other,
-    // last read before the barrier that opens the iteration
-    TileRef cur = fetch();
+    // two slots in turn: a tile is read while the next one lands in the other
+    // slot, last read before the barrier that opens the iteration; the first tile
+    // of a chunk lands in the slot that the last iteration did not read
     int slot = 0;
-    if (cur.fl & kMore) {
-        load_k(cur, 0);
-        load_v(cur, 0);
-    }
-    while (cur.fl & kMore) {
-        sync_tiles();
-        const TileRef nxt = fetch();
-        load_k(nxt, slot ^ 1);
-        load_v(nxt, slot ^ 1);
-        T* const Vs = Vs0 + slot * C::VTILE;
-        if (cur.fl & kNeg) {  // the groups together
-            if (cur.t >= 0) clear_rows<T, BN, D, VW, 256>(Vs, kdoc + cur.t * BN, tid & 255);
-            lds_barrier();
+    for (int base = 0; base < n_kt; base += 64) {
+        TileChunk ch = chunk_at(base);
+        TileRef cur = next(ch, base);
+        if (!(cur.fl & kMore)) continue;
+        load_k(cur, slot);
+        load_v(cur, slot);
+        load_ids(cur, slot);
+        while (cur.fl & kMore) {
+            sync_tiles();
+            const TileRef nxt = next(ch, base);
+            load_k(nxt, slot ^ 1);
+            load_v(nxt, slot ^ 1);
+            load_ids(nxt, slot ^ 1);
+            T* const Vs = Vs0 + slot * C::VTILE;
+            const int* const id = ids[sp][slot] + cur.t % TPD * BN;
+            if (cur.fl & kNeg) {  // the groups together
+                if (cur.t >= 0) clear_rows<T, BN, D, VW, 256>(Vs, id, tid & 255);
+                lds_barrier();
+            }
+            if (cur.fl & kAct) {
+                f32x16 s[NB];
+                s16x8 pk[NPK];
+                qk(Ks0 + slot * C::KTILE, s);
+                score(s, cur, id);
+                softmax(s, pk);
+                pv(Vs, s, pk);
+            }
+            slot ^= 1;
+            cur = nxt;
         }
-        if (cur.fl & kAct) {
-            f32x16 s[NB];
-            s16x8 pk[NPK];
-            qk(Ks0 + slot * C::KTILE, s);
-            score(s, cur);
-            softmax(s, pk);
-            pv(Vs, s, pk);
-        }
-        slot ^= 1;
-        cur = nxt;
     }
     sync_tiles();  // all waves done with the tiles, no copy in flight
 
@@ -497,10 +535,12 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
     constexpr int BN = C::BN, KW = C::KW;
     static_assert(BN == 64, "one range of document ids a tile");
     __shared__ __attribute__((aligned(16))) char smem[C::SMEM_BYTES * KS];
+    __shared__ __attribute__((aligned(16))) int ids[KS][2][64];  // document ids of the tiles
 
     const int tid = threadIdx.x;
     const int lane = tid & 63, wg = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
     const int w = KS == 1 ? wg : wg & 3, sp = KS == 1 ? 0 : wg >> 2;
+    if constexpr (KS == 1) stagger_waves();
     const int2 tord = tile_order<32 * (KS == 1 ? C::MIN_BLOCKS : 1), true>(p.n_tiles);
     const int qt = p.n_tiles - 1 - tord.y;
     const int h = tord.x % p.H, b = tord.x / p.H;
@@ -562,38 +602,37 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
         const int id = qi < p.Sq ? p.q_docs[(int64_t)b * p.q_docs_pad + qi] : -1;
         if (id >= 0) qd = id;
     }
-    uint64_t c_vis = 0, c_act = 0, c_full = 0, c_neg = 0;  // the chunk's tiles
-    int base = -64;
-    auto next = [&]() FA_INLINE -> TileRef {
-        while (c_vis == 0) {
-            base += 64;
-            if (base >= n_kt) {
-                base = n_kt;
-                return TileRef{-1, 0u};
-            }
-            const int t = base + lane, k0 = t * BN;
-            bool v = t < n_kt, a = v && k0 < wlim_hi, f = k0 + BN <= wlim_lo, n = false;
-            if (docs) {
-                const int2 r = v ? krng[t] : make_int2(-1, -1);
-                v = v && docs_meet(r, qr);
-                a = a && v && docs_meet(r, wr);
-                f = f && docs_one(r, wr);
-                n = r.x < 0;
-            }
-            c_vis = __ballot(v);
-            c_act = __ballot(a);
-            c_full = __ballot(f);
-            c_neg = __ballot(n);
+    // key tiles [base, base + 64)
+    auto chunk_at = [&](int base) FA_INLINE -> TileChunk {
+        const int t = base + lane, k0 = t * BN;
+        bool v = t < n_kt, a = v && k0 < wlim_hi;
+        TileChunk c;
+        c.lim = __ballot(k0 + BN <= wlim_lo);
+        c.doc = ~0ull;
+        c.neg = 0;
+        if (docs) {
+            const int2 r = v ? krng[t] : make_int2(-1, -1);
+            v = v && docs_meet(r, qr);
+            a = a && v && docs_meet(r, wr);
+            c.doc = __ballot(docs_one(r, wr));
+            c.neg = __ballot(r.x < 0);
         }
-        const int i = (int)__builtin_ctzll(c_vis);
-        c_vis &= c_vis - 1;
-        return TileRef{base + i, kMore | ((c_act >> i) & 1 ? kAct : 0u) | ((c_full >> i) & 1 ? kFull : 0u) |
-                                     ((c_neg >> i) & 1 ? kNeg : 0u)};
+        c.vis = __ballot(v);
+        c.act = __ballot(a);
+        return c;
     };
-    auto fetch = [&]() FA_INLINE -> TileRef {
-        TileRef r = next();
+    // the next tile of a chunk.  KS = 2: of this group, with kMore and kNeg of the
+    // groups together (they share the barriers)
+    auto next = [&](TileChunk& c, int base) FA_INLINE -> TileRef {
+        auto one = [&]() FA_INLINE -> TileRef {
+            if (c.vis == 0) return TileRef{-1, 0u};
+            const int i = (int)__builtin_ctzll(c.vis);
+            c.vis &= c.vis - 1;
+            return c.ref(base, i);
+        };
+        TileRef r = one();
         if constexpr (KS == 2) {
-            const TileRef r2 = next();
+            const TileRef r2 = one();
             const unsigned both = (r.fl | r2.fl) & (kMore | kNeg);
             if (sp) r = r2;
             r.fl |= both;
@@ -625,6 +664,8 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
             rows.load(src, copy_k ? p.k_ss : p.v_ss, nv, (T*)(buf(s) + (copy_k ? 0 : C::KALLOC)));
         else
             rows.load_untracked(src, copy_k ? p.k_ss : p.v_ss, nv, (const T*)(buf(s) + (copy_k ? 0 : C::KALLOC)));
+        if (docs && w == 0 && r.t >= 0)
+            dma_load4_untracked(buffer_words(kdoc + k0, 256), lds_addr(ids[sp][s]), 4 * lane);
     };
     auto sync_tiles = [&]() FA_INLINE {
         wait_vmem();
@@ -655,27 +696,32 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
             }
         }
     };
-    // ---- dX^T = P^T (dP^T - delta) cap', then dQ^T += K^T dX^T ----
-    auto fin = [&](int k0, const T* Ks, f32x16& s, const f32x16& dp, bool full) FA_INLINE {
-        const int lim = lim_l - k0 - 4 * hi;
-        const float d0 = qpos - (float)(k0 + 4 * hi);
-        uint32_t hide = 0;  // bit r: masked
-        if (!full) {
+    // ---- 16 keys (half ks of the 32): dX^T = P^T (dP^T - delta) cap', then
+    // dQ^T += K^T dX^T ----
+    auto half = [&](int k0, const T* Ks, const int* id, int ks, const f32x16& s, const f32x16& dp, unsigned fl) FA_INLINE {
+        const int ka = k0 + 16 * ks + 4 * hi;  // of element 0; element e is key ka + 8 (e / 4) + e % 4
+        const float d0 = qpos - (float)ka;
+        uint32_t hide = 0;  // bit e: masked
+        if (!(fl & kLim)) {
+            const int lim = lim_l - ka;
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (8 * (r >> 2) + (r & 3) >= lim) hide |= 1u << r;
-            if (docs) {
+            for (int e = 0; e < 8; ++e)
+                if (8 * (e >> 2) + (e & 3) >= lim) hide |= 1u << e;
+        }
+        if (!(fl & kDoc)) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int4 kd = *reinterpret_cast<const int4*>(kdoc + k0 + 8 * g + 4 * hi);
-                    hide |= (kd.x != qd ? 1u : 0u) << (4 * g) | (kd.y != qd ? 2u : 0u) << (4 * g) |
-                            (kd.z != qd ? 4u : 0u) << (4 * g) | (kd.w != qd ? 8u : 0u) << (4 * g);
-                }
+            for (int g = 0; g < 2; ++g) {
+                const int4 kd = *reinterpret_cast<const int4*>(id + 16 * ks + 8 * g + 4 * hi);
+                hide |= (kd.x != qd ? 1u : 0u) << (4 * g) | (kd.y != qd ? 2u : 0u) << (4 * g) |
+                        (kd.z != qd ? 4u : 0u) << (4 * g) | (kd.w != qd ? 8u : 0u) << (4 * g);
             }
         }
+        float ds[8];
+        [[maybe_unused]] float pe[8];  // P
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float ad = __builtin_fabsf(d0 - (float)(8 * (r >> 2) + (r & 3)));
+        for (int e = 0; e < 8; ++e) {
+            const int r = 8 * ks + e;
+            const float ad = __builtin_fabsf(d0 - (float)(8 * (e >> 2) + (e & 3)));
             float pv;
             if constexpr (CAP) {
                 float t = cap.value(s[r]) - lse2;
@@ -684,69 +730,78 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
             } else {
                 pv = fast_exp2(__builtin_fmaf(s[r], c, SLOPE ? __builtin_fmaf(-slope2, ad, -lse2) : -lse2));
             }
-            if constexpr (DSLOPE) {
-                const bool out = !full && ((hide >> r) & 1u);
-                const float pz = out ? 0.f : pv, pdp = out ? 0.f : pv * dp[r];
+            pe[e] = pv;
+            ds[e] = pv * (dp[r] - del);
+            if (CAP) ds[e] *= cap.slope();
+        }
+        if ((fl & kFull) != kFull) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if ((hide >> e) & 1u) pe[e] = ds[e] = 0.f;
+        }
+        if constexpr (DSLOPE) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float ad = __builtin_fabsf(d0 - (float)(8 * (e >> 2) + (e & 3)));
+                // a masked dP may be anything
+                const float pdp = pe[e] == 0.f ? 0.f : pe[e] * dp[8 * ks + e];
                 sum_dp += pdp;
-                sum_d = __builtin_fmaf(pz, ad, sum_d);
+                sum_d = __builtin_fmaf(pe[e], ad, sum_d);
                 sum_ddp = __builtin_fmaf(pdp, ad, sum_ddp);
             }
-            float ds = pv * (dp[r] - del);
-            if (CAP) ds *= cap.slope();
-            s[r] = !full && ((hide >> r) & 1u) ? 0.f : ds;
         }
         if constexpr (C::F32) {
 #pragma unroll
-            for (int t = 0; t < 16; ++t) {
-                const T* kr = Ks + (8 * (t >> 2) + 4 * hi + (t & 3)) * KW + l32;
+            for (int t = 0; t < 8; ++t) {
+                const T* kr = Ks + (16 * ks + 8 * (t >> 2) + 4 * hi + (t & 3)) * KW + l32;
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) dq[i] = mfma_f32(kr[32 * i], s[t], dq[i]);
+                for (int i = 0; i < D / 32; ++i) dq[i] = mfma_f32(kr[32 * i], ds[t], dq[i]);
             }
         } else {
             const int trow = 4 * hi + ((lane & 15) >> 2);
             const int tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            const s16x8 bs8 = pack8<T>(ds);
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                float ts[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) ts[e] = s[8 * ks + e];
-                const s16x8 bs8 = pack8<T>(ts);
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    const T* kp = Ks + (16 * ks + trow) * KW + 32 * i + tcol;
-                    const s16x8 a = cat4(lds_read_tr16(kp), lds_read_tr16(kp + 8 * KW));
-                    dq[i] = Elem<T>::mfma(a, bs8, dq[i]);
-                }
+            for (int i = 0; i < D / 32; ++i) {
+                const T* kp = Ks + (16 * ks + trow) * KW + 32 * i + tcol;
+                const s16x8 a = cat4(lds_read_tr16(kp), lds_read_tr16(kp + 8 * KW));
+                dq[i] = Elem<T>::mfma(a, bs8, dq[i]);
             }
         }
     };
 
     // two buffers in turn: tile j is read while tile j + 1 lands in the other,
     // last read before the barrier that opens the iteration
-    TileRef cur = fetch();
     int bc = 0;
-    if (cur.fl & kMore) issue(cur, 0);
-    while (cur.fl & kMore) {
-        sync_tiles();
-        const TileRef nxt = fetch();
-        issue(nxt, bc ^ 1);
-        T* const Ks = (T*)buf(bc);
-        const T* const Vs = (const T*)(buf(bc) + C::KALLOC);
-        if (cur.fl & kNeg) {
-            if (cur.t >= 0) clear_rows<T, BN, D, KW, 256>(Ks, kdoc + cur.t * BN, tid & 255);
-            lds_barrier();
+    for (int base = 0; base < n_kt; base += 64) {
+        TileChunk ch = chunk_at(base);
+        TileRef cur = next(ch, base);
+        if (!(cur.fl & kMore)) continue;
+        issue(cur, bc);
+        while (cur.fl & kMore) {
+            sync_tiles();
+            const TileRef nxt = next(ch, base);
+            issue(nxt, bc ^ 1);
+            T* const Ks = (T*)buf(bc);
+            const T* const Vs = (const T*)(buf(bc) + C::KALLOC);
+            const int* const id = ids[sp][bc];
+            if (cur.fl & kNeg) {
+                if (cur.t >= 0) clear_rows<T, BN, D, KW, 256>(Ks, id, tid & 255);
+                lds_barrier();
+            }
+            if (cur.fl & kAct) {
+                const int k0 = cur.t * BN;
+                f32x16 s0, dp0, s1, dp1;
+                sdp(Ks, Vs, s0, dp0);
+                sdp(Ks + 32 * KW, Vs + 32 * KW, s1, dp1);
+                half(k0, Ks, id, 0, s0, dp0, cur.fl);
+                half(k0, Ks, id, 1, s0, dp0, cur.fl);
+                half(k0 + 32, Ks + 32 * KW, id + 32, 0, s1, dp1, cur.fl);
+                half(k0 + 32, Ks + 32 * KW, id + 32, 1, s1, dp1, cur.fl);
+            }
+            bc ^= 1;
+            cur = nxt;
         }
-        if (cur.fl & kAct) {
-            const int k0 = cur.t * BN;
-            const bool full = (cur.fl & kFull) != 0;
-            f32x16 s0, dp0, s1, dp1;
-            sdp(Ks, Vs, s0, dp0);
-            sdp(Ks + 32 * KW, Vs + 32 * KW, s1, dp1);
-            fin(k0, Ks, s0, dp0, full);
-            fin(k0 + 32, Ks + 32 * KW, s1, dp1, full);
-        }
-        bc ^= 1;
-        cur = nxt;
     }
     sync_tiles();
     if constexpr (DSLOPE) {
@@ -802,9 +857,14 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
     constexpr int BQ = C::BQ, RW = C::RW;
     static_assert(BQ == 64, "one range of document ids a tile; one dword a lane for LSE and delta");
     __shared__ __attribute__((aligned(16))) char smem[C::SMEM_BYTES];
+    __shared__ __attribute__((aligned(16))) int ids[2][64];  // document ids of the tiles
+    // each key's first query and document id: needed by partly seen tiles only,
+    // and registers are short
+    __shared__ int key_first[C::BK], key_doc[C::BK];
 
     const int tid = threadIdx.x;
     const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
+    stagger_waves();
     const int2 tord = tile_order<32 * (!(Elem<T>::kF32 && D == 128) ? 2 : 1), true>(p.n_tiles);
     const int kt = tord.y;  // the first keys are seen by the most queries
     const int hk = tord.x % p.Hkv, b = tord.x / p.Hkv;
@@ -823,19 +883,23 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
             kreg[i] = ok ? *reinterpret_cast<const uint4*>(krow + d0) : make_uint4(0u, 0u, 0u, 0u);
             vreg[i] = ok ? *reinterpret_cast<const uint4*>(vrow + d0) : make_uint4(0u, 0u, 0u, 0u);
         }
+        // the dP products start from delta and take -V: they give delta - dP, and
+        // the products below sum -dX into dK, whose final scale is negative
+#pragma unroll
+        for (int i = 0; i < KR; ++i) vreg[i] = C::F32 ? neg32x4(vreg[i]) : neg16x8(vreg[i]);
     }
 
-    // ---- the walk over (query head of the group, query tile), downwards ----
+    // ---- the query tiles that the keys are seen by ----
     const int first0 = rule.first(k0);                 // of the block's keys: none of them sooner
     const int wfirst_lo = rule.first(kw0), wfirst_hi = rule.first(kw0 + 31);
-    const int first_l = rule.first(kj);
+    key_first[32 * w + l32] = rule.first(kj);
     const int n_qt = (p.Sq + BQ - 1) / BQ;
     const int t_lo = first0 == INT_MAX ? n_qt : min(n_qt, first0 / BQ);  // tiles [t_lo, n_qt)
     const bool docs = p.q_docs != nullptr;
     const int* qdoc = p.q_docs + (docs ? (int64_t)b * p.q_docs_pad : 0);
     const int2* qrng = p.q_rng + (docs ? (int64_t)b * (p.q_docs_pad / 64) : 0);
     int2 kr = {0, 0}, wr = {0, 0};
-    int kd = -2;
+    int kd = -2;  // no query's id
     if (docs) {
         const int2* krng = p.k_rng + (int64_t)b * (p.k_docs_pad / 64) + k0 / 64;
         const int2 a = uniform2(krng[0]), c = k0 + 64 < p.k_docs_pad ? uniform2(krng[1]) : a;
@@ -844,39 +908,25 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
         const int id = kj < p.Sk ? p.k_docs[(int64_t)b * p.k_docs_pad + kj] : -1;
         if (id >= 0) kd = id;
     }
-    uint64_t c_vis = 0, c_act = 0, c_full = 0, c_neg = 0;  // the chunk's tiles
-    int base = n_qt, g = 0;  // chunk [base, base + 64), head of the group
-    int tile_g = 0;
-    auto next = [&]() FA_INLINE -> TileRef {
-        while (c_vis == 0) {
-            if (base <= t_lo) {
-                if (g + 1 >= p.group || t_lo >= n_qt) {
-                    g = p.group;
-                    return TileRef{-1, 0u};
-                }
-                ++g;
-                base = n_qt;
-            }
-            base -= 64;
-            const int t = base + lane, qa = t * BQ, qz = min(qa + BQ, p.Sq) - 1;  // first and last query
-            bool v = t >= t_lo && t < n_qt, a = v && qz >= wfirst_lo, f = qa >= wfirst_hi, n = false;
-            if (docs) {
-                const int2 r = v ? qrng[t] : make_int2(-1, -1);
-                v = v && docs_meet(r, kr);
-                a = a && v && docs_meet(r, wr);
-                f = f && docs_one(r, wr);
-                n = r.x < 0;
-            }
-            c_vis = __ballot(v);
-            c_act = __ballot(a);
-            c_full = __ballot(f);
-            c_neg = __ballot(n);
+    key_doc[32 * w + l32] = kd;
+    // query tiles [base, base + 64)
+    auto chunk_at = [&](int base) FA_INLINE -> TileChunk {
+        const int t = base + lane, qa = t * BQ, qz = min(qa + BQ, p.Sq) - 1;  // first and last query
+        bool v = t >= t_lo && t < n_qt, a = v && qz >= wfirst_lo;
+        TileChunk c;
+        c.lim = __ballot(qa >= wfirst_hi);
+        c.doc = ~0ull;
+        c.neg = 0;
+        if (docs) {
+            const int2 r = v ? qrng[t] : make_int2(-1, -1);
+            v = v && docs_meet(r, kr);
+            a = a && v && docs_meet(r, wr);
+            c.doc = __ballot(docs_one(r, wr));
+            c.neg = __ballot(r.x < 0);
         }
-        const int i = 63 - (int)__builtin_clzll(c_vis);
-        c_vis &= ~(1ull << i);
-        tile_g = g;
-        return TileRef{base + i, kMore | ((c_act >> i) & 1 ? kAct : 0u) | ((c_full >> i) & 1 ? kFull : 0u) |
-                                     ((c_neg >> i) & 1 ? kNeg : 0u)};
+        c.vis = __ballot(v);
+        c.act = __ballot(a);
+        return c;
     };
 
     f32x16 dk[D / 32], dv[D / 32];
@@ -906,15 +956,16 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
         const uint32_t f = lds_addr(bp + 2 * C::QALLOC);
         dma_load4_untracked(rs, f, 4 * lane);
         dma_load4_untracked(rs, f + 4 * BQ, 4 * (p.sq_pad + lane));
+        if (docs && w == 0 && r.t >= 0) dma_load4_untracked(buffer_words(qdoc + qb0, 256), lds_addr(ids[s]), 4 * lane);
     };
     auto sync_tiles = [&]() FA_INLINE {
         wait_vmem();
         lds_barrier();
     };
-    // ---- S = Q K^T, dP = dO V^T of 32 queries ----
+    // ---- S = Q K^T, delta - dP (dP = dO V^T) of 32 queries ----
     auto sdp = [&](int s, int st, f32x16& sc, f32x16& dpc) FA_INLINE {
         sc = f32x16{};
-        dpc = f32x16{};
+        dpc = delta16((const float*)(buf(s) + 2 * C::QALLOC) + BQ + 32 * st, hi);
         const T* qrow = (const T*)buf(s) + (32 * st + l32) * RW;
         const T* drow = (const T*)(buf(s) + C::QALLOC) + (32 * st + l32) * RW;
 #pragma unroll
@@ -936,21 +987,20 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
             }
         }
     };
-    float pd[16], ds[16];
-    // ---- P and dX = P (dP - delta) cap' ----
-    auto probs = [&](int qb0, int s, int st, float slope2, const f32x16& sc, const f32x16& dpc, bool full) FA_INLINE {
-        const float* lse2 = (const float*)(buf(s) + 2 * C::QALLOC) + 32 * st;
-        const float* dels = lse2 + BQ;
-        const float d0 = (float)(qb0 + 4 * hi + rule.off) - (float)kj;
+    // ---- 16 queries (half ks of the 32): P and -dX = P (delta - dP) cap', packed ----
+    constexpr int NPK = C::F32 ? 1 : 2;
+    auto half = [&](int qb0, int s, int st, int ks, float slope2, f32x16& sc, f32x16& dpc, s16x8 (&bp)[NPK], s16x8 (&bs)[NPK],
+                    unsigned fl) FA_INLINE {
+        const float* lse2 = (const float*)(buf(s) + 2 * C::QALLOC) + 32 * st + 16 * ks + 4 * hi;
+        const int qa = qb0 + 16 * ks + 4 * hi;  // of element 0; element e is query qa + 8 (e / 4) + e % 4
+        const float d0 = (float)(qa + rule.off) - (float)kj;
+        float pd[8], ds[8];
 #pragma unroll
-        for (int gg = 0; gg < 4; ++gg) {
-            const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse2 + 8 * gg + 4 * hi);
-            const f32x4 d4 = *reinterpret_cast<const f32x4*>(dels + 8 * gg + 4 * hi);
-            int4 qd4 = make_int4(0, 0, 0, 0);
-            if (!full && docs) qd4 = *reinterpret_cast<const int4*>(qdoc + qb0 + 8 * gg + 4 * hi);
+        for (int gg = 0; gg < 2; ++gg) {
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse2 + 8 * gg);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int r = 4 * gg + e;
+                const int r = 8 * ks + 4 * gg + e;
                 const float ad = __builtin_fabsf(d0 + (float)(8 * gg + e));
                 float pv;
                 if constexpr (CAP) {
@@ -960,23 +1010,40 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
                 } else {
                     pv = fast_exp2(__builtin_fmaf(sc[r], c, SLOPE ? __builtin_fmaf(-slope2, ad, -l4[e]) : -l4[e]));
                 }
-                float x = pv * (dpc[r] - d4[e]);
-                if (CAP) x *= cap.slope();
-                if (!full) {
-                    const int q = qb0 + 8 * gg + 4 * hi + e;
-                    const int id = e == 0 ? qd4.x : e == 1 ? qd4.y : e == 2 ? qd4.z : qd4.w;
-                    if (q < first_l || (docs && id != kd)) {
-                        pv = 0.f;
-                        x = 0.f;
-                    }
-                }
-                pd[r] = pv;
-                ds[r] = x;
+                pd[4 * gg + e] = pv;
+                ds[4 * gg + e] = CAP ? pv * dpc[r] * cap.slope() : pv * dpc[r];
             }
         }
+        if (!(fl & kLim)) {
+            const int lim = key_first[32 * w + l32] - qa;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (8 * (e >> 2) + (e & 3) < lim) pd[e] = ds[e] = 0.f;
+        }
+        if (!(fl & kDoc)) {
+            const int kd = key_doc[32 * w + l32];
+#pragma unroll
+            for (int gg = 0; gg < 2; ++gg) {
+                const int4 id = *reinterpret_cast<const int4*>(ids[s] + 32 * st + 16 * ks + 8 * gg + 4 * hi);
+                if (id.x != kd) pd[4 * gg] = ds[4 * gg] = 0.f;
+                if (id.y != kd) pd[4 * gg + 1] = ds[4 * gg + 1] = 0.f;
+                if (id.z != kd) pd[4 * gg + 2] = ds[4 * gg + 2] = 0.f;
+                if (id.w != kd) pd[4 * gg + 3] = ds[4 * gg + 3] = 0.f;
+            }
+        }
+        if constexpr (C::F32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                sc[8 * ks + e] = pd[e];
+                dpc[8 * ks + e] = ds[e];
+            }
+        } else {
+            bp[ks] = pack8<T>(pd);
+            bs[ks] = pack8<T>(ds);
+        }
     };
-    // ---- dV^T += dO^T P, dK^T += Q^T dX ----
-    auto acc = [&](int s, int st) FA_INLINE {
+    // ---- dV^T += dO^T P, dK^T -= Q^T dX ----
+    auto acc = [&](int s, int st, const f32x16& pd, const f32x16& ds, const s16x8 (&bp)[NPK], const s16x8 (&bs)[NPK]) FA_INLINE {
         const T* Qs = (const T*)buf(s) + 32 * st * RW;
         const T* Ds = (const T*)(buf(s) + C::QALLOC) + 32 * st * RW;
         if constexpr (C::F32) {
@@ -993,53 +1060,74 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
             const int trow = 4 * hi + ((lane & 15) >> 2);
             const int tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                const s16x8 bp8 = pack8<T>(pd + 8 * ks), bs8 = pack8<T>(ds + 8 * ks);
+            for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int i = 0; i < D / 32; ++i) {
                     const int off = (16 * ks + trow) * RW + 32 * i + tcol;
                     const s16x8 ad = cat4(lds_read_tr16(Ds + off), lds_read_tr16(Ds + off + 8 * RW));
                     const s16x8 aq = cat4(lds_read_tr16(Qs + off), lds_read_tr16(Qs + off + 8 * RW));
-                    dv[i] = Elem<T>::mfma(ad, bp8, dv[i]);
-                    dk[i] = Elem<T>::mfma(aq, bs8, dk[i]);
+                    dv[i] = Elem<T>::mfma(ad, bp[ks], dv[i]);
+                    dk[i] = Elem<T>::mfma(aq, bs[ks], dk[i]);
                 }
-            }
         }
     };
 
-    TileRef cur = next();
-    int cur_h = hk * p.group + tile_g;
+    // chunks of 64 query tiles from the last one, and within a chunk the heads of
+    // the group, each over the chunk's tiles from the last one
     int bc = 0;
-    if (cur.fl & kMore) issue(cur, cur_h, 0);
-    while (cur.fl & kMore) {
-        sync_tiles();
-        const TileRef nxt = next();
-        const int nxt_h = hk * p.group + tile_g;
-        issue(nxt, nxt_h, bc ^ 1);
-        const int q0 = cur.t * BQ;
-        if (cur.fl & kNeg) {
-            clear_rows<T, BQ, D, RW, 256>((T*)buf(bc), qdoc + q0, tid);
-            clear_rows<T, BQ, D, RW, 256>((T*)(buf(bc) + C::QALLOC), qdoc + q0, tid);
-            lds_barrier();
-        }
-        if (cur.fl & kAct) {
-            const float slope2 = SLOPE ? p.slopes[b * p.slopes_sb + cur_h] * kLog2e : 0.f;
-            const bool full = (cur.fl & kFull) != 0;
-#pragma unroll
-            for (int st = 0; st < C::NSUB; ++st) {
-                f32x16 sc, dpc;
-                sdp(bc, st, sc, dpc);
-                probs(q0 + 32 * st, bc, st, slope2, sc, dpc, full);
-                acc(bc, st);
+    for (int base = (n_qt - 1) / 64 * 64; base >= 0 && base + 64 > t_lo; base -= 64) {
+        const TileChunk ch = chunk_at(base);
+        if (ch.vis == 0) continue;
+        uint64_t left = ch.vis;
+        int g = 0;
+        auto next = [&]() FA_INLINE -> TileRef {
+            if (left == 0) {
+                if (++g >= p.group) return TileRef{-1, 0u};
+                left = ch.vis;
             }
+            const int i = 63 - (int)__builtin_clzll(left);
+            left &= ~(1ull << i);
+            return ch.ref(base, i);
+        };
+        TileRef cur = next();
+        int cur_h = hk * p.group;
+        issue(cur, cur_h, bc);
+        while (cur.fl & kMore) {
+            sync_tiles();
+            const TileRef nxt = next();
+            const int nxt_h = hk * p.group + min(g, p.group - 1);
+            issue(nxt, nxt_h, bc ^ 1);
+            const int q0 = cur.t * BQ;
+            if (cur.fl & kNeg) {
+                clear_rows<T, BQ, D, RW, 256>((T*)buf(bc), ids[bc], tid);
+                clear_rows<T, BQ, D, RW, 256>((T*)(buf(bc) + C::QALLOC), ids[bc], tid);
+                lds_barrier();
+            }
+            if (cur.fl & kAct) {
+                const float slope2 = SLOPE ? p.slopes[b * p.slopes_sb + cur_h] * kLog2e : 0.f;
+#pragma unroll
+                for (int st = 0; st < C::NSUB; ++st) {
+                    f32x16 sc, dpc;
+                    s16x8 bp[NPK], bs[NPK];
+                    // (at D = 128 the parts in this order: moved together they need
+                    // more registers than there are)
+                    if constexpr (D == 128) __builtin_amdgcn_sched_barrier(0);
+                    sdp(bc, st, sc, dpc);
+                    if constexpr (D == 128) __builtin_amdgcn_sched_barrier(0);
+                    half(q0 + 32 * st, bc, st, 0, slope2, sc, dpc, bp, bs, cur.fl);
+                    half(q0 + 32 * st, bc, st, 1, slope2, sc, dpc, bp, bs, cur.fl);
+                    if constexpr (D == 128) __builtin_amdgcn_sched_barrier(0);
+                    acc(bc, st, sc, dpc, bp, bs);
+                }
+            }
+            bc ^= 1;
+            cur = nxt;
+            cur_h = nxt_h;
         }
-        bc ^= 1;
-        cur = nxt;
-        cur_h = nxt_h;
     }
     sync_tiles();
     T* const Os = (T*)smem + w * 32 * C::OW;
-    store_rows<T, D>(Os, C::OW, dk, p.scale * (CAP ? 4.f : 1.f), (T*)p.dk + b * p.dk_sb + hk * p.dk_sh, p.dk_ss, kw0,
+    store_rows<T, D>(Os, C::OW, dk, -p.scale * (CAP ? 4.f : 1.f), (T*)p.dk + b * p.dk_sb + hk * p.dk_sh, p.dk_ss, kw0,
                      p.Sk, p.cols, lane, true);
     lds_barrier();
     store_rows<T, D>(Os, C::OW, dv, 1.f, (T*)p.dv + b * p.dv_sb + hk * p.dv_sh, p.dv_ss, kw0, p.Sk, p.cols, lane, true);
