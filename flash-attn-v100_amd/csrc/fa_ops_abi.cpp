@@ -218,6 +218,19 @@ bool few_rows(const fa_scored_args* a, RowsParams& r) {
     return r.o_wgs < (1LL << 31);
 }
 
+// Parts of the dK / dV pass: its workgroups (128 keys of a KV head) walk the
+// queries of every head of the group, and under a causal mask the first keys'
+// walk all of them, so a grid of few workgroups runs for its longest.
+int kv_parts(const fa_scored_args* a) {
+    const int group = a->num_heads / a->num_heads_kv;
+    const int64_t n = ((int64_t)a->seqlen_k + 127) / 128 * a->num_heads_kv * a->batch;
+    return group > 1 && n <= 1024 ? std::min(group, 2) : 1;
+}
+size_t part_bytes(const fa_scored_args* a) {
+    const int n = kv_parts(a);
+    if (n == 1) return 0;
+    return up256((size_t)n * a->batch * a->num_heads_kv * 2 * a->seqlen_k * compiled_dim(a->head_dim) * sizeof(float));
+}
 size_t bwd_rows_bytes(const fa_scored_args* a, int32_t& sq_pad) {
     sq_pad = (a->seqlen_q + 127) / 128 * 128;
     return up256((size_t)a->batch * a->num_heads * 2 * sq_pad * sizeof(float));
@@ -298,7 +311,7 @@ int32_t fa_scored_fwd(const fa_scored_args* a, void* workspace, size_t bytes, vo
 size_t fa_scored_bwd_workspace_size(const fa_scored_args* a) {
     if (fa_scored_check(a, 1)) return 0;
     int32_t pad;
-    size_t n = bwd_rows_bytes(a, pad) + docs_bytes(a);
+    size_t n = bwd_rows_bytes(a, pad) + docs_bytes(a) + part_bytes(a);
     if (a->dslopes) n += up256((size_t)a->batch * a->num_heads * a->seqlen_q * sizeof(float));
     return n;
 }
@@ -320,6 +333,9 @@ int32_t fa_scored_bwd(const fa_scored_args* a, void* workspace, size_t bytes, vo
         p.dslope_rows = (float*)ws;
         ws += up256((size_t)a->batch * a->num_heads * a->seqlen_q * sizeof(float));
     }
+    p.kv_parts = kv_parts(a);
+    p.kv_part = (float*)ws;
+    ws += part_bytes(a);
     if (put_docs(a, p, ws, s) != hipSuccess) return FA_ERR_LAUNCH;
     const int D = compiled_dim(a->head_dim);
     hipError_t e = a->dtype == FA_DTYPE_F32    ? fa::launch_scored_bwd<float>(p, D, s)

@@ -51,6 +51,10 @@ struct ScoredParams {
     float* lse2;
     int sq_pad, ws_stride;
     float* dslope_rows;
+    // dK / dV in parts by groups of a KV head's query heads (1: none): float32
+    // (part, B, Hkv, 2, Sk, D)
+    int kv_parts;
+    float* kv_part;
 };
 
 struct DocParams {

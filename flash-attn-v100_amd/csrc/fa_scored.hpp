@@ -119,15 +119,6 @@ struct TileChunk {
     }
 };
 
-// Two workgroups share a CU, so each SIMD has two waves that alternate between
-// matrix products and the arithmetic of the scores.  At equal priority they fall
-// into step, both in the same phase; with the wave in the odd slot ahead, one's
-// products run beside the other's arithmetic.
-__device__ FA_INLINE inline void stagger_waves() {
-    if (__builtin_amdgcn_s_getreg(4 | (0 << 6) | (0 << 11)) & 1)  // HW_ID, bit 0 of the wave's slot
-        __builtin_amdgcn_s_setprio(2);
-}
-
 // zeros into the rows of a tile that belong to no document (their values may be
 // anything, and 0 times a NaN is none).  All threads of the NT; a barrier follows.
 template <typename T, int R, int D, int W, int NT>
@@ -138,6 +129,23 @@ __device__ FA_INLINE inline void clear_rows(T* tile, const int* docs, int tid) {
         const int row = c / CPR, col = c % CPR;
         if (docs[row] < 0) *reinterpret_cast<uint4*>(tile + row * W + col * EPC) = make_uint4(0u, 0u, 0u, 0u);
     }
+}
+
+// At the head of a rarely taken branch: the compiler would otherwise compute it
+// every time and select (the masks of the forward: 60 of 370 vector instructions
+// a tile)
+__device__ FA_INLINE inline void stay_branch() { asm volatile(""); }
+
+template <int N>
+using template_int = std::integral_constant<int, N>;
+
+// The kernel's arguments, to be read where they are used: what only the epilogue
+// needs would otherwise be read first and take scalar registers from the loop
+// (kept in lanes of vector registers, a read of a lane for each use).
+__device__ FA_INLINE inline const ScoredParams& late_args() {
+    uint64_t a = (uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    return *(const ScoredParams*)(uintptr_t)a;
 }
 
 // -x for four floats
@@ -198,8 +206,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
 
     const int tid = threadIdx.x;
     const int lane = tid & 63, wg = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
-    const int w = KS == 1 ? wg : wg & 3, sp = KS == 1 ? 0 : wg >> 2;
-    if constexpr (KS == 1) stagger_waves();
+    const int w = wg & 3, sp = KS == 1 ? 0 : wg >> 2;  // (& 3: its range decides copies at compile time)
     const int2 tord = tile_order<32 * (KS == 1 ? 2 : 1), true>(p.n_tiles);
     const int qt = p.n_tiles - 1 - tord.y;  // longest causal rows first
     const int h = tord.x % p.H, b = tord.x / p.H;
@@ -337,14 +344,13 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
             }
         }
     };
-    // ---- rules, mask and running max.  A score is held as u, its value in log2
+    // ---- rules, then mask and running max.  A score is held as u, its value in log2
     // units is ua u + ub: u the raw product, or r of the cap (which falls with
     // the score), or the value itself ----
     constexpr bool RCP = CAP && !SLOPE && !C::F32, VALUE = SLOPE || (CAP && C::F32);
     const float ua = VALUE ? 1.f : RCP ? -2.f * cap.top : c, ub = RCP ? cap.top : 0.f;
     constexpr float kHidden = RCP ? INFINITY : -INFINITY;
-    auto score = [&](f32x16 (&s)[NB], const TileRef& r, const int* id) FA_INLINE {
-        const int k0 = r.t * BN;
+    auto rules = [&](f32x16 (&s)[NB], int k0) FA_INLINE {
         if constexpr (RCP) {
 #pragma unroll
             for (int blk = 0; blk < NB; ++blk)
@@ -361,7 +367,11 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
                     s[blk][e] = SLOPE ? __builtin_fmaf(-slope2, __builtin_fabsf(d), t) : t;
                 }
         }
+    };
+    auto mask_max = [&](f32x16 (&s)[NB], const TileRef& r, const int* id) FA_INLINE {
+        const int k0 = r.t * BN;
         if (!(r.fl & kLim)) {
+            stay_branch();
             const int lim = lim_l - k0 - 4 * hi;
 #pragma unroll
             for (int blk = 0; blk < NB; ++blk)
@@ -370,6 +380,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
                     if (32 * blk + 8 * (e >> 2) + (e & 3) >= lim) s[blk][e] = kHidden;
         }
         if (!(r.fl & kDoc)) {
+            stay_branch();
 #pragma unroll
             for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
@@ -381,11 +392,13 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
                     if (kd.w != qd) s[blk][4 * g + 3] = kHidden;
                 }
         }
-        float mx = kHidden;
+        // (four chains: the wave waits out each step of one)
+        float m4[4] = {kHidden, kHidden, kHidden, kHidden};
 #pragma unroll
         for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) mx = RCP ? fminf(mx, s[blk][e]) : fmaxf(mx, s[blk][e]);
+            for (int e = 0; e < 16; ++e) m4[e & 3] = RCP ? fminf(m4[e & 3], s[blk][e]) : fmaxf(m4[e & 3], s[blk][e]);
+        float mx = RCP ? fminf(fminf(m4[0], m4[1]), fminf(m4[2], m4[3])) : fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         mx = pair_max(__builtin_fmaf(mx, ua, ub));
         const float m_new = fmaxf(m_run, mx);
         if (__ballot(m_new > m_run + 8.0f) != 0ull) {
@@ -401,15 +414,16 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
     constexpr int NPK = C::F32 ? 1 : BN / 16;
     auto softmax = [&](f32x16 (&s)[NB], s16x8 (&pk)[NPK]) FA_INLINE {
         const float um = ub - m_run;
-        float psum = 0.f;
+        float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 s[blk][e] = fast_exp2(VALUE ? s[blk][e] + um : __builtin_fmaf(s[blk][e], ua, um));
-                psum += s[blk][e];
+                ps[e & 3] += s[blk][e];
             }
-        l_run += psum;
+        l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        asm volatile("" : "+v"(l_run));  // summed here, beside the products
         if constexpr (!C::F32) {
 #pragma unroll
             for (int ks = 0; ks < BN / 16; ++ks) {
@@ -448,40 +462,100 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
         lds_barrier();
     };
 
-    // two slots in turn: a tile is read while the next one lands in the other
-    // slot, last read before the barrier that opens the iteration; the first tile
-    // of a chunk lands in the slot that the last iteration did not read
-    int slot = 0;
+    // Software pipeline: the products S(j + 1) run beside the probabilities of tile
+    // j, then P(j) V(j) beside the rules of tile j + 1 (a matrix product takes the
+    // matrix unit for 32 cycles and the wave for few of them; two waves on a SIMD
+    // fall into step and overlap nothing by themselves).  K is copied two tiles
+    // ahead and V one: both slots were last read before the barrier that opens the
+    // iteration.  Every wave computes every tile of the workgroup, seen or not
+    // (P = 0): the loop has no branch but the masks'.
+    auto sched = [&](auto n_tag, auto reads_tag, auto valu_tag) FA_INLINE {
+        constexpr int N = decltype(n_tag)::value, RD = decltype(reads_tag)::value, VA = decltype(valu_tag)::value;
+        if constexpr (!C::F32) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * RD, 0);
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, VA, 0);
+                if (n + 2 < N) __builtin_amdgcn_sched_group_barrier(0x100, RD, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    template_int<NB * QR> n_qk;
+    template_int<(BN / 16) * (D / 32)> n_pv;
+    template_int<1> one_read;
+    template_int<2> two_reads;
+    // vector instructions beside a product
+    template_int<(32 * 9 / 2 + NB * QR - 1) / (NB * QR)> va_b;
+    template_int<(32 * (RCP ? 4 : VALUE ? (CAP ? 7 : 3) : 1) + NB * QR - 1) / (NB * QR)> va_a;
+    f32x16 sa[NB], sb[NB];
+    s16x8 pk[NPK];
+    auto iter = [&](int slot, TileRef& cur, TileRef& nxt, const TileRef& nn, f32x16 (&sc)[NB], f32x16 (&sn)[NB]) FA_INLINE {
+        sync_tiles();
+        load_k(nn, slot);
+        load_ids(nn, slot);
+        load_v(nxt, slot ^ 1);
+        T* const Vs = Vs0 + slot * C::VTILE;
+        if (cur.fl & kNeg) {  // the groups together
+            // (the ids of tile j are overwritten by those of tile j + 2: read its rows' ones from memory)
+            if (cur.t >= 0) clear_rows<T, BN, D, VW, 256>(Vs, kdoc + cur.t * BN, tid & 255);
+            lds_barrier();
+        }
+        if constexpr (!C::F32) __builtin_amdgcn_sched_barrier(0);
+        qk(Ks0 + (slot ^ 1) * C::KTILE, sn);
+        softmax(sc, pk);
+        sched(n_qk, one_read, va_b);
+        pv(Vs, sc, pk);
+        rules(sn, nxt.t * BN);
+        // (pinned here: their use below is conditional, and they would move there)
+        if constexpr (RCP || VALUE) {
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk) asm volatile("" : "+v"(sn[blk]));
+        }
+        sched(n_pv, two_reads, va_a);
+        if (nxt.t >= 0) {
+            mask_max(sn, nxt, ids[sp][slot ^ 1] + nxt.t % TPD * BN);
+        } else {  // no tile for this group: P = 0 beside the other's
+            stay_branch();
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sn[blk][e] = kHidden;
+        }
+        cur = nxt;
+        nxt = nn;
+    };
     for (int base = 0; base < n_kt; base += 64) {
         TileChunk ch = chunk_at(base);
         TileRef cur = next(ch, base);
         if (!(cur.fl & kMore)) continue;
-        load_k(cur, slot);
-        load_v(cur, slot);
-        load_ids(cur, slot);
-        while (cur.fl & kMore) {
-            sync_tiles();
-            const TileRef nxt = next(ch, base);
-            load_k(nxt, slot ^ 1);
-            load_v(nxt, slot ^ 1);
-            load_ids(nxt, slot ^ 1);
-            T* const Vs = Vs0 + slot * C::VTILE;
-            const int* const id = ids[sp][slot] + cur.t % TPD * BN;
-            if (cur.fl & kNeg) {  // the groups together
-                if (cur.t >= 0) clear_rows<T, BN, D, VW, 256>(Vs, id, tid & 255);
-                lds_barrier();
-            }
-            if (cur.fl & kAct) {
-                f32x16 s[NB];
-                s16x8 pk[NPK];
-                qk(Ks0 + slot * C::KTILE, s);
-                score(s, cur, id);
-                softmax(s, pk);
-                pv(Vs, s, pk);
-            }
-            slot ^= 1;
-            cur = nxt;
+        TileRef nxt = next(ch, base);
+        // the last iteration of the chunk before read V slot 0 or 1; all slots are
+        // free behind this barrier
+        lds_barrier();
+        load_k(cur, 0);
+        load_ids(cur, 0);
+        load_v(cur, 0);
+        load_k(nxt, 1);
+        load_ids(nxt, 1);
+        sync_tiles();
+        qk(Ks0, sa);
+        rules(sa, cur.t * BN);
+        if (cur.t >= 0) {
+            mask_max(sa, cur, ids[sp][0] + cur.t % TPD * BN);
+        } else {
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sa[blk][e] = kHidden;
         }
+        while (cur.fl & kMore) {
+            iter(0, cur, nxt, next(ch, base), sa, sb);
+            if (!(cur.fl & kMore)) break;
+            iter(1, cur, nxt, next(ch, base), sb, sa);
+        }
+        wait_vmem();  // copies of no tile, still counted
     }
     sync_tiles();  // all waves done with the tiles, no copy in flight
 
@@ -513,13 +587,14 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
     }
 
     // ---- epilogue: normalise, LSE, O^T through LDS as rows ----
+    const ScoredParams& pe = late_args();
     const float l_tot = pair_sum(l_run);
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
     if (sp == 0 && hi == 0 && qi < p.Sq)
-        p.lse[(int64_t)(b * p.H + h) * p.Sq + qi] =
+        pe.lse[(int64_t)(b * pe.H + h) * pe.Sq + qi] =
             l_tot > 0.f ? (m_run + __log2f(l_tot)) * kLn2 : l_tot == 0.f ? -INFINITY : l_tot;
-    store_rows<T, D>(smem + w * 32 * C::OW, C::OW, o, inv, (T*)p.o + b * p.o_sb + h * p.o_sh, p.o_ss,
-                     qw0, p.Sq, p.cols, lane, sp == 0);
+    store_rows<T, D>(smem + w * 32 * C::OW, C::OW, o, inv, (T*)pe.o + b * pe.o_sb + h * pe.o_sh, pe.o_ss,
+                     qw0, pe.Sq, pe.cols, lane, sp == 0);
 }
 
 // ---------------------------------------------------------------------------
@@ -539,8 +614,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
 
     const int tid = threadIdx.x;
     const int lane = tid & 63, wg = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
-    const int w = KS == 1 ? wg : wg & 3, sp = KS == 1 ? 0 : wg >> 2;
-    if constexpr (KS == 1) stagger_waves();
+    const int w = wg & 3, sp = KS == 1 ? 0 : wg >> 2;  // (& 3: its range decides copies at compile time)
     const int2 tord = tile_order<32 * (KS == 1 ? C::MIN_BLOCKS : 1), true>(p.n_tiles);
     const int qt = p.n_tiles - 1 - tord.y;
     const int h = tord.x % p.H, b = tord.x / p.H;
@@ -701,21 +775,6 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
     auto half = [&](int k0, const T* Ks, const int* id, int ks, const f32x16& s, const f32x16& dp, unsigned fl) FA_INLINE {
         const int ka = k0 + 16 * ks + 4 * hi;  // of element 0; element e is key ka + 8 (e / 4) + e % 4
         const float d0 = qpos - (float)ka;
-        uint32_t hide = 0;  // bit e: masked
-        if (!(fl & kLim)) {
-            const int lim = lim_l - ka;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (8 * (e >> 2) + (e & 3) >= lim) hide |= 1u << e;
-        }
-        if (!(fl & kDoc)) {
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const int4 kd = *reinterpret_cast<const int4*>(id + 16 * ks + 8 * g + 4 * hi);
-                hide |= (kd.x != qd ? 1u : 0u) << (4 * g) | (kd.y != qd ? 2u : 0u) << (4 * g) |
-                        (kd.z != qd ? 4u : 0u) << (4 * g) | (kd.w != qd ? 8u : 0u) << (4 * g);
-            }
-        }
         float ds[8];
         [[maybe_unused]] float pe[8];  // P
 #pragma unroll
@@ -734,21 +793,41 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
             ds[e] = pv * (dp[r] - del);
             if (CAP) ds[e] *= cap.slope();
         }
-        if ((fl & kFull) != kFull) {
+        if (!(fl & kLim)) {
+            stay_branch();
+            const int lim = lim_l - ka;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if ((hide >> e) & 1u) pe[e] = ds[e] = 0.f;
+                if (8 * (e >> 2) + (e & 3) >= lim) pe[e] = ds[e] = 0.f;
+        }
+        if (!(fl & kDoc)) {
+            stay_branch();
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const int4 kd = *reinterpret_cast<const int4*>(id + 16 * ks + 8 * g + 4 * hi);
+                if (kd.x != qd) pe[4 * g] = ds[4 * g] = 0.f;
+                if (kd.y != qd) pe[4 * g + 1] = ds[4 * g + 1] = 0.f;
+                if (kd.z != qd) pe[4 * g + 2] = ds[4 * g + 2] = 0.f;
+                if (kd.w != qd) pe[4 * g + 3] = ds[4 * g + 3] = 0.f;
+            }
         }
         if constexpr (DSLOPE) {
+            float x0[2] = {0.f, 0.f}, x1[2] = {0.f, 0.f}, x2[2] = {0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float ad = __builtin_fabsf(d0 - (float)(8 * (e >> 2) + (e & 3)));
                 // a masked dP may be anything
                 const float pdp = pe[e] == 0.f ? 0.f : pe[e] * dp[8 * ks + e];
-                sum_dp += pdp;
-                sum_d = __builtin_fmaf(pe[e], ad, sum_d);
-                sum_ddp = __builtin_fmaf(pdp, ad, sum_ddp);
+                x0[e & 1] += pdp;
+                x1[e & 1] = __builtin_fmaf(pe[e], ad, x1[e & 1]);
+                x2[e & 1] = __builtin_fmaf(pdp, ad, x2[e & 1]);
             }
+            sum_dp += x0[0] + x0[1];
+            sum_d += x1[0] + x1[1];
+            sum_ddp += x2[0] + x2[1];
+            // summed here: moved on, P and dP stay in registers until then, and spill
+            // (2 x 4096 x 32 heads of 128: backward with the slopes' gradient 1683 -> XXXX us)
+            asm volatile("" : "+v"(sum_dp), "+v"(sum_d), "+v"(sum_ddp));
         }
         if constexpr (C::F32) {
 #pragma unroll
@@ -838,41 +917,72 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
             }
         }
     }
+    const ScoredParams& pe = late_args();
     if constexpr (DSLOPE) {
-        if (sp == 0 && hi == 0 && qi < p.Sq)
-            p.dslope_rows[((int64_t)b * p.H + h) * p.Sq + qi] = __builtin_fmaf(sum_dp, sum_d, -sum_ddp);
+        if (sp == 0 && hi == 0 && qi < pe.Sq)
+            pe.dslope_rows[((int64_t)b * pe.H + h) * pe.Sq + qi] = __builtin_fmaf(sum_dp, sum_d, -sum_ddp);
     }
-    store_rows<T, D>((T*)smem + w * 32 * C::OW, C::OW, dq, p.scale * (CAP ? 4.f : 1.f),
-                     (T*)p.dq + b * p.dq_sb + h * p.dq_sh, p.dq_ss, qw0, p.Sq, p.cols, lane, sp == 0);
+    store_rows<T, D>((T*)smem + w * 32 * C::OW, C::OW, dq, pe.scale * (CAP ? 4.f : 1.f),
+                     (T*)pe.dq + b * pe.dq_sb + h * pe.dq_sh, pe.dq_ss, qw0, pe.Sq, pe.cols, lane, sp == 0);
 }
 
 // ---------------------------------------------------------------------------
-// dK and dV of 128 keys of one (batch, KV head): the query heads of the group
-// one after the other, each over the 64-query tiles that the keys are seen by,
-// the last first (so that the workgroups of a head read the same tiles at about
-// the same time).  K and V rows in registers, as in dkdv_kernel.
+// dK and dV of 128 keys of one (batch, KV head): the query heads of the group (or
+// of this part of it) one after the other, each over the query tiles that the
+// keys are seen by, the last first (so that the workgroups of a head read the
+// same tiles at about the same time).  K and V rows in registers, as in
+// dkdv_kernel.
+// 16-bit inputs at D = 128: K, V and the sums take 192 of the 256 registers a
+// lane has (two workgroups a CU); with 64-query tiles in two slots, the LDS left
+// nothing to put beside them, 60 registers spilled, and each reload waited for
+// the tile copies in flight.  There the tiles are of 32 queries in three slots,
+// copied two ahead, and half of K's row chunks stay in LDS (backward of 2 x 4096 x
+// 32 heads, cap: XXXX -> XXXX us).
+template <typename T, int D>
+struct ScoredDkdvCfg {
+    static constexpr bool F32 = Elem<T>::kF32, SMALL = !F32 && D == 128;
+    static constexpr int NW = 4, BK = 32 * NW;
+    static constexpr int NSUB = SMALL ? 1 : 2, BQ = 32 * NSUB, NSLOT = SMALL ? 3 : 2;
+    static constexpr int RW = DkdvCfg<T, D>::RW;
+    using Rows = DmaRowGroups<T, BQ, D, RW, NW / 2>;
+    static constexpr int QALLOC = BQ * RW * (int)sizeof(T);
+    static constexpr int SLOT_BYTES = 2 * QALLOC + 2 * BQ * 4;  // Q rows, dO rows, LSE * log2 e, delta
+    // K chunks in LDS: of each wave's 32 rows, 64 lanes x 16 bytes each
+    static constexpr int KST = SMALL ? 5 : 0, KST_BYTES = KST * NW * 1024;
+    static constexpr int OW = D + (F32 ? 4 : 8);
+    static constexpr int RAW = NSLOT * SLOT_BYTES + KST_BYTES, STAGE = NW * 32 * OW * (int)sizeof(T);
+    static constexpr int SMEM_BYTES = RAW > STAGE ? RAW : STAGE;
+    // copies that each wave has issued for a tile, at least: rows, LSE and delta
+    static constexpr int MIN_COPIES = Rows::NI / (NW / 2) + (SMALL ? 1 : 2);
+    static_assert(SLOT_BYTES % 16 == 0, "16-byte aligned slots");
+};
+
 template <typename T, int D, bool CAP, bool SLOPE>
 __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void scored_dkdv_kernel(const ScoredParams p) {
-    using C = DkdvCfg<T, D>;
-    constexpr int BQ = C::BQ, RW = C::RW;
-    static_assert(BQ == 64, "one range of document ids a tile; one dword a lane for LSE and delta");
+    using C = ScoredDkdvCfg<T, D>;
+    constexpr int BQ = C::BQ, RW = C::RW, NSLOT = C::NSLOT;
+    constexpr int TPD = 64 / BQ;  // tiles per range of document ids
     __shared__ __attribute__((aligned(16))) char smem[C::SMEM_BYTES];
-    __shared__ __attribute__((aligned(16))) int ids[2][64];  // document ids of the tiles
+    __shared__ __attribute__((aligned(16))) int ids[NSLOT][64];  // document ids of the tiles
     // each key's first query and document id: needed by partly seen tiles only,
     // and registers are short
     __shared__ int key_first[C::BK], key_doc[C::BK];
 
     const int tid = threadIdx.x;
-    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
-    stagger_waves();
+    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6) & 3, l32 = lane & 31, hi = lane >> 5;
     const int2 tord = tile_order<32 * (!(Elem<T>::kF32 && D == 128) ? 2 : 1), true>(p.n_tiles);
     const int kt = tord.y;  // the first keys are seen by the most queries
-    const int hk = tord.x % p.Hkv, b = tord.x / p.Hkv;
+    const int part = tord.x % p.kv_parts, bhk = tord.x / p.kv_parts;
+    const int hk = bhk % p.Hkv, b = bhk / p.Hkv;
+    // the query heads of this part
+    const int g0 = p.group * part / p.kv_parts, g1 = p.group * (part + 1) / p.kv_parts;
     const int k0 = kt * C::BK, kw0 = k0 + 32 * w, kj = kw0 + l32;
     const SeqRule rule(p, b);
 
-    constexpr int KR = C::F32 ? D / 8 : D / 16;
-    uint4 kreg[KR], vreg[KR];
+    constexpr int KR = C::F32 ? D / 8 : D / 16, KREG = KR - C::KST;
+    uint4 kreg[KREG], vreg[KR];
+    // this lane's K chunks KREG .. KR - 1
+    char* const kst = smem + NSLOT * C::SLOT_BYTES + w * C::KST * 1024 + lane * 16;
     {
         const T* krow = (const T*)p.k + b * p.k_sb + (int64_t)kj * p.k_ss + hk * p.k_sh;
         const T* vrow = (const T*)p.v + b * p.v_sb + (int64_t)kj * p.v_ss + hk * p.v_sh;
@@ -880,7 +990,11 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
         for (int i = 0; i < KR; ++i) {
             const int d0 = C::F32 ? hi * (D / 2) + 4 * i : 16 * i + 8 * hi;
             const bool ok = kj < rule.len && d0 < p.cols;
-            kreg[i] = ok ? *reinterpret_cast<const uint4*>(krow + d0) : make_uint4(0u, 0u, 0u, 0u);
+            const uint4 x = ok ? *reinterpret_cast<const uint4*>(krow + d0) : make_uint4(0u, 0u, 0u, 0u);
+            if (i < KREG)
+                kreg[i < KREG ? i : 0] = x;
+            else
+                *reinterpret_cast<uint4*>(kst + (i - KREG) * 1024) = x;  // read by this lane only
             vreg[i] = ok ? *reinterpret_cast<const uint4*>(vrow + d0) : make_uint4(0u, 0u, 0u, 0u);
         }
         // the dP products start from delta and take -V: they give delta - dP, and
@@ -918,7 +1032,7 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
         c.doc = ~0ull;
         c.neg = 0;
         if (docs) {
-            const int2 r = v ? qrng[t] : make_int2(-1, -1);
+            const int2 r = v ? qrng[t / TPD] : make_int2(-1, -1);
             v = v && docs_meet(r, kr);
             a = a && v && docs_meet(r, wr);
             c.doc = __ballot(docs_one(r, wr));
@@ -940,8 +1054,9 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
 
     const bool copy_q = w < C::NW / 2;
     typename C::Rows rows;
-    rows.init(copy_q ? p.q_ss : p.do_ss, lane, w % (C::NW / 2), p.cols);
-    auto buf = [&](int s) FA_INLINE -> char* { return smem + s * C::BUF_BYTES; };
+    rows.init(copy_q ? p.q_ss : p.do_ss, lane, w & 1, p.cols);
+    auto buf = [&](int s) FA_INLINE -> char* { return smem + s * C::SLOT_BYTES; };
+    // a tile of no queries (t < 0) is copied too: nothing is read, but the counts stay exact
     auto issue = [&](const TileRef& r, int hh, int s) FA_INLINE {
         const int qb0 = max(r.t, 0) * BQ, nv = r.t < 0 ? 0 : p.Sq - qb0;
         char* bp = buf(s);
@@ -954,13 +1069,14 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
         const float* wrow = p.lse2 + ((int64_t)b * p.H + hh) * p.ws_stride + qb0;  // qb0 + BQ <= sq_pad
         const u32x4 rs = buffer_words(wrow, r.t < 0 ? 0 : (p.ws_stride - qb0) * 4);
         const uint32_t f = lds_addr(bp + 2 * C::QALLOC);
-        dma_load4_untracked(rs, f, 4 * lane);
-        dma_load4_untracked(rs, f + 4 * BQ, 4 * (p.sq_pad + lane));
-        if (docs && w == 0 && r.t >= 0) dma_load4_untracked(buffer_words(qdoc + qb0, 256), lds_addr(ids[s]), 4 * lane);
-    };
-    auto sync_tiles = [&]() FA_INLINE {
-        wait_vmem();
-        lds_barrier();
+        if constexpr (BQ == 32) {  // one instruction: 32 of each
+            dma_load4_untracked(rs, f, 4 * (hi ? p.sq_pad + l32 : l32));
+        } else {
+            dma_load4_untracked(rs, f, 4 * lane);
+            dma_load4_untracked(rs, f + 4 * BQ, 4 * (p.sq_pad + lane));
+        }
+        if (docs && w == 0 && r.t >= 0)
+            dma_load4_untracked(buffer_words(qdoc + qb0 / 64 * 64, 256), lds_addr(ids[s]), 4 * lane);
     };
     // ---- S = Q K^T, delta - dP (dP = dO V^T) of 32 queries ----
     auto sdp = [&](int s, int st, f32x16& sc, f32x16& dpc) FA_INLINE {
@@ -982,7 +1098,9 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
             } else {
                 const s16x8 aq = *reinterpret_cast<const s16x8*>(qrow + 16 * i + 8 * hi);
                 const s16x8 ad = *reinterpret_cast<const s16x8*>(drow + 16 * i + 8 * hi);
-                sc = Elem<T>::mfma(aq, __builtin_bit_cast(s16x8, kreg[i]), sc);
+                const s16x8 bk = i < KREG ? __builtin_bit_cast(s16x8, kreg[i < KREG ? i : 0])
+                                          : *reinterpret_cast<const s16x8*>(kst + (i - KREG) * 1024);
+                sc = Elem<T>::mfma(aq, bk, sc);
                 dpc = Elem<T>::mfma(ad, __builtin_bit_cast(s16x8, vreg[i]), dpc);
             }
         }
@@ -1015,16 +1133,18 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
             }
         }
         if (!(fl & kLim)) {
+            stay_branch();
             const int lim = key_first[32 * w + l32] - qa;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (8 * (e >> 2) + (e & 3) < lim) pd[e] = ds[e] = 0.f;
         }
         if (!(fl & kDoc)) {
+            stay_branch();
             const int kd = key_doc[32 * w + l32];
 #pragma unroll
             for (int gg = 0; gg < 2; ++gg) {
-                const int4 id = *reinterpret_cast<const int4*>(ids[s] + 32 * st + 16 * ks + 8 * gg + 4 * hi);
+                const int4 id = *reinterpret_cast<const int4*>(ids[s] + (qb0 & 63) + 16 * ks + 8 * gg + 4 * hi);
                 if (id.x != kd) pd[4 * gg] = ds[4 * gg] = 0.f;
                 if (id.y != kd) pd[4 * gg + 1] = ds[4 * gg + 1] = 0.f;
                 if (id.z != kd) pd[4 * gg + 2] = ds[4 * gg + 2] = 0.f;
@@ -1040,6 +1160,7 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
         } else {
             bp[ks] = pack8<T>(pd);
             bs[ks] = pack8<T>(ds);
+            asm volatile("" : "+v"(bp[ks]), "+v"(bs[ks]));  // packed here: the unpacked values would stay in registers
         }
     };
     // ---- dV^T += dO^T P, dK^T -= Q^T dX ----
@@ -1073,16 +1194,20 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
     };
 
     // chunks of 64 query tiles from the last one, and within a chunk the heads of
-    // the group, each over the chunk's tiles from the last one
-    int bc = 0;
-    for (int base = (n_qt - 1) / 64 * 64; base >= 0 && base + 64 > t_lo; base -= 64) {
+    // the part, each over the chunk's tiles from the last one.  A tile is copied
+    // NSLOT - 1 ahead, into the slot that was read before the barrier that opens
+    // the iteration.
+    int bc = 0;  // slot of the current tile
+    auto slot_after = [&](int s, int n) FA_INLINE { return s + n >= NSLOT ? s + n - NSLOT : s + n; };
+    for (int base = n_qt > 0 ? (n_qt - 1) / 64 * 64 : -1; base >= 0 && base + 64 > t_lo; base -= 64) {
         const TileChunk ch = chunk_at(base);
         if (ch.vis == 0) continue;
         uint64_t left = ch.vis;
-        int g = 0;
+        int g = g0;
         auto next = [&]() FA_INLINE -> TileRef {
             if (left == 0) {
-                if (++g >= p.group) return TileRef{-1, 0u};
+                if (g + 1 >= g1) return TileRef{-1, 0u};
+                ++g;
                 left = ch.vis;
             }
             const int i = 63 - (int)__builtin_clzll(left);
@@ -1090,18 +1215,33 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
             return ch.ref(base, i);
         };
         TileRef cur = next();
-        int cur_h = hk * p.group;
+        int cur_h = hk * p.group + g0;
         issue(cur, cur_h, bc);
+        [[maybe_unused]] TileRef nxt = {-1, 0u};
+        [[maybe_unused]] int nxt_h = cur_h;
+        if constexpr (NSLOT == 3) {
+            nxt = next();
+            nxt_h = hk * p.group + g;
+            issue(nxt, nxt_h, slot_after(bc, 1));
+        }
         while (cur.fl & kMore) {
-            sync_tiles();
-            const TileRef nxt = next();
-            const int nxt_h = hk * p.group + min(g, p.group - 1);
-            issue(nxt, nxt_h, bc ^ 1);
+            if constexpr (NSLOT == 3) {
+                wait_vmem_below<C::MIN_COPIES>();  // the current tile's copies; the next one's may be in flight
+                barrier_no_fence();
+            } else {
+                wait_vmem();
+                lds_barrier();
+            }
+            const TileRef nn = next();
+            const int nn_h = hk * p.group + g;
+            issue(nn, nn_h, slot_after(bc, NSLOT - 1));
             const int q0 = cur.t * BQ;
             if (cur.fl & kNeg) {
-                clear_rows<T, BQ, D, RW, 256>((T*)buf(bc), ids[bc], tid);
-                clear_rows<T, BQ, D, RW, 256>((T*)(buf(bc) + C::QALLOC), ids[bc], tid);
-                lds_barrier();
+                const int* const id = ids[bc] + (q0 & 63);
+                clear_rows<T, BQ, D, RW, 256>((T*)buf(bc), id, tid);
+                clear_rows<T, BQ, D, RW, 256>((T*)(buf(bc) + C::QALLOC), id, tid);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                barrier_no_fence();
             }
             if (cur.fl & kAct) {
                 const float slope2 = SLOPE ? p.slopes[b * p.slopes_sb + cur_h] * kLog2e : 0.f;
@@ -1109,28 +1249,92 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
                 for (int st = 0; st < C::NSUB; ++st) {
                     f32x16 sc, dpc;
                     s16x8 bp[NPK], bs[NPK];
-                    // (at D = 128 the parts in this order: moved together they need
-                    // more registers than there are)
-                    if constexpr (D == 128) __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (C::SMALL) __builtin_amdgcn_sched_barrier(0);
                     sdp(bc, st, sc, dpc);
-                    if constexpr (D == 128) __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (C::SMALL) __builtin_amdgcn_sched_barrier(0);
                     half(q0 + 32 * st, bc, st, 0, slope2, sc, dpc, bp, bs, cur.fl);
                     half(q0 + 32 * st, bc, st, 1, slope2, sc, dpc, bp, bs, cur.fl);
-                    if constexpr (D == 128) __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (C::SMALL) __builtin_amdgcn_sched_barrier(0);
                     acc(bc, st, sc, dpc, bp, bs);
                 }
             }
-            bc ^= 1;
-            cur = nxt;
-            cur_h = nxt_h;
+            bc = slot_after(bc, 1);
+            if constexpr (NSLOT == 3) {
+                cur = nxt;
+                cur_h = nxt_h;
+                nxt = nn;
+                nxt_h = nn_h;
+            } else {
+                cur = nn;
+                cur_h = nn_h;
+            }
+        }
+        // three slots: the copies of no tile issued last go to slots that the next
+        // chunk's first tiles take; they land before those (in issue order)
+        if constexpr (NSLOT == 3) {
+            wait_vmem();
+            barrier_no_fence();
         }
     }
-    sync_tiles();
-    T* const Os = (T*)smem + w * 32 * C::OW;
-    store_rows<T, D>(Os, C::OW, dk, -p.scale * (CAP ? 4.f : 1.f), (T*)p.dk + b * p.dk_sb + hk * p.dk_sh, p.dk_ss, kw0,
-                     p.Sk, p.cols, lane, true);
+    wait_vmem();
     lds_barrier();
-    store_rows<T, D>(Os, C::OW, dv, 1.f, (T*)p.dv + b * p.dv_sb + hk * p.dv_sh, p.dv_ss, kw0, p.Sk, p.cols, lane, true);
+    const ScoredParams& pe = late_args();
+    if (pe.kv_parts > 1) {  // float32 parts, for kv_sum_kernel
+        if (kj < pe.Sk) {
+            float* row = pe.kv_part + ((((int64_t)part * pe.B + b) * pe.Hkv + hk) * 2 * pe.Sk + kj) * D + 4 * hi;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    f32x4 x, y;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[e] = dk[i][4 * g + e];
+                        y[e] = dv[i][4 * g + e];
+                    }
+                    *reinterpret_cast<f32x4*>(row + 32 * i + 8 * g) = x;
+                    *reinterpret_cast<f32x4*>(row + (int64_t)pe.Sk * D + 32 * i + 8 * g) = y;
+                }
+        }
+        return;
+    }
+    T* const Os = (T*)smem + w * 32 * C::OW;
+    store_rows<T, D>(Os, C::OW, dk, -pe.scale * (CAP ? 4.f : 1.f), (T*)pe.dk + b * pe.dk_sb + hk * pe.dk_sh, pe.dk_ss, kw0,
+                     pe.Sk, pe.cols, lane, true);
+    lds_barrier();
+    store_rows<T, D>(Os, C::OW, dv, 1.f, (T*)pe.dv + b * pe.dv_sb + hk * pe.dv_sh, pe.dv_ss, kw0, pe.Sk, pe.cols, lane, true);
+}
+
+// dK and dV from the float32 parts of a KV head's groups of query heads: one
+// thread 4 columns of a key, the parts in order
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv_sum_kernel(const ScoredParams p, const float k_mul) {
+    const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int col = (int)(gid % (D / 4)) * 4;
+    const int64_t r = gid / (D / 4);  // ((b Hkv + hk) 2 + which) Sk + key
+    if (r >= (int64_t)p.B * p.Hkv * 2 * p.Sk || col >= p.cols) return;
+    const int key = (int)(r % p.Sk), which = (int)(r / p.Sk % 2);
+    const int64_t bh = r / (2 * (int64_t)p.Sk);
+    const int hk = (int)(bh % p.Hkv), b = (int)(bh / p.Hkv);
+    const float* x = p.kv_part + r * D + col;
+    const int64_t step = (int64_t)p.B * p.Hkv * 2 * p.Sk * D;
+    f32x4 acc = *reinterpret_cast<const f32x4*>(x);
+    for (int n = 1; n < p.kv_parts; ++n) {
+        const f32x4 y = *reinterpret_cast<const f32x4*>(x + n * step);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += y[e];
+    }
+    const float mul = which ? 1.f : k_mul;
+    T* out = which ? (T*)p.dv + b * p.dv_sb + (int64_t)key * p.dv_ss + hk * p.dv_sh
+                   : (T*)p.dk + b * p.dk_sb + (int64_t)key * p.dk_ss + hk * p.dk_sh;
+    if constexpr (Elem<T>::kF32) {
+        *reinterpret_cast<f32x4*>(out + col) = f32x4{acc[0] * mul, acc[1] * mul, acc[2] * mul, acc[3] * mul};
+    } else {
+        s16x4 v4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v4[e] = Elem<T>::pack1(acc[e] * mul);
+        *reinterpret_cast<s16x4*>(out + col) = v4;
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -1170,8 +1374,13 @@ hipError_t launch_scored_bwd_t(ScoredParams p, hipStream_t s) {
         }
     }
     p.n_tiles = (p.Sk + CK::BK - 1) / CK::BK;
-    const int64_t nk = (int64_t)p.n_tiles * p.Hkv * p.B;
+    const int64_t nk = (int64_t)p.n_tiles * p.Hkv * p.B * p.kv_parts;
     if (nk > 0) hipLaunchKernelGGL((scored_dkdv_kernel<T, D, CAP, SLOPE>), dim3((unsigned)nk), dim3(256), 0, s, p);
+    if (nk > 0 && p.kv_parts > 1) {
+        const int64_t nt = (int64_t)p.B * p.Hkv * 2 * p.Sk * (D / 4);
+        hipLaunchKernelGGL((kv_sum_kernel<T, D>), dim3((unsigned)((nt + 255) / 256)), dim3(256), 0, s, p,
+                           -p.scale * (CAP ? 4.f : 1.f));
+    }
     return hipGetLastError();
 }
 
