@@ -161,32 +161,40 @@ T ceil_div(T a, T b) { return (a + b - 1) / b; }
 
 void plan_rows(RowsParams& p, int32_t dtype) {
     const int D = compiled_dim(p.cols);
-    const int64_t bn = dtype == FA_DTYPE_F32 ? 32 : 64;
-    const int64_t slots = D == 128 || dtype == FA_DTYPE_F32 ? 256 : 512;
+    const int64_t slots = dtype == FA_DTYPE_F32 && D == 128 ? 256 : 512;  // workgroups that run at once
     const int64_t rows = (int64_t)p.Sq * p.group;
+    p.p_unit = rows * p.B > 64 ? 128 : 32;
     p.o_rt = (int)ceil_div<int64_t>(rows, 32);
-    p.p_rt = p.P > 0 ? (int)ceil_div<int64_t>(rows * p.B, 32) : 0;
+    p.p_rt = p.P > 0 ? (int)ceil_div<int64_t>(rows * p.B, p.p_unit) : 0;
     const int64_t ou = (int64_t)p.B * p.Hkv * p.o_rt, pu = (int64_t)p.Hkv * p.p_rt;
-    const int64_t ont = ceil_div<int64_t>(p.Sk, bn), pnt = ceil_div<int64_t>(p.P, bn);
-    const int64_t chunk = std::max<int64_t>(8, ceil_div(ou * ont + pu * pnt, 2 * slots));
-    p.o_splits = (int)std::max<int64_t>(1, std::min<int64_t>(64, ceil_div(ont, chunk)));
-    p.p_splits = pu ? (int)std::max<int64_t>(1, std::min<int64_t>(64, ceil_div(pnt, chunk))) : 0;
+    const int64_t ont = ceil_div<int64_t>(p.Sk, 64), pnt = ceil_div<int64_t>(p.P, 64);
+    // As many splits as fill the device once, but none below 4 steps of a workgroup
+    // (a step is 128 keys in a unit of 32 rows, 64 keys in one of 128), whose part
+    // would cost more to write and join than its keys: one token of 8 heads
+    // over 512 keys takes 13.1 us in one split a unit and 15.6 us in two.
+    const int64_t chunk = ceil_div<int64_t>(ou * ont + pu * pnt, slots);
+    auto splits = [&](int64_t nt, int64_t least) {
+        return (int)std::max<int64_t>(1, std::min<int64_t>(64, ceil_div(nt, std::max<int64_t>(chunk, least))));
+    };
+    p.o_splits = splits(ont, 8);
+    p.p_splits = pu ? splits(pnt, p.p_unit == 128 ? 4 : 8) : 0;
     p.p_wgs = pu * p.p_splits;
     p.o_wgs = ou * p.o_splits;
+    p.p_rows = p.p_wgs * p.p_unit;
 }
-bool rows_need_parts(const RowsParams& p) { return p.p_wgs > 0 || p.o_splits > 1; }
+bool rows_need_parts(const RowsParams& p) { return p.p_splits + p.o_splits > 1; }
+size_t part_rows(const RowsParams& p) { return (size_t)(p.p_rows + p.o_wgs * 32); }
 size_t rows_bytes(const RowsParams& p) {
     if (!rows_need_parts(p)) return 0;
-    const size_t n = (size_t)(p.p_wgs + p.o_wgs) * 32;
+    const size_t n = part_rows(p);
     return up256(n * sizeof(float2)) + up256(n * compiled_dim(p.cols) * sizeof(float));
 }
 void put_parts(RowsParams& p, void* ws) {
     p.stat = nullptr;
     p.part = nullptr;
     if (!rows_need_parts(p)) return;
-    const size_t n = (size_t)(p.p_wgs + p.o_wgs) * 32;
     p.stat = (float2*)ws;
-    p.part = (float*)((char*)ws + up256(n * sizeof(float2)));
+    p.part = (float*)((char*)ws + up256(part_rows(p) * sizeof(float2)));
 }
 hipError_t run_rows(const RowsParams& p, int32_t dtype, hipStream_t s) {
     const int D = compiled_dim(p.cols);

@@ -98,10 +98,11 @@ struct RowsParams {
     int tail;            // 1: own position of query 0 is len - Sq
     int causal;          // 0: every filled key is seen
     int masked_neg;      // queries at positions below 0 see nothing, the prefix neither
-    // parts: the prefix keys go to p_splits workgroups for each tile of rows
-    // (p_rt tiles a KV head), a sequence's own to o_splits (o_rt tiles)
-    int p_splits, p_rt, o_splits, o_rt;
+    // parts: the prefix keys go to p_splits workgroups for each unit of p_unit rows
+    // (p_rt units a KV head), a sequence's own to o_splits (o_rt units of 32)
+    int p_splits, p_rt, p_unit, o_splits, o_rt;
     int64_t p_wgs, o_wgs;
+    int64_t p_rows;      // part rows of the prefix, p_wgs p_unit
     float2* stat;        // per part row: maximum (log2 units), sum
     float* part;         // per part row: D floats
 };

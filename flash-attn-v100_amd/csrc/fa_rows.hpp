@@ -1,18 +1,21 @@
 // Attention of a few new tokens a sequence over its cache, and over a prefix
 // that all sequences of the batch share; gfx950.
 //
-// A row is one (sequence, new token, query head).  Rows of one KV head are taken
-// 32 at a time: over the prefix the rows of all sequences together (its K and V
-// are read once a tile of rows, not once a sequence), over a sequence's own keys
-// that sequence's rows.  Each tile of rows has its keys split over workgroups;
-// a workgroup's 4 waves walk its 64-key tiles in turn, each copying its own
-// (direct to LDS, two copies in flight), as fwd_decode_kernel does.  A split
-// leaves its rows' maximum, sum and unnormalised output in float32, and
+// A row is one (sequence, new token, query head).  The keys of every unit of rows
+// are split over workgroups:
+//   * a sequence's own keys: units of 32 rows (of one sequence and KV head), whose
+//     keys a workgroup's 4 waves walk in turn, 32 at a time, each copying its own
+//     tiles (direct to LDS, both of a tile's copies in flight) with no barrier;
+//   * the prefix: the rows of all sequences together, units of 128 whose waves
+//     share 64-key tiles, so that K and V are read once for 128 rows, not once a
+//     sequence; units of 32 where there are no more than 64 rows.
+// A split leaves its rows' maximum, sum and unnormalised output in float32, and
 // rows_join_kernel puts the parts of a row together:
 //   O = sum_x 2^(m_x - m) O_x / sum_x 2^(m_x - m) l_x,  m = max_x m_x.
 // Query i of a sequence with n keys of its own stands at own position
 // n - Sq + i and sees its keys up to there; in distances the prefix lies before
-// them.  Bound by the K and V bytes.
+// them.  Bound by the K and V bytes, and over the prefix by the products of its
+// rows.
 #pragma once
 
 #include "fa_common.hpp"
@@ -26,47 +29,73 @@ template <typename T, int D>
 struct RowsCfg {
     static constexpr bool F32 = Elem<T>::kF32;
     static constexpr int NW = 4;
-    static constexpr int BN = F32 ? 32 : 64;
-    static constexpr int NB = BN / 32;
-    static constexpr int KW = D + (F32 ? 4 : 8);
-    static constexpr int VW = F32 ? D + 8 : D + (D == 64 || D == 96 ? 8 : 24);
+    // a wave's own tiles (rows of one 32-row unit): 32 keys, rows of an even
+    // number of 16-byte chunks, so that a tile is whole copy instructions
+    static constexpr int BN = 32;
+    static constexpr int KW = D + (F32 ? 4 : 16);
+    static constexpr int VW = F32 ? D + 8 : D + (D == 128 ? 32 : 16);
     static constexpr int KTILE = BN * KW, VTILE = BN * VW;
     static constexpr int REGION = KTILE + VTILE;
     static_assert((D / 32) * 16 * 64 * 4 <= REGION * (int)sizeof(T), "a wave's O part fits its region");
+    // tiles shared by the waves of a 128-row unit
+    using S = FwdCfg<T, D>;
+    static constexpr int SMEM = NW * REGION > S::SMEM_ELEMS ? NW * REGION : S::SMEM_ELEMS;
+    // two workgroups a CU where registers and LDS allow it
+    static constexpr int PER_CU = F32 && D == 128 ? 1 : 2;
 };
 
-// one tile of rows over keys [0, n_keys) of K / V, keys of split `split` of `splits`
-template <typename T, int D>
-__global__ __launch_bounds__(256, (D <= 64 && !Elem<T>::kF32 ? 2 : 1)) void rows_kernel(const RowsParams p) {
-    using C = RowsCfg<T, D>;
-    constexpr int BN = C::BN, NB = C::NB, KW = C::KW, VW = C::VW, NW = C::NW;
-    __shared__ __attribute__((aligned(16))) T smem[NW * C::REGION];
-    __shared__ float stat[NW][2][32];
+// one row of a unit: its query and the keys [0, lim) it sees
+struct UnitRow {
+    int b, i, h, lim;
+    bool live;
+    float qpos;
+    __device__ FA_INLINE inline UnitRow(const RowsParams& p, bool pre, int row, int hk, int bs) {
+        const int per_seq = p.Sq * p.group, n_rows = pre ? p.B * per_seq : per_seq;
+        live = row < n_rows;
+        const int rr = live ? row : 0;
+        b = pre ? rr / per_seq : bs;
+        const int ig = pre ? rr % per_seq : rr;
+        i = ig / p.group;
+        h = hk * p.group + ig % p.group;
+        const int len = p.lens ? max(0, min(p.Sk, p.lens[b])) : p.Sk;
+        const int off = p.tail ? len - p.Sq : max(-kMaxOffset, min(kMaxOffset, p.offsets ? p.offsets[b] : p.offset0));
+        const int own = off + i;  // the query's position among the sequence's own keys
+        lim = pre ? p.P : p.causal ? min(len, own + 1) : len;
+        if (!live || (p.masked_neg && own < 0)) lim = 0;
+        qpos = (float)(pre ? p.P + own : own);
+    }
+};
 
-    const int tid = threadIdx.x;
-    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
-    const bool pre = (int64_t)blockIdx.x < p.p_wgs;
-    const int nwg = (int)(pre ? p.p_wgs : p.o_wgs);
-    const int id = xcd_remap(pre ? (int)blockIdx.x : (int)(blockIdx.x - p.p_wgs), nwg);
+// scores of 16 keys of a 32-key block in log2 units
+template <bool F32>
+__device__ FA_INLINE inline void row_rules(f32x16& s, const RowsParams& p, Cap<F32>& cap, bool slope, float slope2, float d0) {
+    if (p.cap > 0.f) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = cap.value(s[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] *= p.scale_log2;
+    }
+    if (slope) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            s[e] = __builtin_fmaf(-slope2, __builtin_fabsf(d0 - (float)(8 * (e >> 2) + (e & 3))), s[e]);
+    }
+}
+
+// 32 rows over split `split` of the keys [0, n_keys) (a sequence's own ones, or a
+// prefix that few rows read): each wave walks tiles of its own
+template <typename T, int D>
+__device__ FA_INLINE inline void unit32(const RowsParams& p, bool pre, T* smem, float (*stat)[2][32], int id, int lane, int w) {
+    using C = RowsCfg<T, D>;
+    constexpr int BN = C::BN, KW = C::KW, VW = C::VW, NW = C::NW;
+    const int l32 = lane & 31, hi = lane >> 5;
     const int splits = pre ? p.p_splits : p.o_splits, rts = pre ? p.p_rt : p.o_rt;
     const int split = id % splits, unit = id / splits, rt = unit % rts, bk = unit / rts;
     const int hk = bk % p.Hkv, bs = bk / p.Hkv;  // bs: the sequence (own keys)
-
-    // ---- this lane's row ----
-    const int row = 32 * rt + l32, per_seq = p.Sq * p.group;
-    const int n_rows = pre ? p.B * per_seq : per_seq;
-    const bool live = row < n_rows;
-    const int rr = live ? row : 0;
-    const int b = pre ? rr / per_seq : bs, ig = pre ? rr % per_seq : rr;
-    const int i = ig / p.group, h = hk * p.group + ig % p.group;
-    const int len = p.lens ? max(0, min(p.Sk, p.lens[b])) : p.Sk;
-    const int off = p.tail ? len - p.Sq : max(-kMaxOffset, min(kMaxOffset, p.offsets ? p.offsets[b] : p.offset0));
-    const int own = off + i;  // the query's position among the sequence's own keys
-    int lim = pre ? p.P : p.causal ? min(len, own + 1) : len;  // keys [0, lim) are seen
-    if (!live || (p.masked_neg && own < 0)) lim = 0;
-    const float qpos = (float)(pre ? p.P + own : own);
+    const UnitRow row(p, pre, 32 * rt + l32, hk, bs);
     // keys that some row of the tile sees, and that all do
-    int lim_max = lim, lim_min = live ? lim : INT_MAX;
+    int lim_max = row.lim, lim_min = row.live ? row.lim : INT_MAX;
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) {
         lim_max = max(lim_max, __shfl_xor(lim_max, x));
@@ -107,15 +136,15 @@ __global__ __launch_bounds__(256, (D <= 64 && !Elem<T>::kF32 ? 2 : 1)) void rows
     constexpr int QR = C::F32 ? D / 8 : D / 16;
     uint4 qreg[QR];
     {
-        const T* qrow = (const T*)p.q + b * p.q_sb + (int64_t)i * p.q_ss + h * p.q_sh;
+        const T* qrow = (const T*)p.q + row.b * p.q_sb + (int64_t)row.i * p.q_ss + row.h * p.q_sh;
 #pragma unroll
         for (int kk = 0; kk < QR; ++kk) {
             const int d0 = C::F32 ? hi * (D / 2) + 4 * kk : 16 * kk + 8 * hi;
-            qreg[kk] = live && d0 < p.cols ? *reinterpret_cast<const uint4*>(qrow + d0) : make_uint4(0u, 0u, 0u, 0u);
+            qreg[kk] = row.live && d0 < p.cols ? *reinterpret_cast<const uint4*>(qrow + d0) : make_uint4(0u, 0u, 0u, 0u);
         }
     }
     const bool slope = p.slopes != nullptr;
-    const float slope2 = slope ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
+    const float slope2 = slope ? p.slopes[row.b * p.slopes_sb + row.h] * kLog2e : 0.f;
     wait_vmem();
     asm volatile("" ::: "memory");
 
@@ -136,64 +165,36 @@ __global__ __launch_bounds__(256, (D <= 64 && !Elem<T>::kF32 ? 2 : 1)) void rows
         else
             wait_vmem_below<NVI>();  // K(t); only V(t) may be in flight
         asm volatile("" ::: "memory");
-        f32x16 s[NB];
+        f32x16 s = f32x16{};
+        const T* krow = Ks + l32 * KW;
 #pragma unroll
-        for (int blk = 0; blk < NB; ++blk) {
-            s[blk] = f32x16{};
-            const T* krow = Ks + (32 * blk + l32) * KW;
+        for (int kk = 0; kk < QR; ++kk) {
+            if constexpr (C::F32) {
+                const f32x4 a = *reinterpret_cast<const f32x4*>(krow + hi * (D / 2) + 4 * kk);
+                const f32x4 bq = __builtin_bit_cast(f32x4, qreg[kk]);
 #pragma unroll
-            for (int kk = 0; kk < QR; ++kk) {
-                if constexpr (C::F32) {
-                    const f32x4 a = *reinterpret_cast<const f32x4*>(krow + hi * (D / 2) + 4 * kk);
-                    const f32x4 bq = __builtin_bit_cast(f32x4, qreg[kk]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[blk] = mfma_f32(a[e], bq[e], s[blk]);
-                } else {
-                    const s16x8 a = *reinterpret_cast<const s16x8*>(krow + 16 * kk + 8 * hi);
-                    s[blk] = Elem<T>::mfma(a, __builtin_bit_cast(s16x8, qreg[kk]), s[blk]);
-                }
+                for (int e = 0; e < 4; ++e) s = mfma_f32(a[e], bq[e], s);
+            } else {
+                const s16x8 a = *reinterpret_cast<const s16x8*>(krow + 16 * kk + 8 * hi);
+                s = Elem<T>::mfma(a, __builtin_bit_cast(s16x8, qreg[kk]), s);
             }
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K(t) read before it is overwritten
         if constexpr (!C::F32) copy_k(t + NW);
 
-        // ---- scores in log2 units ----
-        if (p.cap > 0.f) {
-#pragma unroll
-            for (int blk = 0; blk < NB; ++blk)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[blk][e] = cap.value(s[blk][e]);
-        } else {
-#pragma unroll
-            for (int blk = 0; blk < NB; ++blk)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[blk][e] *= p.scale_log2;
-        }
-        if (slope) {
-            const float d0 = qpos - (float)(k0 + 4 * hi);
-#pragma unroll
-            for (int blk = 0; blk < NB; ++blk)
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    s[blk][e] = __builtin_fmaf(-slope2, __builtin_fabsf(d0 - (float)(32 * blk + 8 * (e >> 2) + (e & 3))),
-                                               s[blk][e]);
-        }
+        row_rules(s, p, cap, slope, slope2, row.qpos - (float)(k0 + 4 * hi));
         if (k0 + BN > lim_min) {
-            const int lm = lim - k0 - 4 * hi;
+            stay_branch();
+            const int lm = row.lim - k0 - 4 * hi;
 #pragma unroll
-            for (int blk = 0; blk < NB; ++blk)
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (32 * blk + 8 * (e >> 2) + (e & 3) >= lm) s[blk][e] = -INFINITY;
+            for (int e = 0; e < 16; ++e)
+                if (8 * (e >> 2) + (e & 3) >= lm) s[e] = -INFINITY;
         }
         // ---- softmax ----
-        float mx = -INFINITY;
+        float m2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int blk = 0; blk < NB; ++blk)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[blk][e]);
-        mx = pair_max(mx);
-        const float m_new = fmaxf(m_run, mx);
+        for (int e = 0; e < 16; ++e) m2[e & 1] = fmaxf(m2[e & 1], s[e]);
+        const float m_new = fmaxf(m_run, pair_max(fmaxf(m2[0], m2[1])));
         if (__ballot(m_new > m_run + 8.0f) != 0ull) {
             const float alpha = fast_exp2(m_run - m_new);
             l_run *= alpha;
@@ -203,26 +204,22 @@ __global__ __launch_bounds__(256, (D <= 64 && !Elem<T>::kF32 ? 2 : 1)) void rows
                 for (int e = 0; e < 16; ++e) o[n][e] *= alpha;
             m_run = m_new;
         }
-        float psum = 0.f;
+        float ps[2] = {0.f, 0.f};
 #pragma unroll
-        for (int blk = 0; blk < NB; ++blk)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[blk][e] = fast_exp2(s[blk][e] - m_run);
-                psum += s[blk][e];
-            }
-        l_run += psum;
+        for (int e = 0; e < 16; ++e) {
+            s[e] = fast_exp2(s[e] - m_run);
+            ps[e & 1] += s[e];
+        }
+        l_run += ps[0] + ps[1];
 
         // ---- O^T += V^T P^T ----
         if constexpr (C::F32) {
 #pragma unroll
-            for (int blk = 0; blk < NB; ++blk)
+            for (int x = 0; x < 16; ++x) {
+                const T* vrow = Vs + (8 * (x >> 2) + 4 * hi + (x & 3)) * VW + l32;
 #pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    const T* vrow = Vs + (32 * blk + 8 * (x >> 2) + 4 * hi + (x & 3)) * VW + l32;
-#pragma unroll
-                    for (int n = 0; n < D / 32; ++n) o[n] = mfma_f32(vrow[32 * n], s[blk][x], o[n]);
-                }
+                for (int n = 0; n < D / 32; ++n) o[n] = mfma_f32(vrow[32 * n], s[x], o[n]);
+            }
         } else {
             wait_vmem_below<NKI>();  // V(t); only K(t + 4) may be in flight
             asm volatile("" ::: "memory");
@@ -230,7 +227,7 @@ __global__ __launch_bounds__(256, (D <= 64 && !Elem<T>::kF32 ? 2 : 1)) void rows
             for (int ks = 0; ks < BN / 16; ++ks) {
                 float tmp[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) tmp[e] = s[ks >> 1][8 * (ks & 1) + e];
+                for (int e = 0; e < 8; ++e) tmp[e] = s[8 * ks + e];
                 const s16x8 pk = pack8<T>(tmp);
 #pragma unroll
                 for (int n = 0; n < D / 32; ++n) {
@@ -269,11 +266,11 @@ __global__ __launch_bounds__(256, (D <= 64 && !Elem<T>::kF32 ? 2 : 1)) void rows
         a[x] = fast_exp2(stat[x][0][l32] - mm);
         l_tot = __builtin_fmaf(stat[x][1][l32], a[x], l_tot);
     }
-    const bool only = p.p_wgs == 0 && splits == 1;  // no other part of these rows
-    const int64_t prow = ((pre ? 0 : p.p_wgs) + id) * 32 + l32;
+    const bool only = p.p_splits + p.o_splits == 1;  // no other part of these rows
+    const int64_t prow = (pre ? 0 : p.p_rows) + (int64_t)id * 32 + l32;
     if (!only && w == 0 && hi == 0) p.stat[prow] = make_float2(mm, l_tot);
-    if (only && w == 0 && hi == 0 && live && p.lse)
-        p.lse[(int64_t)(b * p.H + h) * p.Sq + i] =
+    if (only && w == 0 && hi == 0 && row.live && p.lse)
+        p.lse[(int64_t)(row.b * p.H + row.h) * p.Sq + row.i] =
             l_tot > 0.f ? (mm + __log2f(l_tot)) * kLn2 : l_tot == 0.f ? -INFINITY : l_tot;
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
 #pragma unroll
@@ -292,8 +289,8 @@ __global__ __launch_bounds__(256, (D <= 64 && !Elem<T>::kF32 ? 2 : 1)) void rows
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
                 *reinterpret_cast<f32x4*>(op + 8 * q4) = f32x4{om[4 * q4], om[4 * q4 + 1], om[4 * q4 + 2], om[4 * q4 + 3]};
-        } else if (live) {
-            T* ob = (T*)p.o + b * p.o_sb + (int64_t)i * p.o_ss + h * p.o_sh + 32 * n + 4 * hi;
+        } else if (row.live) {
+            T* ob = (T*)p.o + row.b * p.o_sb + (int64_t)row.i * p.o_ss + row.h * p.o_sh + 32 * n + 4 * hi;
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
                 if (32 * n + 8 * q4 + 4 * hi >= p.cols) continue;
@@ -313,36 +310,231 @@ __global__ __launch_bounds__(256, (D <= 64 && !Elem<T>::kF32 ? 2 : 1)) void rows
     }
 }
 
-// the parts of every row, rescaled to their common maximum: one thread per 4
-// columns of a row (D / 4 threads share a row)
+// 128 rows of all sequences over split `split` of the prefix: the waves share its
+// tiles (64 keys, double-buffered), each on 32 rows
 template <typename T, int D>
-__global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p, const int64_t n_rows) {
-    constexpr int TPR = D / 4;
-    const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t r = gid / TPR;
-    const int col = (int)(gid % TPR) * 4;
-    if (r >= n_rows) return;
+__device__ FA_INLINE inline void unit128(const RowsParams& p, T* smem, int id, int lane, int w) {
+    using C = FwdCfg<T, D>;
+    constexpr int BN = C::BN, NB = C::NB, KW = C::KW, VW = C::VW;
+    const int l32 = lane & 31, hi = lane >> 5;
+    const int split = id % p.p_splits, unit = id / p.p_splits, rt = unit % p.p_rt, hk = unit / p.p_rt;
+    const UnitRow row(p, true, 128 * rt + 32 * w + l32, hk, 0);
+    const int nt = (p.P + BN - 1) / BN;
+    const int t0 = (int)((int64_t)nt * split / p.p_splits), t1 = (int)((int64_t)nt * (split + 1) / p.p_splits);
+    const T* __restrict__ kbase = (const T*)p.kp + hk * p.kp_sh;
+    const T* __restrict__ vbase = (const T*)p.vp + hk * p.vp_sh;
+    T* const Ks0 = smem;
+    T* const Vs0 = smem + 2 * C::KTILE;
+    DmaTile<T, BN, D, KW, C::NW> kd;
+    kd.init(p.kp_ss, lane, w, p.cols);
+    DmaTile<T, BN, D, VW, C::NW> vd;
+    vd.init(p.vp_ss, lane, w, p.cols);
+    auto copy = [&](int t, int slot) FA_INLINE {
+        const int nv = t < t1 ? p.P - t * BN : 0;
+        if constexpr (C::F32) {
+            kd.load(kbase + (int64_t)(t * BN) * p.kp_ss, p.kp_ss, nv, Ks0 + slot * C::KTILE, lane);
+            vd.load(vbase + (int64_t)(t * BN) * p.vp_ss, p.vp_ss, nv, Vs0 + slot * C::VTILE, lane);
+        } else {
+            kd.load_untracked(kbase + (int64_t)(t * BN) * p.kp_ss, p.kp_ss, nv, Ks0 + slot * C::KTILE, lane);
+            vd.load_untracked(vbase + (int64_t)(t * BN) * p.vp_ss, p.vp_ss, nv, Vs0 + slot * C::VTILE, lane);
+        }
+    };
+    constexpr int QR = C::F32 ? D / 8 : D / 16;
+    uint4 qreg[QR];
+    {
+        const T* qrow = (const T*)p.q + row.b * p.q_sb + (int64_t)row.i * p.q_ss + row.h * p.q_sh;
+#pragma unroll
+        for (int kk = 0; kk < QR; ++kk) {
+            const int d0 = C::F32 ? hi * (D / 2) + 4 * kk : 16 * kk + 8 * hi;
+            qreg[kk] = row.live && d0 < p.cols ? *reinterpret_cast<const uint4*>(qrow + d0) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    const bool slope = p.slopes != nullptr;
+    const float slope2 = slope ? p.slopes[row.b * p.slopes_sb + row.h] * kLog2e : 0.f;
+    const int lim_w = __builtin_amdgcn_readfirstlane(__ballot(row.live && row.lim == 0) != 0ull ? 0 : p.P);  // seen by all
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) o[n] = f32x16{};
+    float m_run = -1e30f, l_run = 0.f;
+    Cap<C::F32> cap(p);
+
+    int slot = 0;
+    copy(t0, 0);
+    for (int t = t0; t < t1; ++t) {
+        wait_vmem();
+        lds_barrier();
+        copy(t + 1, slot ^ 1);
+        const int k0 = t * BN;
+        f32x16 s[NB];
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk) {
+            s[blk] = f32x16{};
+            const T* krow = Ks0 + slot * C::KTILE + (32 * blk + l32) * KW;
+#pragma unroll
+            for (int kk = 0; kk < QR; ++kk) {
+                if constexpr (C::F32) {
+                    const f32x4 a = *reinterpret_cast<const f32x4*>(krow + hi * (D / 2) + 4 * kk);
+                    const f32x4 bq = __builtin_bit_cast(f32x4, qreg[kk]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[blk] = mfma_f32(a[e], bq[e], s[blk]);
+                } else {
+                    const s16x8 a = *reinterpret_cast<const s16x8*>(krow + 16 * kk + 8 * hi);
+                    s[blk] = Elem<T>::mfma(a, __builtin_bit_cast(s16x8, qreg[kk]), s[blk]);
+                }
+            }
+        }
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk)
+            row_rules(s[blk], p, cap, slope, slope2, row.qpos - (float)(k0 + 32 * blk + 4 * hi));
+        if (k0 + BN > lim_w) {
+            stay_branch();
+            const int lm = row.lim - k0 - 4 * hi;
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (32 * blk + 8 * (e >> 2) + (e & 3) >= lm) s[blk][e] = -INFINITY;
+        }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) m4[e & 3] = fmaxf(m4[e & 3], s[blk][e]);
+        const float m_new = fmaxf(m_run, pair_max(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))));
+        if (__ballot(m_new > m_run + 8.0f) != 0ull) {
+            const float alpha = fast_exp2(m_run - m_new);
+            l_run *= alpha;
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[n][e] *= alpha;
+            m_run = m_new;
+        }
+        float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[blk][e] = fast_exp2(s[blk][e] - m_run);
+                ps[e & 3] += s[blk][e];
+            }
+        l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        const T* const Vs = Vs0 + slot * C::VTILE;
+        if constexpr (C::F32) {
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    const T* vrow = Vs + (32 * blk + 8 * (x >> 2) + 4 * hi + (x & 3)) * VW + l32;
+#pragma unroll
+                    for (int n = 0; n < D / 32; ++n) o[n] = mfma_f32(vrow[32 * n], s[blk][x], o[n]);
+                }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < BN / 16; ++ks) {
+                float tmp[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) tmp[e] = s[ks >> 1][8 * (ks & 1) + e];
+                const s16x8 pk = pack8<T>(tmp);
+#pragma unroll
+                for (int n = 0; n < D / 32; ++n) {
+                    const T* vp = Vs + (16 * ks + 4 * hi + ((lane & 15) >> 2)) * VW + 32 * n + 16 * ((lane >> 4) & 1) +
+                                  4 * (lane & 3);
+                    const s16x8 a = cat4(lds_read_tr16(vp), lds_read_tr16(vp + 8 * VW));
+                    o[n] = Elem<T>::mfma(a, pk, o[n]);
+                }
+            }
+        }
+        slot ^= 1;
+    }
+    wait_vmem();  // (copies of no tile)
+    const float l_w = pair_sum(l_run);
+    const int64_t prow = (int64_t)id * 128 + 32 * w + l32;
+    if (hi == 0) p.stat[prow] = make_float2(m_run, l_w);
+    float* op = p.part + prow * D + 4 * hi;
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4)
+            *reinterpret_cast<f32x4*>(op + 32 * n + 8 * q4) = f32x4{o[n][4 * q4], o[n][4 * q4 + 1], o[n][4 * q4 + 2], o[n][4 * q4 + 3]};
+}
+
+// The units of the prefix, then those of the sequences' own keys, in one launch
+// (the products of the ones beside the bytes of the others).
+template <typename T, int D>
+__global__ __launch_bounds__(256, (RowsCfg<T, D>::PER_CU)) void rows_kernel(const RowsParams p) {
+    using C = RowsCfg<T, D>;
+    __shared__ __attribute__((aligned(16))) T smem[C::SMEM];
+    __shared__ float stat[C::NW][2][32];
+    const int tid = threadIdx.x;
+    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
+    const bool pre = (int64_t)blockIdx.x < p.p_wgs;
+    // splits of a unit are consecutive ids, on one XCD's share of the grid
+    const int id = xcd_remap(pre ? (int)blockIdx.x : (int)(blockIdx.x - p.p_wgs), (int)(pre ? p.p_wgs : p.o_wgs));
+    if (pre && p.p_unit == 128)
+        unit128<T, D>(p, smem, id, lane, w);
+    else
+        unit32<T, D>(p, pre, smem, stat, id, lane, w);
+}
+
+// The parts of every row, rescaled to their common maximum: D / 4 threads a row (4
+// columns each), times G groups that share its parts and meet in LDS.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p, const int64_t n_rows, const int G) {
+    constexpr int TPR = D / 4, SLOTS = 256 / TPR;  // row-groups of a workgroup
+    __shared__ float sm[SLOTS][2], sacc[SLOTS][D];
+    const int slot = (int)threadIdx.x / TPR, col = (int)(threadIdx.x % TPR) * 4;
+    const int g = slot % G;
+    const int64_t r = (int64_t)blockIdx.x * (SLOTS / G) + slot / G;
+    const bool live = r < n_rows;
+    const int64_t rr = live ? r : 0;
     // r = (b H + h) Sq + i
-    const int i = (int)(r % p.Sq), h = (int)((r / p.Sq) % p.H), b = (int)(r / ((int64_t)p.Sq * p.H));
+    const int i = (int)(rr % p.Sq), h = (int)((rr / p.Sq) % p.H), b = (int)(rr / ((int64_t)p.Sq * p.H));
     const int hk = h / p.group, ig = i * p.group + h % p.group, per_seq = p.Sq * p.group;
+    const int U = p.p_unit;
     const int64_t gp = (int64_t)b * per_seq + ig;  // row of the prefix units
-    const int64_t pbase = ((int64_t)hk * p.p_rt + (gp >> 5)) * p.p_splits * 32 + (gp & 31);
-    const int64_t obase = (p.p_wgs + (((int64_t)b * p.Hkv + hk) * p.o_rt + (ig >> 5)) * p.o_splits) * 32 + (ig & 31);
+    const int64_t pbase = ((int64_t)hk * p.p_rt + gp / U) * p.p_splits * U + gp % U;
+    const int64_t obase = p.p_rows + (((int64_t)b * p.Hkv + hk) * p.o_rt + (ig >> 5)) * p.o_splits * 32 + (ig & 31);
+    const int n = p.p_splits + p.o_splits;
+    auto part_row = [&](int x) FA_INLINE { return x < p.p_splits ? pbase + (int64_t)U * x : obase + 32 * (int64_t)(x - p.p_splits); };
     float mm = -1e30f;
-    for (int x = 0; x < p.p_splits; ++x) mm = fmaxf(mm, p.stat[pbase + 32 * x].x);
-    for (int x = 0; x < p.o_splits; ++x) mm = fmaxf(mm, p.stat[obase + 32 * x].x);
+    for (int x = g; x < n; x += G) mm = fmaxf(mm, p.stat[part_row(x)].x);
     float l_tot = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    auto add = [&](int64_t pr) FA_INLINE {
+#pragma unroll 4
+    for (int x = g; x < n; x += G) {
+        const int64_t pr = part_row(x);
         const float2 st = p.stat[pr];
         const float a = fast_exp2(st.x - mm);
         l_tot = __builtin_fmaf(st.y, a, l_tot);
         const f32x4 v = *reinterpret_cast<const f32x4*>(p.part + pr * D + col);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[e], a, acc[e]);
-    };
-    for (int x = 0; x < p.p_splits; ++x) add(pbase + 32 * x);
-    for (int x = 0; x < p.o_splits; ++x) add(obase + 32 * x);
+    }
+    if (G > 1) {
+        if (col == 0) {
+            sm[slot][0] = mm;
+            sm[slot][1] = l_tot;
+        }
+        *reinterpret_cast<f32x4*>(&sacc[slot][col]) = acc;
+        __syncthreads();
+        if (g != 0) return;
+        float m2 = mm;
+        for (int x = 1; x < G; ++x) m2 = fmaxf(m2, sm[slot + x][0]);
+        const float a0 = fast_exp2(mm - m2);
+        l_tot *= a0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] *= a0;
+        for (int x = 1; x < G; ++x) {
+            const float a = fast_exp2(sm[slot + x][0] - m2);
+            l_tot = __builtin_fmaf(sm[slot + x][1], a, l_tot);
+            const f32x4 v = *reinterpret_cast<const f32x4*>(&sacc[slot + x][col]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[e], a, acc[e]);
+        }
+        mm = m2;
+    }
+    if (!live) return;
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
     if (col == 0 && p.lse) p.lse[r] = l_tot > 0.f ? (mm + __log2f(l_tot)) * kLn2 : l_tot == 0.f ? -INFINITY : l_tot;
     if (col >= p.cols) return;
@@ -360,9 +552,13 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p, cons
 template <typename T, int D>
 hipError_t launch_rows_t(const RowsParams& p, hipStream_t s) {
     hipLaunchKernelGGL((rows_kernel<T, D>), dim3((unsigned)(p.p_wgs + p.o_wgs)), dim3(256), 0, s, p);
-    if (p.p_wgs > 0 || p.o_splits > 1) {
-        const int64_t n_rows = (int64_t)p.B * p.H * p.Sq, nt = n_rows * (D / 4);
-        hipLaunchKernelGGL((rows_join_kernel<T, D>), dim3((unsigned)((nt + 255) / 256)), dim3(256), 0, s, p, n_rows);
+    const int n = p.p_splits + p.o_splits;
+    if (n > 1) {
+        const int64_t n_rows = (int64_t)p.B * p.H * p.Sq;
+        constexpr int SLOTS = 256 / (D / 4);
+        const int G = n > 16 ? 8 : n > 4 ? 4 : 1;  // up to 8 row-groups a workgroup at D = 128
+        const int64_t per = SLOTS / G;
+        hipLaunchKernelGGL((rows_join_kernel<T, D>), dim3((unsigned)((n_rows + per - 1) / per)), dim3(256), 0, s, p, n_rows, G);
     }
     return hipGetLastError();
 }
