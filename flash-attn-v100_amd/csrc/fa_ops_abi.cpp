@@ -226,13 +226,27 @@ bool few_rows(const fa_scored_args* a, RowsParams& r) {
     return r.o_wgs < (1LL << 31);
 }
 
-// Parts of the dK / dV pass: its workgroups (128 keys of a KV head) walk the
+// Parts of the dK / dV pass.  A workgroup (128 keys of a KV head) walks the
 // queries of every head of the group, and under a causal mask the first keys'
-// walk all of them, so a grid of few workgroups runs for its longest.
+// walk all of them, so a grid of few workgroups runs for its longest: it is cut
+// into parts of every n-th query tile, whose float32 sums meet in a pass after
+// it.  Worth it while the grid is short of the device (with no causal mask, of
+// half of it) and each part is long; backward in 1, 2, 4 and 8 parts of
+//   1 x 2048, 8 on 2 heads of 128, cap: 521, 304, 195, 143 us
+//   1 x 1024, 8 heads of 128, cap: 105, 89, 78, 80
+//   2 x 1777, 12 heads of 64, cap: 123, 113, 130, 159; 3 documents 61, 72, 85, 113
+//   4 x 700, 12 heads of 128 in float32, cap: 394, 398, 443, 526
+//   2 x 4096, 32 on 8 heads of 128, cap: 1419, 1143, 1187, 1292
+//   2 x 8192, 16 heads of 128, cap: 2168, 2343, 2574, 3143
+//   2 x 2048, 16 heads of 64, cap, not causal: 185, 207
 int kv_parts(const fa_scored_args* a) {
-    const int group = a->num_heads / a->num_heads_kv;
-    const int64_t n = ((int64_t)a->seqlen_k + 127) / 128 * a->num_heads_kv * a->batch;
-    return group > 1 && n <= 1024 ? std::min(group, 2) : 1;
+    const int64_t n = ceil_div<int64_t>(a->seqlen_k, 128) * a->num_heads_kv * a->batch;
+    // queries of a walk (of documents, those of its own)
+    const int64_t walk = (int64_t)(a->num_heads / a->num_heads_kv) * a->seqlen_q / (a->q_documents ? 4 : 1);
+    int parts = 1;
+    const int64_t most = a->causal ? 512 : 256;
+    while (parts < 8 && n * parts <= most && walk >= parts * (n * parts <= 128 ? 512 : 1024)) parts *= 2;
+    return parts;
 }
 size_t part_bytes(const fa_scored_args* a) {
     const int n = kv_parts(a);

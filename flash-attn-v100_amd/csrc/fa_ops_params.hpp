@@ -51,7 +51,7 @@ struct ScoredParams {
     float* lse2;
     int sq_pad, ws_stride;
     float* dslope_rows;
-    // dK / dV in parts by groups of a KV head's query heads (1: none): float32
+    // dK / dV in 1, 2, 4 or 8 parts by query tiles (1: no sums to join): float32
     // (part, B, Hkv, 2, Sk, D)
     int kv_parts;
     float* kv_part;

@@ -927,10 +927,10 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
 }
 
 // ---------------------------------------------------------------------------
-// dK and dV of 128 keys of one (batch, KV head): the query heads of the group (or
-// of this part of it) one after the other, each over the query tiles that the
-// keys are seen by, the last first (so that the workgroups of a head read the
-// same tiles at about the same time).  K and V rows in registers, as in
+// dK and dV of 128 keys of one (batch, KV head): the query heads of the group one
+// after the other, each over the query tiles that the keys are seen by (or this
+// part's of them), the last first (so that the workgroups of a head read the same
+// tiles at about the same time).  K and V rows in registers, as in
 // dkdv_kernel.
 // 16-bit inputs at D = 128: K, V and the sums take 192 of the 256 registers a
 // lane has (two workgroups a CU); with 64-query tiles in two slots, the LDS left
@@ -974,8 +974,9 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
     const int kt = tord.y;  // the first keys are seen by the most queries
     const int part = tord.x % p.kv_parts, bhk = tord.x / p.kv_parts;
     const int hk = bhk % p.Hkv, b = bhk / p.Hkv;
-    // the query heads of this part
-    const int g0 = p.group * part / p.kv_parts, g1 = p.group * (part + 1) / p.kv_parts;
+    // of 64 query tiles, this part's: every kv_parts-th (1, 2, 4 or 8)
+    const uint64_t own = (p.kv_parts == 1 ? ~0ull : p.kv_parts == 2 ? 0x5555555555555555ull
+                          : p.kv_parts == 4 ? 0x1111111111111111ull : 0x0101010101010101ull) << part;
     const int k0 = kt * C::BK, kw0 = k0 + 32 * w, kj = kw0 + l32;
     const SeqRule rule(p, b);
 
@@ -1038,7 +1039,7 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
             c.doc = __ballot(docs_one(r, wr));
             c.neg = __ballot(r.x < 0);
         }
-        c.vis = __ballot(v);
+        c.vis = __ballot(v) & own;
         c.act = __ballot(a);
         return c;
     };
@@ -1203,10 +1204,10 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
         const TileChunk ch = chunk_at(base);
         if (ch.vis == 0) continue;
         uint64_t left = ch.vis;
-        int g = g0;
+        int g = 0;
         auto next = [&]() FA_INLINE -> TileRef {
             if (left == 0) {
-                if (g + 1 >= g1) return TileRef{-1, 0u};
+                if (g + 1 >= p.group) return TileRef{-1, 0u};
                 ++g;
                 left = ch.vis;
             }
@@ -1215,7 +1216,7 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
             return ch.ref(base, i);
         };
         TileRef cur = next();
-        int cur_h = hk * p.group + g0;
+        int cur_h = hk * p.group;
         issue(cur, cur_h, bc);
         [[maybe_unused]] TileRef nxt = {-1, 0u};
         [[maybe_unused]] int nxt_h = cur_h;
@@ -1305,7 +1306,7 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
     store_rows<T, D>(Os, C::OW, dv, 1.f, (T*)pe.dv + b * pe.dv_sb + hk * pe.dv_sh, pe.dv_ss, kw0, pe.Sk, pe.cols, lane, true);
 }
 
-// dK and dV from the float32 parts of a KV head's groups of query heads: one
+// dK and dV from the float32 parts of a KV head (every n-th query tile each): one
 // thread 4 columns of a key, the parts in order
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv_sum_kernel(const ScoredParams p, const float k_mul) {
@@ -1363,14 +1364,27 @@ hipError_t launch_scored_bwd_t(ScoredParams p, hipStream_t s) {
     using CK = DkdvCfg<T, D>;
     p.n_tiles = (p.Sq + CQ::BM - 1) / CQ::BM;
     const int64_t nq = (int64_t)p.n_tiles * p.H * p.B;
+    // as the forward (1 x 2048, 8 on 2 heads of 128, cap: backward 316 -> 303 us;
+    // 2 x 1024, 12 heads of 64, cap: 72 -> 69 us)
+    constexpr bool kTwo = !(CQ::F32 && D == 128);
+    const int ks = kTwo && nq < 256 && p.Sk > CQ::BN ? 2 : 1;
+    auto dq = [&](auto dslope, auto two) {
+        hipLaunchKernelGGL((scored_dq_kernel<T, D, CAP, SLOPE, decltype(dslope)::value, decltype(two)::value ? 2 : 1>),
+                           dim3((unsigned)nq), dim3(256 * ks), 0, s, p);
+    };
+    auto dq_ks = [&](auto dslope) {
+        if constexpr (kTwo)
+            if (ks == 2) return dq(dslope, std::true_type{});
+        dq(dslope, std::false_type{});
+    };
     if (nq > 0) {
         if constexpr (SLOPE) {
             if (p.dslope_rows)
-                hipLaunchKernelGGL((scored_dq_kernel<T, D, CAP, true, true, 1>), dim3((unsigned)nq), dim3(256), 0, s, p);
+                dq_ks(std::true_type{});
             else
-                hipLaunchKernelGGL((scored_dq_kernel<T, D, CAP, true, false, 1>), dim3((unsigned)nq), dim3(256), 0, s, p);
+                dq_ks(std::false_type{});
         } else {
-            hipLaunchKernelGGL((scored_dq_kernel<T, D, CAP, false, false, 1>), dim3((unsigned)nq), dim3(256), 0, s, p);
+            dq_ks(std::false_type{});
         }
     }
     p.n_tiles = (p.Sk + CK::BK - 1) / CK::BK;
