@@ -7,8 +7,11 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include "fa_host_util.hpp"
 #include "fa_ops.h"
@@ -51,6 +54,7 @@ bool none(PyObject* o) { return o == Py_None; }
 const int32_t* lengths(PyObject* o, at::Tensor& keep) {
     if (none(o)) return nullptr;
     keep = THPVariable_Unpack(o);
+    if (keep.scalar_type() == at::kLong) keep = keep.clamp(INT32_MIN, INT32_MAX);  // out of range stays so
     if (keep.scalar_type() != at::kInt || !keep.is_contiguous()) keep = keep.to(at::kInt).contiguous();
     return (const int32_t*)keep.data_ptr();
 }
@@ -59,6 +63,8 @@ const int32_t* documents(PyObject* o, at::Tensor& keep, int64_t& stride) {
     stride = 0;
     if (none(o)) return nullptr;
     keep = THPVariable_Unpack(o);
+    // an id past int32 must not become another one's: it counts as padding
+    if (keep.scalar_type() == at::kLong) keep = at::where(keep.gt(INT32_MAX), -1, keep.clamp_min(-1));
     if (keep.scalar_type() != at::kInt || (keep.size(1) > 1 && keep.stride(1) != 1)) keep = keep.to(at::kInt).contiguous();
     stride = keep.size(0) > 1 ? keep.stride(0) : 0;
     return (const int32_t*)keep.data_ptr();
@@ -319,6 +325,25 @@ PyObject* rotary(PyObject*, PyObject* const* x, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// on_other_stream(tensor or None, ...): whether the gradient of one of them would be
+// handed on to a stream other than its device's current one: the stream that its
+// node (a leaf's accumulator, if an older graph keeps it alive) was made on
+PyObject* on_other_stream(PyObject*, PyObject* const* x, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        if (none(x[i])) continue;
+        if (!all_tensors(x + i, 1)) return nullptr;
+        const at::Tensor& t = THPVariable_Unpack(x[i]);
+        if (!t.requires_grad()) continue;
+        const std::shared_ptr<torch::autograd::Node> node =
+            t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
+        const auto st = node ? node->stream() : std::nullopt;
+        if (st && *st != c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device())) Py_RETURN_TRUE;
+    }
+    Py_RETURN_FALSE;
+    END_HANDLE_TH_ERRORS
+}
+
 // bind_ops(fa_ops_version, sizeof(fa_scored_args), sizeof(fa_prefix_args),
 //     sizeof(fa_rotary_args), then the addresses of the functions above in their
 //     order); refused for another version or other struct sizes, as bind is
@@ -363,5 +388,6 @@ PyMethodDef fa_host::ops_methods[] = {
     {"scored_bwd", (PyCFunction)(void*)scored_bwd, METH_FASTCALL, nullptr},
     {"prefix_fwd", (PyCFunction)(void*)prefix_fwd, METH_FASTCALL, nullptr},
     {"rotary", (PyCFunction)(void*)rotary, METH_FASTCALL, nullptr},
+    {"on_other_stream", (PyCFunction)(void*)on_other_stream, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

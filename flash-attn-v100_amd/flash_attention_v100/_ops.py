@@ -192,6 +192,16 @@ def rotary_table(positions: int, rotary_dim: int, scaling: int, base: float, fac
     return table
 
 
+def check_capture(*inputs) -> None:
+    """Refuses a call to be differentiated inside a stream capture on an input
+    whose gradient would leave the capture: one whose node another stream made, as
+    a leaf's accumulator that an eager graph keeps alive.  The backward would make
+    that stream wait on the capture, which ends the process at the capture's end."""
+    if torch.cuda.is_current_stream_capturing() and host().on_other_stream(*inputs):
+        raise RuntimeError("captured backward: an input belongs to an autograd graph of another stream that is still "
+                           "alive; drop that graph's outputs before the capture, or capture on detached inputs")
+
+
 def optional_lengths(t: Optional[torch.Tensor], name: str, B: int, device) -> Optional[torch.Tensor]:
     """An optional (B,) integer tensor on the inputs' device."""
     if t is None:

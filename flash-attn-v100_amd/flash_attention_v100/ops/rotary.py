@@ -91,15 +91,34 @@ class RotaryFunction(torch.autograd.Function):
         return gq, gk, None, None, None
 
 
-def _overlaps(t: torch.Tensor) -> bool:
+def _overlaps(shape, strides) -> bool:
     """Whether two indices of a tensor may share an element (strides checked from
     the smallest up; a negative answer is exact for views of dense tensors)."""
     end = 0
-    for st, n in sorted((t.stride(d), t.shape[d]) for d in range(t.dim()) if t.shape[d] > 1):
+    for st, n in sorted((st, n) for st, n in zip(strides, shape) if n > 1):
         if st <= end:
             return True
         end += st * (n - 1)
     return False
+
+
+def _disjoint(q: torch.Tensor, k: torch.Tensor) -> bool:
+    """Whether q and k share no element: different storages or address ranges, or
+    heads of one packed tensor."""
+    if q.numel() == 0 or k.numel() == 0 or q.untyped_storage().data_ptr() != k.untyped_storage().data_ptr():
+        return True
+    (q0, q1), (k0, k1) = ((t.storage_offset(), t.storage_offset() + sum((n - 1) * st for n, st in zip(t.shape, t.stride())))
+                          for t in (q, k))
+    if q1 < k0 or k1 < q0:
+        return True
+    sh = q.stride(2) if q.shape[2] > 1 else k.stride(2) if k.shape[2] > 1 else abs(k0 - q0)
+    gap = abs(k0 - q0)
+    first, last = (q, k) if q0 < k0 else (k, q)
+    if sh == 0 or gap % sh or gap // sh < first.shape[2] or any(
+            t.shape[2] > 1 and t.stride(2) != sh for t in (q, k)) or any(
+            q.shape[d] > 1 and q.stride(d) != k.stride(d) for d in (0, 1)):
+        return False
+    return not _overlaps((*first.shape[:2], gap // sh + last.shape[2], first.shape[3]), (*first.stride()[:2], sh, 1))
 
 
 def rotary_embedding_v100(
@@ -159,10 +178,13 @@ def rotary_embedding_v100(
         if grad:
             raise ValueError("inplace=True on inputs that require grad: call it under torch.no_grad()")
         for name, t in (("q", q), ("k", k)):
-            if t is not None and ((D > 1 and t.stride(3) != 1) or _overlaps(t)):
+            if t is not None and ((D > 1 and t.stride(3) != 1) or _overlaps(t.shape, t.stride())):
                 raise ValueError(f"inplace=True needs a {name} with unit column stride and no overlapping elements")
+        if k is not None and not _disjoint(q, k):
+            raise ValueError("inplace=True needs a q and k that share no element")
         return _pair(*_ops.rotary(q, k, table, positions, bool(interleaved), False, True))
     if grad:
+        _ops.check_capture(q, k)
         return RotaryFunction.apply(q, k, table, positions, bool(interleaved))
     return _pair(*_ops.rotary(q, k, table, positions, bool(interleaved), False, False))
 

@@ -145,7 +145,8 @@ def flash_attention_v100_scored(
     ``softcap``: bound of the tanh on the scores (0 or None: none).
     ``distance_slopes``: float32 (H,) or (B, H), differentiable.
     ``documents``: integer ids (B, Sq) or (Sq,) of the queries' documents and,
-    unless ``key_documents`` gives theirs, of the keys'; negative: padding.
+    unless ``key_documents`` gives theirs, of the keys'; negative (or past int32):
+    padding.
     ``prefix_lengths``: (B,), with ``causal``: keys before them are seen by every
     query.  ``key_lengths``: (B,) filled keys.  ``query_offsets``: position of
     query 0 among the keys, an int or (B,); 0 by default (the top-left causal mask
@@ -155,7 +156,9 @@ def flash_attention_v100_scored(
 
     Head dims up to 128 (``NotImplementedError`` above), fp16 / bf16 / fp32.
     Returns O, or (O, LSE) with ``return_softmax_lse``; gradients of q, k, v and
-    ``distance_slopes``.
+    ``distance_slopes``.  Forward and backward may be captured into a HIP graph;
+    inputs that an eager graph of another stream still holds are refused there
+    (``RuntimeError``).
     """
     check_qkv(q, k, v, "flash_attention_v100_scored")
     B, Sq, H, D = q.shape
@@ -190,6 +193,7 @@ def flash_attention_v100_scored(
     rules = _ops.Rules(bool(causal), scale, softcap, slopes, prefix, lens, offsets, offset0, q_docs, k_docs)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (slopes is not None and slopes.requires_grad)):
+        _ops.check_capture(q, k, v, slopes)
         out = ScoredAttentionFunction.apply(q, k, v, slopes, rules, return_softmax_lse)
         o, lse = out if return_softmax_lse else (out, None)
     else:
