@@ -200,6 +200,25 @@ __device__ FA_INLINE inline void store_rows(T* Os, int OW, const f32x16 (&acc)[D
     }
 }
 
+// Which (batch, head) and which block of it, from the longest walk on, a workgroup
+// takes.  With documents the walks are short and of any length, and a sequence of
+// long documents would keep its XCDs busy after the others have drained: there
+// the heads of a group come from all sequences in turn, and the groups are twice
+// as large (2 x 8192 x 16 heads of 128, documents of 153 to 3355 tokens:
+// 1100 -> 962 us a step)
+struct BlockOrder {
+    int b, head, rank;
+};
+template <int SLOTS>
+__device__ FA_INLINE inline BlockOrder block_order(const ScoredParams& p, int heads) {
+    if (p.q_docs) {
+        const int2 t = tile_order<2 * SLOTS, true>(p.n_tiles);
+        return BlockOrder{t.x % p.B, t.x / p.B, t.y};
+    }
+    const int2 t = tile_order<SLOTS, true>(p.n_tiles);
+    return BlockOrder{t.x / heads, t.x % heads, t.y};
+}
+
 // ---------------------------------------------------------------------------
 // Forward, over the tiles of a walk.  KS = 2: two groups of 4 waves on the same
 // queries, taking the walk's tiles in turn, for grids that leave CUs idle.
@@ -215,9 +234,9 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
     const int tid = threadIdx.x;
     const int lane = tid & 63, wg = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
     const int w = wg & 3, sp = KS == 1 ? 0 : wg >> 2;  // (& 3: its range decides copies at compile time)
-    const int2 tord = tile_order<32 * (KS == 1 ? 2 : 1), true>(p.n_tiles);
-    const int qt = p.n_tiles - 1 - tord.y;  // longest causal rows first
-    const int h = tord.x % p.H, b = tord.x / p.H;
+    const BlockOrder ord = block_order<32 * (KS == 1 ? 2 : 1)>(p, p.H);
+    const int qt = p.n_tiles - 1 - ord.rank;  // longest causal rows first
+    const int h = ord.head, b = ord.b;
     const int hk = h / p.group;
     const int q0 = qt * C::BM, qw0 = q0 + 32 * w, qi = qw0 + l32;
     const SeqRule rule(p, b);
@@ -625,9 +644,9 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
     const int tid = threadIdx.x;
     const int lane = tid & 63, wg = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, hi = lane >> 5;
     const int w = wg & 3, sp = KS == 1 ? 0 : wg >> 2;  // (& 3: its range decides copies at compile time)
-    const int2 tord = tile_order<32 * (KS == 1 ? C::MIN_BLOCKS : 1), true>(p.n_tiles);
-    const int qt = p.n_tiles - 1 - tord.y;
-    const int h = tord.x % p.H, b = tord.x / p.H;
+    const BlockOrder ord = block_order<32 * (KS == 1 ? C::MIN_BLOCKS : 1)>(p, p.H);
+    const int qt = p.n_tiles - 1 - ord.rank;
+    const int h = ord.head, b = ord.b;
     const int hk = h / p.group;
     const int q0 = qt * C::BM, qw0 = q0 + 32 * w, qi = qw0 + l32;
     const SeqRule rule(p, b);
@@ -982,10 +1001,9 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
 
     const int tid = threadIdx.x;
     const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6) & 3, l32 = lane & 31, hi = lane >> 5;
-    const int2 tord = tile_order<32 * (!(Elem<T>::kF32 && D == 128) ? 2 : 1), true>(p.n_tiles);
-    const int kt = tord.y;  // the first keys are seen by the most queries
-    const int part = tord.x % p.kv_parts, bhk = tord.x / p.kv_parts;
-    const int hk = bhk % p.Hkv, b = bhk / p.Hkv;
+    const BlockOrder ord = block_order<32 * (!(Elem<T>::kF32 && D == 128) ? 2 : 1)>(p, p.Hkv * p.kv_parts);
+    const int kt = ord.rank;  // the first keys are seen by the most queries
+    const int part = ord.head % p.kv_parts, hk = ord.head / p.kv_parts, b = ord.b;
     // of 64 query tiles, this part's: every kv_parts-th (1, 2, 4 or 8)
     const uint64_t own = (p.kv_parts == 1 ? ~0ull : p.kv_parts == 2 ? 0x5555555555555555ull
                           : p.kv_parts == 4 ? 0x1111111111111111ull : 0x0101010101010101ull) << part;
