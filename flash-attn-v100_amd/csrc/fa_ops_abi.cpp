@@ -285,7 +285,7 @@ int32_t fa_scored_check(const fa_scored_args* a, int32_t backward) {
     if (q) {
         if ((st = check_tensor(a->q, a->q_stride, 4, Sq, D, es)) || (st = check_tensor(a->o, a->o_stride, 4, Sq, D, es)))
             return st;
-        if (!a->lse) return FA_ERR_NULL_ARG;
+        if (backward && !a->lse) return FA_ERR_NULL_ARG;
         if (!aligned(a->lse, 4)) return FA_ERR_ALIGN;
     }
     if (k && ((st = check_tensor(a->k, a->k_stride, 4, Sk, D, es)) || (st = check_tensor(a->v, a->v_stride, 4, Sk, D, es))))

@@ -49,6 +49,10 @@ bool all_tensors(PyObject* const* x, Py_ssize_t n) {
     return true;
 }
 bool none(PyObject* o) { return o == Py_None; }
+int32_t i32(int64_t n) {
+    TORCH_CHECK(n <= INT32_MAX, "size ", n, " exceeds the operators' limit of 2^31 - 1");
+    return (int32_t)n;
+}
 
 // an optional integer array as contiguous int32 (held by `keep`), or null
 const int32_t* lengths(PyObject* o, at::Tensor& keep) {
@@ -111,12 +115,12 @@ void put_sizes(fa_scored_args& a, const at::Tensor& q, const at::Tensor& k, cons
     put_strides(a.q_stride, q);
     put_strides(a.k_stride, k);
     put_strides(a.v_stride, v);
-    a.batch = (int32_t)q.size(0);
-    a.seqlen_q = (int32_t)q.size(1);
-    a.seqlen_k = (int32_t)k.size(1);
-    a.num_heads = (int32_t)q.size(2);
-    a.num_heads_kv = (int32_t)k.size(2);
-    a.head_dim = (int32_t)q.size(3);
+    a.batch = i32(q.size(0));
+    a.seqlen_q = i32(q.size(1));
+    a.seqlen_k = i32(k.size(1));
+    a.num_heads = i32(q.size(2));
+    a.num_heads_kv = i32(k.size(2));
+    a.head_dim = i32(q.size(3));
     a.dtype = dtype_code(q.scalar_type());
 }
 
@@ -130,24 +134,73 @@ PyObject* wrap_or_none(const at::Tensor& t) {
     Py_RETURN_NONE;
 }
 
-// scored_fwd(q, k, v, <rules>, stream) -> (status, o, lse)
+// What the Python entry points look at before every call, in one: False sends them
+// to their own checks, which name what is wrong.
+bool element_type(const at::Tensor& t) { return dtype_code(t.scalar_type()) >= 0; }
+
+// qkv_ok(q, k, v, largest head dim)
+PyObject* qkv_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!check_count(n, 4)) return nullptr;
+    const int64_t most = PyLong_AsLongLong(x[3]);
+    if (PyErr_Occurred()) return nullptr;
+    for (int i = 0; i < 3; ++i)
+        if (!THPVariable_Check(x[i]) || THPVariable_Unpack(x[i]).dim() != 4) Py_RETURN_FALSE;
+    const at::Tensor &q = THPVariable_Unpack(x[0]), &k = THPVariable_Unpack(x[1]), &v = THPVariable_Unpack(x[2]);
+    const int64_t H = q.size(2), Hkv = k.size(2), D = q.size(3);
+    const bool ok = q.is_cuda() && k.device() == q.device() && v.device() == q.device() && element_type(q) &&
+                    k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() &&
+                    k.size(0) == q.size(0) && k.size(3) == D && k.sizes() == v.sizes() && Hkv > 0 && H > 0 &&
+                    H % Hkv == 0 && D > 0 && D <= most;
+    return PyBool_FromLong(ok);
+    END_HANDLE_TH_ERRORS
+}
+
+// rotary_ok(q, k or None, table, positions or None): positions of shape (B, S)
+PyObject* rotary_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!check_count(n, 4)) return nullptr;
+    for (int i = 0; i < 4; ++i)
+        if (!THPVariable_Check(x[i]) && !((i & 1) && none(x[i]))) Py_RETURN_FALSE;
+    const at::Tensor &q = THPVariable_Unpack(x[0]), &t = THPVariable_Unpack(x[2]);
+    if (q.dim() != 4 || t.dim() != 2) Py_RETURN_FALSE;
+    const int64_t B = q.size(0), S = q.size(1), D = q.size(3), R = t.size(1);
+    bool ok = q.is_cuda() && element_type(q) && q.size(2) > 0 && D <= 256 && t.device() == q.device() &&
+              t.scalar_type() == at::kFloat && !t.requires_grad() && R >= 2 && R % 2 == 0 && R <= D && t.size(0) > 0;
+    if (ok && !none(x[1])) {
+        const at::Tensor& k = THPVariable_Unpack(x[1]);
+        ok = k.dim() == 4 && k.device() == q.device() && k.scalar_type() == q.scalar_type() && k.size(0) == B &&
+             k.size(1) == S && k.size(2) > 0 && k.size(3) == D;
+    }
+    if (ok && !none(x[3])) {
+        const at::Tensor& p = THPVariable_Unpack(x[3]);
+        ok = p.dim() == 2 && p.size(0) == B && p.size(1) == S && p.device() == q.device() &&
+             (p.scalar_type() == at::kInt || p.scalar_type() == at::kLong);
+    }
+    return PyBool_FromLong(ok);
+    END_HANDLE_TH_ERRORS
+}
+
+// scored_fwd(q, k, v, <rules>, want_lse, stream) -> (status, o, lse or None)
 PyObject* scored_fwd(PyObject*, PyObject* const* x, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (!check_count(n, 3 + kRules + 1) || !bound() || !all_tensors(x, 3)) return nullptr;
+    if (!check_count(n, 3 + kRules + 2) || !bound() || !all_tensors(x, 3)) return nullptr;
     c10::DeviceGuard guard(THPVariable_Unpack(x[0]).device());
     const at::Tensor q = prepare(THPVariable_Unpack(x[0])), k = prepare(THPVariable_Unpack(x[1])),
                      v = prepare(THPVariable_Unpack(x[2]));
     fa_scored_args a = {};
     Held h;
     if (!put_rules(a, h, x + 3)) return nullptr;
-    void* const stream = PyLong_AsVoidPtr(x[3 + kRules]);
+    const bool want = PyObject_IsTrue(x[3 + kRules]) == 1;
+    void* const stream = PyLong_AsVoidPtr(x[3 + kRules + 1]);
     if (PyErr_Occurred()) return nullptr;
     put_sizes(a, q, k, v);
     const at::Tensor o = at::empty(q.sizes(), q.options());
-    const at::Tensor lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    const at::Tensor lse =
+        want ? at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat)) : at::Tensor();
     a.o = o.data_ptr();
     put_strides(a.o_stride, o);
-    a.lse = (float*)lse.data_ptr();
+    a.lse = (float*)ptr(lse);
     const size_t bytes = p_fwd_size(&a);
     const at::Tensor ws = workspace(bytes, q);
     int32_t st;
@@ -155,7 +208,7 @@ PyObject* scored_fwd(PyObject*, PyObject* const* x, Py_ssize_t n) {
         pybind11::gil_scoped_release no_gil;
         st = p_fwd(&a, ptr(ws), bytes, stream);
     }
-    return Py_BuildValue("(iNN)", (int)st, THPVariable_Wrap(o), THPVariable_Wrap(lse));
+    return Py_BuildValue("(iNN)", (int)st, THPVariable_Wrap(o), wrap_or_none(lse));
     END_HANDLE_TH_ERRORS
 }
 
@@ -233,13 +286,13 @@ PyObject* prefix_fwd(PyObject*, PyObject* const* x, Py_ssize_t n) {
     }
     put_strides(a.k_stride, t[3]);
     put_strides(a.v_stride, t[4]);
-    a.batch = (int32_t)q.size(0);
-    a.seqlen_q = (int32_t)q.size(1);
-    a.prefix_len = (int32_t)t[1].size(0);
-    a.seqlen_k = (int32_t)t[3].size(1);
-    a.num_heads = (int32_t)q.size(2);
-    a.num_heads_kv = (int32_t)t[3].size(2);
-    a.head_dim = (int32_t)q.size(3);
+    a.batch = i32(q.size(0));
+    a.seqlen_q = i32(q.size(1));
+    a.prefix_len = i32(t[1].size(0));
+    a.seqlen_k = i32(t[3].size(1));
+    a.num_heads = i32(q.size(2));
+    a.num_heads_kv = i32(t[3].size(2));
+    a.head_dim = i32(q.size(3));
     a.dtype = dtype_code(q.scalar_type());
     const at::Tensor o = at::empty(q.sizes(), q.options());
     const at::Tensor lse =
@@ -291,11 +344,11 @@ PyObject* rotary(PyObject*, PyObject* const* x, Py_ssize_t n) {
         a.k_out = ko.data_ptr();
         strides(a.k_stride, k);
         strides(a.k_out_stride, ko);
-        a.num_heads_k = (int32_t)k.size(2);
+        a.num_heads_k = i32(k.size(2));
     }
     a.table = (const float*)table.data_ptr();
     a.table_positions = table.size(0);
-    a.rotary_dim = (int32_t)table.size(1);
+    a.rotary_dim = i32(table.size(1));
     if (!none(x[3])) {
         const at::Tensor& p = THPVariable_Unpack(x[3]);  // (B, S), int32 or int64
         a.positions = p.data_ptr();
@@ -307,10 +360,10 @@ PyObject* rotary(PyObject*, PyObject* const* x, Py_ssize_t n) {
     a.inverse = PyObject_IsTrue(x[5]);
     void* const stream = PyLong_AsVoidPtr(x[7]);
     if (PyErr_Occurred()) return nullptr;
-    a.batch = (int32_t)q.size(0);
-    a.seqlen = (int32_t)q.size(1);
-    a.num_heads = (int32_t)q.size(2);
-    a.head_dim = (int32_t)q.size(3);
+    a.batch = i32(q.size(0));
+    a.seqlen = i32(q.size(1));
+    a.num_heads = i32(q.size(2));
+    a.head_dim = i32(q.size(3));
     a.dtype = dtype_code(q.scalar_type());
     int32_t st;
     {
@@ -384,6 +437,8 @@ PyObject* bind_ops(PyObject*, PyObject* const* x, Py_ssize_t n) {
 
 PyMethodDef fa_host::ops_methods[] = {
     {"bind_ops", (PyCFunction)(void*)bind_ops, METH_FASTCALL, nullptr},
+    {"qkv_ok", (PyCFunction)(void*)qkv_ok, METH_FASTCALL, nullptr},
+    {"rotary_ok", (PyCFunction)(void*)rotary_ok, METH_FASTCALL, nullptr},
     {"scored_fwd", (PyCFunction)(void*)scored_fwd, METH_FASTCALL, nullptr},
     {"scored_bwd", (PyCFunction)(void*)scored_bwd, METH_FASTCALL, nullptr},
     {"prefix_fwd", (PyCFunction)(void*)prefix_fwd, METH_FASTCALL, nullptr},

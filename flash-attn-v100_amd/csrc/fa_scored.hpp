@@ -619,7 +619,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
     const ScoredParams& pe = late_args();
     const float l_tot = pair_sum(l_run);
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
-    if (sp == 0 && hi == 0 && qi < p.Sq)
+    if (pe.lse && sp == 0 && hi == 0 && qi < p.Sq)
         pe.lse[(int64_t)(b * pe.H + h) * pe.Sq + qi] =
             l_tot > 0.f ? (m_run + __log2f(l_tot)) * kLn2 : l_tot == 0.f ? -INFINITY : l_tot;
     store_rows<T, D>(smem + w * 32 * C::OW, C::OW, o, inv, (T*)pe.o + b * pe.o_sb + h * pe.o_sh, pe.o_ss,

@@ -5,7 +5,7 @@ prefix, rotary positions.  Same library, host module, status codes and errors as
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -119,28 +119,28 @@ def padded(d: int, dtype: torch.dtype) -> int:
     return -(-d // n) * n
 
 
-class Rules:
+class Rules(NamedTuple):
     """The rules of a scored attention call, in the order the host module takes them."""
 
-    __slots__ = ("causal", "scale", "softcap", "slopes", "prefix", "lens", "offsets", "offset0", "q_docs", "k_docs")
+    causal: bool
+    scale: float
+    softcap: float
+    slopes: Optional[torch.Tensor]
+    prefix: Optional[torch.Tensor]
+    lens: Optional[torch.Tensor]
+    offsets: Optional[torch.Tensor]
+    offset0: int
+    q_docs: Optional[torch.Tensor]
+    k_docs: Optional[torch.Tensor]
 
-    def __init__(self, causal, scale, softcap, slopes, prefix, lens, offsets, offset0, q_docs, k_docs):
-        self.causal, self.scale, self.softcap, self.slopes = causal, scale, softcap, slopes
-        self.prefix, self.lens, self.offsets, self.offset0 = prefix, lens, offsets, offset0
-        self.q_docs, self.k_docs = q_docs, k_docs
 
-    def tuple(self):
-        return (self.causal, self.scale, self.softcap, self.slopes, self.prefix, self.lens, self.offsets, self.offset0,
-                self.q_docs, self.k_docs)
-
-
-def scored_fwd(q, k, v, rules: Rules):
-    """(o, lse) of ``fa_scored_fwd``; checked tensors."""
+def scored_fwd(q, k, v, rules: Rules, want_lse: bool = True):
+    """(o, lse or None) of ``fa_scored_fwd``; checked tensors."""
     D = q.shape[-1]
     dp = padded(D, q.dtype)
     if dp != D:
         q, k, v = (_lib._pad_d(t, dp) for t in (q, k, v))
-    st, o, lse = host().scored_fwd(q, k, v, *rules.tuple(), _lib._raw_stream(q))
+    st, o, lse = host().scored_fwd(q, k, v, *rules, want_lse, _lib._raw_stream(q))
     if st:
         _lib._check("fa_scored_fwd", st)
     return _lib._unpad_d(o, D), lse
@@ -152,7 +152,7 @@ def scored_bwd(q, k, v, o, do, lse, rules: Rules, want_dslopes: bool):
     dp = padded(D, q.dtype)
     if dp != D:
         q, k, v, o, do = (_lib._pad_d(t, dp) for t in (q, k, v, o, do))
-    st, dq, dk, dv, ds = host().scored_bwd(q, k, v, o, do, lse, *rules.tuple(), want_dslopes, _lib._raw_stream(q))
+    st, dq, dk, dv, ds = host().scored_bwd(q, k, v, o, do, lse, *rules, want_dslopes, _lib._raw_stream(q))
     if st:
         _lib._check("fa_scored_bwd", st)
     if dp != D:

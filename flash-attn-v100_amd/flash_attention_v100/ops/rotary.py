@@ -121,25 +121,8 @@ def _disjoint(q: torch.Tensor, k: torch.Tensor) -> bool:
     return not _overlaps((*first.shape[:2], gap // sh + last.shape[2], first.shape[3]), (*first.stride()[:2], sh, 1))
 
 
-def rotary_embedding_v100(
-    q: torch.Tensor,
-    k: Optional[torch.Tensor],
-    table: torch.Tensor,
-    positions: Optional[torch.Tensor] = None,
-    *,
-    interleaved: bool = False,
-    inplace: bool = False,
-) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
-    """q (B, S, H, D) and k (B, S, Hkv, D) with their first ``table.shape[1]``
-    columns rotated: (q', k'), or q' alone for ``k`` None; in one launch.
-
-    ``table`` from :func:`rotary_table_v100`.  ``positions``: int32 or int64
-    (B, S) or (S,), 0 .. S - 1 by default; read on the GPU only: a token at a
-    negative position is left as it is, one at a position past the table becomes
-    NaN.  ``inplace`` writes into q and k and returns them (refused for inputs
-    that require grad while grad mode is on, and for inputs whose elements
-    overlap).  Differentiable in q and k.
-    """
+def _check_inputs(q, k, table, positions):
+    """Raises for what the rotation does not take; positions as (B, S)."""
     for name, t in (("q", q), ("k", k)):
         if t is None and name == "k":
             continue
@@ -173,12 +156,36 @@ def rotary_embedding_v100(
         if positions.device != q.device:
             raise ValueError(f"positions must be on {q.device}, got {positions.device}")
         positions = positions.expand(B, S)
+    return positions
+
+
+def rotary_embedding_v100(
+    q: torch.Tensor,
+    k: Optional[torch.Tensor],
+    table: torch.Tensor,
+    positions: Optional[torch.Tensor] = None,
+    *,
+    interleaved: bool = False,
+    inplace: bool = False,
+) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """q (B, S, H, D) and k (B, S, Hkv, D) with their first ``table.shape[1]``
+    columns rotated: (q', k'), or q' alone for ``k`` None; in one launch.
+
+    ``table`` from :func:`rotary_table_v100`.  ``positions``: int32 or int64
+    (B, S) or (S,), 0 .. S - 1 by default; read on the GPU only: a token at a
+    negative position is left as it is, one at a position past the table becomes
+    NaN.  ``inplace`` writes into q and k and returns them (refused for inputs
+    that require grad while grad mode is on, and for inputs whose elements
+    overlap).  Differentiable in q and k.
+    """
+    if not _ops.host().rotary_ok(q, k, table, positions):
+        positions = _check_inputs(q, k, table, positions)
     grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
     if inplace:
         if grad:
             raise ValueError("inplace=True on inputs that require grad: call it under torch.no_grad()")
         for name, t in (("q", q), ("k", k)):
-            if t is not None and ((D > 1 and t.stride(3) != 1) or _overlaps(t.shape, t.stride())):
+            if t is not None and ((t.shape[3] > 1 and t.stride(3) != 1) or _overlaps(t.shape, t.stride())):
                 raise ValueError(f"inplace=True needs a {name} with unit column stride and no overlapping elements")
         if k is not None and not _disjoint(q, k):
             raise ValueError("inplace=True needs a q and k that share no element")

@@ -30,6 +30,8 @@ SUPPORTED_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
 def check_qkv(q, k, v, what: str) -> None:
     """Shapes, dtypes and devices of q (B, Sq, H, D) and k, v (B, Sk, Hkv, D)."""
+    if _ops.host().qkv_ok(q, k, v, _ops.MAX_HEAD_DIM):
+        return
     for t in (q, k, v):
         if not isinstance(t, torch.Tensor):
             raise TypeError("q, k, v must be torch.Tensor instances")
@@ -57,7 +59,9 @@ def check_scale(scale: Optional[float], D: int) -> float:
 
 
 def check_softcap(softcap: Optional[float]) -> float:
-    c = 0.0 if softcap is None else float(softcap)
+    if softcap is None:
+        return 0.0
+    c = float(softcap)
     # below 2^-60 or so the cap's constants would leave the range of float32
     if not math.isfinite(c) or c < 0 or (0 < c < 1e-6) or c > 1e30:
         raise ValueError(f"softcap must be 0 (none) or within [1e-6, 1e30], got {softcap}")
@@ -165,11 +169,15 @@ def flash_attention_v100_scored(
     Sk = k.shape[1]
     scale = check_scale(scale, D)
     softcap = check_softcap(softcap)
-    slopes = check_slopes(distance_slopes, B, H, q.device)
-    prefix = _ops.optional_lengths(prefix_lengths, "prefix_lengths", B, q.device)
-    if prefix is not None and not causal:
-        raise ValueError("prefix_lengths needs causal=True (without it every key is seen)")
-    lens = _ops.optional_lengths(key_lengths, "key_lengths", B, q.device)
+    slopes = prefix = lens = None
+    if distance_slopes is not None:
+        slopes = check_slopes(distance_slopes, B, H, q.device)
+    if prefix_lengths is not None:
+        prefix = _ops.optional_lengths(prefix_lengths, "prefix_lengths", B, q.device)
+        if not causal:
+            raise ValueError("prefix_lengths needs causal=True (without it every key is seen)")
+    if key_lengths is not None:
+        lens = _ops.optional_lengths(key_lengths, "key_lengths", B, q.device)
     offsets, offset0 = None, 0
     if isinstance(query_offsets, torch.Tensor):
         offsets = _ops.optional_lengths(query_offsets, "query_offsets", B, q.device)
@@ -197,7 +205,7 @@ def flash_attention_v100_scored(
         out = ScoredAttentionFunction.apply(q, k, v, slopes, rules, return_softmax_lse)
         o, lse = out if return_softmax_lse else (out, None)
     else:
-        o, lse = _ops.scored_fwd(q, k, v, rules)
+        o, lse = _ops.scored_fwd(q, k, v, rules, return_softmax_lse)
     if DebugConfig.VALIDATE_OUTPUTS:
         check_tensor_nan_inf(o, "output")
     return (o, lse) if return_softmax_lse else o

@@ -42,7 +42,7 @@ typedef struct fa_scored_args {
     const void* k;
     const void* v;
     void* o;
-    float* lse;                    /* (B, H, Sq) contiguous; written by the forward, read by the backward */
+    float* lse;                    /* (B, H, Sq) contiguous; optional in the forward, read by the backward */
     const void* dout;              /* backward only, as the five below */
     void* dq;
     void* dk;

@@ -304,3 +304,12 @@ def test_gradients_against_differences():
         tol = 2.0 ** -18 * (got[name].double().abs() * step.abs()).sum().item() + 1e-7 * abs(num) + 1e-7
         print(f"{name}: {ana:.8f} against {num:.8f}, tolerance {tol:.2e}", flush=True)
         assert abs(num - ana) <= tol
+
+
+@pytest.mark.parametrize("Sq", [1, 20, 200])
+def test_without_lse(Sq):
+    q, k, v, _ = make(2, Sq, 200, 4, 2, 64, "bf16", seed=12)
+    for kw in (dict(causal=True), dict(softcap=9.0, documents=torch.zeros(Sq, dtype=torch.int32, device=DEV),
+                                       key_documents=torch.zeros(200, dtype=torch.int32, device=DEV))):
+        o, lse = fa.flash_attention_v100_scored(q, k, v, return_softmax_lse=True, **kw)
+        assert torch.equal(fa.flash_attention_v100_scored(q, k, v, **kw), o) and lse.shape == (2, 4, Sq)

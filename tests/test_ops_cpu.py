@@ -97,7 +97,7 @@ SCORED_BAD = [
     ("FA_ERR_RULE", with_(slopes=ADDR, slopes_batch_stride=3)), ("FA_ERR_ALIGN", with_(slopes=ADDR + 2)),
     ("FA_ERR_RULE", with_(q_documents=ADDR)), ("FA_ERR_RULE", with_(k_documents=ADDR)),
     ("FA_ERR_RULE", with_(q_documents=ADDR, k_documents=ADDR, k_documents_stride=-1)),
-    ("FA_ERR_ALIGN", with_(key_lengths=ADDR + 1)), ("FA_ERR_NULL_ARG", with_(q=None)), ("FA_ERR_NULL_ARG", with_(lse=None)),
+    ("FA_ERR_ALIGN", with_(key_lengths=ADDR + 1)), ("FA_ERR_NULL_ARG", with_(q=None)),
     ("FA_ERR_NULL_ARG", with_(v=None)), ("FA_ERR_ALIGN", with_(k=ADDR + 8)), ("FA_ERR_ALIGN", with_(lse=ADDR + 2)),
     ("FA_ERR_STRIDE", with_stride("q_stride", 3, 2)), ("FA_ERR_STRIDE", with_stride("v_stride", 1, 65)),
     ("FA_ERR_STRIDE", with_stride("o_stride", 0, -64)), ("FA_ERR_TOO_LARGE", with_stride("k_stride", 0, 1 << 62)),
@@ -121,7 +121,7 @@ def test_scored_refusals(i):
 
 def test_scored_backward_refusals():
     lib = _ops.load()
-    for code, change in (("FA_ERR_NULL_ARG", with_(dout=None)), ("FA_ERR_NULL_ARG", with_(dk=None)),
+    for code, change in (("FA_ERR_NULL_ARG", with_(dout=None)), ("FA_ERR_NULL_ARG", with_(lse=None)), ("FA_ERR_NULL_ARG", with_(dk=None)),
                          ("FA_ERR_STRIDE", with_stride("dv_stride", 2, 63)), ("FA_ERR_RULE", with_(dslopes=ADDR)),
                          ("FA_ERR_ALIGN", with_(slopes=ADDR, dslopes=ADDR + 2))):
         a = scored_args()
