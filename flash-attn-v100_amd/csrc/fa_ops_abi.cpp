@@ -166,8 +166,15 @@ void plan_rows(RowsParams& p, int32_t dtype) {
     const int64_t rows = (int64_t)p.Sq * p.group;
     p.p_unit = rows * p.B > 64 ? 128 : 32;
     p.o_rt = (int)ceil_div<int64_t>(rows, 32);
-    p.p_rt = p.P > 0 ? (int)ceil_div<int64_t>(rows * p.B, p.p_unit) : 0;
-    const int64_t ou = (int64_t)p.B * p.Hkv * p.o_rt, pu = (int64_t)p.Hkv * p.p_rt;
+    const int64_t ou = (int64_t)p.B * p.Hkv * p.o_rt;
+    // A short prefix before short sequences: one walk over both costs less than a
+    // second launch to join two.  (sequences, KV heads, prefix + own keys), one walk
+    // against two in us: (4, 8, 300 + 40) 7.7 / 11.2; (32, 8, 500 + 100) 12.8 / 17.2;
+    // (64, 8, 400 + 100) 17.6 / 22.0; (4, 8, 900 + 100) 16.2 / 15.3; (16, 8, 1900 +
+    // 100) 24.4 / 16.2
+    p.joined = p.P > 0 && ou <= 512 && (int64_t)p.P + p.Sk <= 640;
+    p.p_rt = p.P > 0 && !p.joined ? (int)ceil_div<int64_t>(rows * p.B, p.p_unit) : 0;
+    const int64_t pu = (int64_t)p.Hkv * p.p_rt;
     const int64_t ont = ceil_div<int64_t>(p.Sk, 64), pnt = ceil_div<int64_t>(p.P, 64);
     // As many splits as fill the device once, but none below 4 steps of a workgroup
     // (a step is 128 keys in a unit of 32 rows, 64 keys in one of 128), whose part
@@ -177,7 +184,7 @@ void plan_rows(RowsParams& p, int32_t dtype) {
     auto splits = [&](int64_t nt, int64_t least) {
         return (int)std::max<int64_t>(1, std::min<int64_t>(64, ceil_div(nt, std::max<int64_t>(chunk, least))));
     };
-    p.o_splits = splits(ont, 8);
+    p.o_splits = p.joined ? 1 : splits(ont, 8);
     p.p_splits = pu ? splits(pnt, p.p_unit == 128 ? 4 : 8) : 0;
     p.p_wgs = pu * p.p_splits;
     p.o_wgs = ou * p.o_splits;

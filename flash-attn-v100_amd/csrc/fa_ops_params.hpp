@@ -101,6 +101,9 @@ struct RowsParams {
     // parts: the prefix keys go to p_splits workgroups for each unit of p_unit rows
     // (p_rt units a KV head), a sequence's own to o_splits (o_rt units of 32)
     int p_splits, p_rt, p_unit, o_splits, o_rt;
+    // the units of a sequence's own keys walk the prefix too, and nothing is joined
+    // (p_splits = 0)
+    int joined;
     int64_t p_wgs, o_wgs;
     int64_t p_rows;      // part rows of the prefix, p_wgs p_unit
     float2* stat;        // per part row: maximum (log2 units), sum

@@ -84,7 +84,8 @@ __device__ FA_INLINE inline void row_rules(f32x16& s, const RowsParams& p, Cap<F
 }
 
 // 32 rows over split `split` of the keys [0, n_keys) (a sequence's own ones, or a
-// prefix that few rows read): each wave walks tiles of its own
+// prefix that few rows read; p.joined: the prefix, then the own ones): each wave
+// walks tiles of its own
 template <typename T, int D>
 __device__ FA_INLINE inline void unit32(const RowsParams& p, bool pre, T* smem, float (*stat)[2][32], int id, int lane, int w) {
     using C = RowsCfg<T, D>;
@@ -103,7 +104,11 @@ __device__ FA_INLINE inline void unit32(const RowsParams& p, bool pre, T* smem, 
     }
     lim_max = __builtin_amdgcn_readfirstlane(lim_max);
     lim_min = __builtin_amdgcn_readfirstlane(lim_min);
-    const int n_keys = max(lim_max, 0), nt = (n_keys + BN - 1) / BN;
+    const int n_keys = max(lim_max, 0);
+    // tiles of the prefix before the own ones (a row that sees any key sees the
+    // prefix and a key of its own)
+    const int pt = p.joined && n_keys > 0 ? (p.P + BN - 1) / BN : 0;
+    const int nt = pt + (n_keys + BN - 1) / BN;
     const int t0 = (int)((int64_t)nt * split / splits), t1 = (int)((int64_t)nt * (split + 1) / splits);
 
     const int64_t k_ss = pre ? p.kp_ss : p.k_ss, v_ss = pre ? p.vp_ss : p.v_ss;
@@ -118,19 +123,29 @@ __device__ FA_INLINE inline void unit32(const RowsParams& p, bool pre, T* smem, 
     constexpr int NKI = decltype(kd)::NI, NVI = decltype(vd)::NI;
     // tiles past the split's end read nothing but are issued, so that the vmcnt
     // counts stay exact (float32 tiles are copied and waited for one by one)
-    auto copy_k = [&](int t) FA_INLINE {
-        const int nv = t < t1 ? n_keys - t * BN : 0;
+    DmaTile<T, BN, D, KW, 1> kpd;  // rows of the prefix, before own ones
+    kpd.init(p.kp_ss, lane, 0, p.cols);
+    DmaTile<T, BN, D, VW, 1> vpd;
+    vpd.init(p.vp_ss, lane, 0, p.cols);
+    auto copy = [&](auto& tile, const T* base, int64_t ss, int k0, int nv, T* dst) FA_INLINE {
         if constexpr (C::F32)
-            kd.load(kbase + (int64_t)(t * BN) * k_ss, k_ss, nv, Ks, lane);
+            tile.load(base + (int64_t)k0 * ss, ss, nv, dst, lane);
         else
-            kd.load_untracked(kbase + (int64_t)(t * BN) * k_ss, k_ss, nv, Ks, lane);
+            tile.load_untracked(base + (int64_t)k0 * ss, ss, nv, dst, lane);
+    };
+    auto copy_k = [&](int t) FA_INLINE {
+        const int k0 = (t < pt ? t : t - pt) * BN;
+        if (t < pt)
+            copy(kpd, (const T*)p.kp + hk * p.kp_sh, p.kp_ss, k0, t < t1 ? p.P - k0 : 0, Ks);
+        else
+            copy(kd, kbase, k_ss, k0, t < t1 ? n_keys - k0 : 0, Ks);
     };
     auto copy_v = [&](int t) FA_INLINE {
-        const int nv = t < t1 ? n_keys - t * BN : 0;
-        if constexpr (C::F32)
-            vd.load(vbase + (int64_t)(t * BN) * v_ss, v_ss, nv, Vs, lane);
+        const int k0 = (t < pt ? t : t - pt) * BN;
+        if (t < pt)
+            copy(vpd, (const T*)p.vp + hk * p.vp_sh, p.vp_ss, k0, t < t1 ? p.P - k0 : 0, Vs);
         else
-            vd.load_untracked(vbase + (int64_t)(t * BN) * v_ss, v_ss, nv, Vs, lane);
+            copy(vd, vbase, v_ss, k0, t < t1 ? n_keys - k0 : 0, Vs);
     };
 
     constexpr int QR = C::F32 ? D / 8 : D / 16;
@@ -158,7 +173,8 @@ __device__ FA_INLINE inline void unit32(const RowsParams& p, bool pre, T* smem, 
     copy_k(t);
     copy_v(t);
     for (; t < t1; t += NW) {
-        const int k0 = t * BN;
+        const bool first = t < pt;
+        const int k0 = (first ? t : t - pt) * BN;
         // ---- S^T = K Q^T ----
         if constexpr (C::F32)
             wait_vmem();
@@ -182,10 +198,10 @@ __device__ FA_INLINE inline void unit32(const RowsParams& p, bool pre, T* smem, 
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K(t) read before it is overwritten
         if constexpr (!C::F32) copy_k(t + NW);
 
-        row_rules(s, p, cap, slope, slope2, row.qpos - (float)(k0 + 4 * hi));
-        if (k0 + BN > lim_min) {
+        row_rules(s, p, cap, slope, slope2, row.qpos - (float)(k0 - (first ? p.P : 0) + 4 * hi));
+        if (k0 + BN > (first && lim_min > 0 ? p.P : lim_min)) {
             stay_branch();
-            const int lm = row.lim - k0 - 4 * hi;
+            const int lm = (first && row.lim > 0 ? p.P : row.lim) - k0 - 4 * hi;
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 if (8 * (e >> 2) + (e & 3) >= lm) s[e] = -INFINITY;

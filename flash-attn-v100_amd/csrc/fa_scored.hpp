@@ -1372,16 +1372,28 @@ __global__ __launch_bounds__(256) void kv_sum_kernel(const ScoredParams p, const
 
 // ---------------------------------------------------------------------------
 // launchers (instantiated in fa_scored_{fwd,bwd}_*.hip)
+// Grids whose blocks get two groups of waves (a workgroup of 512 threads a CU), each
+// on every other tile, so that the longest walk takes half: those of fewer
+// workgroups than CUs, and causal ones of at most two workgroups a CU, whose last
+// blocks' walks are the time.  Forward / backward us, one group against two:
+//   2 x 1777, 12 heads of 64, slopes: 40 / 113, 34 / 104 (336 workgroups)
+//   1 x 4096, 16 heads of 128: 101 / 326, 88 / 309 (512)
+//   2 x 1777, 12 heads of 64 in float32: 181 / 448, 140 / 395 (336)
+//   2 x 2304, 16 heads of 64: 43 / 122, 49 / 131 (576)
+//   1 x 4096, 16 heads of 128, documents: 37 / 143, 47 / 151 (512, short walks)
+//   2 x 1536, 11 heads of 64, not causal: 35 / 98, 45 / 109 (264)
+inline bool two_groups(const ScoredParams& p, int64_t nb, int tile) {
+    return p.Sk > tile && nb < (p.causal && !p.q_docs ? 513 : 256);
+}
 template <typename T, int D, bool CAP, bool SLOPE>
 hipError_t launch_scored_fwd_t(ScoredParams p, hipStream_t s) {
     using C = FwdCfg<T, D>;
     p.n_tiles = (p.Sq + C::BM - 1) / C::BM;
     const int64_t nb = (int64_t)p.n_tiles * p.H * p.B;
     if (nb <= 0) return hipSuccess;
-    // grids of fewer workgroups than CUs: two groups of waves share a block's
-    // keys (fp32 tiles of head dim 128 take the whole LDS)
+    // (fp32 tiles of head dim 128 take the whole LDS)
     if constexpr (!(C::F32 && D == 128)) {
-        if (nb < 256 && p.Sk > C::BN) {
+        if (two_groups(p, nb, C::BN)) {
             hipLaunchKernelGGL((scored_fwd_kernel<T, D, CAP, SLOPE, 2>), dim3((unsigned)nb), dim3(512), 0, s, p);
             return hipGetLastError();
         }
@@ -1396,10 +1408,8 @@ hipError_t launch_scored_bwd_t(ScoredParams p, hipStream_t s) {
     using CK = DkdvCfg<T, D>;
     p.n_tiles = (p.Sq + CQ::BM - 1) / CQ::BM;
     const int64_t nq = (int64_t)p.n_tiles * p.H * p.B;
-    // as the forward (1 x 2048, 8 on 2 heads of 128, cap: backward 316 -> 303 us;
-    // 2 x 1024, 12 heads of 64, cap: 72 -> 69 us)
     constexpr bool kTwo = !(CQ::F32 && D == 128);
-    const int ks = kTwo && nq < 256 && p.Sk > CQ::BN ? 2 : 1;
+    const int ks = kTwo && two_groups(p, nq, CQ::BN) ? 2 : 1;
     auto dq = [&](auto dslope, auto two) {
         hipLaunchKernelGGL((scored_dq_kernel<T, D, CAP, SLOPE, decltype(dslope)::value, decltype(two)::value ? 2 : 1>),
                            dim3((unsigned)nq), dim3(256 * ks), 0, s, p);

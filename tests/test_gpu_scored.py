@@ -313,3 +313,24 @@ def test_without_lse(Sq):
                                        key_documents=torch.zeros(200, dtype=torch.int32, device=DEV))):
         o, lse = fa.flash_attention_v100_scored(q, k, v, return_softmax_lse=True, **kw)
         assert torch.equal(fa.flash_attention_v100_scored(q, k, v, **kw), o) and lse.shape == (2, 4, Sq)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("rule", ["none", "cap", "slopes", "cap+slopes", "docs", "prefix", "all keys"])
+def test_rules_on_larger_grids(rule, D, dt):
+    # 600 blocks of queries and of keys: one group of waves each, no parts
+    B, S, H, Hkv = 5, 500, 30, 30
+    q, k, v, do = make(B, S, S, H, Hkv, D, dt, seed=D)
+    kw = dict(causal=rule != "all keys")
+    if "cap" in rule:
+        kw["softcap"] = 5.0
+    if "slopes" in rule:
+        kw["distance_slopes"] = slopes_for(H)
+    if rule == "docs":
+        kw["documents"] = packed(B, S, [97, 230, 14], pad=9)
+    if rule == "prefix":
+        kw["prefix_lengths"] = torch.tensor([0, 60, 129, 500, 3], device=DEV, dtype=torch.int32)
+        kw["key_lengths"] = torch.tensor([500, 490, 200, 500, 1], device=DEV, dtype=torch.int32)
+    got, ref, names, _ = run(q, k, v, do, **kw)
+    oo.check(got, ref, names, f"{rule} {dt} {D}")

@@ -112,3 +112,21 @@ def test_refuses_gradients():
         fa.flash_attention_v100_shared_prefix(*t)
     with torch.no_grad():
         assert not fa.flash_attention_v100_shared_prefix(*t).requires_grad
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("B,Sq", [(3, 1), (33, 1), (9, 5)])
+def test_long_prefixes(dt, D, B, Sq):
+    # units of 32 and of 128 rows over several parts of a prefix that ends inside a
+    # tile, free slots among them
+    P, Sk, H, Hkv = 1500, 70, 8, 2
+    t = make(B, Sq, P, Sk, H, Hkv, D, dt, seed=21)
+    lens = torch.randint(0, Sk + 1, (B,), generator=torch.Generator("cpu").manual_seed(2)).to(DEV)
+    lens[B // 2] = 0
+    for b in range(B):
+        t[3][b, int(lens[b]):] = math.nan
+    g = torch.Generator("cpu").manual_seed(3)
+    slopes = (0.02 * torch.rand(B, H, generator=g)).to(DEV)
+    run(t, lens, f"{dt} {D} {B}x{Sq}")
+    run(t, lens, f"{dt} {D} {B}x{Sq} cap, slopes", softcap=12.0, distance_slopes=slopes)

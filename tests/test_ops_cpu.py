@@ -182,7 +182,7 @@ def test_prefix_refusals():
         change(a)
         assert lib.fa_prefix_check(ctypes.byref(a)) == CODES[code], code
         assert lib.fa_prefix_fwd(ctypes.byref(a), None, 0, None) == CODES[code], code
-    a = prefix_args()
+    a = prefix_args(P=5000)
     need = lib.fa_prefix_workspace_size(ctypes.byref(a))
     assert need > 0 and lib.fa_prefix_fwd(ctypes.byref(a), ADDR, need - 1, None) == CODES["FA_ERR_WORKSPACE"]
     a = prefix_args(B=0)
