@@ -1391,12 +1391,9 @@ hipError_t launch_scored_fwd_t(ScoredParams p, hipStream_t s) {
     p.n_tiles = (p.Sq + C::BM - 1) / C::BM;
     const int64_t nb = (int64_t)p.n_tiles * p.H * p.B;
     if (nb <= 0) return hipSuccess;
-    // (fp32 tiles of head dim 128 take the whole LDS)
-    if constexpr (!(C::F32 && D == 128)) {
-        if (two_groups(p, nb, C::BN)) {
-            hipLaunchKernelGGL((scored_fwd_kernel<T, D, CAP, SLOPE, 2>), dim3((unsigned)nb), dim3(512), 0, s, p);
-            return hipGetLastError();
-        }
+    if (two_groups(p, nb, C::BN)) {
+        hipLaunchKernelGGL((scored_fwd_kernel<T, D, CAP, SLOPE, 2>), dim3((unsigned)nb), dim3(512), 0, s, p);
+        return hipGetLastError();
     }
     hipLaunchKernelGGL((scored_fwd_kernel<T, D, CAP, SLOPE, 1>), dim3((unsigned)nb), dim3(256), 0, s, p);
     return hipGetLastError();
@@ -1408,7 +1405,7 @@ hipError_t launch_scored_bwd_t(ScoredParams p, hipStream_t s) {
     using CK = DkdvCfg<T, D>;
     p.n_tiles = (p.Sq + CQ::BM - 1) / CQ::BM;
     const int64_t nq = (int64_t)p.n_tiles * p.H * p.B;
-    constexpr bool kTwo = !(CQ::F32 && D == 128);
+    constexpr bool kTwo = !(CQ::F32 && D == 128);  // (whose tiles take the whole LDS)
     const int ks = kTwo && two_groups(p, nq, CQ::BN) ? 2 : 1;
     auto dq = [&](auto dslope, auto two) {
         hipLaunchKernelGGL((scored_dq_kernel<T, D, CAP, SLOPE, decltype(dslope)::value, decltype(two)::value ? 2 : 1>),
