@@ -513,19 +513,36 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p, cons
     const int64_t obase = p.p_rows + (((int64_t)b * p.Hkv + hk) * p.o_rt + (ig >> 5)) * p.o_splits * 32 + (ig & 31);
     const int n = p.p_splits + p.o_splits;
     auto part_row = [&](int x) FA_INLINE { return x < p.p_splits ? pbase + (int64_t)U * x : obase + 32 * (int64_t)(x - p.p_splits); };
-    float mm = -1e30f;
-    for (int x = g; x < n; x += G) mm = fmaxf(mm, p.stat[part_row(x)].x);
-    float l_tot = 0.f;
+    float mm = -1e30f, l_tot = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int x = g; x < n; x += G) {
-        const int64_t pr = part_row(x);
-        const float2 st = p.stat[pr];
-        const float a = fast_exp2(st.x - mm);
-        l_tot = __builtin_fmaf(st.y, a, l_tot);
-        const f32x4 v = *reinterpret_cast<const f32x4*>(p.part + pr * D + col);
+    // four parts at a time, whose loads wait for nothing
+    for (int x0 = g; x0 < n; x0 += 4 * G) {
+        float2 st[4];
+        f32x4 v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[e], a, acc[e]);
+        for (int j = 0; j < 4; ++j) {
+            const bool in = x0 + j * G < n;
+            const int64_t pr = part_row(in ? x0 + j * G : x0);
+            st[j] = p.stat[pr];
+            v[j] = *reinterpret_cast<const f32x4*>(p.part + pr * D + col);
+            if (!in) {
+                st[j] = make_float2(-1e30f, 0.f);
+                v[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+        const float m0 = fmaxf(mm, fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)));
+        const float a0 = fast_exp2(mm - m0);
+        l_tot *= a0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] *= a0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float a = fast_exp2(st[j].x - m0);
+            l_tot = __builtin_fmaf(st[j].y, a, l_tot);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[j][e], a, acc[e]);
+        }
+        mm = m0;
     }
     if (G > 1) {
         if (col == 0) {
