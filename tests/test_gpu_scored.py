@@ -334,3 +334,15 @@ def test_rules_on_larger_grids(rule, D, dt):
         kw["key_lengths"] = torch.tensor([500, 490, 200, 500, 1], device=DEV, dtype=torch.int32)
     got, ref, names, _ = run(q, k, v, do, **kw)
     oo.check(got, ref, names, f"{rule} {dt} {D}")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("B,Sq,Sk,H,Hkv,D", [(1, 100, 900, 8, 2, 128), (2, 33, 400, 6, 1, 64), (1, 300, 1300, 4, 4, 32),
+                                             (40, 20, 90, 6, 2, 64)])
+def test_chunks_over_a_cache(B, Sq, Sk, H, Hkv, D, dt):
+    # many queries at the end of longer caches, filled to different lengths
+    q, k, v, _ = make(B, Sq, Sk, H, Hkv, D, dt, seed=Sq)
+    lens = torch.randint(Sq // 2, Sk + 1, (B,), generator=torch.Generator("cpu").manual_seed(Sq)).to(DEV)
+    for kw in (dict(causal=True), dict(), dict(causal=True, softcap=7.0, distance_slopes=slopes_for(H))):
+        got, ref, names, _ = run(q, k, v, None, False, key_lengths=lens, query_offsets=lens - Sq, **kw)
+        oo.check(got, ref, names, f"{dt} {sorted(kw)}")
