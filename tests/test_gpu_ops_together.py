@@ -442,3 +442,92 @@ def test_rotary_refusals():
     fa.rotary_embedding_v100(y[:, :, :4], y[:, :, 4:], table, inplace=True)
     assert torch.equal(y[:, :, :4], want[0]) and torch.equal(y[:, :, 4:], want[1]) and y._version > n
     assert _ops.MAX_HEAD_DIM == 128
+
+
+# ---------------------------------------------------------------------------
+# the C ABI itself, as a program without the Python entry points calls it
+def test_c_abi():
+    import ctypes
+
+    lib, stream = _ops.load(), torch.cuda.current_stream().cuda_stream
+    B, S, H, Hkv, D = 2, 300, 4, 2, 64
+    q, k, v, do = make(B, S, S, H, Hkv, D, "bf16", seed=9)
+    docs, slopes = packed(B, S, [100, 70], pad=5), slopes_for(H)
+    lens = torch.tensor([300, 211], device=DEV, dtype=torch.int32)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, slopes)]
+    o, lse = fa.flash_attention_v100_scored(*leaves[:3], causal=True, softcap=11.0, distance_slopes=leaves[3], documents=docs,
+                                            key_lengths=lens, return_softmax_lse=True)
+    want = [o.detach(), lse, *torch.autograd.grad(o, leaves, do)]
+    out = [torch.full_like(t, float("nan")) for t in want]
+
+    a = _ops.ScoredArgs()
+    for n, t in zip(("q", "k", "v", "dout", "o", "dq", "dk", "dv"), (q, k, v, do, out[0], *out[2:5])):
+        setattr(a, n, t.data_ptr())
+        getattr(a, ("do" if n == "dout" else n) + "_stride")[:] = t.stride()
+    a.lse, a.slopes, a.dslopes, a.key_lengths = out[1].data_ptr(), slopes.data_ptr(), out[5].data_ptr(), lens.data_ptr()
+    a.q_documents = a.k_documents = docs.data_ptr()
+    a.q_documents_stride = a.k_documents_stride = S
+    a.batch, a.seqlen_q, a.seqlen_k, a.num_heads, a.num_heads_kv, a.head_dim, a.dtype, a.causal = B, S, S, H, Hkv, D, 1, 1
+    a.scale, a.softcap = D ** -0.5, 11.0
+    for size, call in ((lib.fa_scored_fwd_workspace_size, lib.fa_scored_fwd),
+                       (lib.fa_scored_bwd_workspace_size, lib.fa_scored_bwd)):
+        n = size(ctypes.byref(a))
+        ws = torch.full((n + 256,), 255, device=DEV, dtype=torch.uint8)  # NaN where it is read before it is written
+        assert call(ctypes.byref(a), ws.data_ptr(), n, stream) == 0
+        torch.cuda.synchronize()
+        assert (ws[n:] == 255).all()  # nothing behind what was asked for
+    for x, y in zip(out, want):
+        assert torch.equal(x, y)
+
+    kp, vp = k[0, :200].contiguous(), v[0, :200].contiguous()
+    for P, prefix in ((200, (kp, vp)), (3000, (kp.repeat(15, 1, 1), vp.repeat(15, 1, 1)))):
+        want = fa.flash_attention_v100_shared_prefix(q[:, :3], *prefix, k, v, lens, softcap=11.0)
+        out = torch.full((B, 3, H, D), float("nan"), device=DEV, dtype=torch.bfloat16)
+        p = _ops.PrefixArgs()
+        for n, t in zip(("q", "k_prefix", "v_prefix", "k", "v", "o"), (q, *prefix, k, v, out)):
+            setattr(p, n, t.data_ptr())
+            getattr(p, {"k_prefix": "kp", "v_prefix": "vp"}.get(n, n) + "_stride")[:] = t.stride()
+        p.key_lengths = lens.data_ptr()
+        (p.batch, p.seqlen_q, p.prefix_len, p.seqlen_k, p.num_heads, p.num_heads_kv, p.head_dim, p.dtype, p.scale,
+         p.softcap) = B, 3, P, S, H, Hkv, D, 1, D ** -0.5, 11.0
+        n = lib.fa_prefix_workspace_size(ctypes.byref(p))
+        ws = torch.full((n + 256,), 255, device=DEV, dtype=torch.uint8)
+        assert lib.fa_prefix_fwd(ctypes.byref(p), ws.data_ptr(), n, stream) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and (ws[n:] == 255).all()
+
+
+@pytest.mark.parametrize("dt,D", [("bf16", 128), ("fp16", 80), ("fp32", 36), ("fp32", 128)])
+@pytest.mark.parametrize("Sq,Sk", [(130, 130), (700, 70), (3, 500)])
+def test_nothing_is_written_beside_the_outputs(dt, D, Sq, Sk):
+    import ctypes
+
+    lib, stream = _ops.load(), torch.cuda.current_stream().cuda_stream
+    B, H, Hkv = 2, 4, 2
+    q, k, v, do = make(B, Sq, Sk, H, Hkv, D, dt, seed=D)
+    want = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    o = fa.flash_attention_v100_scored(*want, causal=True, query_offsets=Sk - Sq)
+    want = [o.detach(), *torch.autograd.grad(o, want, do)]
+    pad = 4 if dt == "fp32" else 8
+    bufs = [torch.full((B + 1, t.shape[1] + 3, t.shape[2] + 1, D + pad), 7.0, device=DEV, dtype=t.dtype) for t in want]
+    outs = [x[:B, :t.shape[1], :t.shape[2], :D] for x, t in zip(bufs, want)]
+    lse = torch.full((B * H * Sq + 64,), 7.0, device=DEV)
+    a = _ops.ScoredArgs()
+    for n, t in zip(("q", "k", "v", "dout", "o", "dq", "dk", "dv"), (q, k, v, do, *outs)):
+        setattr(a, n, t.data_ptr())
+        getattr(a, ("do" if n == "dout" else n) + "_stride")[:] = t.stride()
+    a.lse, a.query_offset, a.causal, a.scale = lse.data_ptr(), Sk - Sq, 1, D ** -0.5
+    a.batch, a.seqlen_q, a.seqlen_k, a.num_heads, a.num_heads_kv, a.head_dim = B, Sq, Sk, H, Hkv, D
+    a.dtype = {"fp16": 0, "bf16": 1, "fp32": 2}[dt]
+    for size, call in ((lib.fa_scored_fwd_workspace_size, lib.fa_scored_fwd),
+                       (lib.fa_scored_bwd_workspace_size, lib.fa_scored_bwd)):
+        n = size(ctypes.byref(a))
+        ws = torch.full((n + 256,), 255, device=DEV, dtype=torch.uint8)
+        assert call(ctypes.byref(a), ws.data_ptr(), n, stream) == 0
+        torch.cuda.synchronize()
+        assert (ws[n:] == 255).all()
+    for x, y, t in zip(bufs, outs, want):
+        assert torch.equal(y, t)
+        y.fill_(7.0)
+        assert (x == 7.0).all()
+    assert (lse[B * H * Sq:] == 7.0).all()
