@@ -257,13 +257,19 @@ bool few_rows(const fa_scored_args* a, RowsParams& r) {
 //   2 x 4096, 32 on 8 heads of 128, cap: 1419, 1143, 1187, 1292
 //   2 x 8192, 16 heads of 128, cap: 2168, 2343, 2574, 3143
 //   2 x 2048, 16 heads of 64, cap, not causal: 185, 207
+// and over documents of lengths up to
+//   558: 2 x 1464, 12 on 6 heads of 128, cap: 178, 147, 136
+//   1354: 3 x 3718, 4 heads of 80: 196, 182, 198
+//   1286: 1 x 4096, 8 heads of 128: 169, 170, 185
+//   2911: 2 x 8192, 4 on 2 heads of 128: 596, 386, 340, 458
+//   488: 4 x 1000, 16 heads of 64: 64, 84, 108, 165
 int kv_parts(const fa_scored_args* a) {
     const int64_t n = ceil_div<int64_t>(a->seqlen_k, 128) * a->num_heads_kv * a->batch;
-    // queries of a walk (of documents, those of its own)
-    const int64_t walk = (int64_t)(a->num_heads / a->num_heads_kv) * a->seqlen_q / (a->q_documents ? 4 : 1);
+    // queries of a walk (with documents, those of its own: half of all are taken)
+    const int64_t walk = (int64_t)(a->num_heads / a->num_heads_kv) * a->seqlen_q / (a->q_documents ? 2 : 1);
     int parts = 1;
     const int64_t most = a->causal ? 512 : 256;
-    while (parts < 8 && n * parts <= most && walk >= parts * (n * parts <= 128 ? 512 : 1024)) parts *= 2;
+    while (parts < 8 && n * parts <= most && walk >= (n * parts <= 128 ? 512 * parts : 1024 * parts + 1)) parts *= 2;
     return parts;
 }
 size_t part_bytes(const fa_scored_args* a) {

@@ -1385,10 +1385,12 @@ __global__ __launch_bounds__(256) void kv_sum_kernel(const ScoredParams p, const
 //   1 x 4096, 16 heads of 128: 101 / 326, 88 / 309 (512)
 //   2 x 1777, 12 heads of 64 in float32: 181 / 448, 140 / 395 (336)
 //   2 x 2304, 16 heads of 64: 43 / 122, 49 / 131 (576)
-//   1 x 4096, 16 heads of 128, documents: 37 / 143, 47 / 151 (512, short walks)
+//   documents up to 1354: 3 x 3718, 4 heads of 80: 102 / 209, 80 / 182 (360)
+//   up to 1012: 2 x 2048, 16 on 4 heads of 64: 50 / 127, 37 / 113 (512)
+//   of 700: 1 x 4096, 16 heads of 128: 37 / 143, 47 / 151 (512)
 //   2 x 1536, 11 heads of 64, not causal: 35 / 98, 45 / 109 (264)
 inline bool two_groups(const ScoredParams& p, int64_t nb, int tile) {
-    return p.Sk > tile && nb < (p.causal && !p.q_docs ? 513 : 256);
+    return p.Sk > tile && nb < (p.causal ? 513 : 256);
 }
 template <typename T, int D, bool CAP, bool SLOPE>
 hipError_t launch_scored_fwd_t(ScoredParams p, hipStream_t s) {
