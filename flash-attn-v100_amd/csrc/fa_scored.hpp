@@ -16,6 +16,12 @@
 // tanh x = 1 - 2 r, r = 1 / (1 + e^(2x)): one exp2 and one reciprocal a score,
 // and its derivative 1 - tanh^2 = 4 (r - r^2) comes with two more operations.
 //
+// Roundings of 16-bit inputs: P and dS where they enter a product (the matrix
+// instructions take 16 bits), and delta from the rounded O that the caller keeps;
+// sums, statistics and parts are float32.  bf16, cap: the 2-norm of dQ is off by
+// 2.6e-3, of which its own rounding is 1.7e-3 and dS up to 2.4e-3; dS in two pieces
+// would cost another product, an unrounded O another saved tensor.
+//
 // Tiles, operand layouts and pipelines are those of fa_fwd.hpp and fa_bwd.hpp:
 // one workgroup has 4 waves of 32 queries (forward, dQ) or 32 keys (dK/dV).
 // Bound by the vector arithmetic of the scores beside the matrix products, near
