@@ -495,6 +495,7 @@ int32_t fa_rotary_check(const fa_rotary_args* a) {
         for (int i = 0; i < 3; ++i) {
             if (si[i] < 0 || so[i] < 0) return FA_ERR_STRIDE;
             if (si[i] > kMaxStride || so[i] > kMaxStride) return FA_ERR_TOO_LARGE;
+            if (in == out && si[i] != so[i]) return FA_ERR_STRIDE;  // an element would be written before it is read
         }
         return si[3] == 1 && so[3] == 1 ? FA_OK : FA_ERR_STRIDE;
     };

@@ -84,12 +84,15 @@ int32_t fa_ops_version(void);
  * fa_scored_bwd would return for these arguments. */
 int32_t fa_scored_check(const fa_scored_args* args, int32_t backward);
 
-/* Bytes of device workspace; 0 where none is needed and on invalid arguments. */
+/* Bytes of device workspace; 0 where none is needed and on invalid arguments.
+ * Aligned to 16 bytes for the forwards, to 256 for the backward; used until the
+ * call's kernels have run, so calls at once need one each. */
 size_t fa_scored_fwd_workspace_size(const fa_scored_args* args);
 size_t fa_scored_bwd_workspace_size(const fa_scored_args* args);
 
-/* Forward: o and lse.  Few query rows (single tokens over a cache) run with
- * their keys split over workgroups; results differ by the order of float32 sums. */
+/* Forward: o and lse.  Few queries (single tokens and chunks over a longer cache)
+ * run with their keys split over workgroups; results differ by the order of
+ * float32 sums. */
 int32_t fa_scored_fwd(const fa_scored_args* args, void* workspace, size_t workspace_bytes, void* hip_stream);
 
 /* Backward: dq, dk, dv (and dslopes), fully written; deterministic. */
@@ -150,8 +153,9 @@ int32_t fa_rotary_table(float* table, int64_t positions, int32_t rotary_dim, int
 
 /* Rotates the first rotary_dim columns of q (and k): pairs (j, j + rotary_dim / 2),
  * interleaved: (2 j, 2 j + 1).  inverse: the transposed rotation (the gradient of
- * the rotation).  Outputs may be the inputs themselves (the columns past rotary_dim
- * are then left alone, else copied).  A negative position leaves its token as it
+ * the rotation).  Outputs may be the inputs themselves, with equal strides (the
+ * columns past rotary_dim are then left alone, else copied); they may not overlap
+ * in any other way.  A negative position leaves its token as it
  * is, a position past the table makes it NaN.  No alignment beyond the element's
  * is needed; the d stride is 1. */
 typedef struct fa_rotary_args {

@@ -208,6 +208,7 @@ def test_rotary_refusals():
                          ("FA_ERR_HEADS", with_(num_heads=0, num_heads_k=0)), ("FA_ERR_ROTARY", with_(table=None)),
                          ("FA_ERR_ROTARY", with_(table_positions=0)), ("FA_ERR_NULL_ARG", with_(k_out=None)),
                          ("FA_ERR_ALIGN", with_(q=ADDR + 1)), ("FA_ERR_STRIDE", with_stride("q_stride", 3, 2)),
+                         ("FA_ERR_STRIDE", with_stride("k_out_stride", 1, 512)),  # in place, other rows
                          ("FA_ERR_ALIGN", with_(positions=ADDR + 4, positions_64=1)),
                          ("FA_ERR_TOO_LARGE", with_(batch=1 << 20, seqlen=1 << 20))):
         a = rotary_args()
