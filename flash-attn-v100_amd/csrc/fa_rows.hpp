@@ -74,8 +74,14 @@ struct UnitRow {
 template <bool F32>
 __device__ FA_INLINE inline void row_rules(f32x16& s, const RowsParams& p, Cap<F32>& cap, bool slope, float slope2, float d0) {
     if (p.cap > 0.f) {
+        if (F32 || p.cap <= kWideCap) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = cap.value(s[e]);
+            for (int e = 0; e < 16; ++e) s[e] = cap.value(s[e]);
+        } else {
+            Cap<true> wide(p);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = wide.value(s[e]);
+        }
     } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] *= p.scale_log2;

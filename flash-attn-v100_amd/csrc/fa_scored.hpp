@@ -64,10 +64,16 @@ struct SeqRule {
 
 // tanh cap.  value(): cap tanh(x / cap) log2 e of a raw score s (x = scale s);
 // slope(): the derivative / 4.
-// 16-bit inputs: 1 - 2 r, whose cancellation near 0 is at most 2^-23 of the cap
-// in the score.  float32: a series there (through x^13: 2e-8 of the value below
-// 0.45), so that small scores keep their digits.
-template <bool F32>
+// Two forms.  Quick: 1 - 2 r, whose cancellation near 0 leaves an error of about
+// 2^-22 of the cap in the score.  EXACT: a series there (through x^13: 2e-8 of the
+// value below 0.45), so that small scores keep their digits under any cap.  16-bit
+// inputs take the quick form up to kWideCap, where its error in a score, and so in a
+// probability, is at most 2^-14, below the 2^-12 and 2^-9 to which fp16 and bf16
+// round the probabilities; float32 always the series.  2 x 4096, 32 on 8 heads of 128,
+// bf16, causal, quick / series: forward 344 / 461 us, training step 1500 / 1830; single
+// tokens over 16 caches of 8192: 108 / 110.
+constexpr float kWideCap = 256.f;
+template <bool EXACT>
 struct Cap {
     float k1, k2, top;  // scale / cap; that times 2 log2 e; cap log2 e
     float r, t;         // of the last score
@@ -76,7 +82,7 @@ struct Cap {
     __device__ FA_INLINE inline float rcp(float s) { return __builtin_amdgcn_rcpf(1.f + fast_exp2(s * k2)); }
     __device__ FA_INLINE inline float value(float s) {
         r = rcp(s);
-        if constexpr (!F32) {
+        if constexpr (!EXACT) {
             return __builtin_fmaf(-2.f * top, r, top);
         } else {
             const float x = s * k1, u = x * x;
@@ -92,12 +98,20 @@ struct Cap {
         }
     }
     __device__ FA_INLINE inline float slope() const {
-        if constexpr (!F32)
+        if constexpr (!EXACT)
             return __builtin_fmaf(-r, r, r);
         else
             return __builtin_fmaf(-0.25f * t, t, 0.25f);
     }
 };
+
+// CAP of the kernels.  kCapWide (16-bit inputs) is compiled with SLOPE only, whose
+// kernels hold scores as values; a call without slopes has a slope of 0 there.
+constexpr int kCapNone = 0, kCapQuick = 1, kCapWide = 2;
+template <int CAP, bool SLOPE>
+__device__ FA_INLINE inline bool has_slope(const ScoredParams& p) {
+    return SLOPE && (CAP != kCapWide || p.slopes != nullptr);
+}
 
 // ---------------------------------------------------------------------------
 // whether the id ranges of two blocks meet in an id that is not negative
@@ -233,7 +247,7 @@ __device__ FA_INLINE inline BlockOrder block_order(const ScoredParams& p, int he
 // ---------------------------------------------------------------------------
 // Forward, over the tiles of a walk.  KS = 2: two groups of 4 waves on the same
 // queries, taking the walk's tiles in turn, for grids that leave CUs idle.
-template <typename T, int D, bool CAP, bool SLOPE, int KS>
+template <typename T, int D, int CAP, bool SLOPE, int KS>
 __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) ? 2 : 1)) void scored_fwd_kernel(
     const ScoredParams p) {
     using C = FwdCfg<T, D>;
@@ -330,8 +344,8 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
     float m_run = -1e30f;  // running max in log2 units
     float l_run = 0.f;     // lane-partial row sum
     const float c = p.scale_log2;
-    Cap<C::F32> cap(p);
-    const float slope2 = SLOPE ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
+    Cap<(C::F32 || CAP == kCapWide)> cap(p);
+    const float slope2 = has_slope<CAP, SLOPE>(p) ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
     const int qpos = qi + rule.off;  // distances are exact up to 2^24, then rounded once
 
     T* Ks0 = smem + sp * C::SMEM_ELEMS;
@@ -386,7 +400,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
     // ---- rules, then mask and running max.  A score is held as u, its value in log2
     // units is ua u + ub: u the raw product, or r of the cap (which falls with
     // the score), or the value itself ----
-    constexpr bool RCP = CAP && !SLOPE && !C::F32, VALUE = SLOPE || (CAP && C::F32);
+    constexpr bool RCP = CAP == kCapQuick && !SLOPE && !C::F32, VALUE = SLOPE || (CAP && C::F32);
     const float ua = VALUE ? 1.f : RCP ? -2.f * cap.top : c, ub = RCP ? cap.top : 0.f;
     constexpr float kHidden = RCP ? INFINITY : -INFINITY;
     auto rules = [&](f32x16 (&s)[NB], int k0) FA_INLINE {
@@ -644,7 +658,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
 // DSLOPE: also -d loss / d slope of each row, sum_j |d| P (dP - delta) with
 // delta summed from P dP here instead of taken from the rounded output: the sum
 // over all rows is returned in float32, whose digits the rounding would cost.
-template <typename T, int D, bool CAP, bool SLOPE, bool DSLOPE, int KS>
+template <typename T, int D, int CAP, bool SLOPE, bool DSLOPE, int KS>
 __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) void scored_dq_kernel(const ScoredParams p) {
     using C = DqCfg<T, D>;
     constexpr int BN = C::BN, KW = C::KW;
@@ -758,8 +772,8 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) dq[i] = f32x16{};
     const float c = p.scale_log2;
-    Cap<C::F32> cap(p);
-    const float slope2 = SLOPE ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
+    Cap<(C::F32 || CAP == kCapWide)> cap(p);
+    const float slope2 = has_slope<CAP, SLOPE>(p) ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
     const int qpos = qi + rule.off;  // distances are exact up to 2^24, then rounded once
     float sum_dp = 0.f, sum_d = 0.f, sum_ddp = 0.f;  // sums of P dP, |d| P, |d| P dP (DSLOPE)
 
@@ -999,7 +1013,7 @@ struct ScoredDkdvCfg {
     static_assert(SLOT_BYTES % 16 == 0, "16-byte aligned slots");
 };
 
-template <typename T, int D, bool CAP, bool SLOPE>
+template <typename T, int D, int CAP, bool SLOPE>
 __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void scored_dkdv_kernel(const ScoredParams p) {
     using C = ScoredDkdvCfg<T, D>;
     constexpr int BQ = C::BQ, RW = C::RW, NSLOT = C::NSLOT;
@@ -1092,7 +1106,7 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
         dv[i] = f32x16{};
     }
     const float c = p.scale_log2;
-    Cap<C::F32> cap(p);
+    Cap<(C::F32 || CAP == kCapWide)> cap(p);
 
     const bool copy_q = w < C::NW / 2;
     typename C::Rows rows;
@@ -1288,7 +1302,7 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
                 barrier_no_fence();
             }
             if (cur.fl & kAct) {
-                const float slope2 = SLOPE ? p.slopes[b * p.slopes_sb + cur_h] * kLog2e : 0.f;
+                const float slope2 = has_slope<CAP, SLOPE>(p) ? p.slopes[b * p.slopes_sb + cur_h] * kLog2e : 0.f;
 #pragma unroll
                 for (int st = 0; st < C::NSUB; ++st) {
                     f32x16 sc, dpc;
@@ -1398,7 +1412,7 @@ __global__ __launch_bounds__(256) void kv_sum_kernel(const ScoredParams p, const
 inline bool two_groups(const ScoredParams& p, int64_t nb, int tile) {
     return p.Sk > tile && nb < (p.causal ? 513 : 256);
 }
-template <typename T, int D, bool CAP, bool SLOPE>
+template <typename T, int D, int CAP, bool SLOPE>
 hipError_t launch_scored_fwd_t(ScoredParams p, hipStream_t s) {
     using C = FwdCfg<T, D>;
     p.n_tiles = (p.Sq + C::BM - 1) / C::BM;
@@ -1412,7 +1426,7 @@ hipError_t launch_scored_fwd_t(ScoredParams p, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <typename T, int D, bool CAP, bool SLOPE>
+template <typename T, int D, int CAP, bool SLOPE>
 hipError_t launch_scored_bwd_t(ScoredParams p, hipStream_t s) {
     using CQ = DqCfg<T, D>;
     using CK = DkdvCfg<T, D>;
@@ -1453,10 +1467,16 @@ hipError_t launch_scored_bwd_t(ScoredParams p, hipStream_t s) {
 template <typename T>
 hipError_t launch_scored_fwd(const ScoredParams& p, int D, hipStream_t s) {
     const bool cap = p.cap > 0.f, slope = p.slopes != nullptr;
+    [[maybe_unused]] const bool wide = p.cap > kWideCap;
 #define FA_CASE(DD)                                                                                    \
     if (D == DD) {                                                                                     \
-        if (cap) return slope ? launch_scored_fwd_t<T, DD, true, true>(p, s) : launch_scored_fwd_t<T, DD, true, false>(p, s); \
-        return slope ? launch_scored_fwd_t<T, DD, false, true>(p, s) : launch_scored_fwd_t<T, DD, false, false>(p, s);        \
+        if constexpr (!Elem<T>::kF32)                                                                  \
+            if (wide) return launch_scored_fwd_t<T, DD, kCapWide, true>(p, s);                         \
+        if (cap)                                                                                       \
+            return slope ? launch_scored_fwd_t<T, DD, kCapQuick, true>(p, s)                           \
+                         : launch_scored_fwd_t<T, DD, kCapQuick, false>(p, s);                         \
+        return slope ? launch_scored_fwd_t<T, DD, kCapNone, true>(p, s)                                \
+                     : launch_scored_fwd_t<T, DD, kCapNone, false>(p, s);                              \
     }
     FA_CASE(32)
     FA_CASE(64)
@@ -1467,10 +1487,16 @@ hipError_t launch_scored_fwd(const ScoredParams& p, int D, hipStream_t s) {
 template <typename T>
 hipError_t launch_scored_bwd(const ScoredParams& p, int D, hipStream_t s) {
     const bool cap = p.cap > 0.f, slope = p.slopes != nullptr;
+    [[maybe_unused]] const bool wide = p.cap > kWideCap;
 #define FA_CASE(DD)                                                                                    \
     if (D == DD) {                                                                                     \
-        if (cap) return slope ? launch_scored_bwd_t<T, DD, true, true>(p, s) : launch_scored_bwd_t<T, DD, true, false>(p, s); \
-        return slope ? launch_scored_bwd_t<T, DD, false, true>(p, s) : launch_scored_bwd_t<T, DD, false, false>(p, s);        \
+        if constexpr (!Elem<T>::kF32)                                                                  \
+            if (wide) return launch_scored_bwd_t<T, DD, kCapWide, true>(p, s);                         \
+        if (cap)                                                                                       \
+            return slope ? launch_scored_bwd_t<T, DD, kCapQuick, true>(p, s)                           \
+                         : launch_scored_bwd_t<T, DD, kCapQuick, false>(p, s);                         \
+        return slope ? launch_scored_bwd_t<T, DD, kCapNone, true>(p, s)                                \
+                     : launch_scored_bwd_t<T, DD, kCapNone, false>(p, s);                              \
     }
     FA_CASE(32)
     FA_CASE(64)
