@@ -71,17 +71,11 @@ struct UnitRow {
 };
 
 // scores of 16 keys of a 32-key block in log2 units
-template <bool F32>
-__device__ FA_INLINE inline void row_rules(f32x16& s, const RowsParams& p, Cap<F32>& cap, bool slope, float slope2, float d0) {
+template <bool EXACT>
+__device__ FA_INLINE inline void row_rules(f32x16& s, const RowsParams& p, Cap<EXACT>& cap, bool slope, float slope2, float d0) {
     if (p.cap > 0.f) {
-        if (F32 || p.cap <= kWideCap) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = cap.value(s[e]);
-        } else {
-            Cap<true> wide(p);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = wide.value(s[e]);
-        }
+        for (int e = 0; e < 16; ++e) s[e] = cap.value(s[e]);
     } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] *= p.scale_log2;
@@ -96,7 +90,7 @@ __device__ FA_INLINE inline void row_rules(f32x16& s, const RowsParams& p, Cap<F
 // 32 rows over split `split` of the keys [0, n_keys) (a sequence's own ones, or a
 // prefix that few rows read; p.joined: the prefix, then the own ones): each wave
 // walks tiles of its own
-template <typename T, int D>
+template <typename T, int D, bool EXACT>
 __device__ FA_INLINE inline void unit32(const RowsParams& p, bool pre, T* smem, float (*stat)[2][32], int id, int lane, int w) {
     using C = RowsCfg<T, D>;
     constexpr int BN = C::BN, KW = C::KW, VW = C::VW, NW = C::NW;
@@ -177,7 +171,7 @@ __device__ FA_INLINE inline void unit32(const RowsParams& p, bool pre, T* smem, 
 #pragma unroll
     for (int n = 0; n < D / 32; ++n) o[n] = f32x16{};
     float m_run = -1e30f, l_run = 0.f;
-    Cap<C::F32> cap(p);
+    Cap<EXACT> cap(p);
 
     int t = t0 + w;
     copy_k(t);
@@ -338,7 +332,7 @@ __device__ FA_INLINE inline void unit32(const RowsParams& p, bool pre, T* smem, 
 
 // 128 rows of all sequences over split `split` of the prefix: the waves share its
 // tiles (64 keys, double-buffered), each on 32 rows
-template <typename T, int D>
+template <typename T, int D, bool EXACT>
 __device__ FA_INLINE inline void unit128(const RowsParams& p, T* smem, int id, int lane, int w) {
     using C = FwdCfg<T, D>;
     constexpr int BN = C::BN, NB = C::NB, KW = C::KW, VW = C::VW;
@@ -382,7 +376,7 @@ __device__ FA_INLINE inline void unit128(const RowsParams& p, T* smem, int id, i
 #pragma unroll
     for (int n = 0; n < D / 32; ++n) o[n] = f32x16{};
     float m_run = -1e30f, l_run = 0.f;
-    Cap<C::F32> cap(p);
+    Cap<EXACT> cap(p);
 
     int slot = 0;
     copy(t0, 0);
@@ -486,8 +480,9 @@ __device__ FA_INLINE inline void unit128(const RowsParams& p, T* smem, int id, i
 }
 
 // The units of the prefix, then those of the sequences' own keys, in one launch
-// (the products of the ones beside the bytes of the others).
-template <typename T, int D>
+// (the products of the ones beside the bytes of the others).  EXACT: the cap by its
+// series (a branch on it in this kernel costs single tokens 0.2 of 9.0 us).
+template <typename T, int D, bool EXACT>
 __global__ __launch_bounds__(256, (RowsCfg<T, D>::PER_CU)) void rows_kernel(const RowsParams p) {
     using C = RowsCfg<T, D>;
     __shared__ __attribute__((aligned(16))) T smem[C::SMEM];
@@ -498,9 +493,9 @@ __global__ __launch_bounds__(256, (RowsCfg<T, D>::PER_CU)) void rows_kernel(cons
     // splits of a unit are consecutive ids, on one XCD's share of the grid
     const int id = xcd_remap(pre ? (int)blockIdx.x : (int)(blockIdx.x - p.p_wgs), (int)(pre ? p.p_wgs : p.o_wgs));
     if (pre && p.p_unit == 128)
-        unit128<T, D>(p, smem, id, lane, w);
+        unit128<T, D, EXACT>(p, smem, id, lane, w);
     else
-        unit32<T, D>(p, pre, smem, stat, id, lane, w);
+        unit32<T, D, EXACT>(p, pre, smem, stat, id, lane, w);
 }
 
 // The parts of every row, rescaled to their common maximum: D / 4 threads a row (4
@@ -596,7 +591,11 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p, cons
 
 template <typename T, int D>
 hipError_t launch_rows_t(const RowsParams& p, hipStream_t s) {
-    hipLaunchKernelGGL((rows_kernel<T, D>), dim3((unsigned)(p.p_wgs + p.o_wgs)), dim3(256), 0, s, p);
+    const dim3 grid((unsigned)(p.p_wgs + p.o_wgs));
+    if (Elem<T>::kF32 || p.cap > kWideCap)
+        hipLaunchKernelGGL((rows_kernel<T, D, true>), grid, dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL((rows_kernel<T, D, Elem<T>::kF32>), grid, dim3(256), 0, s, p);
     const int n = p.p_splits + p.o_splits;
     if (n > 1) {
         const int64_t n_rows = (int64_t)p.B * p.H * p.Sq;
