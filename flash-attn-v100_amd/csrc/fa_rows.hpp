@@ -48,11 +48,28 @@ struct RowsCfg {
     static constexpr int PER_CU = F32 && D == 128 ? 1 : 2;
 };
 
+// filled keys of a sequence's own, and the position among them of query 0
+__device__ FA_INLINE inline int own_len(const RowsParams& p, int b) {
+    return p.lens ? max(0, min(p.Sk, p.lens[b])) : p.Sk;
+}
+__device__ FA_INLINE inline int own_pos(const RowsParams& p, int b, int len) {
+    return p.tail ? len - p.Sq : max(-kMaxOffset, min(kMaxOffset, p.offsets ? p.offsets[b] : p.offset0));
+}
+// the key nearest to a position: distances are taken from there, as SeqRule::near
+__device__ FA_INLINE inline int near_key(int pos, int len) { return max(0, min(len - 1, pos)); }
+// what the LSE of a row holds for the distance to there (a query after a prefix stands
+// on one of the own keys, or sees nothing)
+__device__ FA_INLINE inline float far_bias(const RowsParams& p, int b, int i, int h) {
+    if (!p.slopes || p.tail) return 0.f;
+    const int len = own_len(p, b), own = own_pos(p, b, len) + i;
+    return p.slopes[b * p.slopes_sb + h] * (float)abs(own - near_key(own, len));
+}
+
 // one row of a unit: its query and the keys [0, lim) it sees
 struct UnitRow {
     int b, i, h, lim;
     bool live;
-    int qpos;
+    int qpos;  // of the nearest key (the prefix before the own ones)
     __device__ FA_INLINE inline UnitRow(const RowsParams& p, bool pre, int row, int hk, int bs) {
         const int per_seq = p.Sq * p.group, n_rows = pre ? p.B * per_seq : per_seq;
         live = row < n_rows;
@@ -61,12 +78,11 @@ struct UnitRow {
         const int ig = pre ? rr % per_seq : rr;
         i = ig / p.group;
         h = hk * p.group + ig % p.group;
-        const int len = p.lens ? max(0, min(p.Sk, p.lens[b])) : p.Sk;
-        const int off = p.tail ? len - p.Sq : max(-kMaxOffset, min(kMaxOffset, p.offsets ? p.offsets[b] : p.offset0));
-        const int own = off + i;  // the query's position among the sequence's own keys
+        const int len = own_len(p, b);
+        const int own = own_pos(p, b, len) + i;  // the query's position among the sequence's own keys
         lim = pre ? p.P : p.causal ? min(len, own + 1) : len;
         if (!live || (p.masked_neg && own < 0)) lim = 0;
-        qpos = pre ? p.P + own : own;
+        qpos = pre ? p.P + own : near_key(own, len);
     }
 };
 
@@ -291,7 +307,8 @@ __device__ FA_INLINE inline void unit32(const RowsParams& p, bool pre, T* smem, 
     if (!only && w == 0 && hi == 0) p.stat[prow] = make_float2(mm, l_tot);
     if (only && w == 0 && hi == 0 && row.live && p.lse)
         p.lse[(int64_t)(row.b * p.H + row.h) * p.Sq + row.i] =
-            l_tot > 0.f ? (mm + __log2f(l_tot)) * kLn2 : l_tot == 0.f ? -INFINITY : l_tot;
+            l_tot > 0.f ? (mm + __log2f(l_tot)) * kLn2 - far_bias(p, row.b, row.i, row.h)
+                        : l_tot == 0.f ? -INFINITY : l_tot;
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
 #pragma unroll
     for (int n0 = 0; n0 < D / 32; n0 += NW) {
@@ -576,7 +593,8 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p, cons
     }
     if (!live) return;
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
-    if (col == 0 && p.lse) p.lse[r] = l_tot > 0.f ? (mm + __log2f(l_tot)) * kLn2 : l_tot == 0.f ? -INFINITY : l_tot;
+    if (col == 0 && p.lse)
+        p.lse[r] = l_tot > 0.f ? (mm + __log2f(l_tot)) * kLn2 - far_bias(p, b, i, h) : l_tot == 0.f ? -INFINITY : l_tot;
     if (col >= p.cols) return;
     T* ob = (T*)p.o + b * p.o_sb + (int64_t)i * p.o_ss + h * p.o_sh + col;
     if constexpr (Elem<T>::kF32) {

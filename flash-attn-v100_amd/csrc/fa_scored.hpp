@@ -56,6 +56,13 @@ struct SeqRule {
     }
     // keys [0, lim(i)) may be seen by query i
     __device__ FA_INLINE inline int lim(int i) const { return causal ? min(len, max(i + off + 1, prefix)) : len; }
+    // The key nearest to query i.  A row's softmax does not change when all of its
+    // distances lose the one to that key, and |i + off - j| less it is
+    // |near(i) - j|: the kernels take distances from there, so that the scores of a
+    // query far from the keys keep their digits, and only the LSE holds
+    // slope far(i).
+    __device__ FA_INLINE inline int near(int i) const { return max(0, min(len - 1, i + off)); }
+    __device__ FA_INLINE inline float far(int i) const { return (float)abs(i + off - near(i)); }
     // queries from first(j) on may see key j
     __device__ FA_INLINE inline int first(int j) const {
         return j >= len ? INT_MAX : (!causal || j < prefix) ? 0 : max(0, j - off);
@@ -346,7 +353,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
     const float c = p.scale_log2;
     Cap<(C::F32 || CAP == kCapWide)> cap(p);
     const float slope2 = has_slope<CAP, SLOPE>(p) ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
-    const int qpos = qi + rule.off;  // distances are exact up to 2^24, then rounded once
+    const int qpos = rule.near(qi);
 
     T* Ks0 = smem + sp * C::SMEM_ELEMS;
     T* Vs0 = Ks0 + 2 * C::KTILE;
@@ -644,9 +651,11 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
     const ScoredParams& pe = late_args();
     const float l_tot = pair_sum(l_run);
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
-    if (pe.lse && sp == 0 && hi == 0 && qi < p.Sq)
+    if (pe.lse && sp == 0 && hi == 0 && qi < p.Sq) {
+        const float far = has_slope<CAP, SLOPE>(pe) ? pe.slopes[b * pe.slopes_sb + h] * rule.far(qi) : 0.f;
         pe.lse[(int64_t)(b * pe.H + h) * pe.Sq + qi] =
-            l_tot > 0.f ? (m_run + __log2f(l_tot)) * kLn2 : l_tot == 0.f ? -INFINITY : l_tot;
+            l_tot > 0.f ? (m_run + __log2f(l_tot)) * kLn2 - far : l_tot == 0.f ? -INFINITY : l_tot;
+    }
     store_rows<T, D>(smem + w * 32 * C::OW, C::OW, o, inv, (T*)pe.o + b * pe.o_sb + h * pe.o_sh, pe.o_ss,
                      qw0, pe.Sq, pe.cols, lane, sp == 0);
 }
@@ -705,8 +714,12 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
         del = pair_sum(del);
     }
     const float lse_in = qi < p.Sq ? p.lse[(int64_t)(b * p.H + h) * p.Sq + qi] : -INFINITY;
-    // a row that sees nothing, and rows past the last: P = exp2(s - inf) = 0
-    const float lse2 = lse_in == -INFINITY ? INFINITY : lse_in * kLog2e;
+    const float slope2 = has_slope<CAP, SLOPE>(p) ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
+    // of distances from the nearest key; a row that sees nothing, and rows past the
+    // last: P = exp2(s - inf) = 0
+    const float lse2 = lse_in == -INFINITY ? INFINITY
+                       : SLOPE             ? __builtin_fmaf(slope2, rule.far(qi), lse_in * kLog2e)
+                                           : lse_in * kLog2e;
     if (sp == 0 && hi == 0) {
         const int64_t wi = ((int64_t)b * p.H + h) * p.ws_stride + qi;  // qi < sq_pad
         p.lse2[wi] = lse2;
@@ -773,8 +786,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
     for (int i = 0; i < D / 32; ++i) dq[i] = f32x16{};
     const float c = p.scale_log2;
     Cap<(C::F32 || CAP == kCapWide)> cap(p);
-    const float slope2 = has_slope<CAP, SLOPE>(p) ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
-    const int qpos = qi + rule.off;  // distances are exact up to 2^24, then rounded once
+    const int qpos = rule.near(qi);
     float sum_dp = 0.f, sum_d = 0.f, sum_ddp = 0.f;  // sums of P dP, |d| P, |d| P dP (DSLOPE)
 
     const T* kbase = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
@@ -1013,7 +1025,10 @@ struct ScoredDkdvCfg {
     static_assert(SLOT_BYTES % 16 == 0, "16-byte aligned slots");
 };
 
-template <typename T, int D, int CAP, bool SLOPE>
+// FAR: queries may stand off the keys, whose distances start at the nearest one (one
+// clamp a score, which in every call would cost 2 x 4096, 32 on 8 heads of 128, bf16,
+// slopes: 1410 -> 1463 us a step).
+template <typename T, int D, int CAP, bool SLOPE, bool FAR>
 __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void scored_dkdv_kernel(const ScoredParams p) {
     using C = ScoredDkdvCfg<T, D>;
     constexpr int BQ = C::BQ, RW = C::RW, NSLOT = C::NSLOT;
@@ -1176,7 +1191,10 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = 8 * ks + 4 * gg + e;
-                const float ad = __builtin_fabsf(d0 + (float)(8 * gg + e));
+                float d = d0 + (float)(8 * gg + e);
+                if constexpr (FAR)  // from the key nearest to the query
+                    d = __builtin_amdgcn_fmed3f(d, (float)-kj, (float)(max(rule.len, 1) - 1 - kj));
+                const float ad = __builtin_fabsf(d);
                 float pv;
                 if constexpr (CAP) {
                     float t = cap.value(sc[r]) - l4[e];
@@ -1455,7 +1473,21 @@ hipError_t launch_scored_bwd_t(ScoredParams p, hipStream_t s) {
     }
     p.n_tiles = (p.Sk + CK::BK - 1) / CK::BK;
     const int64_t nk = (int64_t)p.n_tiles * p.Hkv * p.B * p.kv_parts;
-    if (nk > 0) hipLaunchKernelGGL((scored_dkdv_kernel<T, D, CAP, SLOPE>), dim3((unsigned)nk), dim3(256), 0, s, p);
+    // whether a query may stand off its sequence's keys
+    const bool far = p.slopes && (p.lens || p.offsets || p.offset0 < 0 || (int64_t)p.offset0 + p.Sq > p.Sk);
+    auto dkdv = [&](auto f) {
+        hipLaunchKernelGGL((scored_dkdv_kernel<T, D, CAP, SLOPE, decltype(f)::value>), dim3((unsigned)nk), dim3(256), 0, s, p);
+    };
+    if (nk > 0) {
+        if constexpr (SLOPE) {
+            if (far)
+                dkdv(std::true_type{});
+            else
+                dkdv(std::false_type{});
+        } else {
+            dkdv(std::false_type{});
+        }
+    }
     if (nk > 0 && p.kv_parts > 1) {
         const int64_t nt = (int64_t)p.B * p.Hkv * 2 * p.Sk * (D / 4);
         hipLaunchKernelGGL((kv_sum_kernel<T, D>), dim3((unsigned)((nt + 255) / 256)), dim3(256), 0, s, p,

@@ -1,0 +1,52 @@
+"""Queries far from their keys: the distance to the nearest of them is common to a
+row and leaves no trace in its outputs and gradients, within bounds that grow with
+the spread of the distances only."""
+import pytest
+import torch
+
+import flash_attention_v100 as fa
+import ops_edges_oracle as eo
+import ops_oracle as oo
+from ops_edges_oracle import DEV, make
+
+pytestmark = pytest.mark.gpu
+
+
+FAR = [8192, 65536, 1 << 20, (1 << 24) + 3, (1 << 28) + 1]
+
+
+def forward(q, k, v, slopes, off, label, lens=None, **kw):
+    got = dict(zip(("o", "lse"), fa.flash_attention_v100_scored(
+        q, k, v, query_offsets=off, distance_slopes=slopes, key_lengths=lens, return_softmax_lse=True, **kw)))
+    seen = oo.seen_mask(q.shape[0], q.shape[1], k.shape[1], kw.get("causal", False), None, None, None, lens, off, DEV)
+    oo.check(got, eo.scored(q, k, v, None, 0.0, slopes, off, seen, lens), ["o", "lse"], label)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("off", FAR)
+def test_far_queries(off, D, dt):
+    q, k, v, _ = make(2, 170, 500, 4, 2, D, dt, seed=off % 1000)
+    slopes = torch.tensor([0.5, 0.0625, 0.01, 0.001], device=DEV)
+    forward(q, k, v, slopes, off, f"{off} D={D} {dt}", causal=True)
+    forward(q, k, v, slopes, -off, f"{-off} D={D} {dt}")
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+def test_offsets_inside_and_outside(dt):
+    q, k, v, _ = make(4, 130, 300, 2, 1, 64, dt, seed=7)
+    off = torch.tensor([1 << 20, 200, -5, 100000], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([300, 120, 300, 1], dtype=torch.int32, device=DEV)
+    slopes = torch.tensor([[0.1, -0.004], [0.02, 0.3], [0.5, 0.0], [0.001, 1.0]], device=DEV)
+    forward(q, k, v, slopes, off, dt, lens)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("off", FAR)
+def test_few_far_queries(off, dt):
+    # the few-row kernel: one part a row, and parts that are joined
+    slopes = torch.tensor([0.5, 0.0625, 0.01, 0.001], device=DEV)
+    for Sq, Sk in ((2, 100), (5, 5000)):
+        q, k, v, _ = make(2, Sq, Sk, 4, 2, 64, dt, seed=Sq)
+        forward(q, k, v, slopes, off, f"{Sq} x {Sk}, {off} {dt}", causal=True)
+        forward(q, k, v, slopes, -off, f"{Sq} x {Sk}, {-off} {dt}")
