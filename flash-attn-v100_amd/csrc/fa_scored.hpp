@@ -664,9 +664,15 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
 // dQ, and per query the rows LSE * log2 e and delta = rowsum(dO O) that the
 // dK/dV pass reads after it.  dS goes through the cap's derivative (/ 4, made up
 // for in the final scale).
-// DSLOPE: also -d loss / d slope of each row, sum_j |d| P (dP - delta) with
-// delta summed from P dP here instead of taken from the rounded output: the sum
-// over all rows is returned in float32, whose digits the rounding would cost.
+// SLOPE: P is e^(s - LSE), and the LSE of a query far from the keys is a large number
+// whose rounding is a factor on its row.  The row's sum of P takes it out again: of
+// dQ at the end, and of the LSE that goes to the dK/dV pass (while slope times the
+// distance to the nearest key is below 2^30; then the gradients become NaN).
+// DSLOPE: also -d loss / d slope of each row,
+//   sum_j |d| P (dP - delta) = sum |d| dS - sum |d| P sum dS,  dS = P (dP - delta'),
+// over P and dS that are divided by sum P: with delta' from the rounded output, what
+// is subtracted is small, and delta itself is as good as the sums (the sum over all
+// rows is returned in float32, whose digits the rounding would cost).
 template <typename T, int D, int CAP, bool SLOPE, bool DSLOPE, int KS>
 __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) void scored_dq_kernel(const ScoredParams p) {
     using C = DqCfg<T, D>;
@@ -722,7 +728,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
                                            : lse_in * kLog2e;
     if (sp == 0 && hi == 0) {
         const int64_t wi = ((int64_t)b * p.H + h) * p.ws_stride + qi;  // qi < sq_pad
-        p.lse2[wi] = lse2;
+        if constexpr (!SLOPE) p.lse2[wi] = lse2;  // (else at the end)
         p.lse2[wi + p.sq_pad] = qi < p.Sq ? del : 0.f;
     }
 
@@ -787,7 +793,8 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
     const float c = p.scale_log2;
     Cap<(C::F32 || CAP == kCapWide)> cap(p);
     const int qpos = rule.near(qi);
-    float sum_dp = 0.f, sum_d = 0.f, sum_ddp = 0.f;  // sums of P dP, |d| P, |d| P dP (DSLOPE)
+    // sums of P (SLOPE); of dS, |d| P, |d| dS (DSLOPE)
+    [[maybe_unused]] float sum_p = 0.f, sum_ds = 0.f, sum_d = 0.f, sum_dds = 0.f;
 
     const T* kbase = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
     const T* vbase = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
@@ -879,22 +886,27 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
             }
         }
         if constexpr (DSLOPE) {
-            float x0[2] = {0.f, 0.f}, x1[2] = {0.f, 0.f}, x2[2] = {0.f, 0.f};
+            float xp[2] = {0.f, 0.f}, x0[2] = {0.f, 0.f}, x1[2] = {0.f, 0.f}, x2[2] = {0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float ad = __builtin_fabsf(d0 - (float)(8 * (e >> 2) + (e & 3)));
-                // a masked dP may be anything
-                const float pdp = pe[e] == 0.f ? 0.f : pe[e] * dp[8 * ks + e];
-                x0[e & 1] += pdp;
+                // dS before the cap's derivative (a masked dP may be anything)
+                const float dsn = CAP ? (pe[e] == 0.f ? 0.f : pe[e] * (dp[8 * ks + e] - del)) : ds[e];
+                xp[e & 1] += pe[e];
+                x0[e & 1] += dsn;
                 x1[e & 1] = __builtin_fmaf(pe[e], ad, x1[e & 1]);
-                x2[e & 1] = __builtin_fmaf(pdp, ad, x2[e & 1]);
+                x2[e & 1] = __builtin_fmaf(dsn, ad, x2[e & 1]);
             }
-            sum_dp += x0[0] + x0[1];
+            sum_p += xp[0] + xp[1];
+            sum_ds += x0[0] + x0[1];
             sum_d += x1[0] + x1[1];
-            sum_ddp += x2[0] + x2[1];
+            sum_dds += x2[0] + x2[1];
             // summed here: moved on, P and dP stay in registers until then, and spill
             // (2 x 4096 x 32 heads of 128: backward with the slopes' gradient 1683 -> 1141 us)
-            asm volatile("" : "+v"(sum_dp), "+v"(sum_d), "+v"(sum_ddp));
+            asm volatile("" : "+v"(sum_p), "+v"(sum_ds), "+v"(sum_d), "+v"(sum_dds));
+        } else if constexpr (SLOPE) {
+            sum_p += ((pe[0] + pe[1]) + (pe[2] + pe[3])) + ((pe[4] + pe[5]) + (pe[6] + pe[7]));
+            asm volatile("" : "+v"(sum_p));
         }
         if constexpr (C::F32) {
 #pragma unroll
@@ -951,13 +963,14 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
         }
     }
     sync_tiles();
+    if constexpr (SLOPE) sum_p = pair_sum(sum_p);
     if constexpr (DSLOPE) {
-        sum_dp = pair_sum(sum_dp);
+        sum_ds = pair_sum(sum_ds);
         sum_d = pair_sum(sum_d);
-        sum_ddp = pair_sum(sum_ddp);
+        sum_dds = pair_sum(sum_dds);
     }
     if constexpr (KS == 2) {
-        constexpr int NO = (D / 32) * 16, NF = NO + (DSLOPE ? 3 : 0);
+        constexpr int NO = (D / 32) * 16, NF = NO + (DSLOPE ? 4 : SLOPE ? 1 : 0);
         static_assert(4 * NF * 64 * 4 <= C::SMEM_BYTES, "a group's part fits its tile buffers");
         float* mg = reinterpret_cast<float*>(smem + C::SMEM_BYTES);
         auto at = [&](int f) FA_INLINE { return mg + (w * NF + f) * 64 + lane; };
@@ -966,10 +979,11 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
             for (int i = 0; i < D / 32; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) *at(16 * i + e) = dq[i][e];
+            if (SLOPE) *at(NO) = sum_p;
             if (DSLOPE) {
-                *at(NO) = sum_dp;
-                *at(NO + 1) = sum_d;
-                *at(NO + 2) = sum_ddp;
+                *at(NO + 1) = sum_ds;
+                *at(NO + 2) = sum_d;
+                *at(NO + 3) = sum_dds;
             }
         }
         lds_barrier();
@@ -978,19 +992,27 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
             for (int i = 0; i < D / 32; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) dq[i][e] += *at(16 * i + e);
+            if (SLOPE) sum_p += *at(NO);
             if (DSLOPE) {
-                sum_dp += *at(NO);
-                sum_d += *at(NO + 1);
-                sum_ddp += *at(NO + 2);
+                sum_ds += *at(NO + 1);
+                sum_d += *at(NO + 2);
+                sum_dds += *at(NO + 3);
             }
         }
     }
     const ScoredParams& pe = late_args();
+    float inv = 1.f;  // of sum P
+    if constexpr (SLOPE) {
+        const bool none = lse2 == INFINITY;  // a row that sees nothing
+        inv = none ? 1.f : 1.f / sum_p;
+        if (sp == 0 && hi == 0)
+            pe.lse2[((int64_t)b * pe.H + h) * pe.ws_stride + qi] = none ? lse2 : lse2 + __log2f(sum_p);
+    }
     if constexpr (DSLOPE) {
         if (sp == 0 && hi == 0 && qi < pe.Sq)
-            pe.dslope_rows[((int64_t)b * pe.H + h) * pe.Sq + qi] = __builtin_fmaf(sum_dp, sum_d, -sum_ddp);
+            pe.dslope_rows[((int64_t)b * pe.H + h) * pe.Sq + qi] = __builtin_fmaf(sum_ds * inv, sum_d, -sum_dds) * inv;
     }
-    store_rows<T, D>((T*)smem + w * 32 * C::OW, C::OW, dq, pe.scale * (CAP ? 4.f : 1.f),
+    store_rows<T, D>((T*)smem + w * 32 * C::OW, C::OW, dq, pe.scale * (CAP ? 4.f : 1.f) * inv,
                      (T*)pe.dq + b * pe.dq_sb + h * pe.dq_sh, pe.dq_ss, qw0, pe.Sq, pe.cols, lane, sp == 0);
 }
 

@@ -147,7 +147,9 @@ def flash_attention_v100_scored(
     the formula is in the module docstring.
 
     ``softcap``: bound of the tanh on the scores (0 or None: none).
-    ``distance_slopes``: float32 (H,) or (B, H), differentiable.
+    ``distance_slopes``: float32 (H,) or (B, H), differentiable.  Queries may stand
+    off the keys: results keep their digits at any distance, gradients while slope
+    times the distance to the nearest key stays below 2^30.
     ``documents``: integer ids (B, Sq) or (Sq,) of the queries' documents and,
     unless ``key_documents`` gives theirs, of the keys'; negative (or past int32):
     padding.

@@ -7,7 +7,7 @@ import torch
 import flash_attention_v100 as fa
 import ops_edges_oracle as eo
 import ops_oracle as oo
-from ops_edges_oracle import DEV, make
+from ops_edges_oracle import DEV, make, train
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,29 @@ def test_few_far_queries(off, dt):
         q, k, v, _ = make(2, Sq, Sk, 4, 2, 64, dt, seed=Sq)
         forward(q, k, v, slopes, off, f"{Sq} x {Sk}, {off} {dt}", causal=True)
         forward(q, k, v, slopes, -off, f"{Sq} x {Sk}, {-off} {dt}")
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("off", FAR)
+def test_slopes_of_far_queries(off, D, dt):
+    q, k, v, do = make(2, 70, 500, 4, 2, D, dt, seed=off % 1000)
+    slopes = torch.tensor([0.5, 0.0625, 0.01, 0.001], device=DEV)
+    train(q, k, v, do, f"offset {off} D={D} {dt}", causal=True, query_offsets=off, distance_slopes=slopes)
+    train(q, k, v, do, f"offset {-off} D={D} {dt}", query_offsets=-off, distance_slopes=slopes)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+def test_slopes_of_far_queries_of_other_calls(dt):
+    # offsets and lengths of each sequence (one inside the keys, one before the
+    # first), a cap, slopes of each sequence, negative ones too
+    q, k, v, do = make(4, 130, 300, 2, 1, 64, dt, seed=7)
+    off = torch.tensor([1 << 20, 200, -5, 100000], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([300, 120, 300, 1], dtype=torch.int32, device=DEV)
+    slopes = torch.tensor([[0.1, -0.004], [0.02, 0.3], [0.5, 0.0], [0.001, 1.0]], device=DEV)
+    for kw in ({}, {"softcap": 20.0}):
+        train(q, k, v, do, f"{kw} {dt}", query_offsets=off, key_lengths=lens, distance_slopes=slopes, **kw)
+    # a grid of one group of waves a block
+    q, k, v, do = make(5, 500, 300, 30, 30, 64, dt, seed=8)
+    slopes = torch.exp2(-8.0 * torch.arange(1, 31, device=DEV) / 30)
+    train(q, k, v, do, f"one group {dt}", causal=True, query_offsets=1 << 20, distance_slopes=slopes)
