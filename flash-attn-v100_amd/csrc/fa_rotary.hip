@@ -87,10 +87,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const
         constexpr int NP = INTER ? V / 2 : V;  // pairs of an item
         float c[NP > 0 ? NP : 1], s[NP > 0 ? NP : 1];
 #pragma unroll
-        for (int e = 0; e < NP; ++e) {
-            c[e] = 1.f;
-            s[e] = 0.f;
-        }
+        for (int e = 0; e < NP; ++e) c[e] = s[e] = 0.f;
         if (rot && pos >= 0) {
             const float* row = p.table + (pos < p.n_pos ? pos : 0) * p.R + item * NP;
             const Pack<float, (NP > 4 ? 4 : NP)>* cp = (const Pack<float, (NP > 4 ? 4 : NP)>*)row;
@@ -141,7 +138,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p, const
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (h0 + u * step >= heads) break;
-                if (rot) {
+                if (rot && pos >= 0) {  // (else copied: times 1 and 0 an infinity would become NaN, -0 a 0)
 #pragma unroll
                     for (int e = 0; e < NP; ++e) {
                         T& p0 = INTER ? a[u].e[(2 * e) % V] : a[u].e[e];
