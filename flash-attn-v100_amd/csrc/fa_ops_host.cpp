@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
@@ -138,6 +139,21 @@ PyObject* wrap_or_none(const at::Tensor& t) {
 // to their own checks, which name what is wrong.
 bool element_type(const at::Tensor& t) { return dtype_code(t.scalar_type()) >= 0; }
 
+// A tensor of forward-mode differentiation, whose tangent a kernel would drop.  (It
+// need not require grad; torch has one level of them.)
+bool dual(const at::Tensor& t) {
+    return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined();
+}
+
+// dual(tensor or None, ...): whether one of them is
+PyObject* any_dual(PyObject*, PyObject* const* x, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    for (Py_ssize_t i = 0; i < n; ++i)
+        if (THPVariable_Check(x[i]) && dual(THPVariable_Unpack(x[i]))) Py_RETURN_TRUE;
+    Py_RETURN_FALSE;
+    END_HANDLE_TH_ERRORS
+}
+
 // qkv_ok(q, k, v, largest head dim)
 PyObject* qkv_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -151,7 +167,7 @@ PyObject* qkv_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
     const bool ok = q.is_cuda() && k.device() == q.device() && v.device() == q.device() && element_type(q) &&
                     k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() &&
                     k.size(0) == q.size(0) && k.size(3) == D && k.sizes() == v.sizes() && Hkv > 0 && H > 0 &&
-                    H % Hkv == 0 && D > 0 && D <= most;
+                    H % Hkv == 0 && D > 0 && D <= most && !dual(q) && !dual(k) && !dual(v);
     return PyBool_FromLong(ok);
     END_HANDLE_TH_ERRORS
 }
@@ -166,11 +182,12 @@ PyObject* rotary_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
     if (q.dim() != 4 || t.dim() != 2) Py_RETURN_FALSE;
     const int64_t B = q.size(0), S = q.size(1), D = q.size(3), R = t.size(1);
     bool ok = q.is_cuda() && element_type(q) && q.size(2) > 0 && D <= 256 && t.device() == q.device() &&
-              t.scalar_type() == at::kFloat && !t.requires_grad() && R >= 2 && R % 2 == 0 && R <= D && t.size(0) > 0;
+              t.scalar_type() == at::kFloat && !t.requires_grad() && R >= 2 && R % 2 == 0 && R <= D && t.size(0) > 0 &&
+              !dual(q) && !dual(t);
     if (ok && !none(x[1])) {
         const at::Tensor& k = THPVariable_Unpack(x[1]);
         ok = k.dim() == 4 && k.device() == q.device() && k.scalar_type() == q.scalar_type() && k.size(0) == B &&
-             k.size(1) == S && k.size(2) > 0 && k.size(3) == D;
+             k.size(1) == S && k.size(2) > 0 && k.size(3) == D && !dual(k);
     }
     if (ok && !none(x[3])) {
         const at::Tensor& p = THPVariable_Unpack(x[3]);
@@ -437,6 +454,7 @@ PyObject* bind_ops(PyObject*, PyObject* const* x, Py_ssize_t n) {
 
 PyMethodDef fa_host::ops_methods[] = {
     {"bind_ops", (PyCFunction)(void*)bind_ops, METH_FASTCALL, nullptr},
+    {"dual", (PyCFunction)(void*)any_dual, METH_FASTCALL, nullptr},
     {"qkv_ok", (PyCFunction)(void*)qkv_ok, METH_FASTCALL, nullptr},
     {"rotary_ok", (PyCFunction)(void*)rotary_ok, METH_FASTCALL, nullptr},
     {"scored_fwd", (PyCFunction)(void*)scored_fwd, METH_FASTCALL, nullptr},

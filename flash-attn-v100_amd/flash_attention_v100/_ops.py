@@ -192,6 +192,12 @@ def rotary_table(positions: int, rotary_dim: int, scaling: int, base: float, fac
     return table
 
 
+def check_dual(what: str, *inputs) -> None:
+    """Refuses inputs of forward-mode differentiation: their tangents would be lost."""
+    if host().dual(*inputs):
+        raise NotImplementedError(f"{what} has no forward-mode derivative (torch.autograd.forward_ad)")
+
+
 def check_capture(*inputs) -> None:
     """Refuses a call to be differentiated inside a stream capture on an input
     whose gradient would leave the capture: one whose node another stream made, as

@@ -123,6 +123,7 @@ def _disjoint(q: torch.Tensor, k: torch.Tensor) -> bool:
 
 def _check_inputs(q, k, table, positions):
     """Raises for what the rotation does not take; positions as (B, S)."""
+    _ops.check_dual("rotary_embedding_v100", q, k, table)
     for name, t in (("q", q), ("k", k)):
         if t is None and name == "k":
             continue
@@ -176,7 +177,8 @@ def rotary_embedding_v100(
     negative position is left as it is, one at a position past the table becomes
     NaN.  ``inplace`` writes into q and k and returns them (refused for inputs
     that require grad while grad mode is on, and for inputs whose elements
-    overlap).  Differentiable in q and k.
+    overlap).  Differentiable in q and k, not in forward mode
+    (``NotImplementedError``).
     """
     if not _ops.host().rotary_ok(q, k, table, positions):
         positions = _check_inputs(q, k, table, positions)

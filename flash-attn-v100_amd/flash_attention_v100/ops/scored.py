@@ -32,6 +32,7 @@ def check_qkv(q, k, v, what: str) -> None:
     """Shapes, dtypes and devices of q (B, Sq, H, D) and k, v (B, Sk, Hkv, D)."""
     if _ops.host().qkv_ok(q, k, v, _ops.MAX_HEAD_DIM):
         return
+    _ops.check_dual(what, q, k, v)
     for t in (q, k, v):
         if not isinstance(t, torch.Tensor):
             raise TypeError("q, k, v must be torch.Tensor instances")
@@ -78,6 +79,7 @@ def check_slopes(slopes, B: int, H: int, device):
                          f"{tuple(slopes.shape)}")
     if slopes.device != device:
         raise ValueError(f"distance_slopes must be on {device}, got {slopes.device}")
+    _ops.check_dual("distance_slopes", slopes)
     return slopes
 
 
@@ -162,7 +164,7 @@ def flash_attention_v100_scored(
 
     Head dims up to 128 (``NotImplementedError`` above), fp16 / bf16 / fp32.
     Returns O, or (O, LSE) with ``return_softmax_lse``; gradients of q, k, v and
-    ``distance_slopes``.  Forward and backward may be captured into a HIP graph;
+    ``distance_slopes``, none in forward mode (``NotImplementedError``).  Forward and backward may be captured into a HIP graph;
     inputs that an eager graph of another stream still holds are refused there
     (``RuntimeError``).
     """

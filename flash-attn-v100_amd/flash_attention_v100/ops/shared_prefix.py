@@ -50,6 +50,7 @@ def flash_attention_v100_shared_prefix(
                              f"{tuple(v_prefix.shape) if isinstance(v_prefix, torch.Tensor) else v_prefix}")
         if t.dtype != q.dtype or t.device != q.device:
             raise ValueError("k_prefix, v_prefix must have the dtype and device of q")
+    _ops.check_dual("flash_attention_v100_shared_prefix", k_prefix, v_prefix)
     scale = check_scale(scale, D)
     softcap = check_softcap(softcap)
     slopes = check_slopes(distance_slopes, B, H, q.device)

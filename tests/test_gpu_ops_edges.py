@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import flash_attention_v100 as fa
-from ops_edges_oracle import DEV, DT
+from ops_edges_oracle import DEV, DT, make
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,26 @@ def test_tokens_at_negative_positions_keep_their_bits(D, R, inter, dt):
     z = fa.rotary_embedding_v100(x, None, table, pos, interleaved=inter, inplace=True)
     assert z is x or z.data_ptr() == x.data_ptr()
     assert torch.equal(x.view(bits), y.detach().view(bits))
+
+
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as ad
+
+    q, k, v, _ = make(1, 4, 4, 2, 2, 64, "fp32")
+    slopes = torch.ones(2, device=DEV)
+    table = fa.rotary_table_v100(8, 64, device=DEV)
+    calls = {
+        "scored": (lambda q, k, v, s: fa.flash_attention_v100_scored(q, k, v, distance_slopes=s), (q, k, v, slopes)),
+        "shared": (lambda q, kp, vp, k, v, s: fa.flash_attention_v100_shared_prefix(q, kp, vp, k, v, distance_slopes=s),
+                   (q, k[0], v[0], k, v, slopes)),
+        "rotary": (lambda q, k: fa.rotary_embedding_v100(q, k, table)[0], (q, k)),
+        "rotary, one": (lambda q: fa.rotary_embedding_v100(q, None, table, inplace=True), (q,)),
+    }
+    for name, (f, args) in calls.items():
+        for i in range(len(args)):
+            with ad.dual_level(), torch.no_grad():
+                dual = [ad.make_dual(t, torch.ones_like(t)) if n == i else t for n, t in enumerate(args)]
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    f(*dual)
+                ad.unpack_dual(f(*args))  # a level without duals changes nothing
+        print(name, "refused", flush=True)
