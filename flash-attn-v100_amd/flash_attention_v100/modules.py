@@ -162,8 +162,10 @@ class EnhancedMultiHeadAttention(nn.Module):
         if t is None:
             if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("call the layer once before it is captured: its rotary table is made on first use")
-            t = rotary_table_v100(self.max_positions, self.rotary_dim, self.rotary_base, device=device,
-                                  **self.rotary_scaling)
+            # kept for training too, also where the first call runs in inference mode
+            with torch.inference_mode(False):
+                t = rotary_table_v100(self.max_positions, self.rotary_dim, self.rotary_base, device=device,
+                                      **self.rotary_scaling)
             # made on this stream, read on any: whole before another can see it
             torch.cuda.current_stream(device).synchronize()
             self._tables[device] = t

@@ -60,3 +60,15 @@ def test_forward_mode_derivatives_are_refused():
                     f(*dual)
                 ad.unpack_dual(f(*args))  # a level without duals changes nothing
         print(name, "refused", flush=True)
+
+
+def test_layer_trains_after_inference_mode():
+    torch.manual_seed(3)
+    m = fa.EnhancedMultiHeadAttention(64, 2, rotary_dim=16, softcap=20.0).to(DEV).half()
+    x = torch.randn(2, 30, 64, device=DEV, dtype=torch.half)
+    with torch.inference_mode():
+        a = m(x, is_causal=True)[0]
+    y = m(x, is_causal=True)[0]
+    assert torch.equal(a, y)
+    y.sum().backward()
+    assert m.q_proj.weight.grad is not None

@@ -1,10 +1,13 @@
 """Calls of the operators around attention at the edge of what they document, as far
 as a machine without a GPU shows it."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 import torch.autograd.forward_ad as ad
 
 import flash_attention_v100 as fa
+from flash_attention_v100 import modules
 
 
 def test_forward_mode_derivatives_are_refused():
@@ -22,3 +25,25 @@ def test_forward_mode_derivatives_are_refused():
                     f(*dual)
             with pytest.raises(ValueError, match="no CPU path"):
                 f(*args)
+
+
+def fake_tables(monkeypatch):
+    """rotary_table_v100 of the layer on the CPU: its arguments, in order of the calls."""
+    calls = []
+
+    def table(n, dim, base, device=None, **kw):
+        calls.append((n, dim, base, tuple(sorted(kw.items()))))
+        return torch.zeros(n, dim)
+
+    monkeypatch.setattr(modules, "rotary_table_v100", table)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: SimpleNamespace(synchronize=lambda: None))
+    return calls
+
+
+def test_layer_table_of_inference_mode_serves_training(monkeypatch):
+    calls = fake_tables(monkeypatch)
+    m = fa.EnhancedMultiHeadAttention(64, 4, rotary_dim=16)
+    with torch.inference_mode():
+        t = m._rotary_table(torch.device("cpu"))
+    assert not t.is_inference()
+    assert m._rotary_table(torch.device("cpu")) is t and len(calls) == 1
