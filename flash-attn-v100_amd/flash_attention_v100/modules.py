@@ -127,7 +127,7 @@ class EnhancedMultiHeadAttention(nn.Module):
         self.rotary_scaling, self.max_positions = dict(rotary_scaling or {}), max_positions
         self.softcap = softcap
         self.distance_slopes = nn.Parameter(torch.empty(num_heads)) if distance_bias else None
-        self._tables = {}  # rotary table of each device
+        self._tables = {}  # rotary table of each device and set of options
         self.forward_count = 0
         self._times_ms = []
         self._pending = []
@@ -158,17 +158,20 @@ class EnhancedMultiHeadAttention(nn.Module):
             self.distance_slopes = None
 
     def _rotary_table(self, device: torch.device) -> torch.Tensor:
-        t = self._tables.get(device)
+        # (a table of earlier options stays: a graph captured with it may be replayed)
+        key = (device, self.max_positions, self.rotary_dim, self.rotary_base, tuple(sorted(self.rotary_scaling.items())))
+        t = self._tables.get(key)
         if t is None:
             if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("call the layer once before it is captured: its rotary table is made on first use")
+                raise RuntimeError("call the layer once before it is captured: its rotary table is made on first use, and "
+                                   "again after a change of its options")
             # kept for training too, also where the first call runs in inference mode
             with torch.inference_mode(False):
                 t = rotary_table_v100(self.max_positions, self.rotary_dim, self.rotary_base, device=device,
                                       **self.rotary_scaling)
             # made on this stream, read on any: whole before another can see it
             torch.cuda.current_stream(device).synchronize()
-            self._tables[device] = t
+            self._tables[key] = t
         return t
 
     def _scored(self, q, k, v, attn_mask, key_padding_mask, is_causal, documents):

@@ -72,3 +72,17 @@ def test_layer_trains_after_inference_mode():
     assert torch.equal(a, y)
     y.sum().backward()
     assert m.q_proj.weight.grad is not None
+
+
+def test_layer_follows_its_rotary_options():
+    torch.manual_seed(4)
+    kw = dict(rotary_dim=16, rotary_base=500.0, rotary_scaling={"scaling": "linear", "factor": 2.0}, max_positions=64)
+    m = fa.EnhancedMultiHeadAttention(64, 2, rotary_dim=16, max_positions=32).to(DEV).half()
+    n = fa.EnhancedMultiHeadAttention(64, 2, **kw).to(DEV).half()
+    n.load_state_dict(m.state_dict())
+    x = torch.randn(1, 50, 64, device=DEV, dtype=torch.half)
+    with torch.no_grad():
+        m(x[:, :30])
+        m.rotary_base, m.max_positions = 500.0, 64
+        m.rotary_scaling.update(kw["rotary_scaling"])
+        assert torch.equal(m(x, is_causal=True)[0], n(x, is_causal=True)[0])

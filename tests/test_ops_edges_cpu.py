@@ -47,3 +47,23 @@ def test_layer_table_of_inference_mode_serves_training(monkeypatch):
         t = m._rotary_table(torch.device("cpu"))
     assert not t.is_inference()
     assert m._rotary_table(torch.device("cpu")) is t and len(calls) == 1
+
+
+def test_layer_table_follows_the_options(monkeypatch):
+    calls = fake_tables(monkeypatch)
+    cpu = torch.device("cpu")
+    m = fa.EnhancedMultiHeadAttention(64, 4, rotary_dim=16, max_positions=32)
+    t = m._rotary_table(cpu)
+    for change in (lambda: setattr(m, "max_positions", 64), lambda: setattr(m, "rotary_base", 500.0),
+                   lambda: setattr(m, "rotary_dim", 8), lambda: m.rotary_scaling.update(scaling="linear", factor=2.0)):
+        change()
+        u = m._rotary_table(cpu)
+        assert u is not t and m._rotary_table(cpu) is u
+        t = u
+    assert calls == [(32, 16, 1e4, ()), (64, 16, 1e4, ()), (64, 16, 500.0, ()), (64, 8, 500.0, ()),
+                     (64, 8, 500.0, (("factor", 2.0), ("scaling", "linear")))]
+    # an earlier table is kept: a captured graph may read it
+    assert len(m._tables) == 5
+    m.rotary_dim, m.rotary_base, m.max_positions, m.rotary_scaling = 16, 1e4, 32, {}
+    m._rotary_table(cpu)
+    assert len(calls) == 5
