@@ -78,12 +78,14 @@ size_t doc_bytes(int32_t B, int32_t S) {
     const size_t n = (size_t)B * doc_pad(S);
     return up256(n * 4) + up256(n / 64 * sizeof(int2));
 }
+// (an empty side's array may be null: with no token there the documents rule nothing)
+bool has_docs(const fa_scored_args* a) { return a->q_documents && a->k_documents; }
 bool one_doc_array(const fa_scored_args* a) {
     return a->q_documents == a->k_documents && a->seqlen_q == a->seqlen_k &&
            a->q_documents_stride == a->k_documents_stride;
 }
 size_t docs_bytes(const fa_scored_args* a) {
-    if (!a->q_documents) return 0;
+    if (!has_docs(a)) return 0;
     return doc_bytes(a->batch, a->seqlen_k) + (one_doc_array(a) ? 0 : doc_bytes(a->batch, a->seqlen_q));
 }
 hipError_t make_docs(const int32_t* ids, int64_t sb, int32_t B, int32_t S, char*& ws, const int*& out, const int2*& rng,
@@ -106,7 +108,7 @@ hipError_t put_docs(const fa_scored_args* a, ScoredParams& p, char*& ws, hipStre
     p.q_docs = p.k_docs = nullptr;
     p.q_rng = p.k_rng = nullptr;
     p.q_docs_pad = p.k_docs_pad = 0;
-    if (!a->q_documents) return hipSuccess;
+    if (!has_docs(a)) return hipSuccess;
     hipError_t e = make_docs(a->k_documents, a->k_documents_stride, a->batch, a->seqlen_k, ws, p.k_docs, p.k_rng,
                              p.k_docs_pad, s);
     if (e != hipSuccess) return e;
@@ -222,7 +224,7 @@ hipError_t run_rows(const RowsParams& p, int32_t dtype, hipStream_t s) {
 //   outside the rule: (128, 128, 512, 16 of 128) 149 / 243; (64, 128, 128, 16 of
 //   64) 21 / 41; (64, 16, 16, 16 of 64) 11.7 / 12.2
 bool few_rows(const fa_scored_args* a, RowsParams& r) {
-    if (a->q_documents || a->prefix_lengths || a->seqlen_k == 0) return false;
+    if (has_docs(a) || a->prefix_lengths || a->seqlen_k == 0) return false;
     if (a->seqlen_k < 4 * (int64_t)a->seqlen_q) return false;
     const int64_t blocks = ceil_div<int64_t>(a->seqlen_q, 128) * a->num_heads * a->batch;
     if (a->seqlen_q > 32 && blocks > 128) return false;
@@ -266,7 +268,7 @@ bool few_rows(const fa_scored_args* a, RowsParams& r) {
 int kv_parts(const fa_scored_args* a) {
     const int64_t n = ceil_div<int64_t>(a->seqlen_k, 128) * a->num_heads_kv * a->batch;
     // queries of a walk (with documents, those of its own: half of all are taken)
-    const int64_t walk = (int64_t)(a->num_heads / a->num_heads_kv) * a->seqlen_q / (a->q_documents ? 2 : 1);
+    const int64_t walk = (int64_t)(a->num_heads / a->num_heads_kv) * a->seqlen_q / (has_docs(a) ? 2 : 1);
     int parts = 1;
     const int64_t most = a->causal ? 512 : 256;
     while (parts < 8 && n * parts <= most && walk >= (n * parts <= 128 ? 512 * parts : 1024 * parts + 1)) parts *= 2;
@@ -294,10 +296,11 @@ int32_t fa_scored_check(const fa_scored_args* a, int32_t backward) {
                              a->scale, a->softcap);
     if (st) return st;
     if ((st = check_slopes(a->slopes, a->slopes_batch_stride, a->num_heads))) return st;
-    if (!a->q_documents != !a->k_documents) return FA_ERR_RULE;
+    const bool any = a->batch > 0 && a->seqlen_q > 0 && a->seqlen_k > 0;
+    if (any && !a->q_documents != !a->k_documents) return FA_ERR_RULE;
     for (const int32_t* x : {a->prefix_lengths, a->key_lengths, a->query_offsets, a->q_documents, a->k_documents})
         if (!aligned(x, 4)) return FA_ERR_ALIGN;
-    if (a->q_documents) {
+    if (has_docs(a)) {
         for (int64_t x : {a->q_documents_stride, a->k_documents_stride})
             if (x < 0 || x > kMaxStride) return FA_ERR_RULE;
         if ((int64_t)a->batch * (doc_pad(std::max(a->seqlen_q, a->seqlen_k)) / 64) >= (1LL << 31)) return FA_ERR_TOO_LARGE;

@@ -72,7 +72,7 @@ typedef struct fa_scored_args {
     const int32_t* key_lengths;    /* optional (B) */
     const int32_t* query_offsets;  /* optional (B), else query_offset; held within +-2^30 */
     int32_t query_offset;
-    const int32_t* q_documents;    /* optional (B, Sq), both or none; token stride 1 */
+    const int32_t* q_documents;    /* optional (B, Sq), both or none (any, where one side is empty); token stride 1 */
     const int32_t* k_documents;    /* optional (B, Sk); may be q_documents */
     int64_t q_documents_stride;    /* batch strides in elements */
     int64_t k_documents_stride;

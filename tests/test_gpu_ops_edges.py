@@ -86,3 +86,18 @@ def test_layer_follows_its_rotary_options():
         m.rotary_base, m.max_positions = 500.0, 64
         m.rotary_scaling.update(kw["rotary_scaling"])
         assert torch.equal(m(x, is_causal=True)[0], n(x, is_causal=True)[0])
+
+
+@pytest.mark.parametrize("Sq,Sk", [(0, 5), (5, 0), (0, 0), (0, 300), (300, 0)])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_documents_of_empty_sides(Sq, Sk, dt):
+    q, k, v, do = make(2, Sq, Sk, 2, 1, 64, dt)
+    q, k, v = (t.requires_grad_(True) for t in (q, k, v))
+    s = torch.ones(2, device=DEV).requires_grad_(True)
+    for idt in (torch.int32, torch.int64):
+        ids = lambda n: torch.zeros(2, n, dtype=idt, device=DEV)  # noqa: E731
+        o, lse = fa.flash_attention_v100_scored(q, k, v, documents=ids(Sq), key_documents=ids(Sk), distance_slopes=s,
+                                                return_softmax_lse=True)
+        assert o.shape == q.shape and not o.any() and (lse == -math.inf).all()
+        for g in torch.autograd.grad(o, (q, k, v, s), do):
+            assert not g.any()

@@ -1,5 +1,6 @@
 """Calls of the operators around attention at the edge of what they document, as far
 as a machine without a GPU shows it."""
+import ctypes
 from types import SimpleNamespace
 
 import pytest
@@ -7,7 +8,8 @@ import torch
 import torch.autograd.forward_ad as ad
 
 import flash_attention_v100 as fa
-from flash_attention_v100 import modules
+from flash_attention_v100 import _ops, modules
+from test_ops_cpu import ADDR, CODES, scored_args
 
 
 def test_forward_mode_derivatives_are_refused():
@@ -67,3 +69,16 @@ def test_layer_table_follows_the_options(monkeypatch):
     m.rotary_dim, m.rotary_base, m.max_positions, m.rotary_scaling = 16, 1e4, 32, {}
     m._rotary_table(cpu)
     assert len(calls) == 5
+
+
+@pytest.mark.parametrize("Sq,Sk,q_ids,k_ids", [(0, 5, None, ADDR), (5, 0, ADDR, None), (0, 0, None, None),
+                                               (0, 5, ADDR, None), (5, 5, None, None)])
+def test_documents_of_empty_sides(Sq, Sk, q_ids, k_ids):
+    # an empty tensor's address is null: no sign of a missing array
+    lib, a = _ops.load(), scored_args(Sq=Sq, Sk=Sk)
+    a.q_documents, a.k_documents = q_ids, k_ids
+    for backward in (0, 1):
+        assert lib.fa_scored_check(ctypes.byref(a), backward) == 0
+    assert lib.fa_scored_fwd_workspace_size(ctypes.byref(a)) == 0
+    a.seqlen_q = a.seqlen_k = 5
+    assert lib.fa_scored_check(ctypes.byref(a), 0) == (CODES["FA_ERR_RULE"] if (q_ids is None) != (k_ids is None) else 0)
