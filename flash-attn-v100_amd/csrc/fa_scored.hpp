@@ -662,8 +662,9 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
 
 // ---------------------------------------------------------------------------
 // dQ, and per query the rows LSE * log2 e and delta = rowsum(dO O) that the
-// dK/dV pass reads after it.  dS goes through the cap's derivative (/ 4, made up
-// for in the final scale).
+// dK/dV pass reads after it.  Cap: both passes hold 4 P (the exponent is 2 larger), as
+// the derivative comes divided by 4: dS through it is then what it is, and fp16 rounds
+// neither it nor P sooner as a subnormal number.
 // SLOPE: P is e^(s - LSE), and the LSE of a query far from the keys is a large number
 // whose rounding is a factor on its row.  The row's sum of P takes it out again: of
 // dQ at the end, and of the LSE that goes to the dK/dV pass (while slope times the
@@ -723,9 +724,9 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
     const float slope2 = has_slope<CAP, SLOPE>(p) ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
     // of distances from the nearest key; a row that sees nothing, and rows past the
     // last: P = exp2(s - inf) = 0
-    const float lse2 = lse_in == -INFINITY ? INFINITY
-                       : SLOPE             ? __builtin_fmaf(slope2, rule.far(qi), lse_in * kLog2e)
-                                           : lse_in * kLog2e;
+    const float lse2 = (lse_in == -INFINITY ? INFINITY
+                        : SLOPE             ? __builtin_fmaf(slope2, rule.far(qi), lse_in * kLog2e)
+                                            : lse_in * kLog2e) - (CAP ? 2.f : 0.f);
     if (sp == 0 && hi == 0) {
         const int64_t wi = ((int64_t)b * p.H + h) * p.ws_stride + qi;  // qi < sq_pad
         if constexpr (!SLOPE) p.lse2[wi] = lse2;  // (else at the end)
@@ -1001,18 +1002,19 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
         }
     }
     const ScoredParams& pe = late_args();
-    float inv = 1.f;  // of sum P
+    constexpr float kP = CAP ? 4.f : 1.f;  // sums hold kP P
+    float inv = 1.f;                       // of sum P
     if constexpr (SLOPE) {
         const bool none = lse2 == INFINITY;  // a row that sees nothing
-        inv = none ? 1.f : 1.f / sum_p;
+        inv = none ? 1.f : kP / sum_p;
         if (sp == 0 && hi == 0)
-            pe.lse2[((int64_t)b * pe.H + h) * pe.ws_stride + qi] = none ? lse2 : lse2 + __log2f(sum_p);
+            pe.lse2[((int64_t)b * pe.H + h) * pe.ws_stride + qi] = none ? lse2 : lse2 + __log2f(sum_p * (1.f / kP));
     }
     if constexpr (DSLOPE) {
         if (sp == 0 && hi == 0 && qi < pe.Sq)
-            pe.dslope_rows[((int64_t)b * pe.H + h) * pe.Sq + qi] = __builtin_fmaf(sum_ds * inv, sum_d, -sum_dds) * inv;
+            pe.dslope_rows[((int64_t)b * pe.H + h) * pe.Sq + qi] = __builtin_fmaf(sum_ds * (inv / kP), sum_d, -sum_dds) * (inv / kP);
     }
-    store_rows<T, D>((T*)smem + w * 32 * C::OW, C::OW, dq, pe.scale * (CAP ? 4.f : 1.f) * inv,
+    store_rows<T, D>((T*)smem + w * 32 * C::OW, C::OW, dq, pe.scale * inv,
                      (T*)pe.dq + b * pe.dq_sb + h * pe.dq_sh, pe.dq_ss, qw0, pe.Sq, pe.cols, lane, sp == 0);
 }
 
@@ -1397,16 +1399,16 @@ __global__ __launch_bounds__(256, (!(Elem<T>::kF32 && D == 128) ? 2 : 1)) void s
         return;
     }
     T* const Os = (T*)smem + w * 32 * C::OW;
-    store_rows<T, D>(Os, C::OW, dk, -pe.scale * (CAP ? 4.f : 1.f), (T*)pe.dk + b * pe.dk_sb + hk * pe.dk_sh, pe.dk_ss, kw0,
+    store_rows<T, D>(Os, C::OW, dk, -pe.scale, (T*)pe.dk + b * pe.dk_sb + hk * pe.dk_sh, pe.dk_ss, kw0,
                      pe.Sk, pe.cols, lane, true);
     lds_barrier();
-    store_rows<T, D>(Os, C::OW, dv, 1.f, (T*)pe.dv + b * pe.dv_sb + hk * pe.dv_sh, pe.dv_ss, kw0, pe.Sk, pe.cols, lane, true);
+    store_rows<T, D>(Os, C::OW, dv, CAP ? 0.25f : 1.f, (T*)pe.dv + b * pe.dv_sb + hk * pe.dv_sh, pe.dv_ss, kw0, pe.Sk, pe.cols, lane, true);
 }
 
 // dK and dV from the float32 parts of a KV head (every n-th query tile each): one
 // thread 4 columns of a key, the parts in order
 template <typename T, int D>
-__global__ __launch_bounds__(256) void kv_sum_kernel(const ScoredParams p, const float k_mul) {
+__global__ __launch_bounds__(256) void kv_sum_kernel(const ScoredParams p, const float k_mul, const float v_mul) {
     const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int col = (int)(gid % (D / 4)) * 4;
     const int64_t r = gid / (D / 4);  // ((b Hkv + hk) 2 + which) Sk + key
@@ -1422,7 +1424,7 @@ __global__ __launch_bounds__(256) void kv_sum_kernel(const ScoredParams p, const
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] += y[e];
     }
-    const float mul = which ? 1.f : k_mul;
+    const float mul = which ? v_mul : k_mul;
     T* out = which ? (T*)p.dv + b * p.dv_sb + (int64_t)key * p.dv_ss + hk * p.dv_sh
                    : (T*)p.dk + b * p.dk_sb + (int64_t)key * p.dk_ss + hk * p.dk_sh;
     if constexpr (Elem<T>::kF32) {
@@ -1513,7 +1515,7 @@ hipError_t launch_scored_bwd_t(ScoredParams p, hipStream_t s) {
     if (nk > 0 && p.kv_parts > 1) {
         const int64_t nt = (int64_t)p.B * p.Hkv * 2 * p.Sk * (D / 4);
         hipLaunchKernelGGL((kv_sum_kernel<T, D>), dim3((unsigned)((nt + 255) / 256)), dim3(256), 0, s, p,
-                           -p.scale * (CAP ? 4.f : 1.f));
+                           -p.scale, CAP ? 0.25f : 1.f);
     }
     return hipGetLastError();
 }

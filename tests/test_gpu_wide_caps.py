@@ -1,11 +1,12 @@
 """Caps far above the scores: for |x| far below the cap the result is that without
-one, within bounds that do not grow with the cap."""
+one, within bounds that do not grow with the cap.  Small gradients under a cap."""
 import pytest
 import torch
 
 import flash_attention_v100 as fa
 import ops_edges_oracle as eo
 import ops_oracle as oo
+import test_gpu_scored as ts
 from ops_edges_oracle import DEV, make, train
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +57,15 @@ def test_wide_caps_of_tokens_and_prefixes(cap, dt):
         seen = oo.seen_mask(B, 1, n + 100, True, None, None, None, all_lens, all_lens - 1, DEV)
         ref = eo.scored(q, cat(kp, k), cat(vp, v), None, cap, None, all_lens - 1, seen, all_lens)
         oo.check(got, ref, ["o", "lse"], f"prefix {n} {cap} {dt}")
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("Sq,Sk,D", [(1, 512, 64), (2, 2048, 128), (40, 1500, 32)])
+def test_small_gradients_under_a_cap(Sq, Sk, D, dt):
+    # dS of some 1e-5 and less is subnormal in fp16: rounded once, at its own size
+    q, k, v, do = make(1, Sq, Sk, 2, 2, D, dt, seed=Sq)
+    for kw in ({}, {"distance_slopes": torch.tensor([0.0625, 0.00390625], device=DEV)}):
+        for cap in (2.0, 300.0):
+            got, ref, names, _ = ts.run(q, k, v, do, softcap=cap, **dict(kw))
+            oo.check(got, ref, names, f"{Sq} x {Sk}, {cap} {sorted(kw)}")
