@@ -186,7 +186,16 @@ void plan_rows(RowsParams& p, int32_t dtype) {
     auto splits = [&](int64_t nt, int64_t least) {
         return (int)std::max<int64_t>(1, std::min<int64_t>(64, ceil_div(nt, std::max<int64_t>(chunk, least))));
     };
-    p.o_splits = p.joined ? 1 : splits(ont, 8);
+    // A cache alone is joined for its own parts only: one part under 16 tiles, and where
+    // the device is full, whole parts that fit it once (sequences, queries, keys, query
+    // heads on KV heads of a size; us with the parts of the rule above / with these):
+    // (1, 1, 600, 8 of 64) 11.0 / 9.5; (2, 128, 600, 32 on 4 of 128) 21.1 / 12.9, 1600
+    // keys 26.6 / 20.9; (1, 400, 1600, 32 on 4 of 128) 41.8 / 26.7; (16, 1, 1600, 32 on 8
+    // of 128) 25.8 / 26.4
+    if (p.P == 0)
+        p.o_splits = ont < 16 ? 1 : chunk > 8 ? (int)std::max<int64_t>(1, std::min<int64_t>(64, ont / chunk)) : splits(ont, 8);
+    else
+        p.o_splits = p.joined ? 1 : splits(ont, 8);
     p.p_splits = pu ? splits(pnt, p.p_unit == 128 ? 4 : 8) : 0;
     p.p_wgs = pu * p.p_splits;
     p.o_wgs = ou * p.o_splits;
@@ -217,12 +226,13 @@ hipError_t run_rows(const RowsParams& p, int32_t dtype, hipStream_t s) {
 // other one that is half of the device, over keys of at least four times their
 // number.  us, the 128-query kernel against this one (sequences, queries, keys, query
 // heads on KV heads of a size; bf16, causal at the end of the keys):
-//   (16, 1, 8192, 32 on 8 of 128) 313 / 114; 16 queries 315 / 134, 32 306 / 188,
-//   64 330 / 293; (1, 16, 8192, 32 on 8 of 128) 127 / 18, 128 queries 133 / 41, 512
-//   134 / 106; (1, 1024, 4096, 8 of 128) 68 / 42; (64, 16, 700, 16 of 64) 41 / 35, 64
-//   queries 42 / 43; (2, 128, 600, 32 on 4 of 128) 19 / 22;
-//   outside the rule: (128, 128, 512, 16 of 128) 149 / 243; (64, 128, 128, 16 of
-//   64) 21 / 41; (64, 16, 16, 16 of 64) 11.7 / 12.2
+//   (16, 1, 8192, 32 on 8 of 128) 291 / 108; (1, 1, 600, 8 of 64) 13.7 / 9.5; (64, 16, 700,
+//   16 of 64) 41 / 34; (64, 32, 1000, 32 on 8 of 128) 141 / 95; (128, 8, 64, 16 of 64)
+//   18.9 / 19.2; (2, 128, 600, 32 on 4 of 128) 19.1 / 13.1; (1, 1024, 4096, 8 of 128) 67 /
+//   40; (1, 400, 2500, 32 on 8 of 128) 48 / 37; (4, 128, 512, 32 on 8 of 128) 17.6 / 16.7
+//   outside the rule: (16, 64, 8192, 32 on 8 of 128) 303 / 274; (64, 64, 700, 16 of 64)
+//   42 / 43; (128, 128, 512, 16 of 128) 149 / 243; (64, 128, 128, 16 of 64) 21 / 41; (64,
+//   16, 16, 16 of 64) 11.7 / 12.2
 bool few_rows(const fa_scored_args* a, RowsParams& r) {
     if (has_docs(a) || a->prefix_lengths || a->seqlen_k == 0) return false;
     if (a->seqlen_k < 4 * (int64_t)a->seqlen_q) return false;

@@ -1441,18 +1441,29 @@ __global__ __launch_bounds__(256) void kv_sum_kernel(const ScoredParams p, const
 // launchers (instantiated in fa_scored_{fwd,bwd}_*.hip)
 // Grids whose blocks get two groups of waves (a workgroup of 512 threads a CU), each
 // on every other tile, so that the longest walk takes half: those of fewer
-// workgroups than CUs, and causal ones of at most two workgroups a CU, whose last
-// blocks' walks are the time.  Forward / backward us, one group against two:
+// workgroups than CUs, and causal ones of at most two workgroups a CU on every XCD,
+// whose last blocks' walks are the time.  A group has the start and the end of a
+// block to do for half of its tiles, so short walks take one; the walks over
+// documents are as long as these, which the host does not know: there only long
+// sequences count.  Forward / backward us, one group against two (bf16 unless said):
+//   1 x 256, 16 heads of 128: 12 / 38, 13 / 40; 1 x 1024: 27 / 84, 24 / 80
 //   2 x 1777, 12 heads of 64, slopes: 40 / 113, 34 / 104 (336 workgroups)
-//   1 x 4096, 16 heads of 128: 101 / 326, 88 / 309 (512)
-//   2 x 1777, 12 heads of 64 in float32: 181 / 448, 140 / 395 (336)
+//   2 x 1500, 16 heads of 128: 41 / 139, 36 / 135 (384); 4 x 1024: 33 / 112, 37 / 118 (512)
+//   1 x 4096, 16 heads of 128: 99 / 322, 87 / 304 (512)
+//   1 x 1777, 36 heads of 128: 53 / 192, 69 / 210 (504, of which an XCD has 70)
+//   4 x 512, 20 heads of 64 in float32: 59 / 178, 48 / 167 (320)
 //   2 x 2304, 16 heads of 64: 43 / 122, 49 / 131 (576)
-//   documents up to 1354: 3 x 3718, 4 heads of 80: 102 / 209, 80 / 182 (360)
-//   up to 1012: 2 x 2048, 16 on 4 heads of 64: 50 / 127, 37 / 113 (512)
-//   of 700: 1 x 4096, 16 heads of 128: 37 / 143, 47 / 151 (512)
 //   2 x 1536, 11 heads of 64, not causal: 35 / 98, 45 / 109 (264)
-inline bool two_groups(const ScoredParams& p, int64_t nb, int tile) {
-    return p.Sk > tile && nb < (p.causal ? 513 : 256);
+//   documents of 5 to 603 tokens, 2 x 2048, 16 heads of 128: 35 / 101, 42 / 108 (512)
+//   up to 1596: 3 x 3718, 4 heads of 80: 58 / 151, 50 / 143 (360)
+//   up to 1759: 1 x 4096, 16 heads of 128: 61 / 198, 60 / 197; 700 each: 39 / 158, 49 / 159
+//   up to 3517: 1 x 8192, 8 heads of 128: 106 / 307, 93 / 290; 700 each: 39 / 150, 49 / 161
+//   up to 521: 2 x 1777, 12 heads of 64 in float32: 71 / 228, 78 / 236
+template <typename T>
+inline bool two_groups(const ScoredParams& p, int64_t nb) {
+    if (nb < 256) return p.Sk >= 512;
+    const int64_t on_xcd = ((int64_t)p.B * p.H + 7) / 8 * p.n_tiles;
+    return p.causal && nb <= 512 && on_xcd <= 64 && p.Sk >= (p.q_docs ? 3500 : Elem<T>::kF32 ? 500 : 1500);
 }
 template <typename T, int D, int CAP, bool SLOPE>
 hipError_t launch_scored_fwd_t(ScoredParams p, hipStream_t s) {
@@ -1460,7 +1471,7 @@ hipError_t launch_scored_fwd_t(ScoredParams p, hipStream_t s) {
     p.n_tiles = (p.Sq + C::BM - 1) / C::BM;
     const int64_t nb = (int64_t)p.n_tiles * p.H * p.B;
     if (nb <= 0) return hipSuccess;
-    if (two_groups(p, nb, C::BN)) {
+    if (two_groups<T>(p, nb)) {
         hipLaunchKernelGGL((scored_fwd_kernel<T, D, CAP, SLOPE, 2>), dim3((unsigned)nb), dim3(512), 0, s, p);
         return hipGetLastError();
     }
@@ -1475,7 +1486,7 @@ hipError_t launch_scored_bwd_t(ScoredParams p, hipStream_t s) {
     p.n_tiles = (p.Sq + CQ::BM - 1) / CQ::BM;
     const int64_t nq = (int64_t)p.n_tiles * p.H * p.B;
     constexpr bool kTwo = !(CQ::F32 && D == 128);  // (whose tiles take the whole LDS)
-    const int ks = kTwo && two_groups(p, nq, CQ::BN) ? 2 : 1;
+    const int ks = kTwo && two_groups<T>(p, nq) ? 2 : 1;
     auto dq = [&](auto dslope, auto two) {
         hipLaunchKernelGGL((scored_dq_kernel<T, D, CAP, SLOPE, decltype(dslope)::value, decltype(two)::value ? 2 : 1>),
                            dim3((unsigned)nq), dim3(256 * ks), 0, s, p);
