@@ -123,7 +123,7 @@ hipError_t put_docs(const fa_scored_args* a, ScoredParams& p, char*& ws, hipStre
 
 void put_scored(const fa_scored_args* a, ScoredParams& p) {
     p = ScoredParams{};
-    p.q = a->q; p.k = a->k; p.v = a->v; p.o = a->o; p.lse = a->lse;
+    p.q = a->q; p.k = a->k; p.v = a->v; p.o = a->o; p.lse = a->lse; p.lse_near = a->lse_near;
     p.dout = a->dout; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
     auto put = [](const int64_t st[4], int64_t& sb, int64_t& ss, int64_t& sh) {
         sb = st[0];
@@ -239,7 +239,7 @@ bool few_rows(const fa_scored_args* a, RowsParams& r) {
     const int64_t blocks = ceil_div<int64_t>(a->seqlen_q, 128) * a->num_heads * a->batch;
     if (a->seqlen_q > 32 && blocks > 128) return false;
     r = RowsParams{};
-    r.q = a->q; r.k = a->k; r.v = a->v; r.o = a->o; r.lse = a->lse;
+    r.q = a->q; r.k = a->k; r.v = a->v; r.o = a->o; r.lse = a->lse; r.lse_near = a->lse_near;
     r.q_sb = a->q_stride[0]; r.q_ss = a->q_stride[1]; r.q_sh = a->q_stride[2];
     r.k_sb = a->k_stride[0]; r.k_ss = a->k_stride[1]; r.k_sh = a->k_stride[2];
     r.v_sb = a->v_stride[0]; r.v_ss = a->v_stride[1]; r.v_sh = a->v_stride[2];
@@ -322,7 +322,7 @@ int32_t fa_scored_check(const fa_scored_args* a, int32_t backward) {
         if ((st = check_tensor(a->q, a->q_stride, 4, Sq, D, es)) || (st = check_tensor(a->o, a->o_stride, 4, Sq, D, es)))
             return st;
         if (backward && !a->lse) return FA_ERR_NULL_ARG;
-        if (!aligned(a->lse, 4)) return FA_ERR_ALIGN;
+        if (!aligned(a->lse, 4) || !aligned(a->lse_near, 4)) return FA_ERR_ALIGN;
     }
     if (k && ((st = check_tensor(a->k, a->k_stride, 4, Sk, D, es)) || (st = check_tensor(a->v, a->v_stride, 4, Sk, D, es))))
         return st;

@@ -198,18 +198,26 @@ PyObject* rotary_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// scored_fwd(q, k, v, <rules>, want_lse, stream) -> (status, o, lse or None)
+// Whether the backward needs lse_near beside lse: slopes, and a query may stand so far
+// off the keys that the rounding of its lse is more than the row's sum of P repairs
+// (distances up to 2^16: a factor of 2^(slope / 128) at most)
+bool wants_near(const fa_scored_args& a) {
+    return a.slopes && (a.query_offsets || a.query_offset < -65536 || (int64_t)a.query_offset + a.seqlen_q > 65536);
+}
+
+// scored_fwd(q, k, v, <rules>, want_lse, for a backward, stream)
+//   -> (status, o, lse or None, lse_near or None)
 PyObject* scored_fwd(PyObject*, PyObject* const* x, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (!check_count(n, 3 + kRules + 2) || !bound() || !all_tensors(x, 3)) return nullptr;
+    if (!check_count(n, 3 + kRules + 3) || !bound() || !all_tensors(x, 3)) return nullptr;
     c10::DeviceGuard guard(THPVariable_Unpack(x[0]).device());
     const at::Tensor q = prepare(THPVariable_Unpack(x[0])), k = prepare(THPVariable_Unpack(x[1])),
                      v = prepare(THPVariable_Unpack(x[2]));
     fa_scored_args a = {};
     Held h;
     if (!put_rules(a, h, x + 3)) return nullptr;
-    const bool want = PyObject_IsTrue(x[3 + kRules]) == 1;
-    void* const stream = PyLong_AsVoidPtr(x[3 + kRules + 1]);
+    const bool want = PyObject_IsTrue(x[3 + kRules]) == 1, back = PyObject_IsTrue(x[3 + kRules + 1]) == 1;
+    void* const stream = PyLong_AsVoidPtr(x[3 + kRules + 2]);
     if (PyErr_Occurred()) return nullptr;
     put_sizes(a, q, k, v);
     const at::Tensor o = at::empty(q.sizes(), q.options());
@@ -218,6 +226,8 @@ PyObject* scored_fwd(PyObject*, PyObject* const* x, Py_ssize_t n) {
     a.o = o.data_ptr();
     put_strides(a.o_stride, o);
     a.lse = (float*)ptr(lse);
+    const at::Tensor near = back && wants_near(a) ? at::empty_like(lse) : at::Tensor();
+    a.lse_near = (float*)ptr(near);
     const size_t bytes = p_fwd_size(&a);
     const at::Tensor ws = workspace(bytes, q);
     int32_t st;
@@ -225,15 +235,16 @@ PyObject* scored_fwd(PyObject*, PyObject* const* x, Py_ssize_t n) {
         pybind11::gil_scoped_release no_gil;
         st = p_fwd(&a, ptr(ws), bytes, stream);
     }
-    return Py_BuildValue("(iNN)", (int)st, THPVariable_Wrap(o), wrap_or_none(lse));
+    return Py_BuildValue("(iNNN)", (int)st, THPVariable_Wrap(o), wrap_or_none(lse), wrap_or_none(near));
     END_HANDLE_TH_ERRORS
 }
 
-// scored_bwd(q, k, v, o, do, lse, <rules>, want_dslopes, stream)
+// scored_bwd(q, k, v, o, do, lse, lse_near or None, <rules>, want_dslopes, stream)
 //   -> (status, dq, dk, dv, dslopes or None)
 PyObject* scored_bwd(PyObject*, PyObject* const* x, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (!check_count(n, 6 + kRules + 2) || !bound() || !all_tensors(x, 6)) return nullptr;
+    if (!check_count(n, 7 + kRules + 2) || !bound() || !all_tensors(x, 6)) return nullptr;
+    if (!none(x[6]) && !all_tensors(x + 6, 1)) return nullptr;
     c10::DeviceGuard guard(THPVariable_Unpack(x[0]).device());
     const at::Tensor q = prepare(THPVariable_Unpack(x[0])), k = prepare(THPVariable_Unpack(x[1])),
                      v = prepare(THPVariable_Unpack(x[2])), o = prepare(THPVariable_Unpack(x[3])),
@@ -241,9 +252,9 @@ PyObject* scored_bwd(PyObject*, PyObject* const* x, Py_ssize_t n) {
     const at::Tensor lse = THPVariable_Unpack(x[5]).contiguous();
     fa_scored_args a = {};
     Held h;
-    if (!put_rules(a, h, x + 6)) return nullptr;
-    const bool want = PyObject_IsTrue(x[6 + kRules]) == 1;
-    void* const stream = PyLong_AsVoidPtr(x[6 + kRules + 1]);
+    if (!put_rules(a, h, x + 7)) return nullptr;
+    const bool want = PyObject_IsTrue(x[7 + kRules]) == 1;
+    void* const stream = PyLong_AsVoidPtr(x[7 + kRules + 1]);
     if (PyErr_Occurred()) return nullptr;
     put_sizes(a, q, k, v);
     const at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()),
@@ -252,6 +263,8 @@ PyObject* scored_bwd(PyObject*, PyObject* const* x, Py_ssize_t n) {
     a.o = o.data_ptr();
     a.dout = dout.data_ptr();
     a.lse = (float*)lse.data_ptr();
+    const at::Tensor near = none(x[6]) ? at::Tensor() : THPVariable_Unpack(x[6]).contiguous();
+    a.lse_near = (float*)ptr(near);
     a.dq = dq.data_ptr();
     a.dk = dk.data_ptr();
     a.dv = dv.data_ptr();

@@ -16,6 +16,7 @@ struct ScoredParams {
     const void* v;
     const void* o;  // written by the forward
     float* lse;
+    float* lse_near;  // optional: the LSE over distances from the nearest key
     const void* dout;
     void* dq;
     void* dk;
@@ -82,6 +83,7 @@ struct RowsParams {
     const void* v;
     void* o;
     float* lse;      // optional (B, H, Sq)
+    float* lse_near; // optional, as ScoredParams::lse_near
     int64_t q_sb, q_ss, q_sh;
     int64_t kp_ss, kp_sh, vp_ss, vp_sh;
     int64_t k_sb, k_ss, k_sh;

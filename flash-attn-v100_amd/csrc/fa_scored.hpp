@@ -651,10 +651,12 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
     const ScoredParams& pe = late_args();
     const float l_tot = pair_sum(l_run);
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
-    if (pe.lse && sp == 0 && hi == 0 && qi < p.Sq) {
-        const float far = has_slope<CAP, SLOPE>(pe) ? pe.slopes[b * pe.slopes_sb + h] * rule.far(qi) : 0.f;
-        pe.lse[(int64_t)(b * pe.H + h) * pe.Sq + qi] =
-            l_tot > 0.f ? (m_run + __log2f(l_tot)) * kLn2 - far : l_tot == 0.f ? -INFINITY : l_tot;
+    if (sp == 0 && hi == 0 && qi < p.Sq) {
+        const int64_t at = (int64_t)(b * pe.H + h) * pe.Sq + qi;
+        const float lse = l_tot > 0.f ? (m_run + __log2f(l_tot)) * kLn2 : l_tot == 0.f ? -INFINITY : l_tot;
+        if (SLOPE && pe.lse_near) pe.lse_near[at] = lse;
+        if (pe.lse)
+            pe.lse[at] = has_slope<CAP, SLOPE>(pe) ? __builtin_fmaf(-pe.slopes[b * pe.slopes_sb + h], rule.far(qi), lse) : lse;
     }
     store_rows<T, D>(smem + w * 32 * C::OW, C::OW, o, inv, (T*)pe.o + b * pe.o_sb + h * pe.o_sh, pe.o_ss,
                      qw0, pe.Sq, pe.cols, lane, sp == 0);
@@ -665,10 +667,11 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
 // dK/dV pass reads after it.  Cap: both passes hold 4 P (the exponent is 2 larger), as
 // the derivative comes divided by 4: dS through it is then what it is, and fp16 rounds
 // neither it nor P sooner as a subnormal number.
-// SLOPE: P is e^(s - LSE), and the LSE of a query far from the keys is a large number
-// whose rounding is a factor on its row.  The row's sum of P takes it out again: of
-// dQ at the end, and of the LSE that goes to the dK/dV pass (while slope times the
-// distance to the nearest key is below 2^30; then the gradients become NaN).
+// SLOPE: P is e^(s - LSE) with the LSE over distances from the nearest key.  Where only
+// the other is there, of a query far from the keys, it is a large number whose
+// rounding is a factor on its row.  The row's sum of P takes it out again: of dQ at
+// the end, and of the LSE that goes to the dK/dV pass.  A factor past 2^4 (the digits
+// of P and dS in 16 bits would go too) makes the row's gradients NaN.
 // DSLOPE: also -d loss / d slope of each row,
 //   sum_j |d| P (dP - delta) = sum |d| dS - sum |d| P sum dS,  dS = P (dP - delta'),
 // over P and dS that are divided by sum P: with delta' from the rounded output, what
@@ -720,13 +723,14 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
         }
         del = pair_sum(del);
     }
-    const float lse_in = qi < p.Sq ? p.lse[(int64_t)(b * p.H + h) * p.Sq + qi] : -INFINITY;
+    const float* const lse_rows = SLOPE && p.lse_near ? p.lse_near : p.lse;
+    float lse_in = qi < p.Sq ? lse_rows[(int64_t)(b * p.H + h) * p.Sq + qi] : -INFINITY;
     const float slope2 = has_slope<CAP, SLOPE>(p) ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
     // of distances from the nearest key; a row that sees nothing, and rows past the
     // last: P = exp2(s - inf) = 0
-    const float lse2 = (lse_in == -INFINITY ? INFINITY
-                        : SLOPE             ? __builtin_fmaf(slope2, rule.far(qi), lse_in * kLog2e)
-                                            : lse_in * kLog2e) - (CAP ? 2.f : 0.f);
+    if (has_slope<CAP, SLOPE>(p) && !p.lse_near)
+        lse_in = __builtin_fmaf(p.slopes[b * p.slopes_sb + h], rule.far(qi), lse_in);
+    const float lse2 = (lse_in == -INFINITY ? INFINITY : lse_in * kLog2e) - (CAP ? 2.f : 0.f);
     if (sp == 0 && hi == 0) {
         const int64_t wi = ((int64_t)b * p.H + h) * p.ws_stride + qi;  // qi < sq_pad
         if constexpr (!SLOPE) p.lse2[wi] = lse2;  // (else at the end)
@@ -1006,6 +1010,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
     float inv = 1.f;                       // of sum P
     if constexpr (SLOPE) {
         const bool none = lse2 == INFINITY;  // a row that sees nothing
+        if (!none && !(sum_p > kP / 16.f && sum_p < kP * 16.f)) sum_p = __builtin_nanf("");
         inv = none ? 1.f : kP / sum_p;
         if (sp == 0 && hi == 0)
             pe.lse2[((int64_t)b * pe.H + h) * pe.ws_stride + qi] = none ? lse2 : lse2 + __log2f(sum_p * (1.f / kP));

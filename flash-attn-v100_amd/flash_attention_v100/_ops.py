@@ -11,7 +11,7 @@ import torch
 
 from . import _lib
 
-OPS_VERSION = 1
+OPS_VERSION = 2
 MAX_HEAD_DIM = 128
 
 _I64x2, _I64x3, _I64x4 = ctypes.c_int64 * 2, ctypes.c_int64 * 3, ctypes.c_int64 * 4
@@ -26,7 +26,7 @@ class ScoredArgs(ctypes.Structure):
                                "causal")]
         + [("scale", _F), ("softcap", _F), ("slopes", _P), ("slopes_batch_stride", _I64), ("prefix_lengths", _P),
            ("key_lengths", _P), ("query_offsets", _P), ("query_offset", _I32), ("q_documents", _P),
-           ("k_documents", _P), ("q_documents_stride", _I64), ("k_documents_stride", _I64)])
+           ("k_documents", _P), ("q_documents_stride", _I64), ("k_documents_stride", _I64), ("lse_near", _P)])
 
 
 class PrefixArgs(ctypes.Structure):
@@ -134,25 +134,26 @@ class Rules(NamedTuple):
     k_docs: Optional[torch.Tensor]
 
 
-def scored_fwd(q, k, v, rules: Rules, want_lse: bool = True):
-    """(o, lse or None) of ``fa_scored_fwd``; checked tensors."""
+def scored_fwd(q, k, v, rules: Rules, want_lse: bool = True, for_backward: bool = False):
+    """(o, lse or None, lse_near or None) of ``fa_scored_fwd``; checked tensors.
+    ``for_backward`` (with ``want_lse``): lse_near where ``scored_bwd`` needs it."""
     D = q.shape[-1]
     dp = padded(D, q.dtype)
     if dp != D:
         q, k, v = (_lib._pad_d(t, dp) for t in (q, k, v))
-    st, o, lse = host().scored_fwd(q, k, v, *rules, want_lse, _lib._raw_stream(q))
+    st, o, lse, near = host().scored_fwd(q, k, v, *rules, want_lse, for_backward, _lib._raw_stream(q))
     if st:
         _lib._check("fa_scored_fwd", st)
-    return _lib._unpad_d(o, D), lse
+    return _lib._unpad_d(o, D), lse, near
 
 
-def scored_bwd(q, k, v, o, do, lse, rules: Rules, want_dslopes: bool):
+def scored_bwd(q, k, v, o, do, lse, near, rules: Rules, want_dslopes: bool):
     """(dq, dk, dv, dslopes or None) of ``fa_scored_bwd``."""
     D = q.shape[-1]
     dp = padded(D, q.dtype)
     if dp != D:
         q, k, v, o, do = (_lib._pad_d(t, dp) for t in (q, k, v, o, do))
-    st, dq, dk, dv, ds = host().scored_bwd(q, k, v, o, do, lse, *rules, want_dslopes, _lib._raw_stream(q))
+    st, dq, dk, dv, ds = host().scored_bwd(q, k, v, o, do, lse, near, *rules, want_dslopes, _lib._raw_stream(q))
     if st:
         _lib._check("fa_scored_bwd", st)
     if dp != D:

@@ -100,8 +100,8 @@ class ScoredAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, slopes, rules, return_lse):
-        o, lse = _ops.scored_fwd(q, k, v, rules)
-        ctx.save_for_backward(q, k, v, o, lse, slopes, rules.prefix, rules.lens, rules.offsets, rules.q_docs,
+        o, lse, near = _ops.scored_fwd(q, k, v, rules, True, True)
+        ctx.save_for_backward(q, k, v, o, lse, near, slopes, rules.prefix, rules.lens, rules.offsets, rules.q_docs,
                               None if rules.k_docs is rules.q_docs else rules.k_docs)
         ctx.one_docs = rules.k_docs is rules.q_docs
         ctx.rules = (rules.causal, rules.scale, rules.softcap, rules.offset0)
@@ -114,13 +114,13 @@ class ScoredAttentionFunction(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output, grad_lse=None):
         # the gradient of the LSE output is ignored, as flash_attention_v100 does
-        q, k, v, o, lse, slopes, prefix, lens, offsets, q_docs, k_docs = ctx.saved_tensors
+        q, k, v, o, lse, near, slopes, prefix, lens, offsets, q_docs, k_docs = ctx.saved_tensors
         causal, scale, softcap, offset0 = ctx.rules
         if DebugConfig.VALIDATE_OUTPUTS:
             check_tensor_nan_inf(grad_output, "grad_output")
         rules = _ops.Rules(causal, scale, softcap, slopes, prefix, lens, offsets, offset0, q_docs,
                            q_docs if ctx.one_docs else k_docs)
-        dq, dk, dv, ds = _ops.scored_bwd(q, k, v, o, grad_output, lse, rules,
+        dq, dk, dv, ds = _ops.scored_bwd(q, k, v, o, grad_output, lse, near, rules,
                                          slopes is not None and ctx.needs_input_grad[3])
         if DebugConfig.VALIDATE_OUTPUTS:
             for t, name in ((dq, "grad_q"), (dk, "grad_k"), (dv, "grad_v"), (ds, "grad_distance_slopes")):
@@ -150,8 +150,8 @@ def flash_attention_v100_scored(
 
     ``softcap``: bound of the tanh on the scores (0 or None: none).
     ``distance_slopes``: float32 (H,) or (B, H), differentiable.  Queries may stand
-    off the keys: results keep their digits at any distance, gradients while slope
-    times the distance to the nearest key stays below 2^30.
+    off the keys: outputs and gradients keep their digits at any distance (the LSE
+    holds slope times the distance to the nearest key).
     ``documents``: integer ids (B, Sq) or (Sq,) of the queries' documents and,
     unless ``key_documents`` gives theirs, of the keys'; negative (or past int32):
     padding.
@@ -209,7 +209,7 @@ def flash_attention_v100_scored(
         out = ScoredAttentionFunction.apply(q, k, v, slopes, rules, return_softmax_lse)
         o, lse = out if return_softmax_lse else (out, None)
     else:
-        o, lse = _ops.scored_fwd(q, k, v, rules, return_softmax_lse)
+        o, lse, _ = _ops.scored_fwd(q, k, v, rules, return_softmax_lse)
     if DebugConfig.VALIDATE_OUTPUTS:
         check_tensor_nan_inf(o, "output")
     return (o, lse) if return_softmax_lse else o

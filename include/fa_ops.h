@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define FA_OPS_VERSION 1
+#define FA_OPS_VERSION 2
 
 #define FA_ERR_RULE -15   /* softcap neither 0 nor within [1e-6, 1e30], or an id / length array or its stride invalid */
 #define FA_ERR_ROTARY -16 /* rotary columns not even, more than the head dim, or an invalid base, factor or table */
@@ -35,6 +35,9 @@ extern "C" {
  *         and (no documents or q_documents[b, i] == k_documents[b, j] >= 0)
  * O = softmax over the keys seen, times V; a query that sees no key gets O = 0
  * and lse = -inf (and no gradient).  lse is the natural-log sum of exp(s).
+ * Of a query that stands off the keys (i + offset_b not in 0 .. key_lengths[b] - 1),
+ * lse holds slope times the distance to the nearest key, a number that may leave it
+ * few digits; lse_near is lse without it.
  * Keys from key_lengths[b] on and tokens of a negative document reach no
  * result, whatever their values are. */
 typedef struct fa_scored_args {
@@ -76,6 +79,7 @@ typedef struct fa_scored_args {
     const int32_t* k_documents;    /* optional (B, Sk); may be q_documents */
     int64_t q_documents_stride;    /* batch strides in elements */
     int64_t k_documents_stride;
+    float* lse_near;               /* optional, as lse: written by the forward, read by the backward in its place */
 } fa_scored_args;
 
 int32_t fa_ops_version(void);
@@ -95,7 +99,8 @@ size_t fa_scored_bwd_workspace_size(const fa_scored_args* args);
  * float32 sums. */
 int32_t fa_scored_fwd(const fa_scored_args* args, void* workspace, size_t workspace_bytes, void* hip_stream);
 
-/* Backward: dq, dk, dv (and dslopes), fully written; deterministic. */
+/* Backward: dq, dk, dv (and dslopes), fully written; deterministic.  Slopes and queries
+ * off the keys without lse_near: rows whose lse is too coarse get NaN gradients. */
 int32_t fa_scored_bwd(const fa_scored_args* args, void* workspace, size_t workspace_bytes, void* hip_stream);
 
 /* New tokens of B sequences after a prefix that all of them share.  Query i of

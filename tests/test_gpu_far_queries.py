@@ -12,7 +12,7 @@ from ops_edges_oracle import DEV, make, train
 pytestmark = pytest.mark.gpu
 
 
-FAR = [8192, 65536, 1 << 20, (1 << 24) + 3, (1 << 28) + 1]
+FAR = [8192, 65536, 1 << 20, (1 << 24) + 3, (1 << 28) + 1, 1 << 30]
 
 
 def forward(q, k, v, slopes, off, label, lens=None, **kw):
@@ -76,3 +76,41 @@ def test_slopes_of_far_queries_of_other_calls(dt):
     q, k, v, do = make(5, 500, 300, 30, 30, 64, dt, seed=8)
     slopes = torch.exp2(-8.0 * torch.arange(1, 31, device=DEV) / 30)
     train(q, k, v, do, f"one group {dt}", causal=True, query_offsets=1 << 20, distance_slopes=slopes)
+
+
+def test_an_lse_too_coarse_is_not_passed_over():
+    # the C entry without lse_near: a row's sum of P makes good for the rounding of its
+    # LSE, and where that is no longer possible the gradients are NaN
+    import ctypes
+
+    from flash_attention_v100 import _ops
+
+    lib, stream = _ops.load(), torch.cuda.current_stream().cuda_stream
+    B, Sq, Sk, H, D = 1, 40, 300, 2, 64
+    q, k, v, do = make(B, Sq, Sk, H, H, D, "fp32", seed=3)
+    slopes = torch.tensor([0.5, 0.25], device=DEV)
+    for off, good in ((100000, True), (1 << 24, True), (1 << 30, False)):
+        out = {n: torch.zeros_like(t) for n, t in (("o", q), ("dq", q), ("dk", k), ("dv", v))}
+        lse, ds = torch.zeros(B, H, Sq, device=DEV), torch.zeros(H, device=DEV)
+        a = _ops.ScoredArgs()
+        for n, t in dict(out, q=q, k=k, v=v, dout=do).items():
+            setattr(a, n, t.data_ptr())
+            getattr(a, ("do" if n == "dout" else n) + "_stride")[:] = t.stride()
+        a.lse, a.slopes, a.dslopes, a.query_offset = lse.data_ptr(), slopes.data_ptr(), ds.data_ptr(), off
+        (a.batch, a.seqlen_q, a.seqlen_k, a.num_heads, a.num_heads_kv, a.head_dim, a.dtype,
+         a.scale) = B, Sq, Sk, H, H, D, 2, D ** -0.5
+        for size, call in ((lib.fa_scored_fwd_workspace_size, lib.fa_scored_fwd),
+                           (lib.fa_scored_bwd_workspace_size, lib.fa_scored_bwd)):
+            n = size(ctypes.byref(a))
+            ws = torch.empty(n + 256, device=DEV, dtype=torch.uint8)
+            assert call(ctypes.byref(a), ws.data_ptr(), n, stream) == 0
+        ref = eo.scored(q, k, v, do, 0.0, slopes, off, oo.seen_mask(B, Sq, Sk, device=DEV))
+        got = dict(out, lse=lse, dslopes=ds)
+        oo.check(got, ref, ["o", "lse"], str(off))
+        names = ["dq", "dk", "dv", "dslopes"]
+        if not good:  # a row whose LSE was rounded by little by chance is right, the others are NaN
+            for n in names:
+                nan = torch.isnan(got[n])
+                assert nan.any(), n
+                got[n] = torch.where(nan, ref[n][0].to(got[n].dtype), got[n])
+        oo.check(got, ref, names, str(off))

@@ -82,3 +82,11 @@ def test_documents_of_empty_sides(Sq, Sk, q_ids, k_ids):
     assert lib.fa_scored_fwd_workspace_size(ctypes.byref(a)) == 0
     a.seqlen_q = a.seqlen_k = 5
     assert lib.fa_scored_check(ctypes.byref(a), 0) == (CODES["FA_ERR_RULE"] if (q_ids is None) != (k_ids is None) else 0)
+
+
+def test_lse_near_is_checked():
+    lib, a = _ops.load(), scored_args()
+    for lse_near, code in ((ADDR, 0), (ADDR + 2, CODES["FA_ERR_ALIGN"])):
+        a.lse_near = lse_near
+        for backward in (0, 1):
+            assert lib.fa_scored_check(ctypes.byref(a), backward) == code
