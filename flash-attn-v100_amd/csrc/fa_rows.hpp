@@ -67,7 +67,7 @@ __device__ FA_INLINE inline void put_lse(const RowsParams& p, int b, int h, int 
         const int len = own_len(p, b), own = own_pos(p, b, len) + i;
         lse = __builtin_fmaf(-p.slopes[b * p.slopes_sb + h], (float)abs(own - near_key(own, len)), lse);
     }
-    if (p.lse) p.lse[at] = lse;
+    p.lse[at] = lse;
 }
 
 // one row of a unit: its query and the keys [0, lim) it sees
@@ -310,7 +310,7 @@ __device__ FA_INLINE inline void unit32(const RowsParams& p, bool pre, T* smem, 
     const bool only = p.p_splits + p.o_splits == 1;  // no other part of these rows
     const int64_t prow = (pre ? 0 : p.p_rows) + (int64_t)id * 32 + l32;
     if (!only && w == 0 && hi == 0) p.stat[prow] = make_float2(mm, l_tot);
-    if (only && w == 0 && hi == 0 && row.live && (p.lse || p.lse_near)) put_lse(p, row.b, row.h, row.i, mm, l_tot);
+    if (only && w == 0 && hi == 0 && row.live && p.lse) put_lse(late_args<RowsParams>(), row.b, row.h, row.i, mm, l_tot);
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
 #pragma unroll
     for (int n0 = 0; n0 < D / 32; n0 += NW) {
@@ -595,7 +595,7 @@ __global__ __launch_bounds__(256) void rows_join_kernel(const RowsParams p, cons
     }
     if (!live) return;
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
-    if (col == 0 && (p.lse || p.lse_near)) put_lse(p, b, h, i, mm, l_tot);
+    if (col == 0 && p.lse) put_lse(p, b, h, i, mm, l_tot);
     if (col >= p.cols) return;
     T* ob = (T*)p.o + b * p.o_sb + (int64_t)i * p.o_ss + h * p.o_sh + col;
     if constexpr (Elem<T>::kF32) {

@@ -182,10 +182,11 @@ using template_int = std::integral_constant<int, N>;
 // The kernel's arguments, to be read where they are used: what only the epilogue
 // needs would otherwise be read first and take scalar registers from the loop
 // (kept in lanes of vector registers, a read of a lane for each use).
-__device__ FA_INLINE inline const ScoredParams& late_args() {
+template <typename P = ScoredParams>
+__device__ FA_INLINE inline const P& late_args() {
     uint64_t a = (uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(a));
-    return *(const ScoredParams*)(uintptr_t)a;
+    return *(const P*)(uintptr_t)a;
 }
 
 // -x for four floats
@@ -651,12 +652,11 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
     const ScoredParams& pe = late_args();
     const float l_tot = pair_sum(l_run);
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
-    if (sp == 0 && hi == 0 && qi < p.Sq) {
+    if (pe.lse && sp == 0 && hi == 0 && qi < p.Sq) {
         const int64_t at = (int64_t)(b * pe.H + h) * pe.Sq + qi;
         const float lse = l_tot > 0.f ? (m_run + __log2f(l_tot)) * kLn2 : l_tot == 0.f ? -INFINITY : l_tot;
         if (SLOPE && pe.lse_near) pe.lse_near[at] = lse;
-        if (pe.lse)
-            pe.lse[at] = has_slope<CAP, SLOPE>(pe) ? __builtin_fmaf(-pe.slopes[b * pe.slopes_sb + h], rule.far(qi), lse) : lse;
+        pe.lse[at] = has_slope<CAP, SLOPE>(pe) ? __builtin_fmaf(-pe.slopes[b * pe.slopes_sb + h], rule.far(qi), lse) : lse;
     }
     store_rows<T, D>(smem + w * 32 * C::OW, C::OW, o, inv, (T*)pe.o + b * pe.o_sb + h * pe.o_sh, pe.o_ss,
                      qw0, pe.Sq, pe.cols, lane, sp == 0);

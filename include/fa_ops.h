@@ -79,7 +79,7 @@ typedef struct fa_scored_args {
     const int32_t* k_documents;    /* optional (B, Sk); may be q_documents */
     int64_t q_documents_stride;    /* batch strides in elements */
     int64_t k_documents_stride;
-    float* lse_near;               /* optional, as lse: written by the forward, read by the backward in its place */
+    float* lse_near;               /* optional, beside lse: written by the forward, read by the backward in its place */
 } fa_scored_args;
 
 int32_t fa_ops_version(void);
