@@ -50,6 +50,7 @@ int32_t check_sizes(int32_t B, int32_t Sq, int32_t Sk, int32_t H, int32_t Hkv, i
     if (!std::isfinite(scale) || !(scale > 0.f)) return FA_ERR_SCALE;
     // outside these the constants of the cap leave float32
     if (!std::isfinite(softcap) || (softcap != 0.f && !(softcap >= 1e-6f && softcap <= 1e30f))) return FA_ERR_RULE;
+    if (softcap != 0.f && (double)scale / softcap > 1e37) return FA_ERR_RULE;
     if (Sq >= kMaxLen || Sk >= kMaxLen) return FA_ERR_TOO_LARGE;
     const int64_t tiles = ((int64_t)std::max(Sq, Sk) + 31) / 32;
     if (B > 0 && tiles * (int64_t)H > 0x7fffffffLL / B) return FA_ERR_TOO_LARGE;

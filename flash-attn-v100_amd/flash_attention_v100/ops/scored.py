@@ -59,13 +59,15 @@ def check_scale(scale: Optional[float], D: int) -> float:
     return float(scale)
 
 
-def check_softcap(softcap: Optional[float]) -> float:
+def check_softcap(softcap: Optional[float], scale: float) -> float:
     if softcap is None:
         return 0.0
     c = float(softcap)
     # below 2^-60 or so the cap's constants would leave the range of float32
     if not math.isfinite(c) or c < 0 or (0 < c < 1e-6) or c > 1e30:
         raise ValueError(f"softcap must be 0 (none) or within [1e-6, 1e30], got {softcap}")
+    if c and scale > 1e37 * c:
+        raise ValueError(f"scale must be at most 1e37 times softcap, got {scale} and {softcap}")
     return c
 
 
@@ -172,7 +174,7 @@ def flash_attention_v100_scored(
     B, Sq, H, D = q.shape
     Sk = k.shape[1]
     scale = check_scale(scale, D)
-    softcap = check_softcap(softcap)
+    softcap = check_softcap(softcap, scale)
     slopes = prefix = lens = None
     if distance_slopes is not None:
         slopes = check_slopes(distance_slopes, B, H, q.device)

@@ -52,7 +52,7 @@ def flash_attention_v100_shared_prefix(
             raise ValueError("k_prefix, v_prefix must have the dtype and device of q")
     _ops.check_dual("flash_attention_v100_shared_prefix", k_prefix, v_prefix)
     scale = check_scale(scale, D)
-    softcap = check_softcap(softcap)
+    softcap = check_softcap(softcap, scale)
     slopes = check_slopes(distance_slopes, B, H, q.device)
     lens = _ops.optional_lengths(key_lengths, "key_lengths", B, q.device)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad

@@ -24,7 +24,7 @@ extern "C" {
 
 #define FA_OPS_VERSION 2
 
-#define FA_ERR_RULE -15   /* softcap neither 0 nor within [1e-6, 1e30], or an id / length array or its stride invalid */
+#define FA_ERR_RULE -15   /* softcap neither 0 nor within [1e-6, 1e30], scale over 1e37 softcap, or an id / length array or its stride invalid */
 #define FA_ERR_ROTARY -16 /* rotary columns not even, more than the head dim, or an invalid base, factor or table */
 
 /* Attention with scored rules.  For query i and key j of sequence b, head h:

@@ -9,7 +9,8 @@ import torch.autograd.forward_ad as ad
 
 import flash_attention_v100 as fa
 from flash_attention_v100 import _ops, modules
-from test_ops_cpu import ADDR, CODES, scored_args
+from flash_attention_v100.ops import scored
+from test_ops_cpu import ADDR, CODES, prefix_args, scored_args
 
 
 def test_forward_mode_derivatives_are_refused():
@@ -90,3 +91,18 @@ def test_lse_near_is_checked():
         a.lse_near = lse_near
         for backward in (0, 1):
             assert lib.fa_scored_check(ctypes.byref(a), backward) == code
+
+
+def test_scale_past_the_cap_is_refused():
+    # scale / softcap past float32 would make a score of 0 a NaN
+    lib = _ops.load()
+    for scale, cap, ok in ((1e30, 1e-6, True), (3e38, 1e-6, False), (3e38, 30.0, True), (3e38, 0.0, True)):
+        a = scored_args()
+        a.scale, a.softcap = scale, cap
+        assert lib.fa_scored_check(ctypes.byref(a), 0) == (0 if ok else CODES["FA_ERR_RULE"])
+        p = prefix_args()
+        p.scale, p.softcap = scale, cap
+        assert lib.fa_prefix_check(ctypes.byref(p)) == (0 if ok else CODES["FA_ERR_RULE"])
+    assert scored.check_softcap(1e-6, 1e30) == 1e-6
+    with pytest.raises(ValueError, match="scale"):
+        scored.check_softcap(1e-6, 3e38)
