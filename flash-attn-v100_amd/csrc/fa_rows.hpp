@@ -15,11 +15,14 @@
 // Query i of a sequence with n keys of its own stands at own position
 // n - Sq + i and sees its keys up to there; in distances the prefix lies before
 // them.  Bound by the K and V bytes, and over the prefix by the products of its
-// rows: 16 tokens over caches of up to 8192 keys, 32 on 8 heads of 128: 79 us, 4.5
-// TB/s; 64 tokens after 8192 shared ones and up to 512 of their own: 33 us (51 us
+// rows: 16 tokens over caches of up to 8192 keys, 32 on 8 heads of 128: 78 us, 4.6
+// TB/s; 64 tokens after 8192 shared ones and up to 512 of their own: 37 us (51 us
 // when units of 32 rows read the prefix); 8 x 5 tokens after 20001, 16 on 2 heads:
 // 25 us (43).  Small calls are bound by the launch: 9 us for 8 heads over 512
-// keys, with 4 waves a workgroup as with 8.
+// keys, with 4 waves a workgroup as with 8.  float32, whose tiles are copied and waited
+// for one by one: 16 tokens over 8192 keys, 32 on 8 heads of 128: 270 us with the join, 4.0
+// TB/s; 64 tokens after 8192 and 512: 229 us, of which the products are 61 on the float32
+// matrix instruction.
 #pragma once
 
 #include "fa_common.hpp"

@@ -14,7 +14,9 @@
 // mask that the tile loop walks.  A second ballot marks the tiles that every
 // query of the wave sees whole: only the others run the masking step.
 // tanh x = 1 - 2 r, r = 1 / (1 + e^(2x)): one exp2 and one reciprocal a score,
-// and its derivative 1 - tanh^2 = 4 (r - r^2) comes with two more operations.
+// and its derivative 1 - tanh^2 = 4 (r - r^2) comes with two more operations; by a
+// series under caps far above the scores (Cap).
+// Distances are taken from the key nearest to the query (SeqRule::near).
 //
 // Roundings of 16-bit inputs: P and dS where they enter a product (the matrix
 // instructions take 16 bits), and delta from the rounded O that the caller keeps;
@@ -24,11 +26,15 @@
 //
 // Tiles, operand layouts and pipelines are those of fa_fwd.hpp and fa_bwd.hpp:
 // one workgroup has 4 waves of 32 queries (forward, dQ) or 32 keys (dK/dV).
-// Bound by the vector arithmetic of the scores beside the matrix products, near
-// the power limit of the device; 2 x 4096, 32 on 8 heads of 128, bf16, causal:
-// forward 338 us and backward 1000 us with no rule but the mask, 338 and 1128 with
-// the cap, 308 and 1082 with slopes (1154 with their gradient), 92 and 335 over
-// documents of 700 tokens.
+// The forward with a cap is bound by the vector arithmetic of the scores beside the
+// products: 11 vector instructions for each, two of a quarter of the rate, leave the
+// matrix unit half of the time at most (it has 37%).  The other passes (5 to 8 for
+// each, 30 to 39%) wait: one barrier a tile with two workgroups a CU, and in dQ and
+// dK/dV nothing of a wave between the products of the scores and their arithmetic.
+// The clock is 2.0 to 2.3 GHz under them, of 2.4.  2 x 4096, 32 on 8 heads of 128,
+// bf16, causal: forward 286 us and backward 971 us with no rule but the mask (the dense
+// kernels 255 and 1020), 333 and 1137 with the cap, 311 and 1033 with slopes (1082 with
+// their gradient), 92 and 333 over documents of 700 tokens.
 #pragma once
 
 #include <limits.h>

@@ -39,7 +39,8 @@ def rotary_table_v100(
     ``high_rotations`` times over ``original_positions`` keep their w_j, those of
     at most ``low_rotations`` are divided, blended in between, and cosines and
     sines are multiplied by ``attention_factor`` (0.1 ln factor + 1 unless given;
-    1 for the other scalings)."""
+    1 for the other scalings).  The blend is linear in the rotations; a model that
+    blends over the pairs' index brings a table of its own, of the same layout."""
     if scaling not in _ops.ROTARY_SCALINGS:
         raise ValueError(f"scaling must be one of {tuple(_ops.ROTARY_SCALINGS)}, got {scaling!r}")
     if not isinstance(max_positions, int) or max_positions < 1 or max_positions > 1 << 31:
