@@ -199,10 +199,11 @@ PyObject* rotary_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
 }
 
 // Whether the backward needs lse_near beside lse: slopes, and a query may stand so far
-// off the keys that the rounding of its lse is more than the row's sum of P repairs
-// (distances up to 2^16: a factor of 2^(slope / 128) at most)
+// off the keys that the rounding of its lse counts (up to 512: 2^-16 of P times the slope)
 bool wants_near(const fa_scored_args& a) {
-    return a.slopes && (a.query_offsets || a.query_offset < -65536 || (int64_t)a.query_offset + a.seqlen_q > 65536);
+    const int64_t first = a.query_offset, end = first + a.seqlen_q;
+    const bool off = a.key_lengths || first < 0 || end > a.seqlen_k;
+    return a.slopes && (a.query_offsets || (off && (first < -512 || end > 512)));
 }
 
 // scored_fwd(q, k, v, <rules>, want_lse, for a backward, stream)

@@ -673,11 +673,8 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 && !(Elem<T>::kF32 && D == 128) 
 // dK/dV pass reads after it.  Cap: both passes hold 4 P (the exponent is 2 larger), as
 // the derivative comes divided by 4: dS through it is then what it is, and fp16 rounds
 // neither it nor P sooner as a subnormal number.
-// SLOPE: P is e^(s - LSE) with the LSE over distances from the nearest key.  Where only
-// the other is there, of a query far from the keys, it is a large number whose
-// rounding is a factor on its row.  The row's sum of P takes it out again: of dQ at
-// the end, and of the LSE that goes to the dK/dV pass.  A factor past 2^4 (the digits
-// of P and dS in 16 bits would go too) makes the row's gradients NaN.
+// SLOPE: P is e^(s - LSE) with the LSE over distances from the nearest key: lse_near,
+// or lse less what it holds for them.
 // DSLOPE: also -d loss / d slope of each row,
 //   sum_j |d| P (dP - delta) = sum |d| dS - sum |d| P sum dS,  dS = P (dP - delta'),
 // over P and dS that are divided by sum P: with delta' from the rounded output, what
@@ -739,7 +736,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
     const float lse2 = (lse_in == -INFINITY ? INFINITY : lse_in * kLog2e) - (CAP ? 2.f : 0.f);
     if (sp == 0 && hi == 0) {
         const int64_t wi = ((int64_t)b * p.H + h) * p.ws_stride + qi;  // qi < sq_pad
-        if constexpr (!SLOPE) p.lse2[wi] = lse2;  // (else at the end)
+        p.lse2[wi] = lse2;
         p.lse2[wi + p.sq_pad] = qi < p.Sq ? del : 0.f;
     }
 
@@ -804,7 +801,7 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
     const float c = p.scale_log2;
     Cap<(C::F32 || CAP == kCapWide)> cap(p);
     const int qpos = rule.near(qi);
-    // sums of P (SLOPE); of dS, |d| P, |d| dS (DSLOPE)
+    // sums of P, dS, |d| P, |d| dS (DSLOPE)
     [[maybe_unused]] float sum_p = 0.f, sum_ds = 0.f, sum_d = 0.f, sum_dds = 0.f;
 
     const T* kbase = (const T*)p.k + b * p.k_sb + hk * p.k_sh;
@@ -915,9 +912,6 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
             // summed here: moved on, P and dP stay in registers until then, and spill
             // (2 x 4096 x 32 heads of 128: backward with the slopes' gradient 1683 -> 1141 us)
             asm volatile("" : "+v"(sum_p), "+v"(sum_ds), "+v"(sum_d), "+v"(sum_dds));
-        } else if constexpr (SLOPE) {
-            sum_p += ((pe[0] + pe[1]) + (pe[2] + pe[3])) + ((pe[4] + pe[5]) + (pe[6] + pe[7]));
-            asm volatile("" : "+v"(sum_p));
         }
         if constexpr (C::F32) {
 #pragma unroll
@@ -974,14 +968,14 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
         }
     }
     sync_tiles();
-    if constexpr (SLOPE) sum_p = pair_sum(sum_p);
     if constexpr (DSLOPE) {
+        sum_p = pair_sum(sum_p);
         sum_ds = pair_sum(sum_ds);
         sum_d = pair_sum(sum_d);
         sum_dds = pair_sum(sum_dds);
     }
     if constexpr (KS == 2) {
-        constexpr int NO = (D / 32) * 16, NF = NO + (DSLOPE ? 4 : SLOPE ? 1 : 0);
+        constexpr int NO = (D / 32) * 16, NF = NO + (DSLOPE ? 4 : 0);
         static_assert(4 * NF * 64 * 4 <= C::SMEM_BYTES, "a group's part fits its tile buffers");
         float* mg = reinterpret_cast<float*>(smem + C::SMEM_BYTES);
         auto at = [&](int f) FA_INLINE { return mg + (w * NF + f) * 64 + lane; };
@@ -990,8 +984,8 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
             for (int i = 0; i < D / 32; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) *at(16 * i + e) = dq[i][e];
-            if (SLOPE) *at(NO) = sum_p;
             if (DSLOPE) {
+                *at(NO) = sum_p;
                 *at(NO + 1) = sum_ds;
                 *at(NO + 2) = sum_d;
                 *at(NO + 3) = sum_dds;
@@ -1003,8 +997,8 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
             for (int i = 0; i < D / 32; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) dq[i][e] += *at(16 * i + e);
-            if (SLOPE) sum_p += *at(NO);
             if (DSLOPE) {
+                sum_p += *at(NO);
                 sum_ds += *at(NO + 1);
                 sum_d += *at(NO + 2);
                 sum_dds += *at(NO + 3);
@@ -1012,20 +1006,13 @@ __global__ __launch_bounds__(256 * KS, (KS == 1 ? DqCfg<T, D>::MIN_BLOCKS : 1)) 
         }
     }
     const ScoredParams& pe = late_args();
-    constexpr float kP = CAP ? 4.f : 1.f;  // sums hold kP P
-    float inv = 1.f;                       // of sum P
-    if constexpr (SLOPE) {
-        const bool none = lse2 == INFINITY;  // a row that sees nothing
-        if (!none && !(sum_p > kP / 16.f && sum_p < kP * 16.f)) sum_p = __builtin_nanf("");
-        inv = none ? 1.f : kP / sum_p;
-        if (sp == 0 && hi == 0)
-            pe.lse2[((int64_t)b * pe.H + h) * pe.ws_stride + qi] = none ? lse2 : lse2 + __log2f(sum_p * (1.f / kP));
-    }
     if constexpr (DSLOPE) {
+        // (sums of 4 P and 4 dS under a cap: their quotients are the same)
+        const float inv = sum_p == 0.f ? 0.f : 1.f / sum_p;  // a row that sees nothing
         if (sp == 0 && hi == 0 && qi < pe.Sq)
-            pe.dslope_rows[((int64_t)b * pe.H + h) * pe.Sq + qi] = __builtin_fmaf(sum_ds * (inv / kP), sum_d, -sum_dds) * (inv / kP);
+            pe.dslope_rows[((int64_t)b * pe.H + h) * pe.Sq + qi] = __builtin_fmaf(sum_ds * inv, sum_d, -sum_dds) * inv;
     }
-    store_rows<T, D>((T*)smem + w * 32 * C::OW, C::OW, dq, pe.scale * inv,
+    store_rows<T, D>((T*)smem + w * 32 * C::OW, C::OW, dq, pe.scale,
                      (T*)pe.dq + b * pe.dq_sb + h * pe.dq_sh, pe.dq_ss, qw0, pe.Sq, pe.cols, lane, sp == 0);
 }
 

@@ -99,8 +99,10 @@ size_t fa_scored_bwd_workspace_size(const fa_scored_args* args);
  * float32 sums. */
 int32_t fa_scored_fwd(const fa_scored_args* args, void* workspace, size_t workspace_bytes, void* hip_stream);
 
-/* Backward: dq, dk, dv (and dslopes), fully written; deterministic.  Slopes and queries
- * off the keys without lse_near: rows whose lse is too coarse get NaN gradients. */
+/* Backward: dq, dk, dv (and dslopes), fully written; deterministic.  P is exp(s - lse)
+ * of the lse given (and delta is of the o given), so that dq, dk and dv may be of a part
+ * of the keys of a row whose lse and o are of all; dslopes takes the keys seen for all.
+ * lse_near, of the same keys as lse, keeps the digits of queries far off the keys. */
 int32_t fa_scored_bwd(const fa_scored_args* args, void* workspace, size_t workspace_bytes, void* hip_stream);
 
 /* New tokens of B sequences after a prefix that all of them share.  Query i of
