@@ -23,7 +23,7 @@ INCLUDE = os.path.join(REPO, "include")
 OBJDIR = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "flash_attention_v100", "libfa_gfx950.so")
 HOST_SRC = os.path.join(CSRC, "fa_host.cpp")
-HOST_SRCS = [HOST_SRC, os.path.join(CSRC, "fa_ops_host.cpp")]
+HOST_SRCS = [HOST_SRC, os.path.join(CSRC, "fa_ops_host.cpp"), os.path.join(CSRC, "fa_paged_host.cpp")]
 HOST_LIB = os.path.join(HERE, "flash_attention_v100", "fa_host.so")
 ARCH = "gfx950"
 
@@ -36,7 +36,8 @@ SOURCES = ["fa_abi.cpp", "fa_misc.hip", "fa_fwd_fit.hip", "fa_fwd_decode.hip"] +
     for mode, dts in modes
     for dt in dts
 ] + [f"fa_scored_{pas}_{dt}.hip" for pas in ("bwd", "fwd") for dt in _A] + [f"fa_rows_{dt}.hip" for dt in _A] + [
-    "fa_ops_abi.cpp", "fa_scored_misc.hip", "fa_rotary.hip"]
+    "fa_ops_abi.cpp", "fa_scored_misc.hip", "fa_rotary.hip"] + [f"fa_paged_{dt}.hip" for dt in _A] + [
+    "fa_paged_abi.cpp", "fa_paged_cache.hip"]
 
 # units whose MFMA accumulators may live in AGPRs (the head-dim-256 backward:
 # its dK / dV and dQ kernels need more than 256 registers a lane; with the

@@ -22,6 +22,7 @@
 
 #include "fa_abi.h"
 #include "fa_ops.h"
+#include "fa_paged.h"
 #include "fa_params.hpp"
 
 // Device scratch of fa_bwd_static: the backward workspace for callers that
@@ -352,6 +353,9 @@ const char* fa_strerror(int32_t code) {
             return "softcap must be finite and >= 0; slopes, documents and their strides must be consistent";
         case FA_ERR_ROTARY:
             return "rotary_dim must be even and at most the head dim, with a table and finite positive base and factor";
+        case FA_ERR_PAGES:
+            return "pages hold a multiple of 16 tokens, a pool that is forked or compacted at most 2^20 pages, a tree at "
+                   "most 256 tokens; tables, paths and lengths must be consistent, outputs apart from inputs";
         default: return "unknown status code";
     }
 }

@@ -244,7 +244,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "fa_host", nullptr, -1, methods, nu
 
 PyMODINIT_FUNC PyInit_fa_host(void) {
     PyObject* m = PyModule_Create(&module);
-    if (m && PyModule_AddFunctions(m, fa_host::ops_methods) != 0) {
+    if (m && (PyModule_AddFunctions(m, fa_host::ops_methods) != 0 || PyModule_AddFunctions(m, fa_host::paged_methods) != 0)) {
         Py_DECREF(m);
         return nullptr;
     }

@@ -31,6 +31,7 @@ inline void put_strides(int64_t (&dst)[4], const at::Tensor& t) {
     for (int d = 0; d < 4; ++d) dst[d] = t.stride(d);
 }
 
-extern PyMethodDef ops_methods[];  // fa_ops_host.cpp
+extern PyMethodDef ops_methods[];    // fa_ops_host.cpp
+extern PyMethodDef paged_methods[];  // fa_paged_host.cpp
 
 }  // namespace fa_host

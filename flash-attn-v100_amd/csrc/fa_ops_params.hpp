@@ -114,6 +114,67 @@ struct RowsParams {
 template <typename T>
 hipError_t launch_rows(const RowsParams& p, int D, hipStream_t s);
 
+// Tokens, or trees of drafted tokens, over a cache of pages (fa_paged.hpp): the rows'
+// own keys only (P = 0, tail = 1), k and v a pool of pages
+struct PagedParams : RowsParams {
+    const int* table;      // (B, table_cols) pages, null: sequence b is page b
+    int64_t table_sb;
+    int table_cols, pages;
+    int page_blocks;       // blocks of 16 tokens in a page
+    unsigned page_magic;   // 2^32 / page_blocks, up to one below or above
+    int64_t k_sp, v_sp;    // page strides
+    const int* parents;    // optional (B, Sq), batch stride parents_sb
+    int64_t parents_sb;
+    // work: units of unit_rows rows of one (sequence, KV head), unit_tiles a KV head,
+    // over steps of step_keys keys, shared out to at most `slots` workgroups
+    int unit_tiles, slots;
+};
+template <typename T>
+hipError_t launch_paged(const PagedParams& p, int D, hipStream_t s);
+
+// A pool of pages, as its operators read it (fa_paged_cache.hip); strides in bytes
+struct PoolParams {
+    char* x[2];            // k, v
+    int64_t sl[2], sp[2], sr[2], sh[2];  // layer, page, row, head
+    int layers, pages, page_size, heads, chunks;  // chunks: 16-byte chunks of a head's row
+    int B, cols;
+    const int* table;
+    int64_t table_sb;
+    const int* lens;
+    int room;              // tokens a sequence has room for
+};
+struct CacheWriteParams : PoolParams {
+    const char* in[2];     // (layers, B, N, heads, D)
+    int64_t in_sl[2], in_sb[2], in_ss[2], in_sh[2];
+    int N;
+};
+hipError_t launch_cache_write(const CacheWriteParams& p, hipStream_t s);
+struct CacheAcceptParams : PoolParams {
+    const int* path;
+    int64_t path_sb;
+    int path_cols, N;
+    int* new_lens;
+};
+hipError_t launch_cache_accept(const CacheAcceptParams& p, hipStream_t s);
+struct CacheForkParams : PoolParams {
+    const int* sources;
+    const int* more;
+    int more_all, n_new;
+    int* new_table;
+    int* new_lens;
+    int* free_list;        // workspace: pages to give
+    int4* copies;          // workspace: per new sequence (page from, page to, rows)
+};
+hipError_t launch_cache_fork(const CacheForkParams& p, hipStream_t s);
+struct CacheCompactParams : PoolParams {
+    int* new_table;
+    int* used;
+    int* to;               // workspace: new number of each page
+    int2* moves;           // workspace: (from, to)
+    int* n_moves;
+};
+hipError_t launch_cache_compact(const CacheCompactParams& p, hipStream_t s);
+
 // Rotary positions (fa_rotary.hip)
 struct RotaryTableParams {
     float* table;  // (n, R)

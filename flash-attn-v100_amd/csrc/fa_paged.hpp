@@ -1,0 +1,753 @@
+// Attention of the newest tokens of each sequence, one after another or as a tree
+// of drafted ones, over a cache whose keys lie in pages; gfx950.
+//
+// A row is one (sequence, new token, query head); a unit is 32 rows of one sequence
+// and KV head.  All units' keys, in steps of 128, make one list that the workgroups
+// share out evenly, so that sequences of any lengths keep the device equally busy:
+// a workgroup walks its part of the list, unit after unit, and a unit that it holds
+// only a part of leaves its rows' maximum, sum and unnormalised output in float32 for
+// paged_join_kernel:
+//   O = sum_x 2^(m_x - m) O_x / sum_x 2^(m_x - m) l_x,  m = max_x m_x.
+//
+// Keys come in blocks of 16 tokens, which never leave a page: one lookup and one
+// buffer descriptor a block, whose range ends with the sequence, so that what lies
+// behind it lands as zeros.  A tree's rows hide keys among the newest tokens only: each
+// row's ancestors are bits, and a tile of 32 keys takes its 32 of them.
+#pragma once
+
+#include "fa_common.hpp"
+#include "fa_ops_params.hpp"
+#include "fa_rows.hpp"
+
+namespace fa {
+
+constexpr int kTreeNodes = 256;
+constexpr int kTreeWords = kTreeNodes / 32;
+
+template <typename T, int D>
+struct PagedCfg {
+    static constexpr bool F32 = Elem<T>::kF32;
+    static constexpr int NW = 4;
+    static constexpr int EPC = 16 / (int)sizeof(T);
+    static constexpr int CW = D / EPC;        // 16-byte chunks of a row
+    static constexpr int ROWB = CW * 16;
+    static constexpr int NI16 = CW / 4;       // copies of 64 chunks in a block of 16 rows
+    static constexpr int TILE = 32 * D;       // a wave's 32 keys
+    static constexpr int REGION = 2 * TILE;
+    static constexpr int STEP = NW * 32;      // keys of a step
+    static constexpr int SMEM = NW * REGION;
+    static_assert((D / 32) * 16 * 64 * 4 <= REGION * (int)sizeof(T), "a wave's O part fits its region");
+    static constexpr int PER_CU = F32 && D == 128 ? 1 : 2;
+};
+
+// Rows lie in LDS without padding, the chunks of row r at places c ^ row_swizzle(r).  What
+// one instruction reads then spreads over all banks: the same chunk of 16 rows (K), and 64
+// bytes of each of 4 rows (V^T).
+template <int CW>
+__device__ FA_INLINE inline int row_swizzle(int r) {
+    if constexpr (CW == 4) return (r >> 2) & 3;
+    if constexpr (CW == 8) return ((r & 2) << 1) | ((r >> 2) & 3);
+    return ((r & 3) << 2) | ((r >> 2) & 3);
+}
+
+// scalar loads of what no kernel of the call writes
+typedef const __attribute__((address_space(4))) int const_int;
+__device__ FA_INLINE inline int uniform_load(const int* p, int64_t at) {
+    return ((const_int*)(uintptr_t)p)[at];
+}
+
+// 16 tokens of a sequence: their page, -1 where there is none, and the first one's row
+struct Block16 {
+    int page, row;
+};
+__device__ FA_INLINE inline Block16 block_at(const PagedParams& p, int b, int blk) {
+    if (!p.table) return {b, 16 * blk};
+    int col = (int)__umulhi((unsigned)blk, p.page_magic);
+    int r = blk - col * p.page_blocks;
+    if (r < 0) {
+        --col;
+        r += p.page_blocks;
+    } else if (r >= p.page_blocks) {
+        ++col;
+        r -= p.page_blocks;
+    }
+    const int page = uniform_load(p.table, b * p.table_sb + min(col, p.table_cols - 1));
+    return {(unsigned)page < (unsigned)p.pages ? page : -1, 16 * r};
+}
+
+// copies of 16-row blocks of one KV head's keys or values
+template <typename T, int D>
+struct PageCopy {
+    using C = PagedCfg<T, D>;
+    const T* base;  // the pool's, of the KV head
+    int64_t sp, ss;
+    int cols;
+    int off[C::NI16];
+    __device__ FA_INLINE inline void init(const T* b, int64_t page_stride, int64_t row_stride, int n_cols, int lane) {
+        base = b;
+        sp = page_stride;
+        ss = row_stride;
+        cols = n_cols;
+#pragma unroll
+        for (int x = 0; x < C::NI16; ++x) {
+            const int c = 64 * x + lane, row = c / C::CW, chunk = (c % C::CW) ^ row_swizzle<C::CW>(row);
+            off[x] = chunk < cols / C::EPC ? (row * (int)ss + chunk * C::EPC) * (int)sizeof(T) : kOffNowhere;
+        }
+    }
+    // rows from nv on, and all of a block without a page, land as zeros
+    __device__ FA_INLINE inline void load(Block16 k, int nv, const T* lds) const {
+        const T* at = base + (int64_t)max(k.page, 0) * sp + (int64_t)k.row * ss;
+        const u32x4 rs = row_buffer_words<T, D, 16>(at, ss, k.page < 0 ? 0 : nv, cols);
+        const uint32_t l0 = lds_addr(lds);
+#pragma unroll
+        for (int x = 0; x < C::NI16; ++x) dma_load16_untracked(rs, l0 + 1024 * x, off[x]);
+    }
+};
+
+// ---------------------------------------------------------------------------
+// Trees.  bits[i]: the nodes that node i sees (its ancestors and itself), none for what
+// is no token.  A node's bits are its parent's and its own: ceil(log2 N) rounds, each
+// joining the bits of the node that a node points to and pointing on to where that one
+// points (-1: the context, -2: no token).
+struct TreeBits {
+    unsigned bits[kTreeNodes][kTreeWords];
+    int up[kTreeNodes];
+};
+__device__ FA_INLINE inline void tree_init(const PagedParams& p, TreeBits& t, int b, int tid) {
+    const int N = p.Sq, W = (N + 31) >> 5;
+    __syncthreads();  // (the last unit's rows have read theirs)
+    int up = -2;
+    if (tid < N) {
+        up = p.parents[b * p.parents_sb + tid];
+        if (up < -1 || up >= tid) up = -2;
+        for (int w = 0; w < W; ++w) t.bits[tid][w] = w == (tid >> 5) ? 1u << (tid & 31) : 0u;
+        t.up[tid] = up;
+    }
+    for (int n = 1; n < N; n *= 2) {
+        __syncthreads();
+        unsigned more[kTreeWords];
+        int next = up;
+        if (up >= 0) {
+            for (int w = 0; w < kTreeWords; ++w) more[w] = w < W ? t.bits[up][w] : 0u;
+            next = t.up[up];
+        }
+        __syncthreads();
+        if (up >= 0) {
+            for (int w = 0; w < kTreeWords; ++w)
+                if (w < W) t.bits[tid][w] |= more[w];
+            t.up[tid] = up = next;
+        }
+    }
+    if (tid < N && up != -1)
+        for (int w = 0; w < W; ++w) t.bits[tid][w] = 0u;
+    __syncthreads();
+}
+// the 32 keys from tree position s on (it may be negative: the context) that node i sees
+__device__ FA_INLINE inline unsigned tree_word(const TreeBits& t, int i, int s, int W) {
+    const int w = s >> 5;
+    auto word = [&](int x) FA_INLINE { return x < 0 ? ~0u : x < W ? t.bits[i][x] : 0u; };
+    const uint64_t two = ((uint64_t)word(w + 1) << 32) | word(w);
+    return (unsigned)(two >> (s & 31));
+}
+
+// ---------------------------------------------------------------------------
+// Work.  Steps of all units in one list, by sequence, then unit; every sequence has
+// one at least.  Where no unit is longer than a workgroup's share (or than kLeast steps,
+// whose join would cost more than it saves), a workgroup takes whole units.
+constexpr int kLeast = 4;
+struct PagedWork {
+    int T, W;      // steps, workgroups that have work
+    int per_seq;   // units of a sequence
+    bool whole;    // a workgroup takes whole units
+    template <int STEP>
+    __device__ FA_INLINE inline static int steps(const PagedParams& p, int b) {
+        return b < p.B ? max(1, (own_len(p, b) + STEP - 1) / STEP) : 0;
+    }
+    template <int STEP>
+    __device__ FA_INLINE inline void init(const PagedParams& p, int lane) {
+        int sum = 0, most = 0;
+        if (p.lens) {
+            for (int b0 = 0; b0 < p.B; b0 += 64) {
+                const int st = steps<STEP>(p, b0 + lane);
+                sum += st;
+                most = max(most, st);
+            }
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1) {
+                sum += __shfl_xor(sum, x);
+                most = max(most, __shfl_xor(most, x));
+            }
+        } else {
+            most = steps<STEP>(p, 0);
+            sum = most * p.B;
+        }
+        per_seq = p.Hkv * p.unit_tiles;
+        T = __builtin_amdgcn_readfirstlane(sum) * per_seq;
+        const int share = max(kLeast, (T + p.slots - 1) / p.slots);
+        whole = __builtin_amdgcn_readfirstlane(most) <= share;
+        W = whole ? p.B * per_seq : (T + share - 1) / share;
+    }
+    // the first step of workgroup g (floor(g T / W)), and whose step x is
+    __device__ FA_INLINE inline int first(int g) const { return (int)((int64_t)g * T / W); }
+    __device__ FA_INLINE inline int whose(int x) const { return (int)((((int64_t)x + 1) * W - 1) / T); }
+    // the sequence of step x, its first step and the steps of one of its units
+    template <int STEP>
+    __device__ FA_INLINE inline void locate(const PagedParams& p, int x, int lane, int& b, int& start, int& len) const {
+        if (!p.lens) {
+            len = steps<STEP>(p, 0);
+            b = x / (len * per_seq);
+            start = b * len * per_seq;
+            return;
+        }
+        int before = 0;
+        for (int b0 = 0;; b0 += 64) {
+            const int st = steps<STEP>(p, b0 + lane);
+            int inc = st;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int y = __shfl_up(inc, d);
+                if (lane >= d) inc += y;
+            }
+            const uint64_t past = __ballot((int64_t)(before + inc) * per_seq > x);
+            if (past || b0 + 64 >= p.B) {
+                const int l = past ? (int)__builtin_ctzll(past) : 63;
+                b = b0 + l;
+                len = __builtin_amdgcn_readlane(st, l);
+                start = (before + __builtin_amdgcn_readlane(inc, l) - len) * per_seq;
+                return;
+            }
+            before += __builtin_amdgcn_readlane(inc, 63);
+        }
+    }
+    // the first step of sequence b
+    template <int STEP>
+    __device__ FA_INLINE inline int start_of(const PagedParams& p, int b, int lane) const {
+        if (!p.lens) return b * steps<STEP>(p, 0) * per_seq;
+        int sum = 0;
+        for (int b0 = 0; b0 < b; b0 += 64) sum += b0 + lane < b ? steps<STEP>(p, b0 + lane) : 0;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+        return __builtin_amdgcn_readfirstlane(sum) * per_seq;
+    }
+};
+// parts: a workgroup leaves at most two, of the unit that it begins with (2 g) and of
+// the one that it ends with, begun by it (2 g + 1)
+template <int ROWS>
+__device__ FA_INLINE inline int64_t part_at(int g, bool begun) { return ((int64_t)2 * g + (begun ? 1 : 0)) * ROWS; }
+
+// one row of a unit: keys [0, lim) at most, of which it sees all below `all`
+struct PagedRow {
+    int i, h, lim, all;
+    bool live, valid;  // exists; and sees keys
+    int qpos;
+    __device__ FA_INLINE inline PagedRow(const PagedParams& p, const TreeBits* t, int row, int b, int hk, int len) {
+        live = row < p.Sq * p.group;
+        const int rr = live ? row : 0;
+        i = rr / p.group;
+        h = hk * p.group + rr % p.group;
+        const int c = len - p.Sq;
+        valid = live && c + i >= 0;
+        qpos = c + i;
+        lim = all = c + i + 1;
+        if (t) {
+            const int W = (p.Sq + 31) >> 5;
+            int n = 0;
+            for (int w = 0; w < W; ++w) n += __popc(t->bits[i][w]);
+            valid = valid && n > 0;
+            qpos = c + n - 1;
+            lim = len;
+            all = max(c, 0);
+        }
+        if (!valid) lim = 0;
+    }
+};
+
+// the products of a wave's 32 rows with 32 keys (K tile), log2 units before the rules
+template <typename T, int D>
+__device__ FA_INLINE inline f32x16 tile_scores(const T* Ks, const uint4 (&q)[Elem<T>::kF32 ? D / 8 : D / 16], int l32, int hi) {
+    using C = PagedCfg<T, D>;
+    f32x16 s = f32x16{};
+    const char* row = (const char*)Ks + l32 * C::ROWB;
+    const int sw = row_swizzle<C::CW>(l32);
+    if constexpr (C::F32) {
+#pragma unroll
+        for (int kk = 0; kk < D / 8; ++kk) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(row + (((hi * (D / 8) + kk) ^ sw) << 4));
+            const f32x4 b = __builtin_bit_cast(f32x4, q[kk]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = mfma_f32(a[e], b[e], s);
+        }
+    } else {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+            const s16x8 a = *reinterpret_cast<const s16x8*>(row + (((2 * kk + hi) ^ sw) << 4));
+            s = Elem<T>::mfma(a, __builtin_bit_cast(s16x8, q[kk]), s);
+        }
+    }
+    return s;
+}
+
+// O^T += V^T P^T over 32 keys
+template <typename T, int D>
+__device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16& s, f32x16 (&o)[D / 32], int lane) {
+    using C = PagedCfg<T, D>;
+    const int l32 = lane & 31, hi = lane >> 5;
+    const char* vs = (const char*)Vs;
+    if constexpr (C::F32) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const int r = 8 * (x >> 2) + 4 * hi + (x & 3), sw = row_swizzle<C::CW>(r);
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n) {
+                const float v = *reinterpret_cast<const float*>(vs + r * C::ROWB + (((8 * n + (l32 >> 2)) ^ sw) << 4) + 4 * (l32 & 3));
+                o[n] = mfma_f32(v, s[x], o[n]);
+            }
+        }
+    } else {
+        const int r0 = 4 * hi + ((lane & 15) >> 2);
+        const int sw0 = row_swizzle<C::CW>(r0), sw1 = row_swizzle<C::CW>(r0 + 8);
+        const int chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        const char* vr = vs + r0 * C::ROWB + 8 * (lane & 1);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            float tmp[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) tmp[e] = s[8 * ks + e];
+            const s16x8 pk = pack8<T>(tmp);
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n) {
+                const s16x8 a = cat4(lds_read_tr16(vr + 16 * ks * C::ROWB + (((4 * n + chunk) ^ sw0) << 4)),
+                                     lds_read_tr16(vr + (16 * ks + 8) * C::ROWB + (((4 * n + chunk) ^ sw1) << 4)));
+                o[n] = Elem<T>::mfma(a, pk, o[n]);
+            }
+        }
+    }
+}
+
+// Whether a value of the tile is an infinity or NaN: 0 times it, for a key that a row does
+// not see, would not be 0
+template <typename T, int D>
+__device__ FA_INLINE inline bool tile_odd(const T* Vs, int lane) {
+    using C = PagedCfg<T, D>;
+    constexpr unsigned M = std::is_same<T, bf16>::value ? 0x7F80u : 0x7C00u;
+    bool odd = false;
+#pragma unroll
+    for (int x = 0; x < 32 * C::CW / 64; ++x) {
+        const uint4 v = *reinterpret_cast<const uint4*>((const char*)Vs + 16 * (64 * x + lane));
+        const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (C::F32)
+                odd |= (w[e] & 0x7F800000u) == 0x7F800000u;
+            else
+                odd |= (w[e] & M) == M || ((w[e] >> 16) & M) == M;
+        }
+    }
+    return __ballot(odd) != 0ull;
+}
+// tile_values key by key, each to the rows that see it (bit x of seen: key x)
+template <typename T, int D>
+__device__ FA_INLINE inline void tile_values_seen(const T* Vs, const f32x16& s, unsigned seen, f32x16 (&o)[D / 32], int lane) {
+    using C = PagedCfg<T, D>;
+    const int l32 = lane & 31, hi = lane >> 5;
+#pragma unroll 1
+    for (int g = 0; g < 4; ++g) {
+        float sv[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sv[c] = g == 0 ? s[c] : g == 1 ? s[4 + c] : g == 2 ? s[8 + c] : s[12 + c];
+#pragma unroll
+        for (int xc = 0; xc < 8; ++xc) {
+            const int x = 8 * g + xc;
+            const float p = __shfl(sv[xc & 3], l32 + 32 * (xc >> 2));
+            const bool sees = (seen >> x) & 1;
+            const char* row = (const char*)Vs + x * C::ROWB;
+            const int sw = row_swizzle<C::CW>(x);
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                    float v[4];
+                    if constexpr (C::F32) {
+                        const f32x4 y = *reinterpret_cast<const f32x4*>(row + (((8 * n + 2 * q4 + hi) ^ sw) << 4));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = y[e];
+                    } else {
+                        const s16x4 y = *reinterpret_cast<const s16x4*>(row + (((4 * n + q4) ^ sw) << 4) + 8 * hi);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = Elem<T>::unpack1(y[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float y = __builtin_fmaf(p, v[e], o[n][4 * q4 + e]);
+                        o[n][4 * q4 + e] = sees ? y : o[n][4 * q4 + e];
+                    }
+                }
+        }
+    }
+}
+
+// What a row sees of the 32 keys from k0 on, with bits for the blocks that have a page
+__device__ FA_INLINE inline unsigned row_sees(const PagedParams& p, const TreeBits* t, const PagedRow& r, int k0, int c, unsigned have) {
+    unsigned w;
+    if (t) {
+        w = tree_word(*t, r.i, k0 - c, (p.Sq + 31) >> 5);
+    } else {
+        const int n = r.lim - k0;
+        w = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+    }
+    return r.valid ? w & have : 0u;
+}
+
+// scores of 32 keys through the rules, hidden ones -infinity.  hidden: some row may not
+// see some key
+template <bool EXACT>
+__device__ FA_INLINE inline void tile_rules(f32x16& s, const PagedParams& p, Cap<EXACT>& cap, const PagedRow& r, const TreeBits* t,
+                                           bool slope, float slope2, int k0, int c, unsigned& seen, bool hidden, unsigned have, int hi) {
+    const bool steps = slope && hidden && t;  // distances along the tree
+    row_rules(s, p, cap, slope && !steps, slope2, (float)(r.qpos - k0 - 4 * hi));
+    if (hidden) {
+        stay_branch();
+        seen = row_sees(p, t, r, k0, c, have);
+        const unsigned mine = seen >> (4 * hi);
+        if (steps) {
+            // the tokens from a key to the row's own are those that it sees behind the key
+            const int W = (p.Sq + 31) >> 5, end = k0 - c + 32;
+            int above = 0;
+            for (int w = max(end, 0) >> 5; w < W; ++w) {
+                const unsigned x = t->bits[r.i][w];
+                above += __popc(w == (end >> 5) ? x & (~0u << (end & 31)) : x);
+            }
+            if (end < 0) above += -end;
+            const unsigned word = tree_word(*t, r.i, k0 - c, W);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int x = 8 * (e >> 2) + (e & 3);
+                const int d = above + __popc((word >> (x + 4 * hi)) >> 1);
+                s[e] = __builtin_fmaf(-slope2, (float)d, s[e]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (!((mine >> (8 * (e >> 2) + (e & 3))) & 1)) s[e] = -INFINITY;
+    }
+}
+
+// 32 rows of a unit over its steps [s0, s1): each wave walks tiles of its own.  part:
+// the rows' place among the parts, below 0 where this is all of the unit.
+template <typename T, int D, bool EXACT>
+__device__ FA_INLINE inline void paged_unit32(const PagedParams& p, T* smem, float (*stat)[2][32], const TreeBits* tree, int b, int hk,
+                                             int rt, int s0, int s1, int64_t part, int lane, int w) {
+    using C = PagedCfg<T, D>;
+    constexpr int NW = C::NW;
+    const int l32 = lane & 31, hi = lane >> 5;
+    const int len = __builtin_amdgcn_readfirstlane(own_len(p, b)), c = len - p.Sq;
+    const PagedRow row(p, tree, 32 * rt + l32, b, hk, len);
+    int lim_max = row.lim, lim_min = row.valid ? row.all : INT_MAX;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        lim_max = max(lim_max, __shfl_xor(lim_max, x));
+        lim_min = min(lim_min, __shfl_xor(lim_min, x));
+    }
+    lim_max = __builtin_amdgcn_readfirstlane(lim_max);
+    lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+    const int nt = (lim_max + 31) / 32, t1 = min(NW * s1, nt);
+    const bool uneven = tree || lim_min != lim_max;  // rows see different keys
+
+    T* Ks = smem + w * C::REGION;
+    T* Vs = Ks + C::TILE;
+    PageCopy<T, D> kc, vc;
+    kc.init((const T*)p.k + hk * p.k_sh, p.k_sp, p.k_ss, p.cols, lane);
+    vc.init((const T*)p.v + hk * p.v_sh, p.v_sp, p.v_ss, p.cols, lane);
+    // the two blocks of a tile; what is past the end reads nothing, but is issued, so that
+    // the vmcnt counts stay exact
+    auto blocks = [&](int t, Block16& x, Block16& y) FA_INLINE {
+        const int tt = min(t, max(nt - 1, 0));
+        x = block_at(p, b, 2 * tt);
+        y = block_at(p, b, 2 * tt + 1);
+    };
+    auto copy = [&](const PageCopy<T, D>& pc, int t, Block16 x, Block16 y, const T* dst) FA_INLINE {
+        const int nv = t < t1 ? lim_max - 32 * t : 0;
+        pc.load(x, nv, dst);
+        pc.load(y, nv - 16, dst + 16 * D);
+    };
+
+    constexpr int QR = C::F32 ? D / 8 : D / 16;
+    uint4 q[QR];
+    {
+        const T* qrow = (const T*)p.q + b * p.q_sb + (int64_t)row.i * p.q_ss + row.h * p.q_sh;
+#pragma unroll
+        for (int kk = 0; kk < QR; ++kk) {
+            const int d0 = C::F32 ? hi * (D / 2) + 4 * kk : 16 * kk + 8 * hi;
+            q[kk] = row.live && d0 < p.cols ? *reinterpret_cast<const uint4*>(qrow + d0) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    const bool slope = p.slopes != nullptr;
+    const float slope2 = slope ? p.slopes[b * p.slopes_sb + row.h] * kLog2e : 0.f;
+    wait_vmem();
+    asm volatile("" ::: "memory");
+
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) o[n] = f32x16{};
+    float m_run = -1e30f, l_run = 0.f;
+    Cap<EXACT> cap(p);
+
+    int t = NW * s0 + w;
+    Block16 bx, by;
+    blocks(t, bx, by);
+    copy(kc, t, bx, by, Ks);
+    copy(vc, t, bx, by, Vs);
+    for (; t < t1; t += NW) {
+        const int k0 = 32 * t;
+        const unsigned have = (bx.page < 0 ? 0u : 0xFFFFu) | (by.page < 0 ? 0u : 0xFFFF0000u);
+        wait_vmem_below<2 * C::NI16>();  // K(t); only V(t) may be in flight
+        asm volatile("" ::: "memory");
+        f32x16 s = tile_scores<T, D>(Ks, q, l32, hi);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K(t) read before it is overwritten
+        blocks(t + NW, bx, by);
+        copy(kc, t + NW, bx, by, Ks);
+
+        const bool hidden = k0 + 32 > lim_min || have != ~0u;
+        unsigned seen = ~0u;
+        tile_rules(s, p, cap, row, tree, slope, slope2, k0, c, seen, hidden, have, hi);
+        float m2[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m2[e & 1] = fmaxf(m2[e & 1], s[e]);
+        const float m_new = fmaxf(m_run, pair_max(fmaxf(m2[0], m2[1])));
+        if (__ballot(m_new > m_run + 8.0f) != 0ull) {
+            const float alpha = fast_exp2(m_run - m_new);
+            l_run *= alpha;
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[n][e] *= alpha;
+            m_run = m_new;
+        }
+        float ps[2] = {0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            s[e] = fast_exp2(s[e] - m_run);
+            ps[e & 1] += s[e];
+        }
+        l_run += ps[0] + ps[1];
+
+        wait_vmem_below<2 * C::NI16>();  // V(t); only K(t + 4) may be in flight
+        asm volatile("" ::: "memory");
+        if (hidden && uneven && tile_odd<T, D>(Vs, lane)) {
+            stay_branch();
+            tile_values_seen<T, D>(Vs, s, seen, o, lane);
+        } else {
+            tile_values<T, D>(Vs, s, o, lane);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V(t) read before it is overwritten
+        copy(vc, t + NW, bx, by, Vs);
+    }
+    wait_vmem();  // no copy in flight when the region takes the O part
+    asm volatile("" ::: "memory");
+
+    // ---- the waves' parts, rescaled to their common maximum ----
+    const float l_w = pair_sum(l_run);
+    float* mine = reinterpret_cast<float*>(Ks);
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mine[(16 * n + e) * 64 + lane] = o[n][e];
+    if (hi == 0) {
+        stat[w][0][l32] = m_run;
+        stat[w][1][l32] = l_w;
+    }
+    lds_barrier();
+    float mm = stat[0][0][l32];
+#pragma unroll
+    for (int x = 1; x < NW; ++x) mm = fmaxf(mm, stat[x][0][l32]);
+    float a[NW], l_tot = 0.f;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+        a[x] = fast_exp2(stat[x][0][l32] - mm);
+        l_tot = __builtin_fmaf(stat[x][1][l32], a[x], l_tot);
+    }
+    if (!row.valid) {  // (such a row went along with the others)
+        mm = -1e30f;
+        l_tot = 0.f;
+    }
+    const bool whole = part < 0;
+    const int64_t prow = part + l32;
+    if (!whole && w == 0 && hi == 0) p.stat[prow] = make_float2(mm, l_tot);
+    if (whole && w == 0 && hi == 0 && row.live && p.lse) put_lse(p, b, row.h, row.i, mm, l_tot);
+    const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
+#pragma unroll
+    for (int n0 = 0; n0 < D / 32; n0 += NW) {
+        const int n = n0 + w;
+        if (n >= D / 32) break;
+        f32x16 om = f32x16{};
+#pragma unroll
+        for (int x = 0; x < NW; ++x) {
+            const float* px = reinterpret_cast<const float*>(smem + x * C::REGION);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) om[e] = __builtin_fmaf(px[(16 * n + e) * 64 + lane], a[x], om[e]);
+        }
+        if (!row.valid) om = f32x16{};
+        if (!whole) {
+            float* op = p.part + prow * D + 32 * n + 4 * hi;
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+                *reinterpret_cast<f32x4*>(op + 8 * q4) = f32x4{om[4 * q4], om[4 * q4 + 1], om[4 * q4 + 2], om[4 * q4 + 3]};
+        } else if (row.live) {
+            T* ob = (T*)p.o + b * p.o_sb + (int64_t)row.i * p.o_ss + row.h * p.o_sh + 32 * n + 4 * hi;
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                if (32 * n + 8 * q4 + 4 * hi >= p.cols) continue;
+                if constexpr (C::F32) {
+                    f32x4 v4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v4[e] = om[4 * q4 + e] * inv;
+                    *reinterpret_cast<f32x4*>(ob + 8 * q4) = v4;
+                } else {
+                    s16x4 v4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v4[e] = Elem<T>::pack1(om[4 * q4 + e] * inv);
+                    *reinterpret_cast<s16x4*>(ob + 8 * q4) = v4;
+                }
+            }
+        }
+    }
+    lds_barrier();  // the regions and stat are free for the next unit
+}
+
+template <typename T, int D, bool EXACT, bool TREE>
+__global__ __launch_bounds__(256, (PagedCfg<T, D>::PER_CU)) void paged_kernel(const PagedParams p) {
+    using C = PagedCfg<T, D>;
+    __shared__ __attribute__((aligned(1024))) T smem[C::SMEM];
+    __shared__ float stat[C::NW][2][32];
+    __shared__ typename std::conditional<TREE, TreeBits, int>::type bits;
+    const TreeBits* tree = nullptr;
+    if constexpr (TREE) tree = &bits;
+    const int tid = threadIdx.x;
+    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
+    PagedWork wk;
+    wk.init<C::STEP>(p, lane);
+    if ((int)blockIdx.x >= wk.W) return;
+    const int g = xcd_remap((int)blockIdx.x, wk.W);
+    int x = 0, end = 0, b = 0, start = 0, len = 0, last_b = -1;
+    if (wk.whole) {
+        b = g / wk.per_seq;
+        len = __builtin_amdgcn_readfirstlane(PagedWork::steps<C::STEP>(p, b));
+        start = 0;
+        x = g % wk.per_seq * len;
+        end = x + len;
+    } else {
+        x = wk.first(g);
+        end = wk.first(g + 1);
+    }
+    while (x < end) {
+        if (!wk.whole && (last_b < 0 || x >= start + len * wk.per_seq)) wk.locate<C::STEP>(p, x, lane, b, start, len);
+        const int u = (x - start) / len, s0 = x - start - u * len, s1 = min(len, s0 + end - x);
+        if constexpr (TREE) {
+            if (b != last_b) tree_init(p, bits, b, tid);
+        }
+        last_b = b;
+        const int64_t part = s1 - s0 == len ? -1 : part_at<32>(g, s0 == 0);
+        paged_unit32<T, D, EXACT>(p, smem, stat, tree, b, u / p.unit_tiles, u % p.unit_tiles, s0, s1, part, lane, w);
+        x += s1 - s0;
+    }
+}
+
+// The parts of the rows of units that several workgroups shared: D / 4 threads a row,
+// 4 columns each, a wave's rows all of one sequence (blockIdx.y)
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams p) {
+    using C = PagedCfg<T, D>;
+    constexpr int TPR = D / 4, ROWS = 256 / TPR;
+    const int lane = threadIdx.x & 63, b = blockIdx.y;
+    PagedWork wk;
+    wk.init<C::STEP>(p, lane);
+    if (wk.whole) return;
+    const int start = wk.start_of<C::STEP>(p, b, lane);
+    const int len = __builtin_amdgcn_readfirstlane(PagedWork::steps<C::STEP>(p, b));
+    const int r = (int)blockIdx.x * ROWS + (int)threadIdx.x / TPR, col = (int)(threadIdx.x % TPR) * 4;
+    const int rows = p.Sq * p.group;  // of a KV head
+    if (r >= rows * p.Hkv) return;
+    const int hk = r / rows, ig = r % rows, rt = ig >> 5;
+    const int s = start + (hk * p.unit_tiles + rt) * len;  // the unit's first step
+    const int g0 = wk.whose(s), g1 = wk.whose(s + len - 1);
+    if (g0 == g1) return;
+    float mm = -1e30f, l_tot = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int x0 = g0; x0 <= g1; x0 += 4) {
+        float2 st[4];
+        f32x4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool in = x0 + j <= g1;
+            const int g = in ? x0 + j : g0;
+            const int64_t pr = part_at<32>(g, g == g0) + (ig & 31);  // g0 begins the unit
+            st[j] = p.stat[pr];
+            v[j] = *reinterpret_cast<const f32x4*>(p.part + pr * D + col);
+            if (!in) {
+                st[j] = make_float2(-1e30f, 0.f);
+                v[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+        const float m0 = fmaxf(mm, fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)));
+        const float a0 = fast_exp2(mm - m0);
+        l_tot *= a0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] *= a0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float a = fast_exp2(st[j].x - m0);
+            l_tot = __builtin_fmaf(st[j].y, a, l_tot);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[j][e], a, acc[e]);
+        }
+        mm = m0;
+    }
+    const int i = ig / p.group, h = hk * p.group + ig % p.group;
+    const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
+    if (col == 0 && p.lse) put_lse(p, b, h, i, mm, l_tot);
+    if (col >= p.cols) return;
+    T* ob = (T*)p.o + b * p.o_sb + (int64_t)i * p.o_ss + h * p.o_sh + col;
+    if constexpr (Elem<T>::kF32) {
+        *reinterpret_cast<f32x4*>(ob) = f32x4{acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+    } else {
+        s16x4 v4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v4[e] = Elem<T>::pack1(acc[e] * inv);
+        *reinterpret_cast<s16x4*>(ob) = v4;
+    }
+}
+
+template <typename T, int D>
+hipError_t launch_paged_t(const PagedParams& p, hipStream_t s) {
+    const dim3 grid((unsigned)p.o_wgs);
+    constexpr bool F32 = Elem<T>::kF32;
+    if (p.parents) {
+        if (F32 || p.cap > kWideCap)
+            hipLaunchKernelGGL((paged_kernel<T, D, true, true>), grid, dim3(256), 0, s, p);
+        else
+            hipLaunchKernelGGL((paged_kernel<T, D, F32, true>), grid, dim3(256), 0, s, p);
+    } else {
+        if (F32 || p.cap > kWideCap)
+            hipLaunchKernelGGL((paged_kernel<T, D, true, false>), grid, dim3(256), 0, s, p);
+        else
+            hipLaunchKernelGGL((paged_kernel<T, D, F32, false>), grid, dim3(256), 0, s, p);
+    }
+    if (p.part) {
+        constexpr int ROWS = 256 / (D / 4);
+        const int rows = p.Sq * p.H;
+        hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)((rows + ROWS - 1) / ROWS), (unsigned)p.B), dim3(256), 0, s, p);
+    }
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_paged(const PagedParams& p, int D, hipStream_t s) {
+    switch (D) {
+        case 32: return launch_paged_t<T, 32>(p, s);
+        case 64: return launch_paged_t<T, 64>(p, s);
+        case 128: return launch_paged_t<T, 128>(p, s);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace fa

@@ -7,7 +7,8 @@ launchers (``kernels/forward_kernel.py:246, 445``,
 ``kernels/backward_kernel.py:208``), all backed by hand-written HIP kernels in
 ``libfa_gfx950.so`` (C ABI: ``include/fa_abi.h``), and operators around them (C
 ABI: ``include/fa_ops.h``): attention with scored rules, new tokens after a
-shared prefix, rotary positions.  Importing the package does
+shared prefix, rotary positions; and a paged key/value cache with the attention
+that reads it (C ABI: ``include/fa_paged.h``).  Importing the package does
 not load the library; the first kernel call does, and raises
 ``FlashAttentionExtensionError`` if it is missing.
 """
@@ -33,6 +34,13 @@ from .ops.attention import (  # noqa: F401
     flash_attention_backward,
     flash_attention_forward,
 )
+from .ops.paged import flash_attention_v100_paged  # noqa: F401
+from .ops.paged_cache import (  # noqa: F401
+    paged_cache_accept_v100,
+    paged_cache_compact_v100,
+    paged_cache_fork_v100,
+    paged_cache_write_v100,
+)
 from .ops.rotary import rotary_embedding_v100, rotary_table_v100  # noqa: F401
 from .ops.scored import flash_attention_v100_scored  # noqa: F401
 from .ops.shared_prefix import flash_attention_v100_shared_prefix  # noqa: F401
@@ -50,6 +58,11 @@ __all__ = [
     "flash_attention_memory_mode",
     "flash_attention_v100_scored",
     "flash_attention_v100_shared_prefix",
+    "flash_attention_v100_paged",
+    "paged_cache_write_v100",
+    "paged_cache_accept_v100",
+    "paged_cache_fork_v100",
+    "paged_cache_compact_v100",
     "rotary_table_v100",
     "rotary_embedding_v100",
     "EnhancedMultiHeadAttention",

@@ -14,6 +14,13 @@ from .attention import (  # noqa: F401
     gradient_checkpointing_mode,
     mixed_precision_mode,
 )
+from .paged import flash_attention_v100_paged  # noqa: F401
+from .paged_cache import (  # noqa: F401
+    paged_cache_accept_v100,
+    paged_cache_compact_v100,
+    paged_cache_fork_v100,
+    paged_cache_write_v100,
+)
 from .rotary import rotary_embedding_v100, rotary_table_v100  # noqa: F401
 from .scored import flash_attention_v100_scored  # noqa: F401
 from .shared_prefix import flash_attention_v100_shared_prefix  # noqa: F401
@@ -21,6 +28,11 @@ from .shared_prefix import flash_attention_v100_shared_prefix  # noqa: F401
 __all__ = [
     "flash_attention_v100_scored",
     "flash_attention_v100_shared_prefix",
+    "flash_attention_v100_paged",
+    "paged_cache_write_v100",
+    "paged_cache_accept_v100",
+    "paged_cache_fork_v100",
+    "paged_cache_compact_v100",
     "rotary_table_v100",
     "rotary_embedding_v100",
     "FlashAttentionV100Function",
