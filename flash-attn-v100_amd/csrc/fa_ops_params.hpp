@@ -121,7 +121,7 @@ struct PagedParams : RowsParams {
     int64_t table_sb;
     int table_cols, pages;
     int page_blocks;       // blocks of 16 tokens in a page
-    unsigned page_magic;   // 2^32 / page_blocks, up to one below or above
+    unsigned page_magic;   // 2^32 / page_blocks, rounded up
     int64_t k_sp, v_sp;    // page strides
     const int* parents;    // optional (B, Sq), batch stride parents_sb
     int64_t parents_sb;

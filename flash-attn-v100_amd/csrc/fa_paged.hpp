@@ -17,7 +17,7 @@
 
 #include "fa_common.hpp"
 #include "fa_ops_params.hpp"
-#include "fa_rows.hpp"
+#include "fa_scored.hpp"
 
 namespace fa {
 
@@ -50,6 +50,21 @@ __device__ FA_INLINE inline int row_swizzle(int r) {
     return ((r & 3) << 2) | ((r >> 2) & 3);
 }
 
+// The kernel's arguments, to be read by scalar loads where they are used: read first
+// and kept, they took more scalar registers than there are (200 reads of lanes of vector
+// registers in the loop over tiles).
+typedef const __attribute__((address_space(4))) PagedParams PagedArgs;
+__device__ FA_INLINE inline PagedArgs& paged_args() {
+    uint64_t a = (uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    return *(PagedArgs*)(uintptr_t)a;
+}
+// filled tokens of a sequence
+__device__ FA_INLINE inline int filled_tokens(PagedArgs& p, int b) { return p.lens ? max(0, min(p.Sk, p.lens[b])) : p.Sk; }
+__device__ FA_INLINE inline void put_row_lse(PagedArgs& p, int b, int h, int i, float m, float l) {
+    p.lse[((int64_t)b * p.H + h) * p.Sq + i] = l > 0.f ? (m + __log2f(l)) * kLn2 : l == 0.f ? -INFINITY : l;
+}
+
 // scalar loads of what no kernel of the call writes
 typedef const __attribute__((address_space(4))) int const_int;
 __device__ FA_INLINE inline int uniform_load(const int* p, int64_t at) {
@@ -60,20 +75,21 @@ __device__ FA_INLINE inline int uniform_load(const int* p, int64_t at) {
 struct Block16 {
     int page, row;
 };
-__device__ FA_INLINE inline Block16 block_at(const PagedParams& p, int b, int blk) {
-    if (!p.table) return {b, 16 * blk};
-    int col = (int)__umulhi((unsigned)blk, p.page_magic);
-    int r = blk - col * p.page_blocks;
-    if (r < 0) {
-        --col;
-        r += p.page_blocks;
-    } else if (r >= p.page_blocks) {
-        ++col;
-        r -= p.page_blocks;
+// the lookups of one sequence
+struct PageTable {
+    const int* row;  // null: its tokens are all on page b
+    int b, last_col, pages, blocks;
+    unsigned magic;
+    __device__ FA_INLINE inline PageTable(PagedArgs& p, int b_)
+        : row(p.table ? p.table + b_ * p.table_sb : nullptr), b(b_), last_col(p.table_cols - 1), pages(p.pages), blocks(p.page_blocks),
+          magic(p.page_magic) {}
+    __device__ FA_INLINE inline Block16 block(int blk) const {
+        const int col = blocks == 1 ? blk : (int)__umulhi((unsigned)blk, magic);
+        int page = b;
+        if (row) page = uniform_load(row, min(col, last_col));
+        return {(unsigned)page < (unsigned)pages ? page : -1, 16 * (blk - col * blocks)};
     }
-    const int page = uniform_load(p.table, b * p.table_sb + min(col, p.table_cols - 1));
-    return {(unsigned)page < (unsigned)p.pages ? page : -1, 16 * r};
-}
+};
 
 // copies of 16-row blocks of one KV head's keys or values
 template <typename T, int D>
@@ -113,7 +129,7 @@ struct TreeBits {
     unsigned bits[kTreeNodes][kTreeWords];
     int up[kTreeNodes];
 };
-__device__ FA_INLINE inline void tree_init(const PagedParams& p, TreeBits& t, int b, int tid) {
+__device__ FA_INLINE inline void tree_init(PagedArgs& p, TreeBits& t, int b, int tid) {
     const int N = p.Sq, W = (N + 31) >> 5;
     __syncthreads();  // (the last unit's rows have read theirs)
     int up = -2;
@@ -160,11 +176,11 @@ struct PagedWork {
     int per_seq;   // units of a sequence
     bool whole;    // a workgroup takes whole units
     template <int STEP>
-    __device__ FA_INLINE inline static int steps(const PagedParams& p, int b) {
-        return b < p.B ? max(1, (own_len(p, b) + STEP - 1) / STEP) : 0;
+    __device__ FA_INLINE inline static int steps(PagedArgs& p, int b) {
+        return b < p.B ? max(1, (filled_tokens(p, b) + STEP - 1) / STEP) : 0;
     }
     template <int STEP>
-    __device__ FA_INLINE inline void init(const PagedParams& p, int lane) {
+    __device__ FA_INLINE inline void init(PagedArgs& p, int lane) {
         int sum = 0, most = 0;
         if (p.lens) {
             for (int b0 = 0; b0 < p.B; b0 += 64) {
@@ -192,7 +208,7 @@ struct PagedWork {
     __device__ FA_INLINE inline int whose(int x) const { return (int)((((int64_t)x + 1) * W - 1) / T); }
     // the sequence of step x, its first step and the steps of one of its units
     template <int STEP>
-    __device__ FA_INLINE inline void locate(const PagedParams& p, int x, int lane, int& b, int& start, int& len) const {
+    __device__ FA_INLINE inline void locate(PagedArgs& p, int x, int lane, int& b, int& start, int& len) const {
         if (!p.lens) {
             len = steps<STEP>(p, 0);
             b = x / (len * per_seq);
@@ -221,7 +237,7 @@ struct PagedWork {
     }
     // the first step of sequence b
     template <int STEP>
-    __device__ FA_INLINE inline int start_of(const PagedParams& p, int b, int lane) const {
+    __device__ FA_INLINE inline int start_of(PagedArgs& p, int b, int lane) const {
         if (!p.lens) return b * steps<STEP>(p, 0) * per_seq;
         int sum = 0;
         for (int b0 = 0; b0 < b; b0 += 64) sum += b0 + lane < b ? steps<STEP>(p, b0 + lane) : 0;
@@ -240,7 +256,7 @@ struct PagedRow {
     int i, h, lim, all;
     bool live, valid;  // exists; and sees keys
     int qpos;
-    __device__ FA_INLINE inline PagedRow(const PagedParams& p, const TreeBits* t, int row, int b, int hk, int len) {
+    __device__ FA_INLINE inline PagedRow(PagedArgs& p, const TreeBits* t, int row, int b, int hk, int len) {
         live = row < p.Sq * p.group;
         const int rr = live ? row : 0;
         i = rr / p.group;
@@ -262,27 +278,44 @@ struct PagedRow {
     }
 };
 
+// A lane's place in a tile, as an LDS address that the compiler does not see through: the
+// places of the columns after it are that ^ a constant (a tile begins at a multiple of
+// its row's bytes), one instruction each, which it would otherwise keep in registers
+// from tile to tile.
+typedef __attribute__((address_space(3))) const char* lds_chars;
+__device__ FA_INLINE inline uint32_t lds_place(const void* tile, int bytes) {
+    uint32_t a = lds_addr(tile) + bytes;
+    asm volatile("" : "+v"(a));
+    return a;
+}
+template <typename V>
+__device__ FA_INLINE inline V lds_at(uint32_t a) {
+    return *reinterpret_cast<__attribute__((address_space(3))) const V*>((lds_chars)(uintptr_t)a);
+}
+__device__ FA_INLINE inline s16x4 lds_tr16_at(uint32_t a) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)a);
+}
+
 // the products of a wave's 32 rows with 32 keys (K tile), log2 units before the rules
 template <typename T, int D>
 __device__ FA_INLINE inline f32x16 tile_scores(const T* Ks, const uint4 (&q)[Elem<T>::kF32 ? D / 8 : D / 16], int l32, int hi) {
     using C = PagedCfg<T, D>;
     f32x16 s = f32x16{};
-    const char* row = (const char*)Ks + l32 * C::ROWB;
     const int sw = row_swizzle<C::CW>(l32);
     if constexpr (C::F32) {
+        const uint32_t at = lds_place(Ks, l32 * C::ROWB + (((hi * (D / 8)) ^ sw) << 4));
 #pragma unroll
         for (int kk = 0; kk < D / 8; ++kk) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(row + (((hi * (D / 8) + kk) ^ sw) << 4));
+            const f32x4 a = lds_at<f32x4>(at ^ (kk << 4));
             const f32x4 b = __builtin_bit_cast(f32x4, q[kk]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s = mfma_f32(a[e], b[e], s);
         }
     } else {
+        const uint32_t at = lds_place(Ks, l32 * C::ROWB + ((hi ^ sw) << 4));
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            const s16x8 a = *reinterpret_cast<const s16x8*>(row + (((2 * kk + hi) ^ sw) << 4));
-            s = Elem<T>::mfma(a, __builtin_bit_cast(s16x8, q[kk]), s);
-        }
+        for (int kk = 0; kk < D / 16; ++kk)
+            s = Elem<T>::mfma(lds_at<s16x8>(at ^ (kk << 5)), __builtin_bit_cast(s16x8, q[kk]), s);
     }
     return s;
 }
@@ -292,22 +325,20 @@ template <typename T, int D>
 __device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16& s, f32x16 (&o)[D / 32], int lane) {
     using C = PagedCfg<T, D>;
     const int l32 = lane & 31, hi = lane >> 5;
-    const char* vs = (const char*)Vs;
     if constexpr (C::F32) {
+        // rows 8 (x / 4) + 4 hi + x % 4: their swizzles differ from that of row 4 hi by x alone
+        const uint32_t at = lds_place(Vs, 4 * hi * C::ROWB + (((l32 >> 2) ^ row_swizzle<C::CW>(4 * hi)) << 4) + 4 * (l32 & 3));
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-            const int r = 8 * (x >> 2) + 4 * hi + (x & 3), sw = row_swizzle<C::CW>(r);
+            const int r = 8 * (x >> 2) + (x & 3);
 #pragma unroll
-            for (int n = 0; n < D / 32; ++n) {
-                const float v = *reinterpret_cast<const float*>(vs + r * C::ROWB + (((8 * n + (l32 >> 2)) ^ sw) << 4) + 4 * (l32 & 3));
-                o[n] = mfma_f32(v, s[x], o[n]);
-            }
+            for (int n = 0; n < D / 32; ++n)
+                o[n] = mfma_f32(lds_at<float>((at ^ (((8 * n) ^ row_swizzle<C::CW>(r)) << 4)) + r * C::ROWB), s[x], o[n]);
         }
     } else {
         const int r0 = 4 * hi + ((lane & 15) >> 2);
-        const int sw0 = row_swizzle<C::CW>(r0), sw1 = row_swizzle<C::CW>(r0 + 8);
         const int chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-        const char* vr = vs + r0 * C::ROWB + 8 * (lane & 1);
+        const uint32_t at = lds_place(Vs, r0 * C::ROWB + ((chunk ^ row_swizzle<C::CW>(r0)) << 4) + 8 * (lane & 1));
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             float tmp[8];
@@ -316,8 +347,8 @@ __device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16& s, f32x1
             const s16x8 pk = pack8<T>(tmp);
 #pragma unroll
             for (int n = 0; n < D / 32; ++n) {
-                const s16x8 a = cat4(lds_read_tr16(vr + 16 * ks * C::ROWB + (((4 * n + chunk) ^ sw0) << 4)),
-                                     lds_read_tr16(vr + (16 * ks + 8) * C::ROWB + (((4 * n + chunk) ^ sw1) << 4)));
+                const s16x8 a = cat4(lds_tr16_at((at ^ (n << 6)) + 16 * ks * C::ROWB),
+                                     lds_tr16_at((at ^ ((n << 6) ^ (row_swizzle<C::CW>(8) << 4))) + (16 * ks + 8) * C::ROWB));
                 o[n] = Elem<T>::mfma(a, pk, o[n]);
             }
         }
@@ -351,43 +382,39 @@ __device__ FA_INLINE inline void tile_values_seen(const T* Vs, const f32x16& s, 
     using C = PagedCfg<T, D>;
     const int l32 = lane & 31, hi = lane >> 5;
 #pragma unroll 1
-    for (int g = 0; g < 4; ++g) {
-        float sv[4];
+    for (int x = 0; x < 32; ++x) {
+        float mine = 0.f;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) sv[c] = g == 0 ? s[c] : g == 1 ? s[4 + c] : g == 2 ? s[8 + c] : s[12 + c];
+        for (int e = 0; e < 16; ++e) mine = e == 4 * (x >> 3) + (x & 3) ? s[e] : mine;
+        const float p = __shfl(mine, l32 + 8 * (x & 4));
+        const bool sees = (seen >> x) & 1;
+        const char* row = (const char*)Vs + x * C::ROWB;
+        const int sw = row_swizzle<C::CW>(x);
 #pragma unroll
-        for (int xc = 0; xc < 8; ++xc) {
-            const int x = 8 * g + xc;
-            const float p = __shfl(sv[xc & 3], l32 + 32 * (xc >> 2));
-            const bool sees = (seen >> x) & 1;
-            const char* row = (const char*)Vs + x * C::ROWB;
-            const int sw = row_swizzle<C::CW>(x);
+        for (int n = 0; n < D / 32; ++n)
 #pragma unroll
-            for (int n = 0; n < D / 32; ++n)
+            for (int q4 = 0; q4 < 4; ++q4) {
+                float v[4];
+                if constexpr (C::F32) {
+                    const f32x4 y = *reinterpret_cast<const f32x4*>(row + (((8 * n + 2 * q4 + hi) ^ sw) << 4));
 #pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4) {
-                    float v[4];
-                    if constexpr (C::F32) {
-                        const f32x4 y = *reinterpret_cast<const f32x4*>(row + (((8 * n + 2 * q4 + hi) ^ sw) << 4));
+                    for (int e = 0; e < 4; ++e) v[e] = y[e];
+                } else {
+                    const s16x4 y = *reinterpret_cast<const s16x4*>(row + (((4 * n + q4) ^ sw) << 4) + 8 * hi);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = y[e];
-                    } else {
-                        const s16x4 y = *reinterpret_cast<const s16x4*>(row + (((4 * n + q4) ^ sw) << 4) + 8 * hi);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = Elem<T>::unpack1(y[e]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float y = __builtin_fmaf(p, v[e], o[n][4 * q4 + e]);
-                        o[n][4 * q4 + e] = sees ? y : o[n][4 * q4 + e];
-                    }
+                    for (int e = 0; e < 4; ++e) v[e] = Elem<T>::unpack1(y[e]);
                 }
-        }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float y = __builtin_fmaf(p, v[e], o[n][4 * q4 + e]);
+                    o[n][4 * q4 + e] = sees ? y : o[n][4 * q4 + e];
+                }
+            }
     }
 }
 
 // What a row sees of the 32 keys from k0 on, with bits for the blocks that have a page
-__device__ FA_INLINE inline unsigned row_sees(const PagedParams& p, const TreeBits* t, const PagedRow& r, int k0, int c, unsigned have) {
+__device__ FA_INLINE inline unsigned row_sees(PagedArgs& p, const TreeBits* t, const PagedRow& r, int k0, int c, unsigned have) {
     unsigned w;
     if (t) {
         w = tree_word(*t, r.i, k0 - c, (p.Sq + 31) >> 5);
@@ -401,10 +428,23 @@ __device__ FA_INLINE inline unsigned row_sees(const PagedParams& p, const TreeBi
 // scores of 32 keys through the rules, hidden ones -infinity.  hidden: some row may not
 // see some key
 template <bool EXACT>
-__device__ FA_INLINE inline void tile_rules(f32x16& s, const PagedParams& p, Cap<EXACT>& cap, const PagedRow& r, const TreeBits* t,
+__device__ FA_INLINE inline void tile_rules(f32x16& s, PagedArgs& p, Cap<EXACT>& cap, const PagedRow& r, const TreeBits* t,
                                            bool slope, float slope2, int k0, int c, unsigned& seen, bool hidden, unsigned have, int hi) {
     const bool steps = slope && hidden && t;  // distances along the tree
-    row_rules(s, p, cap, slope && !steps, slope2, (float)(r.qpos - k0 - 4 * hi));
+    if (p.cap > 0.f) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = cap.value(s[e]);
+    } else {
+        const float mul = p.scale_log2;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] *= mul;
+    }
+    if (slope && !steps) {
+        const float d0 = (float)(r.qpos - k0 - 4 * hi);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            s[e] = __builtin_fmaf(-slope2, __builtin_fabsf(d0 - (float)(8 * (e >> 2) + (e & 3))), s[e]);
+    }
     if (hidden) {
         stay_branch();
         seen = row_sees(p, t, r, k0, c, have);
@@ -435,12 +475,13 @@ __device__ FA_INLINE inline void tile_rules(f32x16& s, const PagedParams& p, Cap
 // 32 rows of a unit over its steps [s0, s1): each wave walks tiles of its own.  part:
 // the rows' place among the parts, below 0 where this is all of the unit.
 template <typename T, int D, bool EXACT>
-__device__ FA_INLINE inline void paged_unit32(const PagedParams& p, T* smem, float (*stat)[2][32], const TreeBits* tree, int b, int hk,
+__device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], const TreeBits* tree, int b, int hk,
                                              int rt, int s0, int s1, int64_t part, int lane, int w) {
     using C = PagedCfg<T, D>;
     constexpr int NW = C::NW;
+    PagedArgs& p = paged_args();
     const int l32 = lane & 31, hi = lane >> 5;
-    const int len = __builtin_amdgcn_readfirstlane(own_len(p, b)), c = len - p.Sq;
+    const int len = __builtin_amdgcn_readfirstlane(filled_tokens(p, b)), c = len - p.Sq;
     const PagedRow row(p, tree, 32 * rt + l32, b, hk, len);
     int lim_max = row.lim, lim_min = row.valid ? row.all : INT_MAX;
 #pragma unroll
@@ -460,10 +501,11 @@ __device__ FA_INLINE inline void paged_unit32(const PagedParams& p, T* smem, flo
     vc.init((const T*)p.v + hk * p.v_sh, p.v_sp, p.v_ss, p.cols, lane);
     // the two blocks of a tile; what is past the end reads nothing, but is issued, so that
     // the vmcnt counts stay exact
+    const PageTable table(p, b);
     auto blocks = [&](int t, Block16& x, Block16& y) FA_INLINE {
         const int tt = min(t, max(nt - 1, 0));
-        x = block_at(p, b, 2 * tt);
-        y = block_at(p, b, 2 * tt + 1);
+        x = table.block(2 * tt);
+        y = table.block(2 * tt + 1);
     };
     auto copy = [&](const PageCopy<T, D>& pc, int t, Block16 x, Block16 y, const T* dst) FA_INLINE {
         const int nv = t < t1 ? lim_max - 32 * t : 0;
@@ -546,6 +588,7 @@ __device__ FA_INLINE inline void paged_unit32(const PagedParams& p, T* smem, flo
     asm volatile("" ::: "memory");
 
     // ---- the waves' parts, rescaled to their common maximum ----
+    PagedArgs& pe = paged_args();
     const float l_w = pair_sum(l_run);
     float* mine = reinterpret_cast<float*>(Ks);
 #pragma unroll
@@ -572,8 +615,8 @@ __device__ FA_INLINE inline void paged_unit32(const PagedParams& p, T* smem, flo
     }
     const bool whole = part < 0;
     const int64_t prow = part + l32;
-    if (!whole && w == 0 && hi == 0) p.stat[prow] = make_float2(mm, l_tot);
-    if (whole && w == 0 && hi == 0 && row.live && p.lse) put_lse(p, b, row.h, row.i, mm, l_tot);
+    if (!whole && w == 0 && hi == 0) pe.stat[prow] = make_float2(mm, l_tot);
+    if (whole && w == 0 && hi == 0 && row.live && pe.lse) put_row_lse(pe, b, row.h, row.i, mm, l_tot);
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
 #pragma unroll
     for (int n0 = 0; n0 < D / 32; n0 += NW) {
@@ -588,15 +631,15 @@ __device__ FA_INLINE inline void paged_unit32(const PagedParams& p, T* smem, flo
         }
         if (!row.valid) om = f32x16{};
         if (!whole) {
-            float* op = p.part + prow * D + 32 * n + 4 * hi;
+            float* op = pe.part + prow * D + 32 * n + 4 * hi;
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
                 *reinterpret_cast<f32x4*>(op + 8 * q4) = f32x4{om[4 * q4], om[4 * q4 + 1], om[4 * q4 + 2], om[4 * q4 + 3]};
         } else if (row.live) {
-            T* ob = (T*)p.o + b * p.o_sb + (int64_t)row.i * p.o_ss + row.h * p.o_sh + 32 * n + 4 * hi;
+            T* ob = (T*)pe.o + b * pe.o_sb + (int64_t)row.i * pe.o_ss + row.h * pe.o_sh + 32 * n + 4 * hi;
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
-                if (32 * n + 8 * q4 + 4 * hi >= p.cols) continue;
+                if (32 * n + 8 * q4 + 4 * hi >= pe.cols) continue;
                 if constexpr (C::F32) {
                     f32x4 v4;
 #pragma unroll
@@ -615,8 +658,9 @@ __device__ FA_INLINE inline void paged_unit32(const PagedParams& p, T* smem, flo
 }
 
 template <typename T, int D, bool EXACT, bool TREE>
-__global__ __launch_bounds__(256, (PagedCfg<T, D>::PER_CU)) void paged_kernel(const PagedParams p) {
+__global__ __launch_bounds__(256, (PagedCfg<T, D>::PER_CU)) void paged_kernel(const PagedParams) {
     using C = PagedCfg<T, D>;
+    PagedArgs& p = paged_args();
     __shared__ __attribute__((aligned(1024))) T smem[C::SMEM];
     __shared__ float stat[C::NW][2][32];
     __shared__ typename std::conditional<TREE, TreeBits, int>::type bits;
@@ -640,14 +684,15 @@ __global__ __launch_bounds__(256, (PagedCfg<T, D>::PER_CU)) void paged_kernel(co
         end = wk.first(g + 1);
     }
     while (x < end) {
-        if (!wk.whole && (last_b < 0 || x >= start + len * wk.per_seq)) wk.locate<C::STEP>(p, x, lane, b, start, len);
+        if (!wk.whole && (last_b < 0 || x >= start + len * wk.per_seq)) wk.locate<C::STEP>(paged_args(), x, lane, b, start, len);
         const int u = (x - start) / len, s0 = x - start - u * len, s1 = min(len, s0 + end - x);
         if constexpr (TREE) {
-            if (b != last_b) tree_init(p, bits, b, tid);
+            if (b != last_b) tree_init(paged_args(), bits, b, tid);
         }
         last_b = b;
         const int64_t part = s1 - s0 == len ? -1 : part_at<32>(g, s0 == 0);
-        paged_unit32<T, D, EXACT>(p, smem, stat, tree, b, u / p.unit_tiles, u % p.unit_tiles, s0, s1, part, lane, w);
+        const int tiles = paged_args().unit_tiles;
+        paged_unit32<T, D, EXACT>(smem, stat, tree, b, u / tiles, u % tiles, s0, s1, part, lane, w);
         x += s1 - s0;
     }
 }
@@ -655,8 +700,9 @@ __global__ __launch_bounds__(256, (PagedCfg<T, D>::PER_CU)) void paged_kernel(co
 // The parts of the rows of units that several workgroups shared: D / 4 threads a row,
 // 4 columns each, a wave's rows all of one sequence (blockIdx.y)
 template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams p) {
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams) {
     using C = PagedCfg<T, D>;
+    PagedArgs& p = paged_args();
     constexpr int TPR = D / 4, ROWS = 256 / TPR;
     const int lane = threadIdx.x & 63, b = blockIdx.y;
     PagedWork wk;
@@ -704,7 +750,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams p) {
     }
     const int i = ig / p.group, h = hk * p.group + ig % p.group;
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
-    if (col == 0 && p.lse) put_lse(p, b, h, i, mm, l_tot);
+    if (col == 0 && p.lse) put_row_lse(p, b, h, i, mm, l_tot);
     if (col >= p.cols) return;
     T* ob = (T*)p.o + b * p.o_sb + (int64_t)i * p.o_ss + h * p.o_sh + col;
     if constexpr (Elem<T>::kF32) {

@@ -41,6 +41,8 @@ int32_t check_pool(const fa_page_pool& c, bool table) {
         return FA_ERR_PAGES;
     }
     if (room_of(c) >= kMaxLen || c.page_size >= kMaxLen) return FA_ERR_TOO_LARGE;
+    // blocks of 16 tokens are divided by those of a page with a product of 32 bits, exact up to here
+    if (c.page_table && room_of(c) / 16 * (c.page_size / 16) >= (1LL << 32)) return FA_ERR_TOO_LARGE;
     if (!aligned(c.key_lengths, 4)) return FA_ERR_ALIGN;
     if (c.pages == 0 || c.page_size == 0) return FA_OK;
     for (int x = 0; x < 2; ++x) {
@@ -121,8 +123,9 @@ void put_paged(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& s
     p.table_sb = c.table_stride;
     p.table_cols = c.table_cols;
     p.pages = c.pages;
-    p.page_blocks = std::max(1, c.page_size / 16);
-    p.page_magic = p.page_blocks == 1 ? 0xFFFFFFFFu : (unsigned)((1ull << 32) / (unsigned)p.page_blocks);
+    // (a row of tokens: a page that no block is behind)
+    p.page_blocks = p.table ? c.page_size / 16 : c.page_size / 16 + 1;
+    p.page_magic = (unsigned)(((1ull << 32) + p.page_blocks - 1) / p.page_blocks);
     p.parents = a->parents;
     p.parents_sb = a->parents_stride;
     plan(a, p, grid, shared);
