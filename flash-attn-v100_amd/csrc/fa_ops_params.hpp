@@ -125,9 +125,10 @@ struct PagedParams : RowsParams {
     int64_t k_sp, v_sp;    // page strides
     const int* parents;    // optional (B, Sq), batch stride parents_sb
     int64_t parents_sb;
-    // work: units of unit_rows rows of one (sequence, KV head), unit_tiles a KV head,
-    // over steps of step_keys keys, shared out to at most `slots` workgroups
-    int unit_tiles, slots;
+    // work: units of rows of one (sequence, KV head), unit_tiles a KV head, over steps of
+    // keys, shared out to at most `slots` workgroups
+    int unit_tiles, slots, least;  // least: steps below which units are not shared
+    int wide;              // waves of a unit of 32 rows each that share its tiles; 1: of 32 rows, whose waves share its keys
 };
 template <typename T>
 hipError_t launch_paged(const PagedParams& p, int D, hipStream_t s);

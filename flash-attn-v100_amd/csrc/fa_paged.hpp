@@ -89,6 +89,22 @@ struct PageTable {
         if (row) page = uniform_load(row, min(col, last_col));
         return {(unsigned)page < (unsigned)pages ? page : -1, 16 * (blk - col * blocks)};
     }
+    // bits of a tile's keys that have a page, from block blk on
+    template <int BLOCKS>
+    __device__ FA_INLINE inline uint64_t have(int blk) const {
+        uint64_t w = 0;
+#pragma unroll
+        for (int i = 0; i < BLOCKS; ++i) w |= block(blk + i).page < 0 ? 0ull : 0xFFFFull << (16 * i);
+        return w;
+    }
+    // whether one of blocks [b0, b1) has no page
+    __device__ FA_INLINE inline bool holes(int b0, int b1, int lane) const {
+        if (!row || b0 >= b1) return false;
+        bool none = false;
+        for (int col = b0 / blocks + lane; col <= min((b1 - 1) / blocks, last_col); col += 64)
+            none |= (unsigned)row[col] >= (unsigned)pages;
+        return __ballot(none) != 0ull;
+    }
 };
 
 // copies of 16-row blocks of one KV head's keys or values
@@ -168,9 +184,8 @@ __device__ FA_INLINE inline unsigned tree_word(const TreeBits& t, int i, int s, 
 
 // ---------------------------------------------------------------------------
 // Work.  Steps of all units in one list, by sequence, then unit; every sequence has
-// one at least.  Where no unit is longer than a workgroup's share (or than kLeast steps,
+// one at least.  Where no unit is longer than a workgroup's share (or than p.least steps,
 // whose join would cost more than it saves), a workgroup takes whole units.
-constexpr int kLeast = 4;
 struct PagedWork {
     int T, W;      // steps, workgroups that have work
     int per_seq;   // units of a sequence
@@ -199,9 +214,9 @@ struct PagedWork {
         }
         per_seq = p.Hkv * p.unit_tiles;
         T = __builtin_amdgcn_readfirstlane(sum) * per_seq;
-        const int share = max(kLeast, (T + p.slots - 1) / p.slots);
-        whole = __builtin_amdgcn_readfirstlane(most) <= share;
-        W = whole ? p.B * per_seq : (T + share - 1) / share;
+        W = min(p.slots, (T + p.least - 1) / p.least);
+        whole = __builtin_amdgcn_readfirstlane(most) <= max(p.least, (T + W - 1) / W);
+        if (whole) W = p.B * per_seq;
     }
     // the first step of workgroup g (floor(g T / W)), and whose step x is
     __device__ FA_INLINE inline int first(int g) const { return (int)((int64_t)g * T / W); }
@@ -297,16 +312,18 @@ __device__ FA_INLINE inline s16x4 lds_tr16_at(uint32_t a) {
 }
 
 // the products of a wave's 32 rows with 32 keys (K tile), log2 units before the rules
+// (float32, whose products bound it: only over columns that exist)
 template <typename T, int D>
-__device__ FA_INLINE inline f32x16 tile_scores(const T* Ks, const uint4 (&q)[Elem<T>::kF32 ? D / 8 : D / 16], int l32, int hi) {
+__device__ FA_INLINE inline f32x16 tile_scores(const T* Ks, const uint4 (&q)[Elem<T>::kF32 ? D / 8 : D / 16], int cols, int l32, int hi) {
     using C = PagedCfg<T, D>;
     f32x16 s = f32x16{};
     const int sw = row_swizzle<C::CW>(l32);
     if constexpr (C::F32) {
-        const uint32_t at = lds_place(Ks, l32 * C::ROWB + (((hi * (D / 8)) ^ sw) << 4));
+        const uint32_t at = lds_place(Ks, l32 * C::ROWB + ((hi ^ sw) << 4));
 #pragma unroll
         for (int kk = 0; kk < D / 8; ++kk) {
-            const f32x4 a = lds_at<f32x4>(at ^ (kk << 4));
+            if (kk >= D / 16 && 8 * kk >= cols) break;
+            const f32x4 a = lds_at<f32x4>(at ^ (kk << 5));
             const f32x4 b = __builtin_bit_cast(f32x4, q[kk]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s = mfma_f32(a[e], b[e], s);
@@ -322,7 +339,7 @@ __device__ FA_INLINE inline f32x16 tile_scores(const T* Ks, const uint4 (&q)[Ele
 
 // O^T += V^T P^T over 32 keys
 template <typename T, int D>
-__device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16& s, f32x16 (&o)[D / 32], int lane) {
+__device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16& s, f32x16 (&o)[D / 32], int cols, int lane) {
     using C = PagedCfg<T, D>;
     const int l32 = lane & 31, hi = lane >> 5;
     if constexpr (C::F32) {
@@ -332,8 +349,10 @@ __device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16& s, f32x1
         for (int x = 0; x < 16; ++x) {
             const int r = 8 * (x >> 2) + (x & 3);
 #pragma unroll
-            for (int n = 0; n < D / 32; ++n)
+            for (int n = 0; n < D / 32; ++n) {
+                if (n > 0 && 32 * n >= cols) break;
                 o[n] = mfma_f32(lds_at<float>((at ^ (((8 * n) ^ row_swizzle<C::CW>(r)) << 4)) + r * C::ROWB), s[x], o[n]);
+            }
         }
     } else {
         const int r0 = 4 * hi + ((lane & 15) >> 2);
@@ -362,7 +381,7 @@ __device__ FA_INLINE inline bool tile_odd(const T* Vs, int lane) {
     using C = PagedCfg<T, D>;
     constexpr unsigned M = std::is_same<T, bf16>::value ? 0x7F80u : 0x7C00u;
     bool odd = false;
-#pragma unroll
+#pragma unroll 2
     for (int x = 0; x < 32 * C::CW / 64; ++x) {
         const uint4 v = *reinterpret_cast<const uint4*>((const char*)Vs + 16 * (64 * x + lane));
         const unsigned w[4] = {v.x, v.y, v.z, v.w};
@@ -425,12 +444,12 @@ __device__ FA_INLINE inline unsigned row_sees(PagedArgs& p, const TreeBits* t, c
     return r.valid ? w & have : 0u;
 }
 
-// scores of 32 keys through the rules, hidden ones -infinity.  hidden: some row may not
+// scores of 32 keys through the rules, hidden ones -infinity.  HIDDEN: some row may not
 // see some key
-template <bool EXACT>
+template <bool EXACT, bool HIDDEN>
 __device__ FA_INLINE inline void tile_rules(f32x16& s, PagedArgs& p, Cap<EXACT>& cap, const PagedRow& r, const TreeBits* t,
-                                           bool slope, float slope2, int k0, int c, unsigned& seen, bool hidden, unsigned have, int hi) {
-    const bool steps = slope && hidden && t;  // distances along the tree
+                                           bool slope, float slope2, int k0, int c, unsigned& seen, unsigned have, int hi) {
+    const bool steps = slope && HIDDEN && t;  // distances along the tree
     if (p.cap > 0.f) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = cap.value(s[e]);
@@ -445,8 +464,7 @@ __device__ FA_INLINE inline void tile_rules(f32x16& s, PagedArgs& p, Cap<EXACT>&
         for (int e = 0; e < 16; ++e)
             s[e] = __builtin_fmaf(-slope2, __builtin_fabsf(d0 - (float)(8 * (e >> 2) + (e & 3))), s[e]);
     }
-    if (hidden) {
-        stay_branch();
+    if constexpr (HIDDEN) {
         seen = row_sees(p, t, r, k0, c, have);
         const unsigned mine = seen >> (4 * hi);
         if (steps) {
@@ -502,11 +520,13 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], con
     // the two blocks of a tile; what is past the end reads nothing, but is issued, so that
     // the vmcnt counts stay exact
     const PageTable table(p, b);
+    // (looked up a tile before the copy that needs them)
     auto blocks = [&](int t, Block16& x, Block16& y) FA_INLINE {
         const int tt = min(t, max(nt - 1, 0));
         x = table.block(2 * tt);
         y = table.block(2 * tt + 1);
     };
+    const bool holes = table.holes(2 * NW * s0, 2 * t1, lane);
     auto copy = [&](const PageCopy<T, D>& pc, int t, Block16 x, Block16 y, const T* dst) FA_INLINE {
         const int nv = t < t1 ? lim_max - 32 * t : 0;
         pc.load(x, nv, dst);
@@ -519,7 +539,7 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], con
         const T* qrow = (const T*)p.q + b * p.q_sb + (int64_t)row.i * p.q_ss + row.h * p.q_sh;
 #pragma unroll
         for (int kk = 0; kk < QR; ++kk) {
-            const int d0 = C::F32 ? hi * (D / 2) + 4 * kk : 16 * kk + 8 * hi;
+            const int d0 = C::F32 ? 8 * kk + 4 * hi : 16 * kk + 8 * hi;
             q[kk] = row.live && d0 < p.cols ? *reinterpret_cast<const uint4*>(qrow + d0) : make_uint4(0u, 0u, 0u, 0u);
         }
     }
@@ -539,19 +559,21 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], con
     blocks(t, bx, by);
     copy(kc, t, bx, by, Ks);
     copy(vc, t, bx, by, Vs);
-    for (; t < t1; t += NW) {
+    blocks(t + NW, bx, by);
+    // tiles that every row sees, then the others: the loop over the first ones has no registers
+    // to give to the rules of the second
+    auto tile = [&](auto hidden) FA_INLINE {
+        constexpr bool HIDDEN = decltype(hidden)::value;
         const int k0 = 32 * t;
-        const unsigned have = (bx.page < 0 ? 0u : 0xFFFFu) | (by.page < 0 ? 0u : 0xFFFF0000u);
         wait_vmem_below<2 * C::NI16>();  // K(t); only V(t) may be in flight
         asm volatile("" ::: "memory");
-        f32x16 s = tile_scores<T, D>(Ks, q, l32, hi);
+        f32x16 s = tile_scores<T, D>(Ks, q, kc.cols, l32, hi);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K(t) read before it is overwritten
-        blocks(t + NW, bx, by);
         copy(kc, t + NW, bx, by, Ks);
 
-        const bool hidden = k0 + 32 > lim_min || have != ~0u;
-        unsigned seen = ~0u;
-        tile_rules(s, p, cap, row, tree, slope, slope2, k0, c, seen, hidden, have, hi);
+        unsigned have = ~0u, seen = ~0u;
+        if (HIDDEN && holes) have = (unsigned)table.template have<2>(2 * t);
+        tile_rules<EXACT, HIDDEN>(s, p, cap, row, tree, slope, slope2, k0, c, seen, have, hi);
         float m2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int e = 0; e < 16; ++e) m2[e & 1] = fmaxf(m2[e & 1], s[e]);
@@ -575,15 +597,19 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], con
 
         wait_vmem_below<2 * C::NI16>();  // V(t); only K(t + 4) may be in flight
         asm volatile("" ::: "memory");
-        if (hidden && uneven && tile_odd<T, D>(Vs, lane)) {
+        if (HIDDEN && uneven && tile_odd<T, D>(Vs, lane)) {
             stay_branch();
             tile_values_seen<T, D>(Vs, s, seen, o, lane);
         } else {
-            tile_values<T, D>(Vs, s, o, lane);
+            tile_values<T, D>(Vs, s, o, vc.cols, lane);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V(t) read before it is overwritten
         copy(vc, t + NW, bx, by, Vs);
-    }
+        blocks(t + 2 * NW, bx, by);
+    };
+    const int tv = holes ? 0 : min(t1, lim_min / 32);
+    for (; t < tv; t += NW) tile(std::false_type{});
+    for (; t < t1; t += NW) tile(std::true_type{});
     wait_vmem();  // no copy in flight when the region takes the O part
     asm volatile("" ::: "memory");
 
@@ -657,25 +683,208 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], con
     lds_barrier();  // the regions and stat are free for the next unit
 }
 
-template <typename T, int D, bool EXACT, bool TREE>
-__global__ __launch_bounds__(256, (PagedCfg<T, D>::PER_CU)) void paged_kernel(const PagedParams) {
+// ---------------------------------------------------------------------------
+// Units of 32 NW rows whose NW waves, on 32 rows each, share tiles of 64 keys: K and V
+// are read once for all of them.  NS tiles in LDS, of which NS - 1 are on their way or
+// read; a wave copies one block of 16 keys (NW = 8) or one of K and one of V.
+template <typename T, int D, int NW>
+struct WideCfg {
     using C = PagedCfg<T, D>;
+    static constexpr int STEP = 64;
+    static constexpr int TILE = STEP * D;
+    static constexpr int NS = NW == 8 || D < 128 ? 4 : 2;
+    static constexpr int SMEM = NS * 2 * TILE;
+    static constexpr int COPIES = 8 / NW * C::NI16;  // of a wave, a tile
+    static constexpr int PER_CU = NW == 8 ? 1 : 2;
+};
+
+template <typename T, int D, bool EXACT, int NW>
+__device__ FA_INLINE inline void paged_unit_wide(T* smem, const TreeBits* tree, int b, int hk, int rt, int s0, int s1, int64_t part,
+                                                int lane, int w) {
+    using C = PagedCfg<T, D>;
+    using X = WideCfg<T, D, NW>;
     PagedArgs& p = paged_args();
-    __shared__ __attribute__((aligned(1024))) T smem[C::SMEM];
-    __shared__ float stat[C::NW][2][32];
+    const int l32 = lane & 31, hi = lane >> 5;
+    const int len = __builtin_amdgcn_readfirstlane(filled_tokens(p, b)), c = len - p.Sq;
+    const PagedRow row(p, tree, 32 * (NW * rt + w) + l32, b, hk, len);
+    int lim_min = row.valid ? row.all : INT_MAX, lim_max = row.lim;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        lim_min = min(lim_min, __shfl_xor(lim_min, x));
+        lim_max = max(lim_max, __shfl_xor(lim_max, x));
+    }
+    lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+    const bool uneven = tree || lim_min != __builtin_amdgcn_readfirstlane(lim_max);
+    // keys that some row of the unit may see: all waves copy for all
+    const int top = tree ? len : min(len, c + min(p.Sq, (32 * NW * (rt + 1) - 1) / p.group + 1));
+    const int n_keys = max(top, 0), t1 = min(s1, (n_keys + 63) / 64);
+
+    PageCopy<T, D> kc, vc;
+    if (NW == 4 || w < 4) kc.init((const T*)p.k + hk * p.k_sh, p.k_sp, p.k_ss, p.cols, lane);
+    if (NW == 4) vc.init((const T*)p.v + hk * p.v_sh, p.v_sp, p.v_ss, p.cols, lane);
+    if (NW == 8 && w >= 4) kc.init((const T*)p.v + hk * p.v_sh, p.v_sp, p.v_ss, p.cols, lane);
+    const PageTable table(p, b);
+    const int last = max((n_keys + 15) / 16 - 1, 0);
+    auto look = [&](int t) FA_INLINE { return table.block(min(4 * t + (w & 3), last)); };
+    // tile t, to slot t % NS; what is past the end reads nothing, but is issued, so that the
+    // vmcnt counts stay exact
+    auto issue = [&](int t, Block16 at) FA_INLINE {
+        const int nv = t < t1 ? n_keys - 64 * t - 16 * (w & 3) : 0;
+        T* const dst = smem + (t & (X::NS - 1)) * 2 * X::TILE + 16 * (w & 3) * D;
+        kc.load(at, nv, NW == 8 ? dst + (w >> 2) * X::TILE : dst);
+        if (NW == 4) vc.load(at, nv, dst + X::TILE);
+    };
+    const bool holes = table.holes(4 * s0, 4 * t1, lane);
+
+    constexpr int QR = D / 16;
+    uint4 q[QR];
+    {
+        const T* qrow = (const T*)p.q + b * p.q_sb + (int64_t)row.i * p.q_ss + row.h * p.q_sh;
+#pragma unroll
+        for (int kk = 0; kk < QR; ++kk)
+            q[kk] = row.live && 16 * kk + 8 * hi < p.cols ? *reinterpret_cast<const uint4*>(qrow + 16 * kk + 8 * hi)
+                                                          : make_uint4(0u, 0u, 0u, 0u);
+    }
+    const bool slope = p.slopes != nullptr;
+    const float slope2 = slope ? p.slopes[b * p.slopes_sb + row.h] * kLog2e : 0.f;
+    wait_vmem();
+    asm volatile("" ::: "memory");
+
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) o[n] = f32x16{};
+    float m_run = -1e30f, l_run = 0.f;
+    Cap<EXACT> cap(p);
+
+#pragma unroll
+    for (int x = 0; x < X::NS - 1; ++x) issue(s0 + x, look(s0 + x));
+    Block16 next = look(s0 + X::NS - 1);
+    // (as in paged_unit32: what every row sees first)
+    auto tile = [&](int t, auto hide) FA_INLINE {
+        constexpr bool HIDDEN = decltype(hide)::value;
+        const int k0 = 64 * t;
+        wait_vmem_below<(X::NS - 2) * X::COPIES>();  // this wave's part of tile t
+        barrier_no_fence();                          // everyone's, and tile t - 1 has been read
+        issue(t + X::NS - 1, next);
+        next = look(t + X::NS);
+        const T* const Ks = smem + (t & (X::NS - 1)) * 2 * X::TILE;
+        const T* const Vs = Ks + X::TILE;
+        f32x16 s[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) s[x] = tile_scores<T, D>(Ks + x * 32 * D, q, D, l32, hi);
+        unsigned seen[2] = {~0u, ~0u};
+        uint64_t have = ~0ull;
+        if (HIDDEN && holes) have = table.template have<4>(4 * t);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+            tile_rules<EXACT, HIDDEN>(s[x], p, cap, row, tree, slope, slope2, k0 + 32 * x, c, seen[x], (unsigned)(have >> (32 * x)), hi);
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) m4[e & 3] = fmaxf(m4[e & 3], s[x][e]);
+        const float m_new = fmaxf(m_run, pair_max(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))));
+        if (__ballot(m_new > m_run + 8.0f) != 0ull) {
+            const float alpha = fast_exp2(m_run - m_new);
+            l_run *= alpha;
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[n][e] *= alpha;
+            m_run = m_new;
+        }
+        float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                s[x][e] = fast_exp2(s[x][e] - m_run);
+                ps[e & 3] += s[x][e];
+            }
+        l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            if (HIDDEN && uneven && tile_odd<T, D>(Vs + x * 32 * D, lane)) {
+                stay_branch();
+                tile_values_seen<T, D>(Vs + x * 32 * D, s[x], seen[x], o, lane);
+            } else {
+                tile_values<T, D>(Vs + x * 32 * D, s[x], o, D, lane);
+            }
+        }
+    };
+    const int tv = holes ? s0 : min(t1, lim_min / 64);
+    int t = s0;
+    for (; t < tv; ++t) tile(t, std::false_type{});
+    for (; t < t1; ++t) tile(t, std::true_type{});
+    wait_vmem();  // (copies of no tile)
+
+    PagedArgs& pe = paged_args();
+    float l_tot = pair_sum(l_run);
+    if (!row.valid) {  // (such a row went along with the others)
+        m_run = -1e30f;
+        l_tot = 0.f;
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) o[n] = f32x16{};
+    }
+    if (part >= 0) {
+        const int64_t prow = part + 32 * w + l32;
+        if (hi == 0) pe.stat[prow] = make_float2(m_run, l_tot);
+        float* op = pe.part + prow * D + 4 * hi;
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+                *reinterpret_cast<f32x4*>(op + 32 * n + 8 * q4) = f32x4{o[n][4 * q4], o[n][4 * q4 + 1], o[n][4 * q4 + 2], o[n][4 * q4 + 3]};
+    } else if (row.live) {
+        if (hi == 0 && pe.lse) put_row_lse(pe, b, row.h, row.i, m_run, l_tot);
+        const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
+        T* ob = (T*)pe.o + b * pe.o_sb + (int64_t)row.i * pe.o_ss + row.h * pe.o_sh + 4 * hi;
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+                if (32 * n + 8 * q4 + 4 * hi >= pe.cols) continue;
+                s16x4 v4;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v4[e] = Elem<T>::pack1(o[n][4 * q4 + e] * inv);
+                *reinterpret_cast<s16x4*>(ob + 32 * n + 8 * q4) = v4;
+            }
+    }
+    barrier_no_fence();  // the slots have been read, before the next unit's copies
+}
+
+// ---------------------------------------------------------------------------
+// One workgroup's part of the list.  NW: waves that share tiles (units of 32 NW rows);
+// 1: units of 32 rows, 4 waves.
+template <typename T, int D, int NW>
+struct PagedShape {
+    using X = WideCfg<T, D, NW>;
+    static constexpr int THREADS = 64 * NW, STEP = X::STEP, ROWS = 32 * NW, SMEM = X::SMEM, PER_CU = X::PER_CU;
+};
+template <typename T, int D>
+struct PagedShape<T, D, 1> {
+    using C = PagedCfg<T, D>;
+    static constexpr int THREADS = 256, STEP = C::STEP, ROWS = 32, SMEM = C::SMEM, PER_CU = C::PER_CU;
+};
+
+template <typename T, int D, bool EXACT, bool TREE, int NW>
+__global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 : PagedShape<T, D, NW>::PER_CU)) void paged_kernel(const PagedParams) {
+    using S = PagedShape<T, D, NW>;
+    PagedArgs& p = paged_args();
+    __shared__ __attribute__((aligned(1024))) T smem[S::SMEM];
     __shared__ typename std::conditional<TREE, TreeBits, int>::type bits;
     const TreeBits* tree = nullptr;
     if constexpr (TREE) tree = &bits;
     const int tid = threadIdx.x;
-    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
+    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6) & 7;
     PagedWork wk;
-    wk.init<C::STEP>(p, lane);
+    wk.init<S::STEP>(p, lane);
     if ((int)blockIdx.x >= wk.W) return;
     const int g = xcd_remap((int)blockIdx.x, wk.W);
     int x = 0, end = 0, b = 0, start = 0, len = 0, last_b = -1;
     if (wk.whole) {
         b = g / wk.per_seq;
-        len = __builtin_amdgcn_readfirstlane(PagedWork::steps<C::STEP>(p, b));
+        len = __builtin_amdgcn_readfirstlane(PagedWork::steps<S::STEP>(p, b));
         start = 0;
         x = g % wk.per_seq * len;
         end = x + len;
@@ -684,36 +893,41 @@ __global__ __launch_bounds__(256, (PagedCfg<T, D>::PER_CU)) void paged_kernel(co
         end = wk.first(g + 1);
     }
     while (x < end) {
-        if (!wk.whole && (last_b < 0 || x >= start + len * wk.per_seq)) wk.locate<C::STEP>(paged_args(), x, lane, b, start, len);
+        if (!wk.whole && (last_b < 0 || x >= start + len * wk.per_seq)) wk.locate<S::STEP>(paged_args(), x, lane, b, start, len);
         const int u = (x - start) / len, s0 = x - start - u * len, s1 = min(len, s0 + end - x);
         if constexpr (TREE) {
             if (b != last_b) tree_init(paged_args(), bits, b, tid);
         }
         last_b = b;
-        const int64_t part = s1 - s0 == len ? -1 : part_at<32>(g, s0 == 0);
+        const int64_t part = s1 - s0 == len ? -1 : part_at<S::ROWS>(g, s0 == 0);
         const int tiles = paged_args().unit_tiles;
-        paged_unit32<T, D, EXACT>(smem, stat, tree, b, u / tiles, u % tiles, s0, s1, part, lane, w);
+        if constexpr (NW == 1) {
+            __shared__ float stat[PagedCfg<T, D>::NW][2][32];
+            paged_unit32<T, D, EXACT>(smem, stat, tree, b, u / tiles, u % tiles, s0, s1, part, lane, w);
+        } else {
+            paged_unit_wide<T, D, EXACT, NW>(smem, tree, b, u / tiles, u % tiles, s0, s1, part, lane, w);
+        }
         x += s1 - s0;
     }
 }
 
 // The parts of the rows of units that several workgroups shared: D / 4 threads a row,
 // 4 columns each, a wave's rows all of one sequence (blockIdx.y)
-template <typename T, int D>
+template <typename T, int D, int NW>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams) {
-    using C = PagedCfg<T, D>;
+    using S = PagedShape<T, D, NW>;
     PagedArgs& p = paged_args();
     constexpr int TPR = D / 4, ROWS = 256 / TPR;
     const int lane = threadIdx.x & 63, b = blockIdx.y;
     PagedWork wk;
-    wk.init<C::STEP>(p, lane);
+    wk.init<S::STEP>(p, lane);
     if (wk.whole) return;
-    const int start = wk.start_of<C::STEP>(p, b, lane);
-    const int len = __builtin_amdgcn_readfirstlane(PagedWork::steps<C::STEP>(p, b));
+    const int start = wk.start_of<S::STEP>(p, b, lane);
+    const int len = __builtin_amdgcn_readfirstlane(PagedWork::steps<S::STEP>(p, b));
     const int r = (int)blockIdx.x * ROWS + (int)threadIdx.x / TPR, col = (int)(threadIdx.x % TPR) * 4;
     const int rows = p.Sq * p.group;  // of a KV head
     if (r >= rows * p.Hkv) return;
-    const int hk = r / rows, ig = r % rows, rt = ig >> 5;
+    const int hk = r / rows, ig = r % rows, rt = ig / S::ROWS;
     const int s = start + (hk * p.unit_tiles + rt) * len;  // the unit's first step
     const int g0 = wk.whose(s), g1 = wk.whose(s + len - 1);
     if (g0 == g1) return;
@@ -726,7 +940,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams) {
         for (int j = 0; j < 4; ++j) {
             const bool in = x0 + j <= g1;
             const int g = in ? x0 + j : g0;
-            const int64_t pr = part_at<32>(g, g == g0) + (ig & 31);  // g0 begins the unit
+            const int64_t pr = part_at<S::ROWS>(g, g == g0) + ig % S::ROWS;  // g0 begins the unit
             st[j] = p.stat[pr];
             v[j] = *reinterpret_cast<const f32x4*>(p.part + pr * D + col);
             if (!in) {
@@ -763,35 +977,44 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams) {
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, int NW>
 hipError_t launch_paged_t(const PagedParams& p, hipStream_t s) {
-    const dim3 grid((unsigned)p.o_wgs);
+    using S = PagedShape<T, D, NW>;
+    const dim3 grid((unsigned)p.o_wgs), block(S::THREADS);
     constexpr bool F32 = Elem<T>::kF32;
     if (p.parents) {
         if (F32 || p.cap > kWideCap)
-            hipLaunchKernelGGL((paged_kernel<T, D, true, true>), grid, dim3(256), 0, s, p);
+            hipLaunchKernelGGL((paged_kernel<T, D, true, true, NW>), grid, block, 0, s, p);
         else
-            hipLaunchKernelGGL((paged_kernel<T, D, F32, true>), grid, dim3(256), 0, s, p);
+            hipLaunchKernelGGL((paged_kernel<T, D, F32, true, NW>), grid, block, 0, s, p);
     } else {
         if (F32 || p.cap > kWideCap)
-            hipLaunchKernelGGL((paged_kernel<T, D, true, false>), grid, dim3(256), 0, s, p);
+            hipLaunchKernelGGL((paged_kernel<T, D, true, false, NW>), grid, block, 0, s, p);
         else
-            hipLaunchKernelGGL((paged_kernel<T, D, F32, false>), grid, dim3(256), 0, s, p);
+            hipLaunchKernelGGL((paged_kernel<T, D, F32, false, NW>), grid, block, 0, s, p);
     }
     if (p.part) {
         constexpr int ROWS = 256 / (D / 4);
         const int rows = p.Sq * p.H;
-        hipLaunchKernelGGL((paged_join_kernel<T, D>), dim3((unsigned)((rows + ROWS - 1) / ROWS), (unsigned)p.B), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((paged_join_kernel<T, D, NW>), dim3((unsigned)((rows + ROWS - 1) / ROWS), (unsigned)p.B), dim3(256), 0, s, p);
     }
     return hipGetLastError();
+}
+template <typename T, int D>
+hipError_t launch_paged_d(const PagedParams& p, hipStream_t s) {
+    if constexpr (!Elem<T>::kF32) {
+        if (p.wide == 8) return launch_paged_t<T, D, 8>(p, s);
+        if (p.wide == 4) return launch_paged_t<T, D, 4>(p, s);
+    }
+    return launch_paged_t<T, D, 1>(p, s);
 }
 
 template <typename T>
 hipError_t launch_paged(const PagedParams& p, int D, hipStream_t s) {
     switch (D) {
-        case 32: return launch_paged_t<T, 32>(p, s);
-        case 64: return launch_paged_t<T, 64>(p, s);
-        case 128: return launch_paged_t<T, 128>(p, s);
+        case 32: return launch_paged_d<T, 32>(p, s);
+        case 64: return launch_paged_d<T, 64>(p, s);
+        case 128: return launch_paged_d<T, 128>(p, s);
         default: return hipErrorInvalidValue;
     }
 }

@@ -18,8 +18,6 @@ using namespace fa_ops_check;
 using fa::PagedParams;
 using fa::PoolParams;
 
-constexpr int kLeastSteps = 4;  // steps of a unit that workgroups do not share (fa_paged.hpp: kLeast)
-
 // tokens a sequence has room for, held below 2^28
 int64_t room_of(const fa_page_pool& c) { return (int64_t)c.table_cols * c.page_size; }
 
@@ -80,27 +78,29 @@ void put_pool(const fa_page_pool& c, PoolParams& p) {
 }
 
 // ---------------------------------------------------------------------------
-// attention: units of 32 rows of one (sequence, KV head), steps of 128 keys
+// attention: units of rows of one (sequence, KV head), and their steps
+int unit_rows(const PagedParams& p) { return 32 * p.wide; }
 void plan(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared) {
     const fa_page_pool& c = a->pool;
-    const int step = 128;
+    const bool f32 = c.dtype == FA_DTYPE_F32;
     const int64_t rows = (int64_t)a->seqlen_q * (a->num_heads / c.num_heads_kv);
-    p.unit_tiles = (int)ceil_div<int64_t>(rows, 32);
-    p.slots = c.dtype == FA_DTYPE_F32 && compiled_dim(c.head_dim) == 128 ? 256 : 512;  // workgroups that run at once
+    p.wide = f32 || rows <= 32 ? 1 : rows <= 128 ? 4 : 8;
+    const int step = p.wide == 1 ? 128 : 64;
+    p.unit_tiles = (int)ceil_div<int64_t>(rows, unit_rows(p));
+    p.slots = (f32 && compiled_dim(c.head_dim) == 128) || p.wide == 8 ? 256 : 512;  // workgroups that run at once
+    p.least = f32 ? 1 : 4;
     const int64_t units = (int64_t)c.batch * c.num_heads_kv * p.unit_tiles;
     const int64_t most = std::max<int64_t>(1, ceil_div<int64_t>(p.Sk, step));  // steps of a unit
-    // workgroups that may share units: none where no unit is longer than the least share
-    // or, with every sequence full, than an even one
-    shared = 0;
-    const int64_t share = std::max<int64_t>(kLeastSteps, ceil_div<int64_t>(units * most, p.slots));
-    if (most > kLeastSteps && (c.key_lengths || most > share))
-        shared = std::min<int64_t>(p.slots, ceil_div<int64_t>(units * most, kLeastSteps));
+    // workgroups that may share units (PagedWork): none where no unit is longer than the
+    // least share or, with every sequence full, than an even one
+    const int64_t w = std::min<int64_t>(p.slots, ceil_div<int64_t>(units * most, p.least));
+    shared = most > p.least && (c.key_lengths || most > ceil_div<int64_t>(units * most, w)) ? w : 0;
     grid = std::max(units, shared);
 }
-size_t part_rows(int64_t shared) { return (size_t)(2 * shared * 32); }
+size_t part_rows(const PagedParams& p, int64_t shared) { return (size_t)(2 * shared * unit_rows(p)); }
 size_t paged_bytes(const PagedParams& p, int64_t shared) {
     if (!shared) return 0;
-    return up256(part_rows(shared) * sizeof(float2)) + up256(part_rows(shared) * compiled_dim(p.cols) * sizeof(float));
+    return up256(part_rows(p, shared) * sizeof(float2)) + up256(part_rows(p, shared) * compiled_dim(p.cols) * sizeof(float));
 }
 
 void put_paged(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared) {
@@ -183,7 +183,7 @@ int32_t fa_paged_fwd(const fa_paged_args* a, void* workspace, size_t bytes, void
     if (need && (!workspace || bytes < need || !aligned(workspace, 16))) return FA_ERR_WORKSPACE;
     if (need) {
         p.stat = (float2*)workspace;
-        p.part = (float*)((char*)workspace + up256(part_rows(shared) * sizeof(float2)));
+        p.part = (float*)((char*)workspace + up256(part_rows(p, shared) * sizeof(float2)));
     }
     const int D = compiled_dim(p.cols);
     hipStream_t s = (hipStream_t)stream;
