@@ -147,7 +147,7 @@ struct TreeBits {
 };
 __device__ FA_INLINE inline void tree_init(PagedArgs& p, TreeBits& t, int b, int tid) {
     const int N = p.Sq, W = (N + 31) >> 5;
-    __syncthreads();  // (the last unit's rows have read theirs)
+    lds_barrier();  // (the last unit's rows have read theirs)
     int up = -2;
     if (tid < N) {
         up = p.parents[b * p.parents_sb + tid];
@@ -156,14 +156,14 @@ __device__ FA_INLINE inline void tree_init(PagedArgs& p, TreeBits& t, int b, int
         t.up[tid] = up;
     }
     for (int n = 1; n < N; n *= 2) {
-        __syncthreads();
+        lds_barrier();
         unsigned more[kTreeWords];
         int next = up;
         if (up >= 0) {
             for (int w = 0; w < kTreeWords; ++w) more[w] = w < W ? t.bits[up][w] : 0u;
             next = t.up[up];
         }
-        __syncthreads();
+        lds_barrier();
         if (up >= 0) {
             for (int w = 0; w < kTreeWords; ++w)
                 if (w < W) t.bits[tid][w] |= more[w];
@@ -172,7 +172,7 @@ __device__ FA_INLINE inline void tree_init(PagedArgs& p, TreeBits& t, int b, int
     }
     if (tid < N && up != -1)
         for (int w = 0; w < W; ++w) t.bits[tid][w] = 0u;
-    __syncthreads();
+    lds_barrier();
 }
 // the 32 keys from tree position s on (it may be negative: the context) that node i sees
 __device__ FA_INLINE inline unsigned tree_word(const TreeBits& t, int i, int s, int W) {
@@ -262,28 +262,36 @@ struct PagedWork {
     }
 };
 // parts: a workgroup leaves at most two, of the unit that it begins with (2 g) and of
-// the one that it ends with, begun by it (2 g + 1)
+// the one that it ends with, begun by it (2 g + 1).  Those of 32 rows lie together, in
+// accumulator order (part_of), so that a store of a wave is 1 KB in a row: as rows, 64
+// places of 16 bytes a store, 256 rows took 8 us.
 template <int ROWS>
 __device__ FA_INLINE inline int64_t part_at(int g, bool begun) { return ((int64_t)2 * g + (begun ? 1 : 0)) * ROWS; }
+
+// four columns of a lane's row, 32 n + 8 q4 + 4 (lane / 32) and on, in the part whose first row is `row`
+template <int D>
+__device__ FA_INLINE inline f32x4* part_of(float* part, int64_t row, int n, int q4, int lane) {
+    return reinterpret_cast<f32x4*>(part + row * D) + (4 * n + q4) * 64 + lane;
+}
 
 // one row of a unit: keys [0, lim) at most, of which it sees all below `all`
 struct PagedRow {
     int i, h, lim, all;
     bool live, valid;  // exists; and sees keys
     int qpos;
-    __device__ FA_INLINE inline PagedRow(PagedArgs& p, const TreeBits* t, int row, int b, int hk, int len) {
+    __device__ FA_INLINE inline PagedRow(PagedArgs& p, int row, int hk) {
         live = row < p.Sq * p.group;
         const int rr = live ? row : 0;
         i = rr / p.group;
-        h = hk * p.group + rr % p.group;
-        const int c = len - p.Sq;
+        h = hk * p.group + (rr - i * p.group);
+    }
+    __device__ FA_INLINE inline void rule(const TreeBits* t, int words, int len, int c) {
         valid = live && c + i >= 0;
         qpos = c + i;
         lim = all = c + i + 1;
         if (t) {
-            const int W = (p.Sq + 31) >> 5;
             int n = 0;
-            for (int w = 0; w < W; ++w) n += __popc(t->bits[i][w]);
+            for (int w = 0; w < words; ++w) n += __popc(t->bits[i][w]);
             valid = valid && n > 0;
             qpos = c + n - 1;
             lim = len;
@@ -292,6 +300,10 @@ struct PagedRow {
         if (!valid) lim = 0;
     }
 };
+// keys that some of the rows below `rows` of a unit may see
+__device__ FA_INLINE inline int keys_of(PagedArgs& p, const TreeBits* t, int rows, int len, int c) {
+    return t ? len : max(0, min(len, c + min(p.Sq, (rows - 1) / p.group + 1)));
+}
 
 // A lane's place in a tile, as an LDS address that the compiler does not see through: the
 // places of the columns after it are that ^ a constant (a tile begins at a multiple of
@@ -311,66 +323,89 @@ __device__ FA_INLINE inline s16x4 lds_tr16_at(uint32_t a) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(uintptr_t)a);
 }
 
-// the products of a wave's 32 rows with 32 keys (K tile), log2 units before the rules
-// (float32, whose products bound it: only over columns that exist)
-template <typename T, int D>
-__device__ FA_INLINE inline f32x16 tile_scores(const T* Ks, const uint4 (&q)[Elem<T>::kF32 ? D / 8 : D / 16], int cols, int l32, int hi) {
+// Order of the instructions of a block: reads of LDS ahead of the matrix instructions that
+// take them, `ahead` of them at first and then EACH for one (the compiler's own order
+// reads one operand, waits for it and multiplies).
+template <int MFMAS, int EACH, int AHEAD>
+__device__ FA_INLINE inline void reads_ahead() {
+    constexpr int kMfma = 0x008, kRead = 0x100;
+    __builtin_amdgcn_sched_group_barrier(kRead, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < MFMAS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        if (AHEAD + EACH * i < EACH * MFMAS) __builtin_amdgcn_sched_group_barrier(kRead, EACH, 0);
+    }
+}
+
+// the products of a wave's 32 rows with NB blocks of 32 keys (K tile), log2 units before
+// the rules (float32, whose products bound it: only over columns that exist)
+template <typename T, int D, int NB>
+__device__ FA_INLINE inline void tile_scores(f32x16 (&s)[NB], const T* Ks, const uint4 (&q)[Elem<T>::kF32 ? D / 8 : D / 16], int cols,
+                                            int l32, int hi) {
     using C = PagedCfg<T, D>;
-    f32x16 s = f32x16{};
-    const int sw = row_swizzle<C::CW>(l32);
+    const uint32_t at = lds_place(Ks, l32 * C::ROWB + ((hi ^ row_swizzle<C::CW>(l32)) << 4));
+#pragma unroll
+    for (int x = 0; x < NB; ++x) s[x] = f32x16{};
     if constexpr (C::F32) {
-        const uint32_t at = lds_place(Ks, l32 * C::ROWB + ((hi ^ sw) << 4));
 #pragma unroll
         for (int kk = 0; kk < D / 8; ++kk) {
             if (kk >= D / 16 && 8 * kk >= cols) break;
-            const f32x4 a = lds_at<f32x4>(at ^ (kk << 5));
-            const f32x4 b = __builtin_bit_cast(f32x4, q[kk]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s = mfma_f32(a[e], b[e], s);
+            for (int x = 0; x < NB; ++x) {
+                const f32x4 a = lds_at<f32x4>((at ^ (kk << 5)) + x * 32 * C::ROWB);
+                const f32x4 b = __builtin_bit_cast(f32x4, q[kk]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[x] = mfma_f32(a[e], b[e], s[x]);
+            }
         }
     } else {
-        const uint32_t at = lds_place(Ks, l32 * C::ROWB + ((hi ^ sw) << 4));
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-            s = Elem<T>::mfma(lds_at<s16x8>(at ^ (kk << 5)), __builtin_bit_cast(s16x8, q[kk]), s);
+#pragma unroll
+            for (int x = 0; x < NB; ++x)
+                s[x] = Elem<T>::mfma(lds_at<s16x8>((at ^ (kk << 5)) + x * 32 * C::ROWB), __builtin_bit_cast(s16x8, q[kk]), s[x]);
+        reads_ahead<NB * D / 16, 1, NB * D / 16 < 6 ? NB * D / 16 : 6>();
     }
-    return s;
 }
 
-// O^T += V^T P^T over 32 keys
-template <typename T, int D>
-__device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16& s, f32x16 (&o)[D / 32], int cols, int lane) {
+// O^T += V^T P^T over NB blocks of 32 keys
+template <typename T, int D, int NB>
+__device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16 (&s)[NB], f32x16 (&o)[D / 32], int cols, int lane) {
     using C = PagedCfg<T, D>;
     const int l32 = lane & 31, hi = lane >> 5;
     if constexpr (C::F32) {
         // rows 8 (x / 4) + 4 hi + x % 4: their swizzles differ from that of row 4 hi by x alone
         const uint32_t at = lds_place(Vs, 4 * hi * C::ROWB + (((l32 >> 2) ^ row_swizzle<C::CW>(4 * hi)) << 4) + 4 * (l32 & 3));
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
+        for (int x = 0; x < 16 * NB; ++x) {
             const int r = 8 * (x >> 2) + (x & 3);
 #pragma unroll
             for (int n = 0; n < D / 32; ++n) {
                 if (n > 0 && 32 * n >= cols) break;
-                o[n] = mfma_f32(lds_at<float>((at ^ (((8 * n) ^ row_swizzle<C::CW>(r)) << 4)) + r * C::ROWB), s[x], o[n]);
+                o[n] = mfma_f32(lds_at<float>((at ^ (((8 * n) ^ row_swizzle<C::CW>(r)) << 4)) + r * C::ROWB), s[x >> 4][x & 15], o[n]);
             }
         }
     } else {
         const int r0 = 4 * hi + ((lane & 15) >> 2);
         const int chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
         const uint32_t at = lds_place(Vs, r0 * C::ROWB + ((chunk ^ row_swizzle<C::CW>(r0)) << 4) + 8 * (lane & 1));
+        s16x8 pk[2 * NB];
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
+        for (int ks = 0; ks < 2 * NB; ++ks) {
             float tmp[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) tmp[e] = s[8 * ks + e];
-            const s16x8 pk = pack8<T>(tmp);
+            for (int e = 0; e < 8; ++e) tmp[e] = s[ks >> 1][8 * (ks & 1) + e];
+            pk[ks] = pack8<T>(tmp);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2 * NB; ++ks)
 #pragma unroll
             for (int n = 0; n < D / 32; ++n) {
                 const s16x8 a = cat4(lds_tr16_at((at ^ (n << 6)) + 16 * ks * C::ROWB),
                                      lds_tr16_at((at ^ ((n << 6) ^ (row_swizzle<C::CW>(8) << 4))) + (16 * ks + 8) * C::ROWB));
-                o[n] = Elem<T>::mfma(a, pk, o[n]);
+                o[n] = Elem<T>::mfma(a, pk[ks], o[n]);
             }
-        }
+        reads_ahead<2 * NB * D / 32, 2, 2 * NB * D / 32 < 4 ? 4 * NB * D / 32 : 8>();
     }
 }
 
@@ -410,7 +445,8 @@ __device__ FA_INLINE inline void tile_values_seen(const T* Vs, const f32x16& s, 
         const char* row = (const char*)Vs + x * C::ROWB;
         const int sw = row_swizzle<C::CW>(x);
 #pragma unroll
-        for (int n = 0; n < D / 32; ++n)
+        for (int n = 0; n < D / 32; ++n) {
+            asm volatile("" ::: "memory");  // (the next columns' values are not read ahead: they would need registers)
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
                 float v[4];
@@ -429,14 +465,28 @@ __device__ FA_INLINE inline void tile_values_seen(const T* Vs, const f32x16& s, 
                     o[n][4 * q4 + e] = sees ? y : o[n][4 * q4 + e];
                 }
             }
+        }
     }
 }
 
+// what the rules take from the arguments, read once
+template <bool EXACT>
+struct TileRules {
+    Cap<EXACT> cap;
+    bool capped, slope;
+    float mul, unit, slope2;  // scores times mul, unless unit, their factor in the exponent, is that
+    int words;  // of bits of a tree
+    __device__ FA_INLINE inline TileRules(PagedArgs& p, int b, int h)
+        : cap(p), capped(p.cap > 0.f), slope(p.slopes != nullptr), mul(p.scale_log2), words((p.Sq + 31) >> 5) {
+        unit = capped || slope ? 1.f : mul;
+        slope2 = slope ? p.slopes[b * p.slopes_sb + h] * kLog2e : 0.f;
+    }
+};
 // What a row sees of the 32 keys from k0 on, with bits for the blocks that have a page
-__device__ FA_INLINE inline unsigned row_sees(PagedArgs& p, const TreeBits* t, const PagedRow& r, int k0, int c, unsigned have) {
+__device__ FA_INLINE inline unsigned row_sees(const TreeBits* t, const PagedRow& r, int words, int k0, int c, unsigned have) {
     unsigned w;
     if (t) {
-        w = tree_word(*t, r.i, k0 - c, (p.Sq + 31) >> 5);
+        w = tree_word(*t, r.i, k0 - c, words);
     } else {
         const int n = r.lim - k0;
         w = n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
@@ -447,41 +497,39 @@ __device__ FA_INLINE inline unsigned row_sees(PagedArgs& p, const TreeBits* t, c
 // scores of 32 keys through the rules, hidden ones -infinity.  HIDDEN: some row may not
 // see some key
 template <bool EXACT, bool HIDDEN>
-__device__ FA_INLINE inline void tile_rules(f32x16& s, PagedArgs& p, Cap<EXACT>& cap, const PagedRow& r, const TreeBits* t,
-                                           bool slope, float slope2, int k0, int c, unsigned& seen, unsigned have, int hi) {
-    const bool steps = slope && HIDDEN && t;  // distances along the tree
-    if (p.cap > 0.f) {
+__device__ FA_INLINE inline void tile_rules(f32x16& s, TileRules<EXACT>& u, const PagedRow& r, const TreeBits* t, int k0, int c,
+                                           unsigned& seen, unsigned have, int hi) {
+    const bool steps = u.slope && HIDDEN && t;  // distances along the tree
+    if (u.capped) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = cap.value(s[e]);
-    } else {
-        const float mul = p.scale_log2;
+        for (int e = 0; e < 16; ++e) s[e] = u.cap.value(s[e]);
+    } else if (u.slope) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] *= mul;
+        for (int e = 0; e < 16; ++e) s[e] *= u.mul;
     }
-    if (slope && !steps) {
+    if (u.slope && !steps) {
         const float d0 = (float)(r.qpos - k0 - 4 * hi);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-            s[e] = __builtin_fmaf(-slope2, __builtin_fabsf(d0 - (float)(8 * (e >> 2) + (e & 3))), s[e]);
+            s[e] = __builtin_fmaf(-u.slope2, __builtin_fabsf(d0 - (float)(8 * (e >> 2) + (e & 3))), s[e]);
     }
     if constexpr (HIDDEN) {
-        seen = row_sees(p, t, r, k0, c, have);
+        seen = row_sees(t, r, u.words, k0, c, have);
         const unsigned mine = seen >> (4 * hi);
         if (steps) {
             // the tokens from a key to the row's own are those that it sees behind the key
-            const int W = (p.Sq + 31) >> 5, end = k0 - c + 32;
-            int above = 0;
-            for (int w = max(end, 0) >> 5; w < W; ++w) {
+            const int end = k0 - c + 32;
+            int above = max(-end, 0);
+            for (int w = max(end, 0) >> 5; w < u.words; ++w) {
                 const unsigned x = t->bits[r.i][w];
                 above += __popc(w == (end >> 5) ? x & (~0u << (end & 31)) : x);
             }
-            if (end < 0) above += -end;
-            const unsigned word = tree_word(*t, r.i, k0 - c, W);
+            const unsigned word = tree_word(*t, r.i, k0 - c, u.words);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int x = 8 * (e >> 2) + (e & 3);
                 const int d = above + __popc((word >> (x + 4 * hi)) >> 1);
-                s[e] = __builtin_fmaf(-slope2, (float)d, s[e]);
+                s[e] = __builtin_fmaf(-u.slope2, (float)d, s[e]);
             }
         }
 #pragma unroll
@@ -490,61 +538,104 @@ __device__ FA_INLINE inline void tile_rules(f32x16& s, PagedArgs& p, Cap<EXACT>&
     }
 }
 
+// The running maximum and sum of a row over NB more blocks of scores, which become
+// probabilities: e^(s - m) with an m that is at most 8 (of log2) behind the largest, so
+// that O is rescaled when a maximum grows by more
+template <int D, int NB>
+__device__ FA_INLINE inline void soft_blocks(f32x16 (&s)[NB], float unit, float& m_run, float& l_run, f32x16 (&o)[D / 32]) {
+    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m4[e & 3] = fmaxf(m4[e & 3], s[x][e]);
+    const float m_new = fmaxf(m_run, unit * pair_max(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))));
+    if (__ballot(m_new > m_run + 8.0f) != 0ull) {
+        const float alpha = fast_exp2(m_run - m_new);
+        l_run *= alpha;
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[n][e] *= alpha;
+        m_run = m_new;
+    }
+    float ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < NB; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            s[x][e] = fast_exp2(__builtin_fmaf(s[x][e], unit, -m_run));
+            ps[e & 3] += s[x][e];
+        }
+    l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+}
+
+// A row's q, in the operand order of the products (float32: 4 of each 8 columns a lane)
+template <typename T, int D>
+__device__ FA_INLINE inline void load_q(PagedArgs& p, const PagedRow& row, int b, int hi, uint4 (&q)[Elem<T>::kF32 ? D / 8 : D / 16]) {
+    constexpr int STEP = Elem<T>::kF32 ? 8 : 16;
+    const T* at = (const T*)p.q + b * p.q_sb + (int64_t)row.i * p.q_ss + row.h * p.q_sh;
+#pragma unroll
+    for (int kk = 0; kk < D / STEP; ++kk) {
+        const int d0 = STEP * kk + STEP / 2 * hi;
+        q[kk] = row.live && d0 < p.cols ? *reinterpret_cast<const uint4*>(at + d0) : make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+
 // 32 rows of a unit over its steps [s0, s1): each wave walks tiles of its own.  part:
-// the rows' place among the parts, below 0 where this is all of the unit.
+// the rows' place among the parts, below 0 where this is all of the unit.  The first
+// tiles are on their way before anything else is waited for.
 template <typename T, int D, bool EXACT>
-__device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], const TreeBits* tree, int b, int hk,
-                                             int rt, int s0, int s1, int64_t part, int lane, int w) {
+__device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], TreeBits* tree, bool new_tree, int b, int hk, int rt,
+                                             int s0, int s1, int64_t part, int tid) {
     using C = PagedCfg<T, D>;
     constexpr int NW = C::NW;
     PagedArgs& p = paged_args();
+    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;
     const int l32 = lane & 31, hi = lane >> 5;
+    PagedRow row(p, 32 * rt + l32, hk);
+    uint4 q[C::F32 ? D / 8 : D / 16];
+    load_q<T, D>(p, row, b, hi, q);
+    TileRules<EXACT> rules(p, b, row.h);
     const int len = __builtin_amdgcn_readfirstlane(filled_tokens(p, b)), c = len - p.Sq;
-    const PagedRow row(p, tree, 32 * rt + l32, b, hk, len);
-    int lim_max = row.lim, lim_min = row.valid ? row.all : INT_MAX;
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-        lim_max = max(lim_max, __shfl_xor(lim_max, x));
-        lim_min = min(lim_min, __shfl_xor(lim_min, x));
-    }
-    lim_max = __builtin_amdgcn_readfirstlane(lim_max);
-    lim_min = __builtin_amdgcn_readfirstlane(lim_min);
-    const int nt = (lim_max + 31) / 32, t1 = min(NW * s1, nt);
-    const bool uneven = tree || lim_min != lim_max;  // rows see different keys
+    const int n_keys = keys_of(p, tree, 32 * (rt + 1), len, c);
+    const int nt = (n_keys + 31) / 32, t1 = min(NW * s1, nt);
 
     T* Ks = smem + w * C::REGION;
     T* Vs = Ks + C::TILE;
     PageCopy<T, D> kc, vc;
     kc.init((const T*)p.k + hk * p.k_sh, p.k_sp, p.k_ss, p.cols, lane);
     vc.init((const T*)p.v + hk * p.v_sh, p.v_sp, p.v_ss, p.cols, lane);
-    // the two blocks of a tile; what is past the end reads nothing, but is issued, so that
-    // the vmcnt counts stay exact
+    // the two blocks of a tile, looked up a tile before the copy that needs them; what is
+    // past the end reads nothing, but is issued, so that the vmcnt counts stay exact
     const PageTable table(p, b);
-    // (looked up a tile before the copy that needs them)
     auto blocks = [&](int t, Block16& x, Block16& y) FA_INLINE {
         const int tt = min(t, max(nt - 1, 0));
         x = table.block(2 * tt);
         y = table.block(2 * tt + 1);
     };
-    const bool holes = table.holes(2 * NW * s0, 2 * t1, lane);
     auto copy = [&](const PageCopy<T, D>& pc, int t, Block16 x, Block16 y, const T* dst) FA_INLINE {
-        const int nv = t < t1 ? lim_max - 32 * t : 0;
+        const int nv = t < t1 ? n_keys - 32 * t : 0;
         pc.load(x, nv, dst);
         pc.load(y, nv - 16, dst + 16 * D);
     };
+    int t = NW * s0 + w;
+    Block16 bx, by;
+    blocks(t, bx, by);
+    copy(kc, t, bx, by, Ks);
+    copy(vc, t, bx, by, Vs);
+    blocks(t + NW, bx, by);
 
-    constexpr int QR = C::F32 ? D / 8 : D / 16;
-    uint4 q[QR];
-    {
-        const T* qrow = (const T*)p.q + b * p.q_sb + (int64_t)row.i * p.q_ss + row.h * p.q_sh;
+    if (new_tree) tree_init(p, *tree, b, tid);
+    row.rule(tree, rules.words, len, c);
+    const bool holes = table.holes(2 * NW * s0, 2 * t1, lane);
+    int lim_max = row.lim, lim_min = row.valid ? row.all : INT_MAX;
 #pragma unroll
-        for (int kk = 0; kk < QR; ++kk) {
-            const int d0 = C::F32 ? 8 * kk + 4 * hi : 16 * kk + 8 * hi;
-            q[kk] = row.live && d0 < p.cols ? *reinterpret_cast<const uint4*>(qrow + d0) : make_uint4(0u, 0u, 0u, 0u);
-        }
+    for (int x = 1; x < 32; x <<= 1) {
+        lim_max = max(lim_max, __shfl_xor(lim_max, x));
+        lim_min = min(lim_min, __shfl_xor(lim_min, x));
     }
-    const bool slope = p.slopes != nullptr;
-    const float slope2 = slope ? p.slopes[b * p.slopes_sb + row.h] * kLog2e : 0.f;
+    lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+    const bool uneven = tree || lim_min != __builtin_amdgcn_readfirstlane(lim_max);  // rows see different keys
     wait_vmem();
     asm volatile("" ::: "memory");
 
@@ -552,56 +643,29 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], con
 #pragma unroll
     for (int n = 0; n < D / 32; ++n) o[n] = f32x16{};
     float m_run = -1e30f, l_run = 0.f;
-    Cap<EXACT> cap(p);
-
-    int t = NW * s0 + w;
-    Block16 bx, by;
-    blocks(t, bx, by);
-    copy(kc, t, bx, by, Ks);
-    copy(vc, t, bx, by, Vs);
-    blocks(t + NW, bx, by);
     // tiles that every row sees, then the others: the loop over the first ones has no registers
     // to give to the rules of the second
     auto tile = [&](auto hidden) FA_INLINE {
         constexpr bool HIDDEN = decltype(hidden)::value;
-        const int k0 = 32 * t;
         wait_vmem_below<2 * C::NI16>();  // K(t); only V(t) may be in flight
         asm volatile("" ::: "memory");
-        f32x16 s = tile_scores<T, D>(Ks, q, kc.cols, l32, hi);
+        f32x16 s[1];
+        tile_scores<T, D, 1>(s, Ks, q, kc.cols, l32, hi);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K(t) read before it is overwritten
         copy(kc, t + NW, bx, by, Ks);
 
         unsigned have = ~0u, seen = ~0u;
         if (HIDDEN && holes) have = (unsigned)table.template have<2>(2 * t);
-        tile_rules<EXACT, HIDDEN>(s, p, cap, row, tree, slope, slope2, k0, c, seen, have, hi);
-        float m2[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int e = 0; e < 16; ++e) m2[e & 1] = fmaxf(m2[e & 1], s[e]);
-        const float m_new = fmaxf(m_run, pair_max(fmaxf(m2[0], m2[1])));
-        if (__ballot(m_new > m_run + 8.0f) != 0ull) {
-            const float alpha = fast_exp2(m_run - m_new);
-            l_run *= alpha;
-#pragma unroll
-            for (int n = 0; n < D / 32; ++n)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[n][e] *= alpha;
-            m_run = m_new;
-        }
-        float ps[2] = {0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            s[e] = fast_exp2(s[e] - m_run);
-            ps[e & 1] += s[e];
-        }
-        l_run += ps[0] + ps[1];
+        tile_rules<EXACT, HIDDEN>(s[0], rules, row, tree, 32 * t, c, seen, have, hi);
+        soft_blocks<D, 1>(s, rules.unit, m_run, l_run, o);
 
         wait_vmem_below<2 * C::NI16>();  // V(t); only K(t + 4) may be in flight
         asm volatile("" ::: "memory");
         if (HIDDEN && uneven && tile_odd<T, D>(Vs, lane)) {
             stay_branch();
-            tile_values_seen<T, D>(Vs, s, seen, o, lane);
+            tile_values_seen<T, D>(Vs, s[0], seen, o, lane);
         } else {
-            tile_values<T, D>(Vs, s, o, vc.cols, lane);
+            tile_values<T, D, 1>(Vs, s, o, vc.cols, lane);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V(t) read before it is overwritten
         copy(vc, t + NW, bx, by, Vs);
@@ -640,8 +704,7 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], con
         l_tot = 0.f;
     }
     const bool whole = part < 0;
-    const int64_t prow = part + l32;
-    if (!whole && w == 0 && hi == 0) pe.stat[prow] = make_float2(mm, l_tot);
+    if (!whole && w == 0 && hi == 0) pe.stat[part + l32] = make_float2(mm, l_tot);
     if (whole && w == 0 && hi == 0 && row.live && pe.lse) put_row_lse(pe, b, row.h, row.i, mm, l_tot);
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
 #pragma unroll
@@ -657,10 +720,9 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], con
         }
         if (!row.valid) om = f32x16{};
         if (!whole) {
-            float* op = pe.part + prow * D + 32 * n + 4 * hi;
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
-                *reinterpret_cast<f32x4*>(op + 8 * q4) = f32x4{om[4 * q4], om[4 * q4 + 1], om[4 * q4 + 2], om[4 * q4 + 3]};
+                *part_of<D>(pe.part, part, n, q4, lane) = f32x4{om[4 * q4], om[4 * q4 + 1], om[4 * q4 + 2], om[4 * q4 + 3]};
         } else if (row.live) {
             T* ob = (T*)pe.o + b * pe.o_sb + (int64_t)row.i * pe.o_ss + row.h * pe.o_sh + 32 * n + 4 * hi;
 #pragma unroll
@@ -683,6 +745,36 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], con
     lds_barrier();  // the regions and stat are free for the next unit
 }
 
+// rows [first, first + n) of a sequence without a token
+template <typename T, int D>
+__device__ FA_INLINE inline void empty_unit(PagedArgs& p, int b, int hk, int first, int n, int tid, int threads) {
+    constexpr int CW = PagedCfg<T, D>::CW, EPC = PagedCfg<T, D>::EPC;
+    for (int x = tid; x < n * CW; x += threads) {
+        const PagedRow row(p, first + x / CW, hk);
+        const int col = x % CW * EPC;
+        if (!row.live || col >= p.cols) continue;
+        *reinterpret_cast<uint4*>((T*)p.o + b * p.o_sb + (int64_t)row.i * p.o_ss + row.h * p.o_sh + col) = make_uint4(0u, 0u, 0u, 0u);
+        if (col == 0 && p.lse) put_row_lse(p, b, row.h, row.i, 0.f, 0.f);
+    }
+}
+
+// A wave's 32 rows of O from its LDS (chunks at row_swizzle's places) to their places in
+// memory, whole rows a store
+template <typename T, int D>
+__device__ FA_INLINE inline void store_tile(PagedArgs& p, const T* tile, int b, const PagedRow& row, int lane) {
+    using C = PagedCfg<T, D>;
+    const int64_t mine = row.live ? (int64_t)row.i * p.o_ss + row.h * p.o_sh : -1;
+    T* const ob = (T*)p.o + b * p.o_sb;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // written by this wave alone
+#pragma unroll
+    for (int x = 0; x < 32 * C::CW / 64; ++x) {
+        const int r = (64 * x + lane) / C::CW, chunk = lane % C::CW;
+        const int64_t at = __shfl(mine, r);
+        const uint4 v = *reinterpret_cast<const uint4*>(tile + r * D + ((chunk ^ row_swizzle<C::CW>(r)) * C::EPC));
+        if (at >= 0 && chunk * C::EPC < p.cols) *reinterpret_cast<uint4*>(ob + at + chunk * C::EPC) = v;
+    }
+}
+
 // ---------------------------------------------------------------------------
 // Units of 32 NW rows whose NW waves, on 32 rows each, share tiles of 64 keys: K and V
 // are read once for all of them.  NS tiles in LDS, of which NS - 1 are on their way or
@@ -699,25 +791,20 @@ struct WideCfg {
 };
 
 template <typename T, int D, bool EXACT, int NW>
-__device__ FA_INLINE inline void paged_unit_wide(T* smem, const TreeBits* tree, int b, int hk, int rt, int s0, int s1, int64_t part,
-                                                int lane, int w) {
+__device__ FA_INLINE inline void paged_unit_wide(T* smem, TreeBits* tree, bool new_tree, int b, int hk, int rt, int s0, int s1,
+                                                int64_t part, int tid) {
     using C = PagedCfg<T, D>;
     using X = WideCfg<T, D, NW>;
     PagedArgs& p = paged_args();
+    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6) & (NW - 1);
     const int l32 = lane & 31, hi = lane >> 5;
+    PagedRow row(p, 32 * (NW * rt + w) + l32, hk);
+    uint4 q[D / 16];
+    load_q<T, D>(p, row, b, hi, q);
+    TileRules<EXACT> rules(p, b, row.h);
     const int len = __builtin_amdgcn_readfirstlane(filled_tokens(p, b)), c = len - p.Sq;
-    const PagedRow row(p, tree, 32 * (NW * rt + w) + l32, b, hk, len);
-    int lim_min = row.valid ? row.all : INT_MAX, lim_max = row.lim;
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-        lim_min = min(lim_min, __shfl_xor(lim_min, x));
-        lim_max = max(lim_max, __shfl_xor(lim_max, x));
-    }
-    lim_min = __builtin_amdgcn_readfirstlane(lim_min);
-    const bool uneven = tree || lim_min != __builtin_amdgcn_readfirstlane(lim_max);
-    // keys that some row of the unit may see: all waves copy for all
-    const int top = tree ? len : min(len, c + min(p.Sq, (32 * NW * (rt + 1) - 1) / p.group + 1));
-    const int n_keys = max(top, 0), t1 = min(s1, (n_keys + 63) / 64);
+    // (all waves copy for all)
+    const int n_keys = keys_of(p, tree, 32 * NW * (rt + 1), len, c), t1 = min(s1, (n_keys + 63) / 64);
 
     PageCopy<T, D> kc, vc;
     if (NW == 4 || w < 4) kc.init((const T*)p.k + hk * p.k_sh, p.k_sp, p.k_ss, p.cols, lane);
@@ -734,19 +821,21 @@ __device__ FA_INLINE inline void paged_unit_wide(T* smem, const TreeBits* tree, 
         kc.load(at, nv, NW == 8 ? dst + (w >> 2) * X::TILE : dst);
         if (NW == 4) vc.load(at, nv, dst + X::TILE);
     };
-    const bool holes = table.holes(4 * s0, 4 * t1, lane);
-
-    constexpr int QR = D / 16;
-    uint4 q[QR];
-    {
-        const T* qrow = (const T*)p.q + b * p.q_sb + (int64_t)row.i * p.q_ss + row.h * p.q_sh;
 #pragma unroll
-        for (int kk = 0; kk < QR; ++kk)
-            q[kk] = row.live && 16 * kk + 8 * hi < p.cols ? *reinterpret_cast<const uint4*>(qrow + 16 * kk + 8 * hi)
-                                                          : make_uint4(0u, 0u, 0u, 0u);
+    for (int x = 0; x < X::NS - 1; ++x) issue(s0 + x, look(s0 + x));
+    Block16 next = look(s0 + X::NS - 1);
+
+    if (new_tree) tree_init(p, *tree, b, tid);
+    row.rule(tree, rules.words, len, c);
+    const bool holes = table.holes(4 * s0, 4 * t1, lane);
+    int lim_min = row.valid ? row.all : INT_MAX, lim_max = row.lim;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        lim_min = min(lim_min, __shfl_xor(lim_min, x));
+        lim_max = max(lim_max, __shfl_xor(lim_max, x));
     }
-    const bool slope = p.slopes != nullptr;
-    const float slope2 = slope ? p.slopes[b * p.slopes_sb + row.h] * kLog2e : 0.f;
+    lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+    const bool uneven = tree || lim_min != __builtin_amdgcn_readfirstlane(lim_max);
     wait_vmem();
     asm volatile("" ::: "memory");
 
@@ -754,68 +843,45 @@ __device__ FA_INLINE inline void paged_unit_wide(T* smem, const TreeBits* tree, 
 #pragma unroll
     for (int n = 0; n < D / 32; ++n) o[n] = f32x16{};
     float m_run = -1e30f, l_run = 0.f;
-    Cap<EXACT> cap(p);
-
-#pragma unroll
-    for (int x = 0; x < X::NS - 1; ++x) issue(s0 + x, look(s0 + x));
-    Block16 next = look(s0 + X::NS - 1);
-    // (as in paged_unit32: what every row sees first)
-    auto tile = [&](int t, auto hide) FA_INLINE {
-        constexpr bool HIDDEN = decltype(hide)::value;
-        const int k0 = 64 * t;
+    auto next_tile = [&](int t) FA_INLINE {
         wait_vmem_below<(X::NS - 2) * X::COPIES>();  // this wave's part of tile t
         barrier_no_fence();                          // everyone's, and tile t - 1 has been read
         issue(t + X::NS - 1, next);
         next = look(t + X::NS);
-        const T* const Ks = smem + (t & (X::NS - 1)) * 2 * X::TILE;
-        const T* const Vs = Ks + X::TILE;
-        f32x16 s[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) s[x] = tile_scores<T, D>(Ks + x * 32 * D, q, D, l32, hi);
-        unsigned seen[2] = {~0u, ~0u};
-        uint64_t have = ~0ull;
-        if (HIDDEN && holes) have = table.template have<4>(4 * t);
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-            tile_rules<EXACT, HIDDEN>(s[x], p, cap, row, tree, slope, slope2, k0 + 32 * x, c, seen[x], (unsigned)(have >> (32 * x)), hi);
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) m4[e & 3] = fmaxf(m4[e & 3], s[x][e]);
-        const float m_new = fmaxf(m_run, pair_max(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))));
-        if (__ballot(m_new > m_run + 8.0f) != 0ull) {
-            const float alpha = fast_exp2(m_run - m_new);
-            l_run *= alpha;
-#pragma unroll
-            for (int n = 0; n < D / 32; ++n)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[n][e] *= alpha;
-            m_run = m_new;
-        }
-        float ps[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[x][e] = fast_exp2(s[x][e] - m_run);
-                ps[e & 3] += s[x][e];
-            }
-        l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            if (HIDDEN && uneven && tile_odd<T, D>(Vs + x * 32 * D, lane)) {
-                stay_branch();
-                tile_values_seen<T, D>(Vs + x * 32 * D, s[x], seen[x], o, lane);
-            } else {
-                tile_values<T, D>(Vs + x * 32 * D, s[x], o, D, lane);
-            }
-        }
+        return smem + (t & (X::NS - 1)) * 2 * X::TILE;
     };
+    // (as in paged_unit32: what every row sees first; the others in blocks of 32 keys)
     const int tv = holes ? s0 : min(t1, lim_min / 64);
     int t = s0;
-    for (; t < tv; ++t) tile(t, std::false_type{});
-    for (; t < t1; ++t) tile(t, std::true_type{});
+    for (; t < tv; ++t) {
+        const T* const Ks = next_tile(t);
+        f32x16 s[2];
+        tile_scores<T, D, 2>(s, Ks, q, D, l32, hi);
+        unsigned seen;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) tile_rules<EXACT, false>(s[x], rules, row, tree, 64 * t + 32 * x, c, seen, ~0u, hi);
+        soft_blocks<D, 2>(s, rules.unit, m_run, l_run, o);
+        tile_values<T, D, 2>(Ks + X::TILE, s, o, D, lane);
+    }
+    for (; t < t1; ++t) {
+        const T* const Ks = next_tile(t);
+#pragma unroll 1
+        for (int x = 0; x < 2; ++x) {
+            const T* const Vs = Ks + X::TILE + x * 32 * D;
+            f32x16 s[1];
+            tile_scores<T, D, 1>(s, Ks + x * 32 * D, q, D, l32, hi);
+            unsigned have = ~0u, seen;
+            if (holes) have = (unsigned)table.template have<2>(4 * t + 2 * x);
+            tile_rules<EXACT, true>(s[0], rules, row, tree, 64 * t + 32 * x, c, seen, have, hi);
+            soft_blocks<D, 1>(s, rules.unit, m_run, l_run, o);
+            if (uneven && tile_odd<T, D>(Vs, lane)) {
+                stay_branch();
+                tile_values_seen<T, D>(Vs, s[0], seen, o, lane);
+            } else {
+                tile_values<T, D, 1>(Vs, s, o, D, lane);
+            }
+        }
+    }
     wait_vmem();  // (copies of no tile)
 
     PagedArgs& pe = paged_args();
@@ -826,31 +892,31 @@ __device__ FA_INLINE inline void paged_unit_wide(T* smem, const TreeBits* tree, 
 #pragma unroll
         for (int n = 0; n < D / 32; ++n) o[n] = f32x16{};
     }
+    barrier_no_fence();  // the slots have been read: they take the rows of O, or the next unit's tiles
     if (part >= 0) {
-        const int64_t prow = part + 32 * w + l32;
-        if (hi == 0) pe.stat[prow] = make_float2(m_run, l_tot);
-        float* op = pe.part + prow * D + 4 * hi;
+        if (hi == 0) pe.stat[part + 32 * w + l32] = make_float2(m_run, l_tot);
 #pragma unroll
         for (int n = 0; n < D / 32; ++n)
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
-                *reinterpret_cast<f32x4*>(op + 32 * n + 8 * q4) = f32x4{o[n][4 * q4], o[n][4 * q4 + 1], o[n][4 * q4 + 2], o[n][4 * q4 + 3]};
-    } else if (row.live) {
-        if (hi == 0 && pe.lse) put_row_lse(pe, b, row.h, row.i, m_run, l_tot);
+                *part_of<D>(pe.part, part + 32 * w, n, q4, lane) =
+                    f32x4{o[n][4 * q4], o[n][4 * q4 + 1], o[n][4 * q4 + 2], o[n][4 * q4 + 3]};
+    } else {
+        if (row.live && hi == 0 && pe.lse) put_row_lse(pe, b, row.h, row.i, m_run, l_tot);
         const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
-        T* ob = (T*)pe.o + b * pe.o_sb + (int64_t)row.i * pe.o_ss + row.h * pe.o_sh + 4 * hi;
+        T* const mine = smem + w * 32 * D;
 #pragma unroll
         for (int n = 0; n < D / 32; ++n)
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
-                if (32 * n + 8 * q4 + 4 * hi >= pe.cols) continue;
                 s16x4 v4;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v4[e] = Elem<T>::pack1(o[n][4 * q4 + e] * inv);
-                *reinterpret_cast<s16x4*>(ob + 32 * n + 8 * q4) = v4;
+                *reinterpret_cast<s16x4*>(mine + l32 * D + (((4 * n + q4) ^ row_swizzle<C::CW>(l32)) << 3) + 4 * hi) = v4;
             }
+        store_tile<T, D>(pe, mine, b, row, lane);
+        barrier_no_fence();  // read, before the next unit's copies
     }
-    barrier_no_fence();  // the slots have been read, before the next unit's copies
 }
 
 // ---------------------------------------------------------------------------
@@ -873,10 +939,9 @@ __global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 : Pag
     PagedArgs& p = paged_args();
     __shared__ __attribute__((aligned(1024))) T smem[S::SMEM];
     __shared__ typename std::conditional<TREE, TreeBits, int>::type bits;
-    const TreeBits* tree = nullptr;
+    TreeBits* tree = nullptr;
     if constexpr (TREE) tree = &bits;
-    const int tid = threadIdx.x;
-    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6) & 7;
+    const int tid = threadIdx.x, lane = tid & 63;
     PagedWork wk;
     wk.init<S::STEP>(p, lane);
     if ((int)blockIdx.x >= wk.W) return;
@@ -895,84 +960,91 @@ __global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 : Pag
     while (x < end) {
         if (!wk.whole && (last_b < 0 || x >= start + len * wk.per_seq)) wk.locate<S::STEP>(paged_args(), x, lane, b, start, len);
         const int u = (x - start) / len, s0 = x - start - u * len, s1 = min(len, s0 + end - x);
-        if constexpr (TREE) {
-            if (b != last_b) tree_init(paged_args(), bits, b, tid);
-        }
-        last_b = b;
         const int64_t part = s1 - s0 == len ? -1 : part_at<S::ROWS>(g, s0 == 0);
         const int tiles = paged_args().unit_tiles;
-        if constexpr (NW == 1) {
+        if (len == 1 && filled_tokens(paged_args(), b) == 0) {
+            empty_unit<T, D>(paged_args(), b, u / tiles, u % tiles * S::ROWS, S::ROWS, tid, S::THREADS);
+        } else if constexpr (NW == 1) {
             __shared__ float stat[PagedCfg<T, D>::NW][2][32];
-            paged_unit32<T, D, EXACT>(smem, stat, tree, b, u / tiles, u % tiles, s0, s1, part, lane, w);
+            paged_unit32<T, D, EXACT>(smem, stat, tree, TREE && b != last_b, b, u / tiles, u % tiles, s0, s1, part, tid);
         } else {
-            paged_unit_wide<T, D, EXACT, NW>(smem, tree, b, u / tiles, u % tiles, s0, s1, part, lane, w);
+            paged_unit_wide<T, D, EXACT, NW>(smem, tree, TREE && b != last_b, b, u / tiles, u % tiles, s0, s1, part, tid);
         }
+        last_b = b;
         x += s1 - s0;
     }
 }
 
-// The parts of the rows of units that several workgroups shared: D / 4 threads a row,
-// 4 columns each, a wave's rows all of one sequence (blockIdx.y)
+// The parts of 32 rows (blockIdx.x: KV head, unit, its rows) of a unit that several
+// workgroups shared, 32 columns (blockIdx.y) of them: each wave takes every fourth part,
+// and their sums meet in LDS.
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams) {
     using S = PagedShape<T, D, NW>;
     PagedArgs& p = paged_args();
-    constexpr int TPR = D / 4, ROWS = 256 / TPR;
-    const int lane = threadIdx.x & 63, b = blockIdx.y;
+    __shared__ float sums[4][16][64], stat[4][2][32];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+    const int l32 = lane & 31, hi = lane >> 5, n = blockIdx.y, b = blockIdx.z;
     PagedWork wk;
     wk.init<S::STEP>(p, lane);
     if (wk.whole) return;
     const int start = wk.start_of<S::STEP>(p, b, lane);
     const int len = __builtin_amdgcn_readfirstlane(PagedWork::steps<S::STEP>(p, b));
-    const int r = (int)blockIdx.x * ROWS + (int)threadIdx.x / TPR, col = (int)(threadIdx.x % TPR) * 4;
-    const int rows = p.Sq * p.group;  // of a KV head
-    if (r >= rows * p.Hkv) return;
-    const int hk = r / rows, ig = r % rows, rt = ig / S::ROWS;
-    const int s = start + (hk * p.unit_tiles + rt) * len;  // the unit's first step
+    const int u = blockIdx.x / NW, first_row = S::ROWS * (u % p.unit_tiles) + 32 * (blockIdx.x % NW);
+    const int s = start + u * len;  // the unit's first step
     const int g0 = wk.whose(s), g1 = wk.whose(s + len - 1);
     if (g0 == g1) return;
-    float mm = -1e30f, l_tot = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int x0 = g0; x0 <= g1; x0 += 4) {
-        float2 st[4];
+    float m = -1e30f, l = 0.f;
+    f32x4 acc[4];
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) acc[q4] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int g = g0 + w; g <= g1; g += 4) {
+        const int64_t part = part_at<S::ROWS>(g, g == g0) + 32 * (blockIdx.x % NW);  // g0 begins the unit
+        const float2 st = p.stat[part + l32];
         f32x4 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const bool in = x0 + j <= g1;
-            const int g = in ? x0 + j : g0;
-            const int64_t pr = part_at<S::ROWS>(g, g == g0) + ig % S::ROWS;  // g0 begins the unit
-            st[j] = p.stat[pr];
-            v[j] = *reinterpret_cast<const f32x4*>(p.part + pr * D + col);
-            if (!in) {
-                st[j] = make_float2(-1e30f, 0.f);
-                v[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            }
-        }
-        const float m0 = fmaxf(mm, fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)));
-        const float a0 = fast_exp2(mm - m0);
-        l_tot *= a0;
+        for (int q4 = 0; q4 < 4; ++q4) v[q4] = *part_of<D>(p.part, part, n, q4, lane);
+        const float m0 = fmaxf(m, st.x), a0 = fast_exp2(m - m0), a1 = fast_exp2(st.x - m0);
+        l = __builtin_fmaf(st.y, a1, l * a0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] *= a0;
+        for (int q4 = 0; q4 < 4; ++q4)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float a = fast_exp2(st[j].x - m0);
-            l_tot = __builtin_fmaf(st[j].y, a, l_tot);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(v[j][e], a, acc[e]);
-        }
-        mm = m0;
+            for (int e = 0; e < 4; ++e) acc[q4][e] = __builtin_fmaf(v[q4][e], a1, acc[q4][e] * a0);
+        m = m0;
     }
-    const int i = ig / p.group, h = hk * p.group + ig % p.group;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sums[w][e][lane] = acc[e >> 2][e & 3];
+    if (hi == 0) {
+        stat[w][0][l32] = m;
+        stat[w][1][l32] = l;
+    }
+    __syncthreads();
+    // each thread 4 columns of a row: 8 threads a row
+    const int r = threadIdx.x >> 3, c4 = threadIdx.x & 7;
+    const PagedRow row(p, first_row + r, u / p.unit_tiles);
+    if (!row.live) return;
+    float mm = stat[0][0][r], l_tot = 0.f;
+#pragma unroll
+    for (int x = 1; x < 4; ++x) mm = fmaxf(mm, stat[x][0][r]);
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        const float a = fast_exp2(stat[x][0][r] - mm);
+        l_tot = __builtin_fmaf(stat[x][1][r], a, l_tot);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(sums[x][4 * (c4 >> 1) + e][32 * (c4 & 1) + r], a, o[e]);
+    }
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
-    if (col == 0 && p.lse) put_row_lse(p, b, h, i, mm, l_tot);
+    if (n == 0 && c4 == 0 && p.lse) put_row_lse(p, b, row.h, row.i, mm, l_tot);
+    const int col = 32 * n + 4 * c4;
     if (col >= p.cols) return;
-    T* ob = (T*)p.o + b * p.o_sb + (int64_t)i * p.o_ss + h * p.o_sh + col;
+    T* ob = (T*)p.o + b * p.o_sb + (int64_t)row.i * p.o_ss + row.h * p.o_sh + col;
     if constexpr (Elem<T>::kF32) {
-        *reinterpret_cast<f32x4*>(ob) = f32x4{acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+        *reinterpret_cast<f32x4*>(ob) = f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     } else {
         s16x4 v4;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v4[e] = Elem<T>::pack1(acc[e] * inv);
+        for (int e = 0; e < 4; ++e) v4[e] = Elem<T>::pack1(o[e] * inv);
         *reinterpret_cast<s16x4*>(ob) = v4;
     }
 }
@@ -994,9 +1066,8 @@ hipError_t launch_paged_t(const PagedParams& p, hipStream_t s) {
             hipLaunchKernelGGL((paged_kernel<T, D, F32, false, NW>), grid, block, 0, s, p);
     }
     if (p.part) {
-        constexpr int ROWS = 256 / (D / 4);
-        const int rows = p.Sq * p.H;
-        hipLaunchKernelGGL((paged_join_kernel<T, D, NW>), dim3((unsigned)((rows + ROWS - 1) / ROWS), (unsigned)p.B), dim3(256), 0, s, p);
+        const dim3 tiles((unsigned)(p.Hkv * p.unit_tiles * NW), D / 32, (unsigned)p.B);
+        hipLaunchKernelGGL((paged_join_kernel<T, D, NW>), tiles, dim3(256), 0, s, p);
     }
     return hipGetLastError();
 }
