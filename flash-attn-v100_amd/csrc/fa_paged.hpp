@@ -337,9 +337,34 @@ __device__ FA_INLINE inline void reads_ahead() {
     }
 }
 
+// Scores of one block of 32 keys (D / 16 products) beside the exponentials of another, then
+// that one's values (D / 16 products, two reads each) beside the maximum of the scores
+template <int D>
+__device__ FA_INLINE inline void block_order() {
+    constexpr int kMfma = 0x008, kRead = 0x100, kVector = 0x002, N = D / 16, AHEAD = N < 4 ? N : 4;
+    __builtin_amdgcn_sched_group_barrier(kRead, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kVector, 64 / N, 0);
+        if (AHEAD + i < N)
+            __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+        else
+            __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kVector, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
+    }
+}
+
 // the products of a wave's 32 rows with NB blocks of 32 keys (K tile), log2 units before
 // the rules (float32, whose products bound it: only over columns that exist)
-template <typename T, int D, int NB>
+// (ORDERED: its place among other instructions is the caller's to say)
+template <typename T, int D, int NB, bool ORDERED = false>
 __device__ FA_INLINE inline void tile_scores(f32x16 (&s)[NB], const T* Ks, const uint4 (&q)[Elem<T>::kF32 ? D / 8 : D / 16], int cols,
                                             int l32, int hi) {
     using C = PagedCfg<T, D>;
@@ -364,12 +389,12 @@ __device__ FA_INLINE inline void tile_scores(f32x16 (&s)[NB], const T* Ks, const
 #pragma unroll
             for (int x = 0; x < NB; ++x)
                 s[x] = Elem<T>::mfma(lds_at<s16x8>((at ^ (kk << 5)) + x * 32 * C::ROWB), __builtin_bit_cast(s16x8, q[kk]), s[x]);
-        reads_ahead<NB * D / 16, 1, NB * D / 16 < 6 ? NB * D / 16 : 6>();
+        if constexpr (!ORDERED) reads_ahead<NB * D / 16, 1, NB * D / 16 < 6 ? NB * D / 16 : 6>();
     }
 }
 
 // O^T += V^T P^T over NB blocks of 32 keys
-template <typename T, int D, int NB>
+template <typename T, int D, int NB, bool ORDERED = false>
 __device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16 (&s)[NB], f32x16 (&o)[D / 32], int cols, int lane) {
     using C = PagedCfg<T, D>;
     const int l32 = lane & 31, hi = lane >> 5;
@@ -405,7 +430,7 @@ __device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16 (&s)[NB],
                                      lds_tr16_at((at ^ ((n << 6) ^ (row_swizzle<C::CW>(8) << 4))) + (16 * ks + 8) * C::ROWB));
                 o[n] = Elem<T>::mfma(a, pk[ks], o[n]);
             }
-        reads_ahead<2 * NB * D / 32, 2, 2 * NB * D / 32 < 4 ? 4 * NB * D / 32 : 8>();
+        if constexpr (!ORDERED) reads_ahead<2 * NB * D / 32, 2, 2 * NB * D / 32 < 4 ? 4 * NB * D / 32 : 8>();
     }
 }
 
@@ -542,7 +567,7 @@ __device__ FA_INLINE inline void tile_rules(f32x16& s, TileRules<EXACT>& u, cons
 // probabilities: e^(s - m) with an m that is at most 8 (of log2) behind the largest, so
 // that O is rescaled when a maximum grows by more
 template <int D, int NB>
-__device__ FA_INLINE inline void soft_blocks(f32x16 (&s)[NB], float unit, float& m_run, float& l_run, f32x16 (&o)[D / 32]) {
+__device__ FA_INLINE inline void soft_max(const f32x16 (&s)[NB], float unit, float& m_run, float& l_run, f32x16 (&o)[D / 32]) {
     float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int x = 0; x < NB; ++x)
@@ -558,6 +583,9 @@ __device__ FA_INLINE inline void soft_blocks(f32x16 (&s)[NB], float unit, float&
             for (int e = 0; e < 16; ++e) o[n][e] *= alpha;
         m_run = m_new;
     }
+}
+template <int NB>
+__device__ FA_INLINE inline void soft_exp(f32x16 (&s)[NB], float unit, float m_run, float& l_run) {
     float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int x = 0; x < NB; ++x)
@@ -657,7 +685,8 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], Tre
         unsigned have = ~0u, seen = ~0u;
         if (HIDDEN && holes) have = (unsigned)table.template have<2>(2 * t);
         tile_rules<EXACT, HIDDEN>(s[0], rules, row, tree, 32 * t, c, seen, have, hi);
-        soft_blocks<D, 1>(s, rules.unit, m_run, l_run, o);
+        soft_max<D, 1>(s, rules.unit, m_run, l_run, o);
+        soft_exp<1>(s, rules.unit, m_run, l_run);
 
         wait_vmem_below<2 * C::NI16>();  // V(t); only K(t + 4) may be in flight
         asm volatile("" ::: "memory");
@@ -855,13 +884,22 @@ __device__ FA_INLINE inline void paged_unit_wide(T* smem, TreeBits* tree, bool n
     int t = s0;
     for (; t < tv; ++t) {
         const T* const Ks = next_tile(t);
-        f32x16 s[2];
-        tile_scores<T, D, 2>(s, Ks, q, D, l32, hi);
+        const T* const Vs = Ks + X::TILE;
+        // the second block's scores beside the first one's exponentials, the first one's values
+        // beside the second one's maximum
         unsigned seen;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) tile_rules<EXACT, false>(s[x], rules, row, tree, 64 * t + 32 * x, c, seen, ~0u, hi);
-        soft_blocks<D, 2>(s, rules.unit, m_run, l_run, o);
-        tile_values<T, D, 2>(Ks + X::TILE, s, o, D, lane);
+        f32x16 sa[1], sb[1];
+        tile_scores<T, D, 1>(sa, Ks, q, D, l32, hi);
+        tile_rules<EXACT, false>(sa[0], rules, row, tree, 64 * t, c, seen, ~0u, hi);
+        soft_max<D, 1>(sa, rules.unit, m_run, l_run, o);
+        tile_scores<T, D, 1, true>(sb, Ks + 32 * D, q, D, l32, hi);
+        soft_exp<1>(sa, rules.unit, m_run, l_run);
+        tile_values<T, D, 1, true>(Vs, sa, o, D, lane);
+        block_order<D>();
+        tile_rules<EXACT, false>(sb[0], rules, row, tree, 64 * t + 32, c, seen, ~0u, hi);
+        soft_max<D, 1>(sb, rules.unit, m_run, l_run, o);
+        soft_exp<1>(sb, rules.unit, m_run, l_run);
+        tile_values<T, D, 1>(Vs + 32 * D, sb, o, D, lane);
     }
     for (; t < t1; ++t) {
         const T* const Ks = next_tile(t);
@@ -873,7 +911,8 @@ __device__ FA_INLINE inline void paged_unit_wide(T* smem, TreeBits* tree, bool n
             unsigned have = ~0u, seen;
             if (holes) have = (unsigned)table.template have<2>(4 * t + 2 * x);
             tile_rules<EXACT, true>(s[0], rules, row, tree, 64 * t + 32 * x, c, seen, have, hi);
-            soft_blocks<D, 1>(s, rules.unit, m_run, l_run, o);
+            soft_max<D, 1>(s, rules.unit, m_run, l_run, o);
+        soft_exp<1>(s, rules.unit, m_run, l_run);
             if (uneven && tile_odd<T, D>(Vs, lane)) {
                 stay_branch();
                 tile_values_seen<T, D>(Vs, s[0], seen, o, lane);
