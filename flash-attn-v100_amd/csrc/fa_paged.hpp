@@ -184,25 +184,38 @@ __device__ FA_INLINE inline unsigned tree_word(const TreeBits& t, int i, int s, 
 
 // ---------------------------------------------------------------------------
 // Work.  Steps of all units in one list, by sequence, then unit; every sequence has
-// one at least.  Where no unit is longer than a workgroup's share (or than p.least steps,
-// whose join would cost more than it saves), a workgroup takes whole units.
+// one at least, and every unit p.extra more that stand for what it costs beside its keys.
+// Where no unit is longer than a workgroup's share, or than p.alone steps, a workgroup takes
+// whole units.
 struct PagedWork {
     int T, W;      // steps, workgroups that have work
     int per_seq;   // units of a sequence
     bool whole;    // a workgroup takes whole units
+    int st0, inc0; // of sequence `lane`: its steps, and those up to its end
     template <int STEP>
     __device__ FA_INLINE inline static int steps(PagedArgs& p, int b) {
-        return b < p.B ? max(1, (filled_tokens(p, b) + STEP - 1) / STEP) : 0;
+        return b < p.B ? max(1, (filled_tokens(p, b) + STEP - 1) / STEP) + p.extra : 0;
+    }
+    __device__ FA_INLINE inline static int scan(int x, int lane) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_up(x, d);
+            if (lane >= d) x += y;
+        }
+        return x;
     }
     template <int STEP>
     __device__ FA_INLINE inline void init(PagedArgs& p, int lane) {
         int sum = 0, most = 0;
         if (p.lens) {
-            for (int b0 = 0; b0 < p.B; b0 += 64) {
+            most = st0 = steps<STEP>(p, lane);
+            for (int b0 = 64; b0 < p.B; b0 += 64) {
                 const int st = steps<STEP>(p, b0 + lane);
                 sum += st;
                 most = max(most, st);
             }
+            inc0 = scan(st0, lane);
+            sum += st0;
 #pragma unroll
             for (int x = 1; x < 64; x <<= 1) {
                 sum += __shfl_xor(sum, x);
@@ -215,12 +228,17 @@ struct PagedWork {
         per_seq = p.Hkv * p.unit_tiles;
         T = __builtin_amdgcn_readfirstlane(sum) * per_seq;
         W = min(p.slots, (T + p.least - 1) / p.least);
-        whole = __builtin_amdgcn_readfirstlane(most) <= max(p.least, (T + W - 1) / W);
+        whole = __builtin_amdgcn_readfirstlane(most) - p.extra <= max(p.alone, (T + W - 1) / W);
         if (whole) W = p.B * per_seq;
     }
-    // the first step of workgroup g (floor(g T / W)), and whose step x is
-    __device__ FA_INLINE inline int first(int g) const { return (int)((int64_t)g * T / W); }
-    __device__ FA_INLINE inline int whose(int x) const { return (int)((((int64_t)x + 1) * W - 1) / T); }
+    // the first step of workgroup g (floor(g T / W)), and whose step x is; in 32 bits where
+    // they suffice
+    __device__ FA_INLINE inline int first(int g) const {
+        return (int64_t)T * W < INT_MAX ? (int)((unsigned)(g * T) / (unsigned)W) : (int)((int64_t)g * T / W);
+    }
+    __device__ FA_INLINE inline int whose(int x) const {
+        return (int64_t)T * W < INT_MAX ? (int)((unsigned)((x + 1) * W - 1) / (unsigned)T) : (int)((((int64_t)x + 1) * W - 1) / T);
+    }
     // the sequence of step x, its first step and the steps of one of its units
     template <int STEP>
     __device__ FA_INLINE inline void locate(PagedArgs& p, int x, int lane, int& b, int& start, int& len) const {
@@ -232,13 +250,7 @@ struct PagedWork {
         }
         int before = 0;
         for (int b0 = 0;; b0 += 64) {
-            const int st = steps<STEP>(p, b0 + lane);
-            int inc = st;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const int y = __shfl_up(inc, d);
-                if (lane >= d) inc += y;
-            }
+            const int st = b0 ? steps<STEP>(p, b0 + lane) : st0, inc = b0 ? scan(st, lane) : inc0;
             const uint64_t past = __ballot((int64_t)(before + inc) * per_seq > x);
             if (past || b0 + 64 >= p.B) {
                 const int l = past ? (int)__builtin_ctzll(past) : 63;
@@ -250,15 +262,23 @@ struct PagedWork {
             before += __builtin_amdgcn_readlane(inc, 63);
         }
     }
-    // the first step of sequence b
+    // the first step of sequence b and the steps of one of its units
     template <int STEP>
-    __device__ FA_INLINE inline int start_of(PagedArgs& p, int b, int lane) const {
-        if (!p.lens) return b * steps<STEP>(p, 0) * per_seq;
-        int sum = 0;
-        for (int b0 = 0; b0 < b; b0 += 64) sum += b0 + lane < b ? steps<STEP>(p, b0 + lane) : 0;
+    __device__ FA_INLINE inline void sequence(PagedArgs& p, int b, int lane, int& start, int& len) const {
+        if (!p.lens) {
+            len = steps<STEP>(p, 0);
+            start = b * len * per_seq;
+        } else if (b < 64) {
+            len = __builtin_amdgcn_readlane(st0, b);
+            start = (__builtin_amdgcn_readlane(inc0, b) - len) * per_seq;
+        } else {
+            int sum = st0;
+            for (int b0 = 64; b0 < b; b0 += 64) sum += b0 + lane < b ? steps<STEP>(p, b0 + lane) : 0;
 #pragma unroll
-        for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
-        return __builtin_amdgcn_readfirstlane(sum) * per_seq;
+            for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+            len = __builtin_amdgcn_readfirstlane(steps<STEP>(p, b));
+            start = __builtin_amdgcn_readfirstlane(sum) * per_seq;
+        }
     }
 };
 // parts: a workgroup leaves at most two, of the unit that it begins with (2 g) and of
@@ -985,7 +1005,8 @@ __global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 : Pag
     wk.init<S::STEP>(p, lane);
     if ((int)blockIdx.x >= wk.W) return;
     const int g = xcd_remap((int)blockIdx.x, wk.W);
-    int x = 0, end = 0, b = 0, start = 0, len = 0, last_b = -1;
+    const int extra = p.extra;
+    int x = 0, end = 0, b = 0, start = 0, len = 0, last_b = -1;  // len: of a unit, with the extra steps
     if (wk.whole) {
         b = g / wk.per_seq;
         len = __builtin_amdgcn_readfirstlane(PagedWork::steps<S::STEP>(p, b));
@@ -998,10 +1019,12 @@ __global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 : Pag
     }
     while (x < end) {
         if (!wk.whole && (last_b < 0 || x >= start + len * wk.per_seq)) wk.locate<S::STEP>(paged_args(), x, lane, b, start, len);
-        const int u = (x - start) / len, s0 = x - start - u * len, s1 = min(len, s0 + end - x);
-        const int64_t part = s1 - s0 == len ? -1 : part_at<S::ROWS>(g, s0 == 0);
+        const int u = (x - start) / len, s0 = x - start - u * len, n = len - extra, s1 = min(n, s0 + end - x);
+        x = min(end, start + (u + 1) * len);
+        if (s0 >= s1) continue;  // (the extra steps of a unit that ended in another workgroup)
+        const int64_t part = s1 - s0 == n ? -1 : part_at<S::ROWS>(g, s0 == 0);
         const int tiles = paged_args().unit_tiles;
-        if (len == 1 && filled_tokens(paged_args(), b) == 0) {
+        if (n == 1 && filled_tokens(paged_args(), b) == 0) {
             empty_unit<T, D>(paged_args(), b, u / tiles, u % tiles * S::ROWS, S::ROWS, tid, S::THREADS);
         } else if constexpr (NW == 1) {
             __shared__ float stat[PagedCfg<T, D>::NW][2][32];
@@ -1010,81 +1033,106 @@ __global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 : Pag
             paged_unit_wide<T, D, EXACT, NW>(smem, tree, TREE && b != last_b, b, u / tiles, u % tiles, s0, s1, part, tid);
         }
         last_b = b;
-        x += s1 - s0;
     }
 }
 
 // The parts of 32 rows (blockIdx.x: KV head, unit, its rows) of a unit that several
-// workgroups shared, 32 columns (blockIdx.y) of them: each wave takes every fourth part,
-// and their sums meet in LDS.
+// workgroups shared: for 32 columns G waves, each of which takes every G-th part, two at
+// a time, and whose sums meet in LDS.  Units of 32 rows are few and in up to 64 parts: four
+// waves, 32 columns a workgroup (one token over 65536 keys: 39 us a call, 45 with two and all
+// columns); wide units are in two or three, and what a workgroup finds out about its unit
+// serves all columns (16 trees of 64 over up to 8192: 13 us, 18 with 32 columns).
+template <int D, int NW>
+struct JoinShape {
+    static constexpr int G = NW == 1 ? 4 : 2, BLOCKS = NW == 1 ? 1 : D / 32;  // of 32 columns
+};
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(256) void paged_join_kernel(const PagedParams) {
+__global__ __launch_bounds__((64 * JoinShape<D, NW>::G * JoinShape<D, NW>::BLOCKS)) void paged_join_kernel(const PagedParams) {
     using S = PagedShape<T, D, NW>;
+    using J = JoinShape<D, NW>;
+    constexpr int G = J::G;
     PagedArgs& p = paged_args();
-    __shared__ float sums[4][16][64], stat[4][2][32];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
-    const int l32 = lane & 31, hi = lane >> 5, n = blockIdx.y, b = blockIdx.z;
+    __shared__ float sums[J::BLOCKS][G][16][64], stat[G][2][32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l32 = lane & 31, hi = lane >> 5, b = blockIdx.z;
+    const int w = wave % G, block = wave / G, n = blockIdx.y * J::BLOCKS + block;
     PagedWork wk;
     wk.init<S::STEP>(p, lane);
     if (wk.whole) return;
-    const int start = wk.start_of<S::STEP>(p, b, lane);
-    const int len = __builtin_amdgcn_readfirstlane(PagedWork::steps<S::STEP>(p, b));
-    const int u = blockIdx.x / NW, first_row = S::ROWS * (u % p.unit_tiles) + 32 * (blockIdx.x % NW);
+    int start, len;
+    wk.sequence<S::STEP>(p, b, lane, start, len);
+    const int u = blockIdx.x / NW, r0 = 32 * (blockIdx.x % NW);
     const int s = start + u * len;  // the unit's first step
-    const int g0 = wk.whose(s), g1 = wk.whose(s + len - 1);
+    const int g0 = wk.whose(s), g1 = wk.whose(s + len - p.extra - 1);
     if (g0 == g1) return;
     float m = -1e30f, l = 0.f;
     f32x4 acc[4];
 #pragma unroll
     for (int q4 = 0; q4 < 4; ++q4) acc[q4] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int g = g0 + w; g <= g1; g += 4) {
-        const int64_t part = part_at<S::ROWS>(g, g == g0) + 32 * (blockIdx.x % NW);  // g0 begins the unit
-        const float2 st = p.stat[part + l32];
-        f32x4 v[4];
+    for (int g = g0 + w; g <= g1; g += 2 * G) {
+        float2 st[2];
+        f32x4 v[2][4];
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) v[q4] = *part_of<D>(p.part, part, n, q4, lane);
-        const float m0 = fmaxf(m, st.x), a0 = fast_exp2(m - m0), a1 = fast_exp2(st.x - m0);
-        l = __builtin_fmaf(st.y, a1, l * a0);
+        for (int x = 0; x < 2; ++x) {
+            const bool in = g + G * x <= g1;
+            const int gx = in ? g + G * x : g;
+            const int64_t part = part_at<S::ROWS>(gx, gx == g0) + r0;  // g0 begins the unit
+            st[x] = p.stat[part + l32];
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) v[x][q4] = *part_of<D>(p.part, part, n, q4, lane);
+            if (!in) {
+                st[x] = make_float2(-1e30f, 0.f);
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) v[x][q4] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+        }
+        const float m0 = fmaxf(m, fmaxf(st[0].x, st[1].x)), a0 = fast_exp2(m - m0);
+        const float a[2] = {fast_exp2(st[0].x - m0), fast_exp2(st[1].x - m0)};
+        l = __builtin_fmaf(st[1].y, a[1], __builtin_fmaf(st[0].y, a[0], l * a0));
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[q4][e] = __builtin_fmaf(v[q4][e], a1, acc[q4][e] * a0);
+            for (int e = 0; e < 4; ++e)
+                acc[q4][e] = __builtin_fmaf(v[1][q4][e], a[1], __builtin_fmaf(v[0][q4][e], a[0], acc[q4][e] * a0));
         m = m0;
     }
 #pragma unroll
-    for (int e = 0; e < 16; ++e) sums[w][e][lane] = acc[e >> 2][e & 3];
-    if (hi == 0) {
+    for (int e = 0; e < 16; ++e) sums[block][w][e][lane] = acc[e >> 2][e & 3];
+    if (block == 0 && hi == 0) {
         stat[w][0][l32] = m;
         stat[w][1][l32] = l;
     }
     __syncthreads();
-    // each thread 4 columns of a row: 8 threads a row
-    const int r = threadIdx.x >> 3, c4 = threadIdx.x & 7;
-    const PagedRow row(p, first_row + r, u / p.unit_tiles);
+    const PagedRow row(p, S::ROWS * (u % p.unit_tiles) + r0 + l32, u / p.unit_tiles);
     if (!row.live) return;
-    float mm = stat[0][0][r], l_tot = 0.f;
+    float mm = stat[0][0][l32], l_tot = 0.f, a[G];
 #pragma unroll
-    for (int x = 1; x < 4; ++x) mm = fmaxf(mm, stat[x][0][r]);
-    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int x = 1; x < G; ++x) mm = fmaxf(mm, stat[x][0][l32]);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-        const float a = fast_exp2(stat[x][0][r] - mm);
-        l_tot = __builtin_fmaf(stat[x][1][r], a, l_tot);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(sums[x][4 * (c4 >> 1) + e][32 * (c4 & 1) + r], a, o[e]);
+    for (int x = 0; x < G; ++x) {
+        a[x] = fast_exp2(stat[x][0][l32] - mm);
+        l_tot = __builtin_fmaf(stat[x][1][l32], a[x], l_tot);
     }
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
-    if (n == 0 && c4 == 0 && p.lse) put_row_lse(p, b, row.h, row.i, mm, l_tot);
-    const int col = 32 * n + 4 * c4;
-    if (col >= p.cols) return;
-    T* ob = (T*)p.o + b * p.o_sb + (int64_t)row.i * p.o_ss + row.h * p.o_sh + col;
-    if constexpr (Elem<T>::kF32) {
-        *reinterpret_cast<f32x4*>(ob) = f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-    } else {
-        s16x4 v4;
+    if (n == 0 && w == 0 && hi == 0 && p.lse) put_row_lse(p, b, row.h, row.i, mm, l_tot);
+    T* ob = (T*)p.o + b * p.o_sb + (int64_t)row.i * p.o_ss + row.h * p.o_sh + 32 * n + 4 * hi;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v4[e] = Elem<T>::pack1(o[e] * inv);
-        *reinterpret_cast<s16x4*>(ob) = v4;
+    for (int q = 0; q < 4 / G; ++q) {
+        const int q4 = w * (4 / G) + q;
+        if (32 * n + 8 * q4 + 4 * hi >= p.cols) continue;
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < G; ++x)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(sums[block][x][4 * q4 + e][lane], a[x], o[e]);
+        if constexpr (Elem<T>::kF32) {
+            *reinterpret_cast<f32x4*>(ob + 8 * q4) = f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+        } else {
+            s16x4 v4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v4[e] = Elem<T>::pack1(o[e] * inv);
+            *reinterpret_cast<s16x4*>(ob + 8 * q4) = v4;
+        }
     }
 }
 
@@ -1105,8 +1153,9 @@ hipError_t launch_paged_t(const PagedParams& p, hipStream_t s) {
             hipLaunchKernelGGL((paged_kernel<T, D, F32, false, NW>), grid, block, 0, s, p);
     }
     if (p.part) {
-        const dim3 tiles((unsigned)(p.Hkv * p.unit_tiles * NW), D / 32, (unsigned)p.B);
-        hipLaunchKernelGGL((paged_join_kernel<T, D, NW>), tiles, dim3(256), 0, s, p);
+        using J = JoinShape<D, NW>;
+        const dim3 tiles((unsigned)(p.Hkv * p.unit_tiles * NW), D / 32 / J::BLOCKS, (unsigned)p.B);
+        hipLaunchKernelGGL((paged_join_kernel<T, D, NW>), tiles, dim3(64 * J::G * J::BLOCKS), 0, s, p);
     }
     return hipGetLastError();
 }

@@ -84,17 +84,39 @@ void plan(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared
     const fa_page_pool& c = a->pool;
     const bool f32 = c.dtype == FA_DTYPE_F32;
     const int64_t rows = (int64_t)a->seqlen_q * (a->num_heads / c.num_heads_kv);
-    p.wide = f32 || rows <= 32 ? 1 : rows <= 128 ? 4 : 8;
+    // Waves that share tiles read K and V once for 128 or 256 rows, but leave larger parts and
+    // fewer units: worth it where a workgroup gets enough steps of units that are full enough.
+    // us of trees of N on 32 and 8 heads of 128, units of 32, 128 and 256 rows (sequences of up
+    // to, N): 16 x 8192, 64: 271, 180, 160; 24 x 4096, 64: 190, 142, 130; 16 x 4000, 64: 152, 134,
+    // 140; 2 x 16000, 48: 94, 74, 83; 16 x 8192, 16: 114, 100, 132; the other way 8 x 1000, 48: 35,
+    // 41, 45; 16 x 4000, 12: 70, 79, 136; 1 x 1000, 64: 22, 32, 37
+    auto busy = [&](int64_t unit, int64_t keys, int64_t workgroups) {
+        const int64_t tiles = ceil_div<int64_t>(rows, unit);
+        return (double)c.batch * c.num_heads_kv * ceil_div<int64_t>(p.Sk, keys) * tiles / workgroups;
+    };
+    auto full = [&](int64_t unit) { return (double)rows / (double)(unit * ceil_div<int64_t>(rows, unit)); };
+    p.wide = f32 || rows <= 32 || busy(32, 128, 512) * full(128) < 10 ? 1 : rows <= 128 || busy(256, 64, 256) * full(256) < 40 ? 4 : 8;
     const int step = p.wide == 1 ? 128 : 64;
     p.unit_tiles = (int)ceil_div<int64_t>(rows, unit_rows(p));
     p.slots = (f32 && compiled_dim(c.head_dim) == 128) || p.wide == 8 ? 256 : 512;  // workgroups that run at once
-    p.least = f32 ? 1 : 4;
     const int64_t units = (int64_t)c.batch * c.num_heads_kv * p.unit_tiles;
     const int64_t most = std::max<int64_t>(1, ceil_div<int64_t>(p.Sk, step));  // steps of a unit
-    // workgroups that may share units (PagedWork): none where no unit is longer than the
-    // least share or, with every sequence full, than an even one
-    const int64_t w = std::min<int64_t>(p.slots, ceil_div<int64_t>(units * most, p.least));
-    shared = most > p.least && (c.key_lengths || most > ceil_div<int64_t>(units * most, w)) ? w : 0;
+    // Where no sequence has room for more than 4 steps, units are not shared: the join would
+    // cost more than it saves (one token of 8 heads over 512 keys 8.4 us, with a join 11.0).
+    // Where it is launched, all of more than `alone` steps are, down to `least` a workgroup.  us
+    // with units of 4 steps whole / shared: trees of 12 over up to 1000 21.7 / 16.3; least of 1, 2
+    // and 4: of 24 over up to 4000 21.0, 18.5, 20.6; one token over 8192 16.2, 15.3, 16.6.
+    // float32, whose steps take longer, from the second step on.
+    const int join_from = f32 ? 1 : 4;
+    p.alone = p.wide == 1 && most > join_from ? 1 : 4;
+    p.least = f32 || (p.wide == 1 && most <= 16) ? 1 : p.wide == 1 ? 2 : 4;
+    // a wide unit's tree, rows and parts take about as long as 3 of its steps: 16 x 8192, trees of
+    // 64: 166 us without, 158 with them in the balance
+    p.extra = p.wide == 1 ? 0 : 3;
+    // workgroups that may share units (PagedWork): none where no unit is that long or, with
+    // every sequence full, longer than an even share
+    const int64_t T = units * (most + p.extra), w = std::min<int64_t>(p.slots, ceil_div<int64_t>(T, p.least));
+    shared = most > join_from && (c.key_lengths || most > ceil_div<int64_t>(T, w)) ? w : 0;
     grid = std::max(units, shared);
 }
 size_t part_rows(const PagedParams& p, int64_t shared) { return (size_t)(2 * shared * unit_rows(p)); }
