@@ -159,6 +159,11 @@ struct CacheAcceptParams : PoolParams {
     int* new_lens;
 };
 hipError_t launch_cache_accept(const CacheAcceptParams& p, hipStream_t s);
+// what a sequence of the new batch takes of its source
+struct ForkPlan {
+    int src, len, kept, part;  // len below 0: dropped; kept: pages; part: rows of a partly filled page
+    int page, copy, need, first;  // its number; whether it goes to a new page; new ones, from `first` of the free on
+};
 struct CacheForkParams : PoolParams {
     const int* sources;
     const int* more;
@@ -166,13 +171,14 @@ struct CacheForkParams : PoolParams {
     int* new_table;
     int* new_lens;
     int* free_list;        // workspace: pages to give
+    int* heirs;            // workspace, per source
+    ForkPlan* plan;        // workspace, per new sequence
     int4* copies;          // workspace: per new sequence (page from, page to, rows)
 };
 hipError_t launch_cache_fork(const CacheForkParams& p, hipStream_t s);
 struct CacheCompactParams : PoolParams {
     int* new_table;
     int* used;
-    int* to;               // workspace: new number of each page
     int2* moves;           // workspace: (from, to)
     int* n_moves;
 };

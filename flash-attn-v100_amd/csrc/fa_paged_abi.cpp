@@ -222,7 +222,7 @@ int32_t fa_cache_write_check(const fa_cache_write_args* a) {
     int32_t st = check_pool(c, false);
     if (st) return st;
     if (a->tokens < 0) return FA_ERR_SHAPE;
-    if ((int64_t)c.batch * a->tokens >= (1LL << 31)) return FA_ERR_TOO_LARGE;
+    if ((int64_t)c.batch * a->tokens >= (1LL << 30)) return FA_ERR_TOO_LARGE;
     if (c.batch == 0 || a->tokens == 0 || empty_pool(c)) return FA_OK;
     const int es = elem_size(c.dtype);
     if ((st = check_tensor(a->k, a->k_stride, 5, a->tokens, c.head_dim, es)) ||
@@ -298,7 +298,8 @@ int32_t fa_cache_fork_check(const fa_cache_fork_args* a) {
 
 size_t fa_cache_fork_workspace_size(const fa_cache_fork_args* a) {
     if (fa_cache_fork_check(a) || a->new_batch == 0) return 0;
-    return up256((size_t)a->new_batch * sizeof(int4)) + up256(((size_t)a->pool.pages + a->pool.batch) * 4);
+    return up256((size_t)a->new_batch * sizeof(int4)) + up256((size_t)a->new_batch * sizeof(fa::ForkPlan)) +
+           up256(((size_t)a->pool.pages + a->pool.batch) * 4);
 }
 
 int32_t fa_cache_fork(const fa_cache_fork_args* a, void* workspace, size_t bytes, void* stream) {
@@ -315,8 +316,13 @@ int32_t fa_cache_fork(const fa_cache_fork_args* a, void* workspace, size_t bytes
     p.n_new = a->new_batch;
     p.new_table = a->new_table;
     p.new_lens = a->new_lengths;
-    p.copies = (int4*)workspace;
-    p.free_list = (int*)((char*)workspace + up256((size_t)a->new_batch * sizeof(int4)));
+    char* ws = (char*)workspace;
+    p.copies = (int4*)ws;
+    ws += up256((size_t)a->new_batch * sizeof(int4));
+    p.plan = (fa::ForkPlan*)ws;
+    ws += up256((size_t)a->new_batch * sizeof(fa::ForkPlan));
+    p.free_list = (int*)ws;
+    p.heirs = p.free_list + a->pool.pages;
     return fa::launch_cache_fork(p, (hipStream_t)stream) == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
@@ -336,7 +342,7 @@ int32_t fa_cache_compact_check(const fa_cache_compact_args* a) {
 
 size_t fa_cache_compact_workspace_size(const fa_cache_compact_args* a) {
     if (fa_cache_compact_check(a)) return 0;
-    return up256((size_t)a->pool.pages * sizeof(int2)) + up256((size_t)a->pool.pages * 4) + 256;
+    return up256((size_t)a->pool.pages * sizeof(int2)) + 256;
 }
 
 int32_t fa_cache_compact(const fa_cache_compact_args* a, void* workspace, size_t bytes, void* stream) {
@@ -351,7 +357,6 @@ int32_t fa_cache_compact(const fa_cache_compact_args* a, void* workspace, size_t
     char* ws = (char*)workspace;
     p.n_moves = (int*)ws;
     p.moves = (int2*)(ws + 256);
-    p.to = (int*)(ws + 256 + up256((size_t)a->pool.pages * sizeof(int2)));
     return fa::launch_cache_compact(p, (hipStream_t)stream) == hipSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 

@@ -30,11 +30,12 @@ __device__ FA_INLINE inline Place place_of(const PoolParams& p, int b, int x) {
 __device__ FA_INLINE inline char* row_at(const PoolParams& p, int kv, int layer, Place at) {
     return p.x[kv] + layer * p.sl[kv] + at.page * p.sp[kv] + at.row * p.sr[kv];
 }
-// chunk c of a row, of the pool and of a tensor with head stride sh (bytes)
-struct Chunk {
-    int head, col;
-    __device__ FA_INLINE inline Chunk(const PoolParams& p, int c) : head(c / p.chunks), col(16 * (c - c / p.chunks * p.chunks)) {}
-};
+// byte offset of chunk c of a row whose heads lie sh bytes apart
+__device__ FA_INLINE inline int64_t chunk_at(const PoolParams& p, int64_t sh, int c) {
+    if (sh == 16 * p.chunks) return 16 * c;  // (heads in a row: no division)
+    const int head = c / p.chunks;
+    return head * sh + 16 * (c - head * p.chunks);
+}
 
 // ---------------------------------------------------------------------------
 // R rows a wave, whose loads are in flight together
@@ -42,7 +43,7 @@ template <int R>
 __global__ __launch_bounds__(256) void cache_write_kernel(const CacheWriteParams p) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kv = blockIdx.y & 1, layer = blockIdx.y >> 1;
-    const int64_t r0 = ((int64_t)blockIdx.x * 4 + w) * R, rows = (int64_t)p.B * p.N;
+    const int r0 = (blockIdx.x * 4 + w) * R, rows = p.B * p.N;  // below 2^31
     const char* from[R];
     char* to[R];
 #pragma unroll
@@ -50,7 +51,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheWriteParams
         from[r] = nullptr;
         to[r] = nullptr;
         if (r0 + r >= rows) continue;
-        const int b = (int)((r0 + r) / p.N), i = (int)((r0 + r) % p.N);
+        const int b = (r0 + r) / p.N, i = (r0 + r) - b * p.N;
         const int x = __builtin_amdgcn_readfirstlane(filled(p, b)) - p.N + i;
         if (x < 0) continue;
         const Place at = place_of(p, b, x);
@@ -61,94 +62,97 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheWriteParams
     const int n = p.heads * p.chunks;
     for (int c0 = 0; c0 < n; c0 += 64) {
         if (c0 + lane >= n) break;
-        const Chunk c(p, c0 + lane);
+        const int64_t in = chunk_at(p, p.in_sh[kv], c0 + lane), out = chunk_at(p, p.sh[kv], c0 + lane);
         chunk_t v[R];
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            if (to[r]) v[r] = *reinterpret_cast<const chunk_t*>(from[r] + c.head * p.in_sh[kv] + c.col);
+            if (to[r]) v[r] = *reinterpret_cast<const chunk_t*>(from[r] + in);
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            if (to[r]) *reinterpret_cast<chunk_t*>(to[r] + c.head * p.sh[kv] + c.col) = v[r];
+            if (to[r]) *reinterpret_cast<chunk_t*>(to[r] + out) = v[r];
     }
 }
 
 // ---------------------------------------------------------------------------
 // A wave takes 64 chunks of all rows of one path.  Its entries ascend, so that row j
 // takes from row j or one behind it: rows are read in groups of 8, before any of them is
-// written, and nothing that is still to be read has been written before.
+// written, and nothing that is still to be read has been written before.  Lane j looks up
+// the places of entry j: read one after the other, they took 8 of the 15 us of 64 paths of
+// up to 9 in 8 layers.
 __global__ __launch_bounds__(256) void cache_accept_kernel(const CacheAcceptParams p) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = p.heads * p.chunks, blocks = (n + 63) / 64;
-    const int64_t item = (int64_t)blockIdx.x * 4 + w;
-    const int per_seq = 2 * p.layers * blocks;
-    const int b = (int)(item / per_seq), x = (int)(item % per_seq);
+    const int item = blockIdx.x * 4 + w, per_seq = 2 * p.layers * blocks;  // items: below 2^31
+    const int b = item / per_seq, x = item - b * per_seq;
     if (b >= p.B) return;
-    const int kv = x & 1, layer = (x >> 1) / blocks, c0 = 64 * ((x >> 1) % blocks);
-    const int len = __builtin_amdgcn_readfirstlane(filled(p, b)), first = len - p.N;
+    const int kv = x & 1, layer = (x >> 1) / blocks, c0 = 64 * ((x >> 1) - layer * blocks);
     const int* path = p.path + b * p.path_sb;
-    int count = 0;
-    if (first >= 0) {
-        for (int last = -1; count < p.path_cols; count += 64) {
-            const int j = count + lane;
-            const int a = j < p.path_cols ? path[j] : -1;
-            int before = __shfl_up(a, 1);
-            if (lane == 0) before = last;
-            const uint64_t end = __ballot(a <= before || a >= p.N);
-            if (end) {
-                count += (int)__builtin_ctzll(end);
-                break;
-            }
-            last = __builtin_amdgcn_readlane(a, 63);
-        }
-        count = min(count, p.path_cols);
-    }
-    if (x == 0 && lane == 0) p.new_lens[b] = first >= 0 ? first + count : len;
+    int a = lane < p.path_cols ? path[lane] : -1;
+    const int len = __builtin_amdgcn_readfirstlane(filled(p, b)), first = len - p.N;
     const bool mine = c0 + lane < n;
-    const Chunk c(p, mine ? c0 + lane : 0);
-    const int64_t off = c.head * p.sh[kv] + c.col;
-    for (int j0 = 0; j0 < count; j0 += 8) {
-        chunk_t v[8];
-        char* to[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            to[u] = nullptr;
-            const int j = j0 + u;
-            if (j >= count) continue;
-            const int a = __builtin_amdgcn_readfirstlane(path[j]);
-            if (a == j) continue;
-            const Place src = place_of(p, b, first + a), dst = place_of(p, b, first + j);
-            if (src.page < 0 || dst.page < 0) continue;
-            to[u] = row_at(p, kv, layer, dst);
-            if (mine) v[u] = *reinterpret_cast<const chunk_t*>(row_at(p, kv, layer, src) + off);
+    char* const rows = row_at(p, kv, layer, Place{0, 0}) + (mine ? chunk_at(p, p.sh[kv], c0 + lane) : 0);
+    int count = 0;
+    for (int j0 = 0, last = -1; first >= 0 && j0 < p.path_cols; j0 += 64) {
+        if (j0) a = j0 + lane < p.path_cols ? path[j0 + lane] : -1;
+        int before = __shfl_up(a, 1);
+        if (lane == 0) before = last;
+        const uint64_t end = __ballot(a <= before || a >= p.N);
+        const int m = end ? (int)__builtin_ctzll(end) : 64;
+        int64_t from = -1, to = -1;
+        if (lane < m && a != j0 + lane) {
+            const Place src = place_of(p, b, first + a), dst = place_of(p, b, first + j0 + lane);
+            if (src.page >= 0 && dst.page >= 0) {
+                from = src.page * p.sp[kv] + src.row * p.sr[kv];
+                to = dst.page * p.sp[kv] + dst.row * p.sr[kv];
+            }
         }
+        for (int g = 0; g < m; g += 8) {
+            chunk_t v[8];
+            int64_t at[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-            if (to[u] && mine) *reinterpret_cast<chunk_t*>(to[u] + off) = v[u];
+            for (int u = 0; u < 8; ++u) {
+                const int64_t src = __shfl(from, g + u);
+                at[u] = __shfl(to, g + u);
+                if (src >= 0 && mine) v[u] = *reinterpret_cast<const chunk_t*>(rows + src);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (at[u] >= 0 && mine) *reinterpret_cast<chunk_t*>(rows + at[u]) = v[u];
+        }
+        count = j0 + m;
+        if (end) break;
+        last = __builtin_amdgcn_readlane(a, 63);
     }
+    if (x == 0 && lane == 0) p.new_lens[b] = first >= 0 ? first + min(count, p.path_cols) : len;
 }
 
 // ---------------------------------------------------------------------------
-// Pages in use as bits in LDS, by one workgroup: 16 KB for up to 2^17 pages, 128 KB for
-// up to 2^20.
+// Pages in use as bits in LDS, by one workgroup: 16 KB for up to 2^17 pages (and there what
+// is known of up to 1024 sequences), 128 KB for up to 2^20.  Bound by the round trips to
+// memory, one after the other.
 constexpr int kPlan = 1024;  // threads
+constexpr int kSmallWords = 1 << 12, kLargeWords = 1 << 15;
 
 // sum of x over the workgroup's threads before this one, and the total
-__device__ FA_INLINE inline int scan(int x, int* sums, int& total) {
+template <typename I>
+__device__ FA_INLINE inline I scan(I x, I* sums, I& total) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int inc = x;
+    I inc = x;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(inc, d);
+        const I y = __shfl_up(inc, d);
         if (lane >= d) inc += y;
     }
     __syncthreads();  // (the sums of a call before this one have been read)
     if (lane == 63) sums[w] = inc;
     __syncthreads();
-    int before = 0;
+    I before = 0;
     total = 0;
+#pragma unroll
     for (int i = 0; i < kPlan / 64; ++i) {
-        if (i < w) before += sums[i];
-        total += sums[i];
+        const I y = sums[i];
+        if (i < w) before += y;
+        total += y;
     }
     return before + inc - x;
 }
@@ -157,56 +161,68 @@ __device__ FA_INLINE inline void mark(const PoolParams& p, unsigned* bits, int p
     if ((unsigned)page < (unsigned)p.pages) atomicOr(&bits[page >> 5], 1u << (page & 31));
 }
 
-// what sequence b of the new batch has of its source
-struct Forked {
-    int src, len, part, kept, need;  // part: rows of a partly filled page; kept: pages; need: new ones
-    bool drop, copy;                 // no room in the table; the part goes to a new page
-    __device__ FA_INLINE inline Forked(const CacheForkParams& p, const int* heirs, int b) {
-        src = p.sources[b];
-        len = part = kept = need = 0;
-        drop = copy = false;
-        if ((unsigned)src >= (unsigned)p.B) {
-            src = -1;
-            return;
-        }
-        const int n = filled(p, src), full = n / p.page_size;
-        const int64_t all = (int64_t)n + max(0, p.more ? p.more[b] : p.more_all);
-        drop = all > p.room;
-        if (drop) return;
-        len = (int)all;
-        part = n - full * p.page_size;
-        kept = full;
-        if (part) {
-            const int page = p.table[src * p.table_sb + full];
-            copy = heirs[src] != b && (unsigned)page < (unsigned)p.pages;
-            if (!copy) ++kept;
-        }
-        need = (len + p.page_size - 1) / p.page_size - kept;
-    }
-};
-
-// p.copies doubles as the place of (first new page, 1 where dropped) between the passes
 template <int WORDS>
 __global__ __launch_bounds__(kPlan) void fork_plan_kernel(const CacheForkParams p) {
+    constexpr bool SMALL = WORDS == kSmallWords;
+    constexpr int NEAR = SMALL ? 1024 : 1, LIST = SMALL ? 4096 : 1;
     __shared__ unsigned bits[WORDS];
-    __shared__ int sums[kPlan / 64];
+    __shared__ int sums[kPlan / 64], near_heirs[NEAR], near_list[LIST];
+    __shared__ ForkPlan near_plan[NEAR];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    int* heirs = p.free_list + p.pages;  // per source the first that continues it
+    // per source the first that continues it; per sequence what it takes; pages to give
+    int* const heirs = SMALL && p.B <= NEAR ? near_heirs : p.heirs;
+    ForkPlan* const plan = SMALL && p.n_new <= NEAR ? near_plan : p.plan;
+    int* const list = SMALL && p.pages <= LIST ? near_list : p.free_list;
     for (int i = tid; i < (p.pages + 31) / 32; i += kPlan) bits[i] = 0u;
     for (int i = tid; i < p.B; i += kPlan) heirs[i] = INT_MAX;
     __threadfence_block();
     __syncthreads();
-    for (int i = tid; i < p.n_new; i += kPlan) {
-        const int s = p.sources[i];
-        if ((unsigned)s >= (unsigned)p.B) continue;
-        // one without room for its new tokens does not keep the partly filled page
-        if ((int64_t)filled(p, s) + max(0, p.more ? p.more[i] : p.more_all) <= p.room) atomicMin(&heirs[s], i);
+    for (int b = tid; b < p.n_new; b += kPlan) {
+        ForkPlan f = {};
+        f.src = p.sources[b];
+        f.len = -1;  // dropped, or no source
+        if ((unsigned)f.src < (unsigned)p.B) {
+            const int n = filled(p, f.src);
+            const int64_t all = (int64_t)n + max(0, p.more ? p.more[b] : p.more_all);
+            if (all <= p.room) {
+                f.len = (int)all;
+                f.kept = n / p.page_size;
+                f.part = n - f.kept * p.page_size;
+                // the page that the part is in (one that is none stays with all)
+                f.page = f.part ? p.table[f.src * p.table_sb + f.kept] : -1;
+                atomicMin(&heirs[f.src], b);
+            }
+        }
+        plan[b] = f;
+    }
+    __threadfence_block();
+    __syncthreads();
+    // what each needs, in the batch's order: counts that no pool holds stay beyond it
+    int wanted = 0;
+    for (int b0 = 0; b0 < p.n_new; b0 += kPlan) {
+        const int b = b0 + tid;
+        int total;
+        ForkPlan f = {};
+        if (b < p.n_new) {
+            f = plan[b];
+            if (f.len >= 0) {
+                f.copy = f.part && (unsigned)f.page < (unsigned)p.pages &&
+                         __hip_atomic_load(&heirs[f.src], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != b;
+                if (f.part && !f.copy) ++f.kept;
+                f.need = (f.len + p.page_size - 1) / p.page_size - f.kept;
+            }
+        }
+        const int before = scan(min(f.need, p.pages + 1), sums, total);
+        f.first = wanted + before;
+        if (b < p.n_new) plan[b] = f;
+        wanted = (int)min((int64_t)p.pages + 1, (int64_t)wanted + total);
     }
     __threadfence_block();
     __syncthreads();
     // pages that the new batch shares or keeps
     for (int b = w; b < p.n_new; b += kPlan / 64) {
-        const Forked f(p, heirs, b);
+        const ForkPlan f = plan[b];
+        if (f.len < 0) continue;
         for (int m = lane; m < f.kept; m += 64) mark(p, bits, p.table[f.src * p.table_sb + m]);
     }
     __syncthreads();
@@ -219,39 +235,23 @@ __global__ __launch_bounds__(kPlan) void fork_plan_kernel(const CacheForkParams 
     int mine = 0, have;
     for (int i = i0; i < i1; ++i) mine += __popc(free_bits(i));
     int rank = scan(mine, sums, have);
-    // what each sequence needs, in the batch's order
-    int wanted = 0;
-    for (int b0 = 0; b0 < p.n_new; b0 += kPlan) {
-        const int b = b0 + tid;
-        int need = 0, total;
-        if (b < p.n_new) need = Forked(p, heirs, b).need;
-        // (sums of parts of a batch stay below 2^31: 1024 sequences of up to 2^20 pages that exist)
-        const int before = scan(min(need, p.pages + 1), sums, total);
-        if (b < p.n_new) {
-            const bool out = need > 0 && (int64_t)wanted + before + need > have;
-            p.copies[b] = make_int4(wanted + before, out ? 1 : 0, 0, 0);
-        }
-        wanted = (int)min((int64_t)p.pages + 1, (int64_t)wanted + total);
-    }
     for (int i = i0; i < i1 && rank < wanted; ++i)
-        for (unsigned x = free_bits(i); x; x &= x - 1) p.free_list[rank++] = 32 * i + __ffs(x) - 1;
+        for (unsigned x = free_bits(i); x; x &= x - 1) list[rank++] = 32 * i + __ffs(x) - 1;
     __threadfence_block();
     __syncthreads();
     for (int b = w; b < p.n_new; b += kPlan / 64) {
-        const Forked f(p, heirs, b);
-        const int4 plan = p.copies[b];
-        const bool gone = f.src < 0 || f.drop || plan.y;
+        const ForkPlan f = plan[b];
+        const bool gone = f.len < 0 || (f.need > 0 && (int64_t)f.first + f.need > have);
         const int pages = gone ? 0 : f.kept + f.need;
         int* row = p.new_table + (int64_t)b * p.cols;
         for (int m = lane; m < p.cols; m += 64) {
             int page = -1;
-            if (m < pages) page = m < f.kept ? p.table[f.src * p.table_sb + m] : p.free_list[plan.x + m - f.kept];
+            if (m < pages) page = m < f.kept ? p.table[f.src * p.table_sb + m] : list[f.first + m - f.kept];
             row[m] = (unsigned)page < (unsigned)p.pages ? page : -1;
         }
         if (lane == 0) {
             p.new_lens[b] = gone ? 0 : f.len;
-            p.copies[b] = !gone && f.copy ? make_int4(p.table[f.src * p.table_sb + f.kept], p.free_list[plan.x], f.part, 0)
-                                          : make_int4(-1, -1, 0, 0);
+            p.copies[b] = !gone && f.copy ? make_int4(f.page, list[f.first], f.part, 0) : make_int4(-1, -1, 0, 0);
         }
     }
 }
@@ -261,6 +261,7 @@ __device__ FA_INLINE inline void copy_rows(const PoolParams& p, int kv, int laye
     const char* src = row_at(p, kv, layer, Place{from, 0});
     char* dst = row_at(p, kv, layer, Place{to, 0});
     const int n = p.heads * p.chunks, all = rows * n;
+    const bool flat = p.sh[kv] == 16 * p.chunks && p.sr[kv] == 16 * n;  // (rows in a row: no division)
     for (int x0 = first; x0 < all; x0 += 4 * step) {
         chunk_t v[4];
         int64_t off[4];
@@ -268,9 +269,12 @@ __device__ FA_INLINE inline void copy_rows(const PoolParams& p, int kv, int laye
         for (int u = 0; u < 4; ++u) {
             const int x = x0 + u * step;
             if (x >= all) break;
-            const int r = x / n;
-            const Chunk c(p, x - r * n);
-            off[u] = r * p.sr[kv] + c.head * p.sh[kv] + c.col;
+            if (flat) {
+                off[u] = (int64_t)16 * x;
+            } else {
+                const int r = x / n;
+                off[u] = r * p.sr[kv] + chunk_at(p, p.sh[kv], x - r * n);
+            }
             v[u] = *reinterpret_cast<const chunk_t*>(src + off[u]);
         }
 #pragma unroll
@@ -289,7 +293,8 @@ __global__ __launch_bounds__(256) void fork_copy_kernel(const CacheForkParams p)
 template <int WORDS>
 __global__ __launch_bounds__(kPlan) void compact_plan_kernel(const CacheCompactParams p) {
     __shared__ unsigned bits[WORDS];
-    __shared__ int sums[kPlan / 64];
+    __shared__ int sums[kPlan / 64], live_before[kPlan];
+    __shared__ unsigned long long sums2[kPlan / 64];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int words = (p.pages + 31) / 32;
     for (int i = tid; i < words; i += kPlan) bits[i] = 0u;
@@ -302,16 +307,19 @@ __global__ __launch_bounds__(kPlan) void compact_plan_kernel(const CacheCompactP
     const int per = (words + kPlan - 1) / kPlan, i0 = min(words, tid * per), i1 = min(words, i0 + per);
     int live = 0, used;
     for (int i = i0; i < i1; ++i) live += __popc(bits[i]);
-    const int before = scan(live, sums, used);
+    live_before[tid] = scan(live, sums, used);
     // bits of pages below the number of used ones
     auto low = [&](int i) { return used >= 32 * i + 32 ? ~0u : used <= 32 * i ? 0u : (1u << (used - 32 * i)) - 1u; };
-    int hole = 0, holes;
-    for (int i = i0; i < i1; ++i) hole += __popc(~bits[i] & low(i));
-    int at = scan(hole, sums, holes);
-    // pages in use from `used` on: as many as holes; those before this thread's words
-    int kept = 0, total;
-    for (int i = i0; i < i1; ++i) kept += __popc(bits[i] & low(i));
-    int from = before - scan(kept, sums, total);
+    // free ones and used ones among them: as many are free as are used from there on
+    unsigned hole = 0, kept = 0;
+    for (int i = i0; i < i1; ++i) {
+        hole += __popc(~bits[i] & low(i));
+        kept += __popc(bits[i] & low(i));
+    }
+    unsigned long long totals;
+    const unsigned long long before = scan((unsigned long long)hole << 32 | kept, sums2, totals);
+    const int holes = (int)(totals >> 32), stay = (int)(unsigned)totals;
+    int at = (int)(before >> 32), from = live_before[tid] - (int)(unsigned)before;
     for (int i = i0; i < i1; ++i) {
         for (unsigned x = ~bits[i] & low(i); x; x &= x - 1) p.moves[at++].y = 32 * i + __ffs(x) - 1;
         for (unsigned x = bits[i] & ~low(i); x; x &= x - 1) p.moves[from++].x = 32 * i + __ffs(x) - 1;
@@ -322,16 +330,20 @@ __global__ __launch_bounds__(kPlan) void compact_plan_kernel(const CacheCompactP
     }
     __threadfence_block();
     __syncthreads();
-    for (int k = tid; k < holes; k += kPlan) p.to[p.moves[k].x] = p.moves[k].y;
-    __threadfence_block();
-    __syncthreads();
+    // a page that moves is the k-th used one from there on
+    auto moved = [&](int page) {
+        const int i = page >> 5, t = i / per;
+        int k = live_before[t] - stay + __popc(bits[i] & ((1u << (page & 31)) - 1u));
+        for (int j = t * per; j < i; ++j) k += __popc(bits[j]);
+        return p.moves[k].y;
+    };
     for (int b = w; b < p.B; b += kPlan / 64) {
         const int n = (filled(p, b) + p.page_size - 1) / p.page_size;
         int* row = p.new_table + (int64_t)b * p.cols;
         for (int m = lane; m < p.cols; m += 64) {
             int page = m < n ? p.table[b * p.table_sb + m] : -1;
             if ((unsigned)page >= (unsigned)p.pages) page = -1;
-            row[m] = page >= used ? p.to[page] : page;
+            row[m] = page >= used ? moved(page) : page;
         }
     }
 }
@@ -344,8 +356,6 @@ __global__ __launch_bounds__(256) void compact_copy_kernel(const CacheCompactPar
         copy_rows(p, x & 1, x >> 1, m.x, m.y, p.page_size, threadIdx.x, 256);
     }
 }
-
-constexpr int kSmallWords = 1 << 12, kLargeWords = 1 << 15;
 
 }  // namespace
 

@@ -104,52 +104,101 @@ bool wants_grad(const at::Tensor& t) { return t.requires_grad() && c10::GradMode
 
 // What the Python entry points look at before every call, in one: False sends them to
 // their own checks, which name what is wrong.
-// pool_ok(k, v, table or None, lengths or None, batch or None, written): the batch is
-// that of the table where None
-PyObject* pool_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
-    HANDLE_TH_ERRORS
-    if (n != 6) {
-        PyErr_Format(PyExc_TypeError, "expected 6 arguments, got %zd", n);
-        return nullptr;
-    }
-    for (int i = 0; i < 4; ++i)
-        if (!THPVariable_Check(x[i]) && !(i >= 2 && none(x[i]))) Py_RETURN_FALSE;
-    const at::Tensor &k = THPVariable_Unpack(x[0]), &v = THPVariable_Unpack(x[1]);
-    const bool written = PyObject_IsTrue(x[5]) == 1;
+bool integer(PyObject* o, const at::Tensor& k, int64_t dim) {
+    if (!THPVariable_Check(o)) return false;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    return t.dim() == dim && t.device() == k.device() && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong);
+}
+// a cache and its table and lengths (or None) of `batch` sequences (below 0: of the table's)
+bool cache_ok(PyObject* ok, PyObject* ov, PyObject* table, PyObject* lens, int64_t batch, bool written) {
+    if (!THPVariable_Check(ok) || !THPVariable_Check(ov)) return false;
+    const at::Tensor &k = THPVariable_Unpack(ok), &v = THPVariable_Unpack(ov);
     const int64_t d = k.dim();
     if ((d != 4 && !(written && d == 5)) || !k.is_cuda() || k.sizes() != v.sizes() || v.device() != k.device() ||
         v.scalar_type() != k.scalar_type() || dtype_code(k.scalar_type()) < 0 || dual(k) || dual(v) || wants_grad(k) || wants_grad(v))
-        Py_RETURN_FALSE;
+        return false;
     const int64_t es = k.element_size(), D = k.size(d - 1);
-    if (D <= 0 || D > 128 || D * es % 16 != 0 || k.size(d - 2) <= 0 || (d == 5 && k.size(0) <= 0)) Py_RETURN_FALSE;
+    if (D <= 0 || D > 128 || D * es % 16 != 0 || k.size(d - 2) <= 0 || (d == 5 && k.size(0) <= 0)) return false;
     for (const at::Tensor* t : {&k, &v}) {
-        if ((uintptr_t)t->data_ptr() & 15 || t->stride(d - 1) != 1) Py_RETURN_FALSE;
+        if ((uintptr_t)t->data_ptr() & 15 || t->stride(d - 1) != 1) return false;
         for (int64_t i = 0; i + 1 < d; ++i)
-            if (t->stride(i) < 0 || t->stride(i) * es % 16 != 0) Py_RETURN_FALSE;
-        if (written && !t->is_contiguous()) Py_RETURN_FALSE;
+            if (t->stride(i) < 0 || t->stride(i) * es % 16 != 0) return false;
+        if (written && !t->is_contiguous()) return false;
     }
-    if (written && k.numel() && k.data_ptr() == v.data_ptr()) Py_RETURN_FALSE;
-    int64_t batch = -1;
-    if (!none(x[4])) {
-        batch = PyLong_AsLongLong(x[4]);
-        if (PyErr_Occurred()) return nullptr;
-    }
-    auto integer = [&](const at::Tensor& t) {
-        return t.device() == k.device() && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong);
-    };
-    if (!none(x[2])) {
-        const at::Tensor& t = THPVariable_Unpack(x[2]);
-        if (t.dim() != 2 || !integer(t) || (batch >= 0 && t.size(0) != batch) || k.size(d - 3) % 16 != 0 || k.size(d - 3) == 0)
-            Py_RETURN_FALSE;
-        batch = t.size(0);
+    if (written && k.numel() && k.data_ptr() == v.data_ptr()) return false;
+    if (!none(table)) {
+        if (!integer(table, k, 2) || k.size(d - 3) % 16 != 0 || k.size(d - 3) == 0) return false;
+        const int64_t n = THPVariable_Unpack(table).size(0);
+        if (batch >= 0 && n != batch) return false;
+        batch = n;
     } else if (batch < 0 || k.size(d - 4) != batch) {
-        Py_RETURN_FALSE;
+        return false;
     }
-    if (!none(x[3])) {
-        const at::Tensor& t = THPVariable_Unpack(x[3]);
-        if (t.dim() != 1 || !integer(t) || t.size(0) != batch) Py_RETURN_FALSE;
-    }
-    Py_RETURN_TRUE;
+    return none(lens) || (integer(lens, k, 1) && THPVariable_Unpack(lens).size(0) == batch);
+}
+// new rows or queries (.., batch, tokens, heads, d) beside a cache
+bool rows_ok(PyObject* o, const at::Tensor& k, int64_t dim) {
+    if (!THPVariable_Check(o)) return false;
+    const at::Tensor& t = THPVariable_Unpack(o);
+    return t.dim() == dim && t.device() == k.device() && t.scalar_type() == k.scalar_type() && t.size(dim - 1) == k.size(k.dim() - 1) &&
+           !dual(t) && !wants_grad(t);
+}
+bool check_count(Py_ssize_t n, Py_ssize_t want) {
+    if (n == want) return true;
+    PyErr_Format(PyExc_TypeError, "expected %zd arguments, got %zd", want, n);
+    return false;
+}
+
+// pool_ok(k, v, table or None, lengths or None, batch or None, written)
+PyObject* pool_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!check_count(n, 6)) return nullptr;
+    const int64_t batch = none(x[4]) ? -1 : PyLong_AsLongLong(x[4]);
+    if (PyErr_Occurred()) return nullptr;
+    return PyBool_FromLong(cache_ok(x[0], x[1], x[2], x[3], batch, PyObject_IsTrue(x[5]) == 1));
+    END_HANDLE_TH_ERRORS
+}
+// paged_ok(q, k, v, lengths, table (or None each))
+PyObject* paged_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!check_count(n, 5)) return nullptr;
+    if (!THPVariable_Check(x[0]) || THPVariable_Unpack(x[0]).dim() != 4) Py_RETURN_FALSE;
+    const at::Tensor& q = THPVariable_Unpack(x[0]);
+    if (!cache_ok(x[1], x[2], x[4], x[3], q.size(0), false)) Py_RETURN_FALSE;
+    const at::Tensor& k = THPVariable_Unpack(x[1]);
+    return PyBool_FromLong(rows_ok(x[0], k, 4) && q.size(2) > 0 && q.size(2) % k.size(2) == 0);
+    END_HANDLE_TH_ERRORS
+}
+// write_ok(k_new, v_new, k, v, lengths, table (or None each))
+PyObject* write_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!check_count(n, 6)) return nullptr;
+    if (!THPVariable_Check(x[0]) || !THPVariable_Check(x[2])) Py_RETURN_FALSE;
+    const at::Tensor &kn = THPVariable_Unpack(x[0]), &k = THPVariable_Unpack(x[2]);
+    const int64_t d = kn.dim();
+    if (d != k.dim() || d < 4 || !cache_ok(x[2], x[3], x[5], x[4], kn.size(d - 4), true)) Py_RETURN_FALSE;
+    return PyBool_FromLong(rows_ok(x[0], k, d) && rows_ok(x[1], k, d) && kn.sizes() == THPVariable_Unpack(x[1]).sizes() &&
+                           kn.size(d - 2) == k.size(d - 2) && (d == 4 || kn.size(0) == k.size(0)));
+    END_HANDLE_TH_ERRORS
+}
+// accept_ok(k, v, path, lengths, table (or None each))
+PyObject* accept_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!check_count(n, 5)) return nullptr;
+    if (!THPVariable_Check(x[2]) || THPVariable_Unpack(x[2]).dim() != 2) Py_RETURN_FALSE;
+    return PyBool_FromLong(cache_ok(x[0], x[1], x[4], x[3], THPVariable_Unpack(x[2]).size(0), true) &&
+                           integer(x[2], THPVariable_Unpack(x[0]), 2));
+    END_HANDLE_TH_ERRORS
+}
+// fork_ok(k, v, table, sources, lengths or None, new tokens): an int is for the caller to look at
+PyObject* fork_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!check_count(n, 6)) return nullptr;
+    if (none(x[2]) || !cache_ok(x[0], x[1], x[2], x[4], -1, true)) Py_RETURN_FALSE;
+    const at::Tensor& k = THPVariable_Unpack(x[0]);
+    if (!integer(x[3], k, 1)) Py_RETURN_FALSE;
+    return PyBool_FromLong(!THPVariable_Check(x[5]) ||
+                           (integer(x[5], k, 1) && THPVariable_Unpack(x[5]).size(0) == THPVariable_Unpack(x[3]).size(0)));
     END_HANDLE_TH_ERRORS
 }
 
@@ -372,6 +421,10 @@ PyObject* bind_paged(PyObject*, PyObject* const* x, Py_ssize_t n) {
 PyMethodDef fa_host::paged_methods[] = {
     {"bind_paged", (PyCFunction)(void*)bind_paged, METH_FASTCALL, nullptr},
     {"pool_ok", (PyCFunction)(void*)pool_ok, METH_FASTCALL, nullptr},
+    {"paged_ok", (PyCFunction)(void*)paged_ok, METH_FASTCALL, nullptr},
+    {"write_ok", (PyCFunction)(void*)write_ok, METH_FASTCALL, nullptr},
+    {"accept_ok", (PyCFunction)(void*)accept_ok, METH_FASTCALL, nullptr},
+    {"fork_ok", (PyCFunction)(void*)fork_ok, METH_FASTCALL, nullptr},
     {"paged_fwd", (PyCFunction)(void*)paged_fwd, METH_FASTCALL, nullptr},
     {"cache_write", (PyCFunction)(void*)cache_write, METH_FASTCALL, nullptr},
     {"cache_accept", (PyCFunction)(void*)cache_accept, METH_FASTCALL, nullptr},

@@ -25,6 +25,26 @@ from ..utils import check_tensor_nan_inf
 from .scored import check_scale, check_slopes, check_softcap
 
 
+WHAT = "flash_attention_v100_paged"
+
+
+def _check_inputs(q, k_cache, v_cache, key_lengths, page_table) -> None:
+    """Raises for what the attention does not take."""
+    if not isinstance(q, torch.Tensor):
+        raise TypeError("q must be a torch.Tensor")
+    if q.dim() != 4:
+        raise ValueError("q must be 4-dimensional [batch, tokens, num_heads, head_dim]")
+    _paged.check_cache(WHAT, k_cache, v_cache, page_table, key_lengths, q.shape[0], False)
+    if q.dtype != k_cache.dtype or q.device != k_cache.device or k_cache.shape[3] != q.shape[3]:
+        raise ValueError(f"q {tuple(q.shape)} {q.dtype} does not match k_cache {tuple(k_cache.shape)} {k_cache.dtype}, or "
+                         "its device")
+    if q.shape[2] == 0 or q.shape[2] % k_cache.shape[2]:
+        raise ValueError(f"num_heads {q.shape[2]} must be a positive multiple of num_heads_kv {k_cache.shape[2]}")
+    _ops.check_dual(WHAT, q)
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise NotImplementedError(f"{WHAT} has no backward: call it under torch.no_grad()")
+
+
 def flash_attention_v100_paged(
     q: torch.Tensor,
     k_cache: torch.Tensor,
@@ -64,19 +84,9 @@ def flash_attention_v100_paged(
     Inputs that require grad are refused while grad mode is on
     (``NotImplementedError``).
     """
-    what = "flash_attention_v100_paged"
-    if not isinstance(q, torch.Tensor):
-        raise TypeError("q must be a torch.Tensor")
-    if q.dim() != 4:
-        raise ValueError("q must be 4-dimensional [batch, tokens, num_heads, head_dim]")
+    if not _paged.host().paged_ok(q, k_cache, v_cache, key_lengths, page_table):
+        _check_inputs(q, k_cache, v_cache, key_lengths, page_table)
     B, N, H, D = q.shape
-    _paged.check_cache(what, k_cache, v_cache, page_table, key_lengths, B, False)
-    if q.dtype != k_cache.dtype or q.device != k_cache.device or k_cache.shape[3] != D:
-        raise ValueError(f"q {tuple(q.shape)} {q.dtype} does not match k_cache {tuple(k_cache.shape)} {k_cache.dtype}, or "
-                         "its device")
-    if H == 0 or H % k_cache.shape[2]:
-        raise ValueError(f"num_heads {H} must be a positive multiple of num_heads_kv {k_cache.shape[2]}")
-    _ops.check_dual(what, q)
     scale = check_scale(scale, D)
     softcap = check_softcap(softcap, scale)
     slopes = None if distance_slopes is None else check_slopes(distance_slopes, B, H, q.device)
@@ -84,8 +94,8 @@ def flash_attention_v100_paged(
         _paged.check_ints(parents, "parents", ((N,), (B, N)), q.device)
         if N > _paged.MAX_TREE_NODES:
             raise NotImplementedError(f"a tree has at most {_paged.MAX_TREE_NODES} tokens, got {N}")
-    if torch.is_grad_enabled() and (q.requires_grad or (slopes is not None and slopes.requires_grad)):
-        raise NotImplementedError(f"{what} has no backward: call it under torch.no_grad()")
+    if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"{WHAT} has no backward: call it under torch.no_grad()")
     o, lse = _paged.paged_fwd(q, k_cache, v_cache, key_lengths, page_table, parents, slopes, scale, softcap,
                               return_softmax_lse)
     if DebugConfig.VALIDATE_OUTPUTS:

@@ -33,6 +33,13 @@ def paged_cache_write_v100(
     sequence.  Returns (k_cache, v_cache), which are written in place; two sequences
     that share a page must not write the same place of it.
     """
+    if not _paged.host().write_ok(k, v, k_cache, v_cache, key_lengths, page_table):
+        _check_write(k, v, k_cache, v_cache, key_lengths, page_table)
+    _paged.cache_write(k, v, k_cache, v_cache, key_lengths, page_table)
+    return k_cache, v_cache
+
+
+def _check_write(k, v, k_cache, v_cache, key_lengths, page_table) -> None:
     what = "paged_cache_write_v100"
     for name, t in (("k", k), ("v", v)):
         if not isinstance(t, torch.Tensor):
@@ -50,8 +57,6 @@ def paged_cache_write_v100(
     _ops.check_dual(what, k, v)
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
         raise NotImplementedError(f"{what} has no backward: call it under torch.no_grad()")
-    _paged.cache_write(k, v, k_cache, v_cache, key_lengths, page_table)
-    return k_cache, v_cache
 
 
 def paged_cache_accept_v100(
@@ -70,6 +75,15 @@ def paged_cache_accept_v100(
     ``drafted`` tokens stays as it is.  The drafted tokens' pages must not be shared
     with another sequence.
     """
+    if not _paged.host().accept_ok(k_cache, v_cache, path, key_lengths, page_table):
+        _check_accept(k_cache, v_cache, key_lengths, path, page_table)
+    drafted = int(drafted)
+    if drafted < 0 or drafted >= 1 << 31:
+        raise ValueError(f"drafted must not be negative, got {drafted}")
+    return _paged.cache_accept(k_cache, v_cache, path, key_lengths, page_table, drafted)
+
+
+def _check_accept(k_cache, v_cache, key_lengths, path, page_table) -> None:
     what = "paged_cache_accept_v100"
     if not isinstance(path, torch.Tensor):
         raise TypeError("path must be a torch.Tensor")
@@ -77,10 +91,6 @@ def paged_cache_accept_v100(
         raise ValueError(f"path must be 2-dimensional [batch, tokens], got shape {tuple(path.shape)}")
     _paged.check_cache(what, k_cache, v_cache, page_table, key_lengths, path.shape[0], True)
     _paged.check_ints(path, "path", (tuple(path.shape),), k_cache.device)
-    drafted = int(drafted)
-    if drafted < 0 or drafted >= 1 << 31:
-        raise ValueError(f"drafted must not be negative, got {drafted}")
-    return _paged.cache_accept(k_cache, v_cache, path, key_lengths, page_table, drafted)
 
 
 def paged_cache_fork_v100(
@@ -107,6 +117,17 @@ def paged_cache_fork_v100(
     page; the old ones are left as they are, and no longer valid once new tokens are
     written.  Pools of at most 2^20 pages (``NotImplementedError`` above).
     """
+    if not _paged.host().fork_ok(k_cache, v_cache, page_table, sources, key_lengths, new_tokens):
+        _check_fork(k_cache, v_cache, page_table, key_lengths, sources, new_tokens)
+    if not isinstance(new_tokens, torch.Tensor):
+        new_tokens = int(new_tokens)
+        if new_tokens < 0 or new_tokens >= 1 << 31:
+            raise ValueError(f"new_tokens must not be negative, got {new_tokens}")
+    _check_pages("paged_cache_fork_v100", k_cache)
+    return _paged.cache_fork(k_cache, v_cache, page_table, sources, key_lengths, new_tokens)
+
+
+def _check_fork(k_cache, v_cache, page_table, key_lengths, sources, new_tokens) -> None:
     what = "paged_cache_fork_v100"
     if page_table is None:
         raise TypeError("page_table must be a torch.Tensor")
@@ -118,12 +139,6 @@ def paged_cache_fork_v100(
     _paged.check_ints(sources, "sources", (tuple(sources.shape),), k_cache.device)
     if isinstance(new_tokens, torch.Tensor):
         _paged.check_ints(new_tokens, "new_tokens", (tuple(sources.shape),), k_cache.device)
-    else:
-        new_tokens = int(new_tokens)
-        if new_tokens < 0 or new_tokens >= 1 << 31:
-            raise ValueError(f"new_tokens must not be negative, got {new_tokens}")
-    _check_pages(what, k_cache)
-    return _paged.cache_fork(k_cache, v_cache, page_table, sources, key_lengths, new_tokens)
 
 
 def paged_cache_compact_v100(
