@@ -161,6 +161,28 @@ __device__ FA_INLINE inline void mark(const PoolParams& p, unsigned* bits, int p
     if ((unsigned)page < (unsigned)p.pages) atomicOr(&bits[page >> 5], 1u << (page & 31));
 }
 
+// f(row, column, page of the table or -1) for every column of every one of `rows` rows, whose
+// first kept(row) columns are read of row source(row): four reads of a thread in flight
+template <typename K, typename S, typename F>
+__device__ FA_INLINE inline void each_column(const PoolParams& p, int rows, K&& kept, S&& source, F&& f) {
+    const int64_t all = (int64_t)rows * p.cols;
+    for (int64_t x0 = threadIdx.x; x0 < all; x0 += 4 * kPlan) {
+        int page[4], row[4], col[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t x = x0 + u * kPlan;
+            row[u] = -1;
+            if (x >= all) continue;
+            row[u] = (int)((unsigned)x / (unsigned)p.cols);  // (rows times columns: below 2^31)
+            col[u] = (int)x - row[u] * p.cols;
+            page[u] = col[u] < kept(row[u]) ? p.table[source(row[u]) * p.table_sb + col[u]] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (row[u] >= 0) f(row[u], col[u], page[u]);
+    }
+}
+
 template <int WORDS>
 __global__ __launch_bounds__(kPlan) void fork_plan_kernel(const CacheForkParams p) {
     constexpr bool SMALL = WORDS == kSmallWords;
@@ -168,7 +190,7 @@ __global__ __launch_bounds__(kPlan) void fork_plan_kernel(const CacheForkParams 
     __shared__ unsigned bits[WORDS];
     __shared__ int sums[kPlan / 64], near_heirs[NEAR], near_list[LIST];
     __shared__ ForkPlan near_plan[NEAR];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int tid = threadIdx.x;
     // per source the first that continues it; per sequence what it takes; pages to give
     int* const heirs = SMALL && p.B <= NEAR ? near_heirs : p.heirs;
     ForkPlan* const plan = SMALL && p.n_new <= NEAR ? near_plan : p.plan;
@@ -220,11 +242,9 @@ __global__ __launch_bounds__(kPlan) void fork_plan_kernel(const CacheForkParams 
     __threadfence_block();
     __syncthreads();
     // pages that the new batch shares or keeps
-    for (int b = w; b < p.n_new; b += kPlan / 64) {
-        const ForkPlan f = plan[b];
-        if (f.len < 0) continue;
-        for (int m = lane; m < f.kept; m += 64) mark(p, bits, p.table[f.src * p.table_sb + m]);
-    }
+    auto kept = [&](int b) { return plan[b].kept; };  // (0 where dropped)
+    auto source = [&](int b) { return (int64_t)plan[b].src; };
+    each_column(p, p.n_new, kept, source, [&](int, int, int page) { mark(p, bits, page); });
     __syncthreads();
     // the free ones, lowest first
     const int words = (p.pages + 31) / 32, per = (words + kPlan - 1) / kPlan, i0 = min(words, tid * per), i1 = min(words, i0 + per);
@@ -239,28 +259,26 @@ __global__ __launch_bounds__(kPlan) void fork_plan_kernel(const CacheForkParams 
         for (unsigned x = free_bits(i); x; x &= x - 1) list[rank++] = 32 * i + __ffs(x) - 1;
     __threadfence_block();
     __syncthreads();
-    for (int b = w; b < p.n_new; b += kPlan / 64) {
+    auto gone = [&](const ForkPlan& f) { return f.len < 0 || (f.need > 0 && (int64_t)f.first + f.need > have); };
+    each_column(p, p.n_new, kept, source, [&](int b, int m, int page) {
         const ForkPlan f = plan[b];
-        const bool gone = f.len < 0 || (f.need > 0 && (int64_t)f.first + f.need > have);
-        const int pages = gone ? 0 : f.kept + f.need;
-        int* row = p.new_table + (int64_t)b * p.cols;
-        for (int m = lane; m < p.cols; m += 64) {
-            int page = -1;
-            if (m < pages) page = m < f.kept ? p.table[f.src * p.table_sb + m] : list[f.first + m - f.kept];
-            row[m] = (unsigned)page < (unsigned)p.pages ? page : -1;
-        }
-        if (lane == 0) {
-            p.new_lens[b] = gone ? 0 : f.len;
-            p.copies[b] = !gone && f.copy ? make_int4(f.page, list[f.first], f.part, 0) : make_int4(-1, -1, 0, 0);
-        }
+        if (m >= f.kept && m < f.kept + f.need) page = gone(f) ? -1 : list[f.first + m - f.kept];
+        if (gone(f) || (unsigned)page >= (unsigned)p.pages) page = -1;
+        p.new_table[(int64_t)b * p.cols + m] = page;
+    });
+    for (int b = tid; b < p.n_new; b += kPlan) {
+        const ForkPlan f = plan[b];
+        p.new_lens[b] = gone(f) ? 0 : f.len;
+        p.copies[b] = !gone(f) && f.copy ? make_int4(f.page, list[f.first], f.part, 0) : make_int4(-1, -1, 0, 0);
     }
 }
 
-// rows [0, rows) of one page to another, one layer's keys or values
-__device__ FA_INLINE inline void copy_rows(const PoolParams& p, int kv, int layer, int from, int to, int rows, int first, int step) {
+// rows [0, rows) of one page to another, one layer's keys or values: chunks `first` and every
+// step-th after it, of `most` from the workgroup's first on
+__device__ FA_INLINE inline void copy_rows(const PoolParams& p, int kv, int layer, int from, int to, int rows, int first, int step, int most) {
     const char* src = row_at(p, kv, layer, Place{from, 0});
     char* dst = row_at(p, kv, layer, Place{to, 0});
-    const int n = p.heads * p.chunks, all = rows * n;
+    const int n = p.heads * p.chunks, all = min(rows * n, first - (int)threadIdx.x + most);
     const bool flat = p.sh[kv] == 16 * p.chunks && p.sr[kv] == 16 * n;  // (rows in a row: no division)
     for (int x0 = first; x0 < all; x0 += 4 * step) {
         chunk_t v[4];
@@ -286,7 +304,8 @@ __device__ FA_INLINE inline void copy_rows(const PoolParams& p, int kv, int laye
 __global__ __launch_bounds__(256) void fork_copy_kernel(const CacheForkParams p) {
     const int4 c = p.copies[blockIdx.x];
     if (c.z == 0) return;
-    copy_rows(p, blockIdx.y & 1, blockIdx.y >> 1, c.x, c.y, c.z, blockIdx.z * 256 + threadIdx.x, 256 * gridDim.z);
+    for (int x = blockIdx.z * 1024; x < c.z * p.heads * p.chunks; x += gridDim.z * 1024)
+        copy_rows(p, blockIdx.y & 1, blockIdx.y >> 1, c.x, c.y, c.z, x + threadIdx.x, 256, 1024);
 }
 
 // ---------------------------------------------------------------------------
@@ -295,14 +314,16 @@ __global__ __launch_bounds__(kPlan) void compact_plan_kernel(const CacheCompactP
     __shared__ unsigned bits[WORDS];
     __shared__ int sums[kPlan / 64], live_before[kPlan];
     __shared__ unsigned long long sums2[kPlan / 64];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    __shared__ int near_kept[kPlan];
+    const int tid = threadIdx.x;
     const int words = (p.pages + 31) / 32;
+    auto pages_of = [&](int b) { return (filled(p, b) + p.page_size - 1) / p.page_size; };
+    if (tid < p.B) near_kept[tid] = pages_of(tid);
     for (int i = tid; i < words; i += kPlan) bits[i] = 0u;
     __syncthreads();
-    for (int b = w; b < p.B; b += kPlan / 64) {
-        const int n = (filled(p, b) + p.page_size - 1) / p.page_size;
-        for (int m = lane; m < n; m += 64) mark(p, bits, p.table[b * p.table_sb + m]);
-    }
+    auto kept_of = [&](int b) { return b < kPlan ? near_kept[b] : pages_of(b); };
+    auto source = [](int b) { return (int64_t)b; };
+    each_column(p, p.B, kept_of, source, [&](int, int, int page) { mark(p, bits, page); });
     __syncthreads();
     const int per = (words + kPlan - 1) / kPlan, i0 = min(words, tid * per), i1 = min(words, i0 + per);
     int live = 0, used;
@@ -337,23 +358,20 @@ __global__ __launch_bounds__(kPlan) void compact_plan_kernel(const CacheCompactP
         for (int j = t * per; j < i; ++j) k += __popc(bits[j]);
         return p.moves[k].y;
     };
-    for (int b = w; b < p.B; b += kPlan / 64) {
-        const int n = (filled(p, b) + p.page_size - 1) / p.page_size;
-        int* row = p.new_table + (int64_t)b * p.cols;
-        for (int m = lane; m < p.cols; m += 64) {
-            int page = m < n ? p.table[b * p.table_sb + m] : -1;
-            if ((unsigned)page >= (unsigned)p.pages) page = -1;
-            row[m] = page >= used ? moved(page) : page;
-        }
-    }
+    each_column(p, p.B, kept_of, source, [&](int b, int m, int page) {
+        if ((unsigned)page >= (unsigned)p.pages) page = -1;
+        p.new_table[(int64_t)b * p.cols + m] = page >= used ? moved(page) : page;
+    });
 }
 
-__global__ __launch_bounds__(256) void compact_copy_kernel(const CacheCompactParams p) {
-    const int64_t items = (int64_t)*p.n_moves * 2 * p.layers;
+// 16 KB of a page at a time
+__global__ __launch_bounds__(256) void compact_copy_kernel(const CacheCompactParams p, const int pieces) {
+    const int per_move = 2 * p.layers * pieces;
+    const int64_t items = (int64_t)*p.n_moves * per_move;
     for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
-        const int x = (int)(i % (2 * p.layers));
-        const int2 m = p.moves[i / (2 * p.layers)];
-        copy_rows(p, x & 1, x >> 1, m.x, m.y, p.page_size, threadIdx.x, 256);
+        const int k = (int)(i / per_move), x = (int)(i - (int64_t)k * per_move), side = x / pieces;
+        const int2 m = p.moves[k];
+        copy_rows(p, side & 1, side >> 1, m.x, m.y, p.page_size, (x - side * pieces) * 1024 + threadIdx.x, 256, 1024);
     }
 }
 
@@ -362,8 +380,10 @@ __global__ __launch_bounds__(256) void compact_copy_kernel(const CacheCompactPar
 hipError_t launch_cache_write(const CacheWriteParams& p, hipStream_t s) {
     const int64_t rows = (int64_t)p.B * p.N;
     const unsigned y = 2 * p.layers;
-    if (rows * y >= 16384)
+    if (rows * y >= 65536)
         hipLaunchKernelGGL((cache_write_kernel<4>), dim3((unsigned)((rows + 15) / 16), y), dim3(256), 0, s, p);
+    else if (rows * y >= 8192)
+        hipLaunchKernelGGL((cache_write_kernel<2>), dim3((unsigned)((rows + 7) / 8), y), dim3(256), 0, s, p);
     else
         hipLaunchKernelGGL((cache_write_kernel<1>), dim3((unsigned)((rows + 3) / 4), y), dim3(256), 0, s, p);
     return hipGetLastError();
@@ -381,7 +401,7 @@ hipError_t launch_cache_fork(const CacheForkParams& p, hipStream_t s) {
     else
         hipLaunchKernelGGL((fork_plan_kernel<kLargeWords>), dim3(1), dim3(kPlan), 0, s, p);
     const int z = (p.page_size * p.heads * p.chunks + 1023) / 1024;
-    hipLaunchKernelGGL(fork_copy_kernel, dim3((unsigned)p.n_new, (unsigned)(2 * p.layers), (unsigned)min(z, 64)), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(fork_copy_kernel, dim3((unsigned)p.n_new, (unsigned)(2 * p.layers), (unsigned)min(z, 1024)), dim3(256), 0, s, p);
     return hipGetLastError();
 }
 
@@ -390,8 +410,9 @@ hipError_t launch_cache_compact(const CacheCompactParams& p, hipStream_t s) {
         hipLaunchKernelGGL((compact_plan_kernel<kSmallWords>), dim3(1), dim3(kPlan), 0, s, p);
     else
         hipLaunchKernelGGL((compact_plan_kernel<kLargeWords>), dim3(1), dim3(kPlan), 0, s, p);
-    const int64_t most = (int64_t)(p.pages / 2) * 2 * p.layers;
-    if (most > 0) hipLaunchKernelGGL(compact_copy_kernel, dim3((unsigned)min(most, (int64_t)2048)), dim3(256), 0, s, p);
+    const int pieces = (p.page_size * p.heads * p.chunks + 1023) / 1024;
+    const int64_t most = (int64_t)(p.pages / 2) * 2 * p.layers * pieces;
+    if (most > 0) hipLaunchKernelGGL(compact_copy_kernel, dim3((unsigned)min(most, (int64_t)8192)), dim3(256), 0, s, p, pieces);
     return hipGetLastError();
 }
 

@@ -38,6 +38,8 @@ import torch.nn as nn
 
 from .interface import flash_attention_performance_mode, flash_attention_v100
 from .ops.attention import gradient_checkpointing_mode
+from .ops.paged import flash_attention_v100_paged
+from .ops.paged_cache import paged_cache_write_v100
 from .ops.rotary import rotary_embedding_v100, rotary_table_v100
 from .ops.scored import flash_attention_v100_scored
 
@@ -272,6 +274,48 @@ class EnhancedMultiHeadAttention(nn.Module):
             ev1.record()
             self._pending.append((ev0, ev1))
         return out, weights
+
+    @torch.no_grad()
+    def decode(self,
+               query: torch.Tensor,
+               k_cache: torch.Tensor,
+               v_cache: torch.Tensor,
+               key_lengths: Optional[torch.Tensor] = None,
+               page_table: Optional[torch.Tensor] = None,
+               parents: Optional[torch.Tensor] = None,
+               positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The layer's output for the newest N tokens of each sequence, (B, N, E) or
+        (N, B, E) as ``batch_first`` says, whose keys and values it writes into the cache
+        (:func:`paged_cache_write_v100`) and then attends over
+        (:func:`flash_attention_v100_paged`): causal, or through the tree of
+        ``parents``.  ``key_lengths`` count the new tokens.  ``positions``: their rotary
+        positions, (B, N) or (N,): their places in the sequence by default, to be given
+        with ``parents`` (a tree's tokens stand at the context's length and their depth).
+        With ``softcap`` and ``distance_bias``; no dropout, no gradients."""
+        if self.training and self.dropout > 0.0:
+            raise ValueError("decode has no attention dropout: call eval() or use dropout=0.0")
+        if not self.batch_first:
+            query = query.transpose(0, 1)
+        B, N, E = query.shape
+        q, k, v = (lin(query).view(B, N, self.num_heads, self.head_dim) for lin in (self.q_proj, self.k_proj, self.v_proj))
+        if self.rotary_dim:
+            if positions is None:
+                if parents is not None:
+                    raise ValueError("a tree's rotary positions must be given")
+                n = key_lengths
+                if n is None:
+                    room = k_cache.shape[-3] * (1 if page_table is None else page_table.shape[1])
+                    n = torch.full((B,), room, dtype=torch.int32, device=q.device)
+                positions = n[:, None] - N + torch.arange(N, dtype=n.dtype, device=q.device)
+            q, k = rotary_embedding_v100(q, k, self._rotary_table(q.device), positions, interleaved=self.rotary_interleaved)
+        elif positions is not None:
+            raise ValueError("positions need rotary_dim > 0")
+        paged_cache_write_v100(k, v, k_cache, v_cache, key_lengths, page_table)
+        slopes = None if self.distance_slopes is None else self.distance_slopes.float()
+        out = flash_attention_v100_paged(q, k_cache, v_cache, key_lengths, page_table, parents=parents,
+                                         softcap=self.softcap, distance_slopes=slopes)
+        out = self.out_proj(out.reshape(B, N, E))
+        return out if self.batch_first else out.transpose(0, 1)
 
     def get_performance_stats(self) -> Optional[Dict[str, Any]]:
         """Forward count and HIP-event times (ms) when monitoring is enabled."""
