@@ -125,10 +125,10 @@ struct PagedParams : RowsParams {
     int64_t k_sp, v_sp;    // page strides
     const int* parents;    // optional (B, Sq), batch stride parents_sb
     int64_t parents_sb;
-    // work: units of rows of one (sequence, KV head), unit_tiles a KV head, over steps of
-    // keys, shared out to at most `slots` workgroups
-    int unit_tiles, slots;
-    int alone, least;      // steps of units that are not shared; those of a workgroup, at least
+    // work (PagedWork): units of rows of one (sequence, KV head), unit_tiles a KV head, over
+    // steps of keys, shared out to at most `groups` workgroups a unit
+    int unit_tiles, groups;
+    int alone, least;      // steps of sequences that are not shared; those of a group, at least
     int extra;             // steps that a unit counts beside its keys'
     int wide;              // waves of a unit of 32 rows each that share its tiles; 1: of 32 rows, whose waves share its keys
 };

@@ -183,14 +183,16 @@ __device__ FA_INLINE inline unsigned tree_word(const TreeBits& t, int i, int s, 
 }
 
 // ---------------------------------------------------------------------------
-// Work.  Steps of all units in one list, by sequence, then unit; every sequence has
-// one at least, and every unit p.extra more that stand for what it costs beside its keys.
-// Where no unit is longer than a workgroup's share, or than p.alone steps, a workgroup takes
-// whole units.
+// Work.  A sequence's units (of every KV head) have the same keys, in steps: one at least,
+// and p.extra more that stand for what a unit costs beside its keys.  The steps of all
+// sequences, one after the other, are shared out evenly to W groups of workgroups, one
+// workgroup of a group for each unit: they walk the same tokens side by side, whose
+// heads lie side by side in memory (and several units of one KV head read its tiles
+// through one L2).  Where no sequence is longer than a group's share, or than p.alone
+// steps, there is a group for each sequence.
 struct PagedWork {
-    int T, W;      // steps, workgroups that have work
-    int per_seq;   // units of a sequence
-    bool whole;    // a workgroup takes whole units
+    int T, W;      // steps, groups
+    bool whole;    // a group for each sequence
     int st0, inc0; // of sequence `lane`: its steps, and those up to its end
     template <int STEP>
     __device__ FA_INLINE inline static int steps(PagedArgs& p, int b) {
@@ -225,64 +227,63 @@ struct PagedWork {
             most = steps<STEP>(p, 0);
             sum = most * p.B;
         }
-        per_seq = p.Hkv * p.unit_tiles;
-        T = __builtin_amdgcn_readfirstlane(sum) * per_seq;
-        W = min(p.slots, (T + p.least - 1) / p.least);
-        whole = __builtin_amdgcn_readfirstlane(most) - p.extra <= max(p.alone, (T + W - 1) / W);
-        if (whole) W = p.B * per_seq;
+        T = __builtin_amdgcn_readfirstlane(sum);
+        W = min(p.groups, (T + p.least - 1) / p.least);
+        whole = W <= 1 || __builtin_amdgcn_readfirstlane(most) - p.extra <= max(p.alone, (T + W - 1) / W);
+        if (whole) W = p.B;
     }
-    // the first step of workgroup g (floor(g T / W)), and whose step x is; in 32 bits where
-    // they suffice
+    // the first step of group g (floor(g T / W)), and whose step x is; in 32 bits where they
+    // suffice
     __device__ FA_INLINE inline int first(int g) const {
         return (int64_t)T * W < INT_MAX ? (int)((unsigned)(g * T) / (unsigned)W) : (int)((int64_t)g * T / W);
     }
     __device__ FA_INLINE inline int whose(int x) const {
         return (int64_t)T * W < INT_MAX ? (int)((unsigned)((x + 1) * W - 1) / (unsigned)T) : (int)((((int64_t)x + 1) * W - 1) / T);
     }
-    // the sequence of step x, its first step and the steps of one of its units
+    // the sequence of step x, its first step and its steps
     template <int STEP>
     __device__ FA_INLINE inline void locate(PagedArgs& p, int x, int lane, int& b, int& start, int& len) const {
         if (!p.lens) {
             len = steps<STEP>(p, 0);
-            b = x / (len * per_seq);
-            start = b * len * per_seq;
+            b = x / len;
+            start = b * len;
             return;
         }
         int before = 0;
         for (int b0 = 0;; b0 += 64) {
             const int st = b0 ? steps<STEP>(p, b0 + lane) : st0, inc = b0 ? scan(st, lane) : inc0;
-            const uint64_t past = __ballot((int64_t)(before + inc) * per_seq > x);
+            const uint64_t past = __ballot(before + inc > x);
             if (past || b0 + 64 >= p.B) {
                 const int l = past ? (int)__builtin_ctzll(past) : 63;
                 b = b0 + l;
                 len = __builtin_amdgcn_readlane(st, l);
-                start = (before + __builtin_amdgcn_readlane(inc, l) - len) * per_seq;
+                start = before + __builtin_amdgcn_readlane(inc, l) - len;
                 return;
             }
             before += __builtin_amdgcn_readlane(inc, 63);
         }
     }
-    // the first step of sequence b and the steps of one of its units
+    // the first step of sequence b, and its steps
     template <int STEP>
     __device__ FA_INLINE inline void sequence(PagedArgs& p, int b, int lane, int& start, int& len) const {
         if (!p.lens) {
             len = steps<STEP>(p, 0);
-            start = b * len * per_seq;
+            start = b * len;
         } else if (b < 64) {
             len = __builtin_amdgcn_readlane(st0, b);
-            start = (__builtin_amdgcn_readlane(inc0, b) - len) * per_seq;
+            start = __builtin_amdgcn_readlane(inc0, b) - len;
         } else {
             int sum = st0;
             for (int b0 = 64; b0 < b; b0 += 64) sum += b0 + lane < b ? steps<STEP>(p, b0 + lane) : 0;
 #pragma unroll
             for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
             len = __builtin_amdgcn_readfirstlane(steps<STEP>(p, b));
-            start = __builtin_amdgcn_readfirstlane(sum) * per_seq;
+            start = __builtin_amdgcn_readfirstlane(sum);
         }
     }
 };
-// parts: a workgroup leaves at most two, of the unit that it begins with (2 g) and of
-// the one that it ends with, begun by it (2 g + 1).  Those of 32 rows lie together, in
+// parts: a workgroup (g) leaves at most two, of the sequence that it begins with (2 g) and
+// of the one that it ends with, begun by it (2 g + 1).  Those of 32 rows lie together, in
 // accumulator order (part_of), so that a store of a wave is 1 KB in a row: as rows, 64
 // places of 16 bytes a store, 256 rows took 8 us.
 template <int ROWS>
@@ -753,7 +754,7 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], Tre
         l_tot = 0.f;
     }
     const bool whole = part < 0;
-    if (!whole && w == 0 && hi == 0) pe.stat[part + l32] = make_float2(mm, l_tot);
+    if (!whole && w == 0 && hi == 0 && row.live) pe.stat[part + l32] = make_float2(mm, l_tot);
     if (whole && w == 0 && hi == 0 && row.live && pe.lse) put_row_lse(pe, b, row.h, row.i, mm, l_tot);
     const float inv = l_tot > 0.f || l_tot != l_tot ? 1.f / l_tot : 0.f;
 #pragma unroll
@@ -768,11 +769,12 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], Tre
             for (int e = 0; e < 16; ++e) om[e] = __builtin_fmaf(px[(16 * n + e) * 64 + lane], a[x], om[e]);
         }
         if (!row.valid) om = f32x16{};
+        if (!row.live) continue;
         if (!whole) {
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
                 *part_of<D>(pe.part, part, n, q4, lane) = f32x4{om[4 * q4], om[4 * q4 + 1], om[4 * q4 + 2], om[4 * q4 + 3]};
-        } else if (row.live) {
+        } else {
             T* ob = (T*)pe.o + b * pe.o_sb + (int64_t)row.i * pe.o_ss + row.h * pe.o_sh + 32 * n + 4 * hi;
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
@@ -953,12 +955,12 @@ __device__ FA_INLINE inline void paged_unit_wide(T* smem, TreeBits* tree, bool n
     }
     barrier_no_fence();  // the slots have been read: they take the rows of O, or the next unit's tiles
     if (part >= 0) {
-        if (hi == 0) pe.stat[part + 32 * w + l32] = make_float2(m_run, l_tot);
+        if (row.live && hi == 0) pe.stat[part + 32 * w + l32] = make_float2(m_run, l_tot);
 #pragma unroll
         for (int n = 0; n < D / 32; ++n)
 #pragma unroll
             for (int q4 = 0; q4 < 4; ++q4)
-                *part_of<D>(pe.part, part + 32 * w, n, q4, lane) =
+                if (row.live) *part_of<D>(pe.part, part + 32 * w, n, q4, lane) =
                     f32x4{o[n][4 * q4], o[n][4 * q4 + 1], o[n][4 * q4 + 2], o[n][4 * q4 + 3]};
     } else {
         if (row.live && hi == 0 && pe.lse) put_row_lse(pe, b, row.h, row.i, m_run, l_tot);
@@ -1003,34 +1005,32 @@ __global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 : Pag
     const int tid = threadIdx.x, lane = tid & 63;
     PagedWork wk;
     wk.init<S::STEP>(p, lane);
-    if ((int)blockIdx.x >= wk.W) return;
-    const int g = xcd_remap((int)blockIdx.x, wk.W);
-    const int extra = p.extra;
+    const int units = p.Hkv * p.unit_tiles, extra = p.extra;
+    if ((int64_t)blockIdx.x >= (int64_t)wk.W * units) return;
+    const int g = xcd_remap((int)blockIdx.x, wk.W * units), group = g / units, u = g - group * units;
+    const int tiles = p.unit_tiles, hk = u / tiles, rt = u - hk * tiles;
     int x = 0, end = 0, b = 0, start = 0, len = 0, last_b = -1;  // len: of a unit, with the extra steps
     if (wk.whole) {
-        b = g / wk.per_seq;
+        b = group;
         len = __builtin_amdgcn_readfirstlane(PagedWork::steps<S::STEP>(p, b));
-        start = 0;
-        x = g % wk.per_seq * len;
-        end = x + len;
+        end = len;
     } else {
-        x = wk.first(g);
-        end = wk.first(g + 1);
+        x = wk.first(group);
+        end = wk.first(group + 1);
     }
     while (x < end) {
-        if (!wk.whole && (last_b < 0 || x >= start + len * wk.per_seq)) wk.locate<S::STEP>(paged_args(), x, lane, b, start, len);
-        const int u = (x - start) / len, s0 = x - start - u * len, n = len - extra, s1 = min(n, s0 + end - x);
-        x = min(end, start + (u + 1) * len);
+        if (!wk.whole) wk.locate<S::STEP>(paged_args(), x, lane, b, start, len);
+        const int s0 = x - start, n = len - extra, s1 = min(n, end - start);
+        x = min(end, start + len);
         if (s0 >= s1) continue;  // (the extra steps of a unit that ended in another workgroup)
         const int64_t part = s1 - s0 == n ? -1 : part_at<S::ROWS>(g, s0 == 0);
-        const int tiles = paged_args().unit_tiles;
         if (n == 1 && filled_tokens(paged_args(), b) == 0) {
-            empty_unit<T, D>(paged_args(), b, u / tiles, u % tiles * S::ROWS, S::ROWS, tid, S::THREADS);
+            empty_unit<T, D>(paged_args(), b, hk, rt * S::ROWS, S::ROWS, tid, S::THREADS);
         } else if constexpr (NW == 1) {
             __shared__ float stat[PagedCfg<T, D>::NW][2][32];
-            paged_unit32<T, D, EXACT>(smem, stat, tree, TREE && b != last_b, b, u / tiles, u % tiles, s0, s1, part, tid);
+            paged_unit32<T, D, EXACT>(smem, stat, tree, TREE && b != last_b, b, hk, rt, s0, s1, part, tid);
         } else {
-            paged_unit_wide<T, D, EXACT, NW>(smem, tree, TREE && b != last_b, b, u / tiles, u % tiles, s0, s1, part, tid);
+            paged_unit_wide<T, D, EXACT, NW>(smem, tree, TREE && b != last_b, b, hk, rt, s0, s1, part, tid);
         }
         last_b = b;
     }
@@ -1061,10 +1061,10 @@ __global__ __launch_bounds__((64 * JoinShape<D, NW>::G * JoinShape<D, NW>::BLOCK
     if (wk.whole) return;
     int start, len;
     wk.sequence<S::STEP>(p, b, lane, start, len);
-    const int u = blockIdx.x / NW, r0 = 32 * (blockIdx.x % NW);
-    const int s = start + u * len;  // the unit's first step
-    const int g0 = wk.whose(s), g1 = wk.whose(s + len - p.extra - 1);
+    const int g0 = wk.whose(start), g1 = wk.whose(start + len - p.extra - 1);
     if (g0 == g1) return;
+    const int units = p.Hkv * p.unit_tiles, u = blockIdx.x / NW, r0 = 32 * (blockIdx.x % NW);
+    const PagedRow row(p, S::ROWS * (u % p.unit_tiles) + r0 + l32, u / p.unit_tiles);
     float m = -1e30f, l = 0.f;
     f32x4 acc[4];
 #pragma unroll
@@ -1076,11 +1076,12 @@ __global__ __launch_bounds__((64 * JoinShape<D, NW>::G * JoinShape<D, NW>::BLOCK
         for (int x = 0; x < 2; ++x) {
             const bool in = g + G * x <= g1;
             const int gx = in ? g + G * x : g;
-            const int64_t part = part_at<S::ROWS>(gx, gx == g0) + r0;  // g0 begins the unit
-            st[x] = p.stat[part + l32];
+            const int64_t part = part_at<S::ROWS>(gx * units + u, gx == g0) + r0;  // g0 begins the sequence
+            if (in && row.live) {
+                st[x] = p.stat[part + l32];
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) v[x][q4] = *part_of<D>(p.part, part, n, q4, lane);
-            if (!in) {
+                for (int q4 = 0; q4 < 4; ++q4) v[x][q4] = *part_of<D>(p.part, part, n, q4, lane);
+            } else {
                 st[x] = make_float2(-1e30f, 0.f);
 #pragma unroll
                 for (int q4 = 0; q4 < 4; ++q4) v[x][q4] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1103,7 +1104,6 @@ __global__ __launch_bounds__((64 * JoinShape<D, NW>::G * JoinShape<D, NW>::BLOCK
         stat[w][1][l32] = l;
     }
     __syncthreads();
-    const PagedRow row(p, S::ROWS * (u % p.unit_tiles) + r0 + l32, u / p.unit_tiles);
     if (!row.live) return;
     float mm = stat[0][0][l32], l_tot = 0.f, a[G];
 #pragma unroll

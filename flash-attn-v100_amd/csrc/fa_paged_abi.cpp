@@ -98,9 +98,14 @@ void plan(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared
     p.wide = f32 || rows <= 32 || busy(32, 128, 512) * full(128) < 10 ? 1 : rows <= 128 || busy(256, 64, 256) * full(256) < 40 ? 4 : 8;
     const int step = p.wide == 1 ? 128 : 64;
     p.unit_tiles = (int)ceil_div<int64_t>(rows, unit_rows(p));
-    p.slots = (f32 && compiled_dim(c.head_dim) == 128) || p.wide == 8 ? 256 : 512;  // workgroups that run at once
-    const int64_t units = (int64_t)c.batch * c.num_heads_kv * p.unit_tiles;
+    const int64_t slots = (f32 && compiled_dim(c.head_dim) == 128) || p.wide == 8 ? 256 : 512;  // workgroups that run at once
+    const int64_t units = (int64_t)c.num_heads_kv * p.unit_tiles;  // of a sequence
     const int64_t most = std::max<int64_t>(1, ceil_div<int64_t>(p.Sk, step));  // steps of a unit
+    // groups of a workgroup for each unit that fill the device once, or (more than 1 in 7 of it
+    // would stay empty) twice
+    int64_t groups = slots / units;
+    if (groups * units * 7 < slots * 6) groups = 2 * slots / units;
+    p.groups = (int)std::max<int64_t>(groups, 1);
     // Where no sequence has room for more than 4 steps, units are not shared: the join would
     // cost more than it saves (one token of 8 heads over 512 keys 8.4 us, with a join 11.0).
     // Where it is launched, all of more than `alone` steps are, down to `least` a workgroup.  us
@@ -113,11 +118,11 @@ void plan(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared
     // a wide unit's tree, rows and parts take about as long as 3 of its steps: 16 x 8192, trees of
     // 64: 166 us without, 158 with them in the balance
     p.extra = p.wide == 1 ? 0 : 3;
-    // workgroups that may share units (PagedWork): none where no unit is that long or, with
-    // every sequence full, longer than an even share
-    const int64_t T = units * (most + p.extra), w = std::min<int64_t>(p.slots, ceil_div<int64_t>(T, p.least));
-    shared = most > join_from && (c.key_lengths || most > ceil_div<int64_t>(T, w)) ? w : 0;
-    grid = std::max(units, shared);
+    // workgroups that may share sequences: none where none is that long or, with all of them
+    // full, longer than an even share
+    const int64_t T = c.batch * (most + p.extra), w = std::min<int64_t>(p.groups, ceil_div<int64_t>(T, p.least));
+    shared = w > 1 && most > join_from && (c.key_lengths || most > ceil_div<int64_t>(T, w)) ? w * units : 0;
+    grid = std::max(units * c.batch, shared);
 }
 size_t part_rows(const PagedParams& p, int64_t shared) { return (size_t)(2 * shared * unit_rows(p)); }
 size_t paged_bytes(const PagedParams& p, int64_t shared) {
