@@ -934,7 +934,7 @@ __device__ FA_INLINE inline void paged_unit_wide(T* smem, TreeBits* tree, bool n
             if (holes) have = (unsigned)table.template have<2>(4 * t + 2 * x);
             tile_rules<EXACT, true>(s[0], rules, row, tree, 64 * t + 32 * x, c, seen, have, hi);
             soft_max<D, 1>(s, rules.unit, m_run, l_run, o);
-        soft_exp<1>(s, rules.unit, m_run, l_run);
+            soft_exp<1>(s, rules.unit, m_run, l_run);
             if (uneven && tile_odd<T, D>(Vs, lane)) {
                 stay_branch();
                 tile_values_seen<T, D>(Vs, s[0], seen, o, lane);

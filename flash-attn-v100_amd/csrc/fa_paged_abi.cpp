@@ -87,15 +87,15 @@ void plan(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared
     // Waves that share tiles read K and V once for 128 or 256 rows, but leave larger parts and
     // fewer units: worth it where a workgroup gets enough steps of units that are full enough.
     // us of trees of N on 32 and 8 heads of 128, units of 32, 128 and 256 rows (sequences of up
-    // to, N): 16 x 8192, 64: 271, 180, 160; 24 x 4096, 64: 190, 142, 130; 16 x 4000, 64: 152, 134,
-    // 140; 2 x 16000, 48: 94, 74, 83; 16 x 8192, 16: 114, 100, 132; the other way 8 x 1000, 48: 35,
-    // 41, 45; 16 x 4000, 12: 70, 79, 136; 1 x 1000, 64: 22, 32, 37
+    // to, N): 16 x 8192, 64: 269, 168, 156; 24 x 4096, 64: 197, 135, 129; 16 x 4000, 64: 151, 125,
+    // 141; 2 x 16000, 48: 73, 64, 68; 8 x 4000, 24: 42, 39, 65; the other way 2 x 1000, 64: 25,
+    // 34, 39; 16 x 4000, 12: 61, 77, 134; 4 x 16000, 12: 40, 49, 84
     auto busy = [&](int64_t unit, int64_t keys, int64_t workgroups) {
         const int64_t tiles = ceil_div<int64_t>(rows, unit);
         return (double)c.batch * c.num_heads_kv * ceil_div<int64_t>(p.Sk, keys) * tiles / workgroups;
     };
     auto full = [&](int64_t unit) { return (double)rows / (double)(unit * ceil_div<int64_t>(rows, unit)); };
-    p.wide = f32 || rows <= 32 || busy(32, 128, 512) * full(128) < 10 ? 1 : rows <= 128 || busy(256, 64, 256) * full(256) < 40 ? 4 : 8;
+    p.wide = f32 || rows <= 32 || busy(32, 128, 512) * full(128) < 8 ? 1 : rows <= 128 || busy(256, 64, 256) * full(256) < 40 ? 4 : 8;
     const int step = p.wide == 1 ? 128 : 64;
     p.unit_tiles = (int)ceil_div<int64_t>(rows, unit_rows(p));
     const int64_t slots = (f32 && compiled_dim(c.head_dim) == 128) || p.wide == 8 ? 256 : 512;  // workgroups that run at once
