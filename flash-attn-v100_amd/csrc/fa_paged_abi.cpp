@@ -150,9 +150,10 @@ void put_paged(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& s
     p.table_sb = c.table_stride;
     p.table_cols = c.table_cols;
     p.pages = c.pages;
-    // (a row of tokens: a page that no block is behind)
-    p.page_blocks = p.table ? c.page_size / 16 : c.page_size / 16 + 1;
-    p.page_magic = (unsigned)(((1ull << 32) + p.page_blocks - 1) / p.page_blocks);
+    // (a row of tokens: every block is in the first column; rows may be longer than pages that
+    // the product divides by exactly)
+    p.page_blocks = p.table ? c.page_size / 16 : 2;
+    p.page_magic = p.table ? (unsigned)(((1ull << 32) + p.page_blocks - 1) / p.page_blocks) : 0u;
     p.parents = a->parents;
     p.parents_sb = a->parents_stride;
     plan(a, p, grid, shared);
@@ -183,11 +184,12 @@ int32_t fa_paged_check(const fa_paged_args* a) {
     if ((st = check_tensor(a->q, a->q_stride, 4, a->seqlen_q, c.head_dim, es)) ||
         (st = check_tensor(a->o, a->o_stride, 4, a->seqlen_q, c.head_dim, es)))
         return st;
-    // all units' steps in 32 bits
+    // all units' steps in 32 bits, a grid's threads too
     const int64_t rows = (int64_t)a->seqlen_q * (a->num_heads / c.num_heads_kv);
     const double steps = (double)c.batch * c.num_heads_kv * (double)ceil_div<int64_t>(rows, 32) *
                          (double)std::max<int64_t>(1, ceil_div<int64_t>(room_of(c), 64));
-    if (steps >= 2e9 || c.batch > 65535) return FA_ERR_TOO_LARGE;
+    if (steps >= 2e9 || c.batch > 65535 || (double)c.batch * c.num_heads_kv * (double)ceil_div<int64_t>(rows, 32) >= 1 << 24)
+        return FA_ERR_TOO_LARGE;
     return FA_OK;
 }
 
@@ -227,7 +229,7 @@ int32_t fa_cache_write_check(const fa_cache_write_args* a) {
     int32_t st = check_pool(c, false);
     if (st) return st;
     if (a->tokens < 0) return FA_ERR_SHAPE;
-    if ((int64_t)c.batch * a->tokens >= (1LL << 30)) return FA_ERR_TOO_LARGE;
+    if ((int64_t)c.batch * a->tokens >= (1LL << 28)) return FA_ERR_TOO_LARGE;
     if (c.batch == 0 || a->tokens == 0 || empty_pool(c)) return FA_OK;
     const int es = elem_size(c.dtype);
     if ((st = check_tensor(a->k, a->k_stride, 5, a->tokens, c.head_dim, es)) ||
@@ -292,7 +294,8 @@ int32_t fa_cache_fork_check(const fa_cache_fork_args* a) {
     if (st) return st;
     if (a->new_batch < 0) return FA_ERR_SHAPE;
     if (c.pages > FA_MAX_POOL_PAGES) return FA_ERR_PAGES;
-    if ((int64_t)a->new_batch * c.table_cols >= (1LL << 31) || (int64_t)c.page_size * c.num_heads_kv * 32 >= (1LL << 30))
+    if ((int64_t)a->new_batch * c.table_cols >= (1LL << 31) || a->new_batch >= 1 << 24 ||
+        (int64_t)c.page_size * c.num_heads_kv * 32 >= (1LL << 30))
         return FA_ERR_TOO_LARGE;
     if (a->new_batch == 0) return FA_OK;
     if (!a->sources || !a->new_lengths || (c.table_cols > 0 && !a->new_table)) return FA_ERR_NULL_ARG;
@@ -338,7 +341,8 @@ int32_t fa_cache_compact_check(const fa_cache_compact_args* a) {
     const int32_t st = check_pool(c, true);
     if (st) return st;
     if (c.pages > FA_MAX_POOL_PAGES) return FA_ERR_PAGES;
-    if ((int64_t)c.batch * c.table_cols >= (1LL << 31) || (int64_t)c.page_size * c.num_heads_kv * 32 >= (1LL << 30))
+    const int64_t chunks = (int64_t)c.page_size * c.num_heads_kv * 32;
+    if ((int64_t)c.batch * c.table_cols >= (1LL << 31) || chunks >= (1LL << 30) || c.layers * (chunks / 512 + 2) >= (1LL << 31))
         return FA_ERR_TOO_LARGE;
     if (!a->used || (c.batch > 0 && c.table_cols > 0 && !a->new_table)) return FA_ERR_NULL_ARG;
     if (!aligned(a->used, 4) || !aligned(a->new_table, 4)) return FA_ERR_ALIGN;

@@ -89,7 +89,8 @@ int32_t fa_paged_fwd(const fa_paged_args* args, void* workspace, size_t workspac
 
 /* Writes the rows of N = tokens new tokens: row i of sequence b to place
  * key_lengths[b] - N + i of every layer (a negative place is not written).  Two
- * sequences that share a page may not write the same row of it. */
+ * sequences that share a page may not write the same row of it; k and v do not overlap
+ * the pool. */
 typedef struct fa_cache_write_args {
     fa_page_pool pool;
     const void* k;          /* (layers, B, N, Hkv, D): strides in that order */

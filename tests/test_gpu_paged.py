@@ -241,6 +241,24 @@ def test_pool_past_32_bits():
     assert torch.equal(fa.flash_attention_v100_paged(small[0], kc, vc, ints(lens), ints(far)), want)
 
 
+def test_rows_of_millions_of_tokens():
+    # the last tokens of rows longer than a page may be: what they hold decides
+    size, D, N = 2 ** 21 + 16, 32, 2
+    g = torch.Generator(DEV).manual_seed(18)
+    kc = torch.zeros(2, size, 1, D, dtype=torch.float16, device=DEV)
+    vc = torch.zeros_like(kc)
+    q = torch.zeros(2, N, 1, D, dtype=torch.float16, device=DEV)
+    q[..., 0] = 30.0
+    kc[:, -40:, :, 0] = 3.0                                    # e^90 against e^0 of 2^21 others
+    vc[:, -40:] = torch.randn(2, 40, 1, D, generator=g, device=DEV).half()
+    o = fa.flash_attention_v100_paged(q, kc, vc, scale=1.0)
+    for i in range(N):
+        want = vc[:, size - 40:size - N + i + 1, 0].double().mean(1)
+        # the products and sums of up to 40 probabilities (one each, e^-90 times 2^21 beside them) in fp16 and float32
+        bound = want.abs() * 2.0 ** -11 + vc[:, -40:, 0].double().abs().mean(1) * (2.0 ** -11 + 41 * 2.0 ** -24) + 2.0 ** -25
+        assert ((o[:, i, 0].double() - want).abs() <= bound).all()
+
+
 def test_empty_sides():
     q, kc, vc, table = make([16, 5], 2, 1, 16, 4, 2, 64, "bf16", seed=16)
     ints = lambda x: torch.tensor(x, device=DEV, dtype=torch.int32)  # noqa: E731

@@ -184,6 +184,29 @@ def test_trees_and_rows_of_tokens():
     assert status("fa_paged", a) == CODES["FA_ERR_PAGES"]
 
 
+def test_grids_that_no_launch_takes():
+    # 2^32 threads a grid: units of 32 rows of 256, rows of 64 of 4 rows, forks of 256 each
+    a = paged_args(N=2000, H=4, Hkv=4, cols=1, batch=65535)    # 63 units of each of 4 heads: 16.5 million, below 2^24
+    assert status("fa_paged", a) == 0
+    a = paged_args(N=2100, H=4, Hkv=4, cols=1, batch=65535)    # 66: 17.3 million
+    assert status("fa_paged", a) == CODES["FA_ERR_TOO_LARGE"]
+    a = write_args(N=1 << 10)
+    a.pool.batch = 1 << 17
+    assert status("fa_cache_write", a) == 0
+    a.pool.batch = 1 << 18
+    assert status("fa_cache_write", a) == CODES["FA_ERR_TOO_LARGE"]
+    a = fork_args(new_batch=(1 << 24) - 1)
+    assert status("fa_cache_fork", a) == 0
+    a.new_batch += 1
+    assert status("fa_cache_fork", a) == CODES["FA_ERR_TOO_LARGE"]
+    # pieces of 16 KB of all layers of a page, in 31 bits
+    a = compact_args()
+    a.pool.page_size, a.pool.num_heads_kv, a.pool.layers = 1 << 14, 1 << 9, 1 << 11
+    assert status("fa_cache_compact", a) == 0
+    a.pool.layers = 1 << 12
+    assert status("fa_cache_compact", a) == CODES["FA_ERR_TOO_LARGE"]
+
+
 def test_workspaces_and_refusals_before_any_launch():
     lib = _paged.load()
     size = lib.fa_paged_workspace_size
