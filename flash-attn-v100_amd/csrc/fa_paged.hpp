@@ -879,14 +879,11 @@ __device__ FA_INLINE inline void paged_unit_wide(T* smem, TreeBits* tree, bool n
     if (new_tree) tree_init(p, *tree, b, tid);
     row.rule(tree, rules.words, len, c);
     const bool holes = table.holes(4 * s0, 4 * t1, lane);
-    int lim_min = row.valid ? row.all : INT_MAX, lim_max = row.lim;
+    int lim_min = row.valid ? row.all : INT_MAX;
 #pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-        lim_min = min(lim_min, __shfl_xor(lim_min, x));
-        lim_max = max(lim_max, __shfl_xor(lim_max, x));
-    }
+    for (int x = 1; x < 32; x <<= 1) lim_min = min(lim_min, __shfl_xor(lim_min, x));
     lim_min = __builtin_amdgcn_readfirstlane(lim_min);
-    const bool uneven = tree || lim_min != __builtin_amdgcn_readfirstlane(lim_max);
+    const bool uneven = lim_min < n_keys;  // a row does not see what others, or other waves' rows, see
     wait_vmem();
     asm volatile("" ::: "memory");
 

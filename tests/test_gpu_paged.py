@@ -179,6 +179,23 @@ def test_hidden_infinities(dt, tree, N):
     assert (o[:, -1, :, 7] == math.inf).all() and torch.isfinite(o[:, :-1]).all()
 
 
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+def test_hidden_infinities_of_waves_of_one_token(dt):
+    # 64 heads of a KV head: all rows of a wave are one token's, and other waves of the unit see more
+    N, lens = 8, [2048, 1000, 2047, 8, 1999, 64, 1500, 777, 2048, 130, 1, 0, 1024, 2048, 31, 1600]
+    t = make(lens, N, 128, 16, 64, 1, 32, dt, seed=11)
+    kc, vc = t[1].clone(), t[2].clone()
+    for b, n in enumerate(lens):
+        if n:
+            p, r = po.place(t[3], b, n - 1, 16)
+            kc[p, r, :, 5] = vc[p, r, :, ::3] = math.inf
+    ints = lambda x: torch.tensor(x, device=DEV)  # noqa: E731
+    o, lse = fa.flash_attention_v100_paged(t[0], kc, vc, ints(lens), ints(t[3]), return_softmax_lse=True)
+    ref = po.attention(*t[:3], lens, t[3])
+    oo.check({"o": o[:, :-1], "lse": lse[:, :, :-1]},
+             {"o": tuple(x[:, :-1] for x in ref["o"]), "lse": tuple(x[:, :, :-1] for x in ref["lse"])}, ["o", "lse"], dt)
+
+
 def test_pages_that_are_none():
     N, lens = 4, [200, 64, 130]
     t = make(lens, N, 13, 16, 4, 2, 64, "bf16", seed=12)
