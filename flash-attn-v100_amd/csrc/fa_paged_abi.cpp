@@ -57,7 +57,7 @@ void put_pool(const fa_page_pool& c, PoolParams& p) {
     const int64_t es = elem_size(c.dtype);
     p.x[0] = (char*)c.k;
     p.x[1] = (char*)c.v;
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < 2 && c.pages && c.page_size; ++x) {  // (strides of nothing have not been checked)
         const int64_t* st = x ? c.v_stride : c.k_stride;
         p.sl[x] = st[0] * es;
         p.sp[x] = st[1] * es;
@@ -184,10 +184,9 @@ int32_t fa_paged_check(const fa_paged_args* a) {
     if ((st = check_tensor(a->q, a->q_stride, 4, a->seqlen_q, c.head_dim, es)) ||
         (st = check_tensor(a->o, a->o_stride, 4, a->seqlen_q, c.head_dim, es)))
         return st;
-    // all units' steps in 32 bits, a grid's threads too
+    // the steps of all sequences in 32 bits, a grid's threads too
     const int64_t rows = (int64_t)a->seqlen_q * (a->num_heads / c.num_heads_kv);
-    const double steps = (double)c.batch * c.num_heads_kv * (double)ceil_div<int64_t>(rows, 32) *
-                         (double)std::max<int64_t>(1, ceil_div<int64_t>(room_of(c), 64));
+    const double steps = (double)c.batch * (double)(ceil_div<int64_t>(room_of(c), 64) + 4);
     if (steps >= 2e9 || c.batch > 65535 || (double)c.batch * c.num_heads_kv * (double)ceil_div<int64_t>(rows, 32) >= 1 << 24)
         return FA_ERR_TOO_LARGE;
     return FA_OK;

@@ -192,6 +192,18 @@ def test_fork_and_compact_large_pools():
     same((kc, vc, *got), want)
 
 
+@pytest.mark.parametrize("B,Bn,P", [(1100, 1500, 6000), (1100, 70, 3000), (60, 1500, 9000)])
+def test_batches_of_more_than_a_workgroup(B, Bn, P):
+    lens, table, sources, more = random_fork(B + Bn, B, Bn, 3, P, 16, 1, 20)
+    kc, vc = pools(1, P, 16, 1, 8, "bf16", seed=Bn)
+    want = po.fork(kc, vc, table, lens, sources, more)
+    got = fa.paged_cache_fork_v100(kc, vc, ints(table), ints(lens), ints(sources), ints(more))
+    same((kc, vc, *got), want)
+    want = po.compact(kc, vc, got[0].tolist(), got[1].tolist())
+    got = fa.paged_cache_compact_v100(kc, vc, *got)
+    same((kc, vc, *got), want)
+
+
 @pytest.mark.parametrize("seed", range(8))
 def test_compact(seed):
     B, M, P, size, L = [(5, 6, 60, 16, 2), (1, 3, 40, 32, 1), (40, 5, 260, 16, 3), (3, 2, 6, 48, 1)][seed % 4]
