@@ -3,7 +3,11 @@
 //
 // All of them move rows of a token (every KV head's columns, 16-byte chunks); a wave
 // takes 64 chunks of a row, so that a row's place is found by scalar instructions.
-// Bound by the bytes read and written; small calls by the launch.
+// Bound by the bytes read and written: prompts of 2048 tokens (50 MB in and out) 9.0 us,
+// 5.6 TB/s (the writes stay in the last cache); drafts of 64 tokens of 64 sequences in 8
+// layers (283 MB with the accepted rows) 53 + 8 us, 4.6 TB/s; a pool of 2520 pages compacted
+// (165 MB) 36 us for the rows, 4.6 TB/s, after 8 for its plan.  A small call (one token, a
+// fork, a plan) is bound by its launch and a few round trips to memory, 2 to 8 us.
 #include <hip/hip_runtime.h>
 
 #include "fa_common.hpp"
