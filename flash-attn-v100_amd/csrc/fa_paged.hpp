@@ -73,17 +73,20 @@ __device__ FA_INLINE inline PagedArgs& paged_args() {
     asm volatile("" : "+s"(a));
     return *(PagedArgs*)(uintptr_t)a;
 }
-// filled tokens of a sequence
-__device__ FA_INLINE inline int filled_tokens(PagedArgs& p, int b) { return p.lens ? max(0, min(p.Sk, p.lens[b])) : p.Sk; }
-__device__ FA_INLINE inline void put_row_lse(PagedArgs& p, int b, int h, int i, float m, float l) {
-    p.lse[((int64_t)b * p.H + h) * p.Sq + i] = l > 0.f ? (m + __log2f(l)) * kLn2 : l == 0.f ? -INFINITY : l;
-}
-
 // scalar loads of what no kernel of the call writes
 typedef const __attribute__((address_space(4))) int const_int;
 __device__ FA_INLINE inline int uniform_load(const int* p, int64_t at) {
     return ((const_int*)(uintptr_t)p)[at];
 }
+// filled tokens of a sequence; of one that is the same for a wave
+__device__ FA_INLINE inline int filled_here(PagedArgs& p, int b) {
+    return p.lens ? max(0, min(p.Sk, uniform_load(p.lens, __builtin_amdgcn_readfirstlane(b)))) : p.Sk;
+}
+__device__ FA_INLINE inline int filled_tokens(PagedArgs& p, int b) { return p.lens ? max(0, min(p.Sk, p.lens[b])) : p.Sk; }
+__device__ FA_INLINE inline void put_row_lse(PagedArgs& p, int b, int h, int i, float m, float l) {
+    p.lse[((int64_t)b * p.H + h) * p.Sq + i] = l > 0.f ? (m + __log2f(l)) * kLn2 : l == 0.f ? -INFINITY : l;
+}
+
 
 // 16 tokens of a sequence: their page, -1 where there is none, and the first one's row
 struct Block16 {
@@ -212,6 +215,10 @@ struct PagedWork {
     __device__ FA_INLINE inline static int steps(PagedArgs& p, int b) {
         return b < p.B ? max(1, (filled_tokens(p, b) + STEP - 1) / STEP) + p.extra : 0;
     }
+    template <int STEP>
+    __device__ FA_INLINE inline static int steps_here(PagedArgs& p, int b) {
+        return max(1, (filled_here(p, b) + STEP - 1) / STEP) + p.extra;
+    }
     __device__ FA_INLINE inline static int scan(int x, int lane) {
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -222,6 +229,11 @@ struct PagedWork {
     }
     template <int STEP>
     __device__ FA_INLINE inline void init(PagedArgs& p, int lane) {
+        if (!p.part) {  // (nothing may be shared: no lengths are needed to know it)
+            whole = true;
+            W = p.B;
+            return;
+        }
         int sum = 0, most = 0;
         if (p.lens) {
             most = st0 = steps<STEP>(p, lane);
@@ -231,12 +243,12 @@ struct PagedWork {
                 most = max(most, st);
             }
             inc0 = scan(st0, lane);
-            sum += st0;
 #pragma unroll
             for (int x = 1; x < 64; x <<= 1) {
-                sum += __shfl_xor(sum, x);
+                if (p.B > 64) sum += __shfl_xor(sum, x);
                 most = max(most, __shfl_xor(most, x));
             }
+            sum += __builtin_amdgcn_readlane(inc0, 63);
         } else {
             most = steps<STEP>(p, 0);
             sum = most * p.B;
@@ -659,7 +671,7 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], Tre
     uint4 q[C::F32 ? D / 8 : D / 16];
     load_q<T, D>(p, row, b, hi, q);
     TileRules<EXACT> rules(p, b, row.h);
-    const int len = __builtin_amdgcn_readfirstlane(filled_tokens(p, b)), c = len - p.Sq;
+    const int len = filled_here(p, b), c = len - p.Sq;
     const int n_keys = keys_of(p, tree, 32 * (rt + 1), len, c);
     const int nt = (n_keys + 31) / 32, t1 = min(NW * s1, nt);
 
@@ -671,10 +683,10 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], Tre
     // the two blocks of a tile, looked up a tile before the copy that needs them; what is
     // past the end reads nothing, but is issued, so that the vmcnt counts stay exact
     const PageTable table(p, b);
+    // (those behind the sequence are of some page, and their copies read nothing)
     auto blocks = [&](int t, Block16& x, Block16& y) FA_INLINE {
-        const int tt = min(t, max(nt - 1, 0));
-        x = table.block(2 * tt);
-        y = table.block(2 * tt + 1);
+        x = table.block(2 * t);
+        y = table.block(2 * t + 1);
     };
     auto copy = [&](const PageCopy<T, D>& pc, int t, Block16 x, Block16 y, const T* dst) FA_INLINE {
         const int nv = t < t1 ? n_keys - 32 * t : 0;
@@ -867,7 +879,7 @@ __device__ FA_INLINE inline void paged_unit_wide(T* smem, TreeBits* tree, bool n
     uint4 q[D / 16];
     load_q<T, D>(p, row, b, hi, q);
     TileRules<EXACT> rules(p, b, row.h);
-    const int len = __builtin_amdgcn_readfirstlane(filled_tokens(p, b)), c = len - p.Sq;
+    const int len = filled_here(p, b), c = len - p.Sq;
     // (all waves copy for all)
     const int n_keys = keys_of(p, tree, 32 * NW * (rt + 1), len, c), t1 = min(s1, (n_keys + 63) / 64);
 
@@ -876,8 +888,7 @@ __device__ FA_INLINE inline void paged_unit_wide(T* smem, TreeBits* tree, bool n
     if (NW == 4) vc.init((const T*)p.v + hk * p.v_sh, p.v_sp, p.v_ss, p.cols, lane);
     if (NW == 8 && w >= 4) kc.init((const T*)p.v + hk * p.v_sh, p.v_sp, p.v_ss, p.cols, lane);
     const PageTable table(p, b);
-    const int last = max((n_keys + 15) / 16 - 1, 0);
-    auto look = [&](int t) FA_INLINE { return table.block(min(4 * t + (w & 3), last)); };
+    auto look = [&](int t) FA_INLINE { return table.block(4 * t + (w & 3)); };
     // tile t, to slot t % NS; what is past the end reads nothing, but is issued, so that the
     // vmcnt counts stay exact
     auto issue = [&](int t, Block16 at) FA_INLINE {
@@ -1023,7 +1034,7 @@ __global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 : Pag
     int x = 0, end = 0, b = 0, start = 0, len = 0, last_b = -1;  // len: of a unit, with the extra steps
     if (wk.whole) {
         b = group;
-        len = __builtin_amdgcn_readfirstlane(PagedWork::steps<S::STEP>(p, b));
+        len = PagedWork::steps_here<S::STEP>(p, b);
         end = len;
     } else {
         x = wk.first(group);
@@ -1035,7 +1046,7 @@ __global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 : Pag
         x = min(end, start + len);
         if (s0 >= s1) continue;  // (the extra steps of a unit that ended in another workgroup)
         const int64_t part = s1 - s0 == n ? -1 : part_at<S::ROWS>(g, s0 == 0);
-        if (n == 1 && filled_tokens(paged_args(), b) == 0) {
+        if (n == 1 && filled_here(paged_args(), b) == 0) {
             empty_unit<T, D>(paged_args(), b, hk, rt * S::ROWS, S::ROWS, tid, S::THREADS);
         } else if constexpr (NW == 1) {
             __shared__ float stat[PagedCfg<T, D>::NW][2][32];
