@@ -486,21 +486,24 @@ __device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16 (&s)[NB],
 template <typename T, int D>
 __device__ FA_INLINE inline bool tile_odd(const T* Vs, int lane) {
     using C = PagedCfg<T, D>;
-    constexpr unsigned M = std::is_same<T, bf16>::value ? 0x7F80u : 0x7C00u;
-    bool odd = false;
-#pragma unroll 2
+    // the largest magnitude, as integers: an infinity's or above
+    constexpr unsigned short M = std::is_same<T, bf16>::value ? 0x7F80 : 0x7C00;
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    unsigned top = 0u;
+    u16x2 top2 = {0, 0};
+#pragma unroll 4
     for (int x = 0; x < 32 * C::CW / 64; ++x) {
         const uint4 v = *reinterpret_cast<const uint4*>((const char*)Vs + 16 * (64 * x + lane));
         const unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if constexpr (C::F32)
-                odd |= (w[e] & 0x7F800000u) == 0x7F800000u;
+                top = max(top, w[e] & 0x7FFFFFFFu);
             else
-                odd |= (w[e] & M) == M || ((w[e] >> 16) & M) == M;
+                top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(u16x2, w[e] & 0x7FFF7FFFu));
         }
     }
-    return __ballot(odd) != 0ull;
+    return __ballot(C::F32 ? top >= 0x7F800000u : top2.x >= M || top2.y >= M) != 0ull;
 }
 // tile_values key by key, each to the rows that see it (bit x of seen: key x)
 template <typename T, int D>
@@ -854,17 +857,20 @@ __device__ FA_INLINE inline void store_tile(PagedArgs& p, const T* tile, int b, 
 
 // ---------------------------------------------------------------------------
 // Units of 32 NW rows whose NW waves, on 32 rows each, share tiles of 64 keys: K and V
-// are read once for all of them.  NS tiles in LDS, of which NS - 1 are on their way or
-// read; a wave copies one block of 16 keys (NW = 8) or one of K and one of V.
+// are read once for all of them.  NW = 8 for 128 columns only: up to 64 leave registers for
+// three workgroups of four waves a CU (28 trees of 91 over up to 13755 keys, 4 heads of 64:
+// 130 us with two, 113 with three, 118 with four, which spill).  NS tiles in LDS, of which
+// NS - 1 are on their way or read; a wave copies one block of 16 keys (NW = 8) or one of K and
+// one of V.
 template <typename T, int D, int NW>
 struct WideCfg {
     using C = PagedCfg<T, D>;
     static constexpr int STEP = 64;
     static constexpr int TILE = STEP * D;
-    static constexpr int NS = NW == 8 || D < 128 ? 4 : 2;
+    static constexpr int NS = NW == 8 ? 4 : 2;
     static constexpr int SMEM = NS * 2 * TILE;
     static constexpr int COPIES = 8 / NW * C::NI16;  // of a wave, a tile
-    static constexpr int PER_CU = NW == 8 ? 1 : 2;
+    static constexpr int PER_CU = NW == 8 ? 1 : D < 128 ? 3 : 2;
 };
 
 template <typename T, int D, bool EXACT, int NW>
@@ -1017,7 +1023,7 @@ struct PagedShape<T, D, 1> {
 };
 
 template <typename T, int D, bool EXACT, bool TREE, int NW>
-__global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 : PagedShape<T, D, NW>::PER_CU)) void paged_kernel(const PagedParams) {
+__global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 * PagedShape<T, D, NW>::PER_CU : PagedShape<T, D, NW>::PER_CU)) void paged_kernel(const PagedParams) {
     using S = PagedShape<T, D, NW>;
     PagedArgs& p = paged_args();
     __shared__ __attribute__((aligned(1024))) T smem[S::SMEM];
@@ -1061,18 +1067,20 @@ __global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 : Pag
 // The parts of 32 rows (blockIdx.x: KV head, unit, its rows) of a unit that several
 // workgroups shared: for 32 columns G waves, each of which takes every G-th part, two at
 // a time, and whose sums meet in LDS.  Units of 32 rows are few and in up to 64 parts: four
-// waves, 32 columns a workgroup (one token over 65536 keys: 39 us a call, 45 with two and all
+// waves (16 where a sequence may be in more than 40 parts: one token over 8192 keys in 32
+// parts 16.9 us with four, 17.8 with 16; 15 tokens of 2 heads in 54 parts 20.2 and 18.3; one over
+// 65536 in 64 parts 40.5 and 39.1), 32 columns a workgroup (one token over 65536 keys: 39 us a call, 45 with two and all
 // columns); wide units are in two or three, and what a workgroup finds out about its unit
 // serves all columns (16 trees of 64 over up to 8192: 13 us, 18 with 32 columns).
-template <int D, int NW>
+template <int D, int NW, bool MANY>
 struct JoinShape {
-    static constexpr int G = NW == 1 ? 4 : 2, BLOCKS = NW == 1 ? 1 : D / 32;  // of 32 columns
+    static constexpr int G = NW > 1 ? 2 : MANY ? 16 : 4, BLOCKS = NW == 1 ? 1 : D / 32;  // of 32 columns
 };
-template <typename T, int D, int NW>
-__global__ __launch_bounds__((64 * JoinShape<D, NW>::G * JoinShape<D, NW>::BLOCKS)) void paged_join_kernel(const PagedParams) {
+template <typename T, int D, int NW, bool MANY>
+__global__ __launch_bounds__((64 * JoinShape<D, NW, MANY>::G * JoinShape<D, NW, MANY>::BLOCKS)) void paged_join_kernel(const PagedParams) {
     using S = PagedShape<T, D, NW>;
-    using J = JoinShape<D, NW>;
-    constexpr int G = J::G;
+    using J = JoinShape<D, NW, MANY>;
+    constexpr int G = J::G, OUT = G < 4 ? G : 4;  // waves that write the sums
     PagedArgs& p = paged_args();
     __shared__ float sums[J::BLOCKS][G][16][64], stat[G][2][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1126,7 +1134,7 @@ __global__ __launch_bounds__((64 * JoinShape<D, NW>::G * JoinShape<D, NW>::BLOCK
         stat[w][1][l32] = l;
     }
     __syncthreads();
-    if (!row.live) return;
+    if (!row.live || w >= OUT) return;
     float mm = stat[0][0][l32], l_tot = 0.f, a[G];
 #pragma unroll
     for (int x = 1; x < G; ++x) mm = fmaxf(mm, stat[x][0][l32]);
@@ -1139,8 +1147,8 @@ __global__ __launch_bounds__((64 * JoinShape<D, NW>::G * JoinShape<D, NW>::BLOCK
     if (n == 0 && w == 0 && hi == 0 && p.lse) put_row_lse(p, b, row.h, row.i, mm, l_tot);
     T* ob = (T*)p.o + b * p.o_sb + (int64_t)row.i * p.o_ss + row.h * p.o_sh + 32 * n + 4 * hi;
 #pragma unroll
-    for (int q = 0; q < 4 / G; ++q) {
-        const int q4 = w * (4 / G) + q;
+    for (int q = 0; q < 4 / OUT; ++q) {
+        const int q4 = w * (4 / OUT) + q;
         if (32 * n + 8 * q4 + 4 * hi >= p.cols) continue;
         float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -1175,16 +1183,24 @@ hipError_t launch_paged_t(const PagedParams& p, hipStream_t s) {
             hipLaunchKernelGGL((paged_kernel<T, D, F32, false, NW>), grid, block, 0, s, p);
     }
     if (p.part) {
-        using J = JoinShape<D, NW>;
-        const dim3 tiles((unsigned)(p.Hkv * p.unit_tiles * NW), D / 32 / J::BLOCKS, (unsigned)p.B);
-        hipLaunchKernelGGL((paged_join_kernel<T, D, NW>), tiles, dim3(64 * J::G * J::BLOCKS), 0, s, p);
+        auto join = [&](auto many) {
+            using J = JoinShape<D, NW, decltype(many)::value>;
+            const dim3 tiles((unsigned)(p.Hkv * p.unit_tiles * NW), D / 32 / J::BLOCKS, (unsigned)p.B);
+            hipLaunchKernelGGL((paged_join_kernel<T, D, NW, decltype(many)::value>), tiles, dim3(64 * J::G * J::BLOCKS), 0, s, p);
+        };
+        if (NW == 1 && p.many)
+            join(std::integral_constant<bool, NW == 1>{});
+        else
+            join(std::false_type{});
     }
     return hipGetLastError();
 }
 template <typename T, int D>
 hipError_t launch_paged_d(const PagedParams& p, hipStream_t s) {
     if constexpr (!Elem<T>::kF32) {
-        if (p.wide == 8) return launch_paged_t<T, D, 8>(p, s);
+        if constexpr (D == 128) {
+            if (p.wide == 8) return launch_paged_t<T, D, 8>(p, s);
+        }
         if (p.wide == 4) return launch_paged_t<T, D, 4>(p, s);
     }
     return launch_paged_t<T, D, 1>(p, s);

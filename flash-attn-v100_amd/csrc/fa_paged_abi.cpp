@@ -82,23 +82,29 @@ void put_pool(const fa_page_pool& c, PoolParams& p) {
 int unit_rows(const PagedParams& p) { return 32 * p.wide; }
 void plan(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared) {
     const fa_page_pool& c = a->pool;
-    const bool f32 = c.dtype == FA_DTYPE_F32;
+    const bool f32 = c.dtype == FA_DTYPE_F32, d128 = compiled_dim(c.head_dim) == 128;
     const int64_t rows = (int64_t)a->seqlen_q * (a->num_heads / c.num_heads_kv);
     // Waves that share tiles read K and V once for 128 or 256 rows, but leave larger parts and
     // fewer units: worth it where a workgroup gets enough steps of units that are full enough.
     // us of trees of N on 32 and 8 heads of 128, units of 32, 128 and 256 rows (sequences of up
     // to, N): 16 x 8192, 64: 269, 168, 156; 24 x 4096, 64: 197, 135, 129; 16 x 4000, 64: 151, 125,
     // 141; 2 x 16000, 48: 73, 64, 68; 8 x 4000, 24: 42, 39, 65; the other way 2 x 1000, 64: 25,
-    // 34, 39; 16 x 4000, 12: 61, 77, 134; 4 x 16000, 12: 40, 49, 84
+    // 34, 39; 16 x 4000, 12: 61, 77, 134; 4 x 16000, 12: 40, 49, 84.  Head dims up to 64 have three
+    // workgroups of 128 rows a CU: 16 x 8192, 64: 169, 104, 103 (64 on 8 heads 300, 174, 178); chunks
+    // of 189 in 28 x 546, 96 on 12 heads: 290, 178, 232
     auto busy = [&](int64_t unit, int64_t keys, int64_t workgroups) {
         const int64_t tiles = ceil_div<int64_t>(rows, unit);
         return (double)c.batch * c.num_heads_kv * ceil_div<int64_t>(p.Sk, keys) * tiles / workgroups;
     };
     auto full = [&](int64_t unit) { return (double)rows / (double)(unit * ceil_div<int64_t>(rows, unit)); };
-    p.wide = f32 || rows <= 32 || busy(32, 128, 512) * full(128) < 8 ? 1 : rows <= 128 || busy(256, 64, 256) * full(256) < 40 ? 4 : 8;
+    if (f32 || rows <= 32 || busy(32, 128, 512) * full(128) < 8)
+        p.wide = 1;
+    else
+        p.wide = !d128 || rows <= 128 || busy(256, 64, 256) * full(256) < 40 ? 4 : 8;
     const int step = p.wide == 1 ? 128 : 64;
     p.unit_tiles = (int)ceil_div<int64_t>(rows, unit_rows(p));
-    const int64_t slots = (f32 && compiled_dim(c.head_dim) == 128) || p.wide == 8 ? 256 : 512;  // workgroups that run at once
+    // workgroups that run at once
+    const int64_t slots = p.wide == 1 ? (f32 && d128 ? 256 : 512) : p.wide == 8 ? 256 : d128 ? 512 : 768;
     const int64_t units = (int64_t)c.num_heads_kv * p.unit_tiles;  // of a sequence
     const int64_t most = std::max<int64_t>(1, ceil_div<int64_t>(p.Sk, step));  // steps of a unit
     // groups of a workgroup for each unit that fill the device once, or (more than 1 in 7 of it
@@ -122,6 +128,7 @@ void plan(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared
     // full, longer than an even share
     const int64_t T = c.batch * (most + p.extra), w = std::min<int64_t>(p.groups, ceil_div<int64_t>(T, p.least));
     shared = w > 1 && most > join_from && (c.key_lengths || most > ceil_div<int64_t>(T, w)) ? w * units : 0;
+    p.many = w > 40 * (int64_t)c.batch;
     grid = std::max(units * c.batch, shared);
 }
 size_t part_rows(const PagedParams& p, int64_t shared) { return (size_t)(2 * shared * unit_rows(p)); }

@@ -39,7 +39,7 @@ template <typename T>
 hipError_t launch_paged(const PagedParams& p, int D, hipStream_t) {
     ++g_launches;
     CHECK(D >= p.cols && (D == 32 || D == 64 || D == 128) && p.H == p.Hkv * p.group);
-    CHECK(p.wide == 1 || ((p.wide == 4 || p.wide == 8) && sizeof(T) == 2));
+    CHECK(p.wide == 1 || ((p.wide == 4 || (p.wide == 8 && D == 128)) && sizeof(T) == 2));
     const int64_t rows = (int64_t)p.Sq * p.group, unit = 32 * p.wide, units = (int64_t)p.Hkv * p.unit_tiles;
     const int step = p.wide == 1 ? 128 : 64;
     CHECK(p.unit_tiles * unit >= rows && (p.unit_tiles - 1) * unit < rows && rows < (1LL << 31));
