@@ -77,6 +77,36 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const CacheWriteParams
     }
 }
 
+// Rows of at most half a wave's chunks: a wave takes as many rows side by side as fit, R times,
+// each lane looking up its own (3120 tokens of each of 59 sequences, one head of 128, 185 MB: 99 us
+// with a row a wave, 45 so; 700 of 16, two heads of 64: 9.2 and 5.8)
+template <int R>
+__global__ __launch_bounds__(256) void cache_write_short_kernel(const CacheWriteParams p) {
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kv = blockIdx.y & 1, layer = blockIdx.y >> 1;
+    const int n = p.heads * p.chunks, per = 64 / n, sub = lane / n, c = lane - sub * n, rows = p.B * p.N;
+    if (sub >= per) return;
+    const int64_t in = chunk_at(p, p.in_sh[kv], c), out = chunk_at(p, p.sh[kv], c);
+    const int r0 = (blockIdx.x * 4 + w) * R * per + sub;  // below 2^31: at most 64 R past the rows
+    chunk_t v[R];
+    char* to[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        to[r] = nullptr;
+        const int row = r0 + r * per;
+        if (row >= rows) continue;
+        const int b = row / p.N, i = row - b * p.N, x = filled(p, b) - p.N + i;
+        if (x < 0) continue;
+        const Place at = place_of(p, b, x);
+        if (at.page < 0) continue;
+        to[r] = row_at(p, kv, layer, at) + out;
+        v[r] = *reinterpret_cast<const chunk_t*>(p.in[kv] + layer * p.in_sl[kv] + b * p.in_sb[kv] + i * p.in_ss[kv] + in);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (to[r]) *reinterpret_cast<chunk_t*>(to[r]) = v[r];
+}
+
 // ---------------------------------------------------------------------------
 // A wave takes 64 chunks of all rows of one path.  Its entries ascend, so that row j
 // takes from row j or one behind it: rows are read in groups of 8, before any of them is
@@ -384,7 +414,13 @@ __global__ __launch_bounds__(256) void compact_copy_kernel(const CacheCompactPar
 hipError_t launch_cache_write(const CacheWriteParams& p, hipStream_t s) {
     const int64_t rows = (int64_t)p.B * p.N;
     const unsigned y = 2 * p.layers;
-    if (rows * y >= 65536)
+    const int per = 64 / (p.heads * p.chunks);  // rows that fit a wave
+    if (per >= 2) {
+        if (rows * y >= 65536)
+            hipLaunchKernelGGL((cache_write_short_kernel<4>), dim3((unsigned)((rows + 16 * per - 1) / (16 * per)), y), dim3(256), 0, s, p);
+        else
+            hipLaunchKernelGGL((cache_write_short_kernel<1>), dim3((unsigned)((rows + 4 * per - 1) / (4 * per)), y), dim3(256), 0, s, p);
+    } else if (rows * y >= 65536)
         hipLaunchKernelGGL((cache_write_kernel<4>), dim3((unsigned)((rows + 15) / 16), y), dim3(256), 0, s, p);
     else if (rows * y >= 8192)
         hipLaunchKernelGGL((cache_write_kernel<2>), dim3((unsigned)((rows + 7) / 8), y), dim3(256), 0, s, p);

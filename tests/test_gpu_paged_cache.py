@@ -54,6 +54,19 @@ def test_write_layers(L, N):
     same((kc, vc), want)
 
 
+@pytest.mark.parametrize("dt,Hkv,D", [("fp16", 1, 8), ("fp32", 1, 36), ("bf16", 3, 80), ("bf16", 1, 128), ("fp16", 4, 64)])
+def test_write_many_short_rows(dt, Hkv, D):
+    # rows of 1, 9, 30, 16 and 32 chunks, several rows a wave (64, 7, 2, 4, 2), heads apart in the pool
+    L, N, lens = 2, 5500, [5500, 3000, 5511]
+    table = po.draw_table(po.rng(dt, D), lens, 32, 173, 460)
+    kc, vc = pools(L, 460, 32, Hkv, D, dt)
+    vc = vc.transpose(2, 3).contiguous().transpose(2, 3)
+    k, v = pools(L, 3, N, Hkv, D, dt, seed=1)
+    want = po.write(kc, vc, k, v, lens, table)
+    fa.paged_cache_write_v100(k, v, kc, vc, ints(lens), ints(table))
+    same((kc, vc), want)
+
+
 def test_write_rows_strides_and_no_pages():
     # rows of tokens; strided inputs and pools; pages that are none; lengths past the room
     kc, vc = pools(1, 3, 50, 2, 64, "fp16")
