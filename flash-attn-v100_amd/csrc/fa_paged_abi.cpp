@@ -97,7 +97,11 @@ void plan(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared
         return (double)c.batch * c.num_heads_kv * ceil_div<int64_t>(p.Sk, keys) * tiles / workgroups;
     };
     auto full = [&](int64_t unit) { return (double)rows / (double)(unit * ceil_div<int64_t>(rows, unit)); };
-    if (f32 || rows <= 32 || busy(32, 128, 512) * full(128) < 8)
+    // Short sequences, whose units cost their beginnings and ends (trees of 64 over up to 300: 32
+    // sequences 57 -> 33, 16 31 -> 24, 8 17 -> 22; of 12: 32 sequences 18 -> 25): where units alone
+    // fill the device and are filled by their rows.
+    const double units128 = (double)c.batch * c.num_heads_kv * ceil_div<int64_t>(rows, 128);
+    if (f32 || rows <= 32 || (busy(32, 128, 512) * full(128) < 8 && units128 * full(128) * full(128) < 140))
         p.wide = 1;
     else
         p.wide = !d128 || rows <= 128 || busy(256, 64, 256) * full(256) < 40 ? 4 : 8;
@@ -117,9 +121,12 @@ void plan(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared
     // Where it is launched, all of more than `alone` steps are, down to `least` a workgroup.  us
     // with units of 4 steps whole / shared: trees of 12 over up to 1000 21.7 / 16.3; least of 1, 2
     // and 4: of 24 over up to 4000 21.0, 18.5, 20.6; one token over 8192 16.2, 15.3, 16.6.
-    // float32, whose steps take longer, from the second step on.
-    const int join_from = f32 ? 1 : 4;
-    p.alone = p.wide == 1 && most > join_from ? 1 : 4;
+    // float32, whose steps take longer, from the third step on (64 tokens over up to 250 keys, 16 on 8
+    // heads of 128: 51 us shared from the second on, 46 so); wide units, whose parts are large,
+    // from the ninth (16 trees of 64 over up to 300 keys 37 us shared, 24 whole; 16 trees of 48 over
+    // up to 600, head dim 64, 29 and, were they whole, 33).
+    const int join_from = f32 ? 2 : p.wide == 1 ? 4 : 8;
+    p.alone = p.wide == 1 ? (most > join_from ? 1 : 4) : 8;
     p.least = f32 || (p.wide == 1 && most <= 16) ? 1 : p.wide == 1 ? 2 : 4;
     // a wide unit's tree, rows and parts take about as long as 3 of its steps: 16 x 8192, trees of
     // 64: 166 us without, 158 with them in the balance

@@ -92,6 +92,23 @@ def test_units_shared_by_workgroups(dt, D, N, tree):
     run(*t[:3], lens, t[3], f"{dt} {N}", [po.draw_tree(rng, N) for _ in lens] if tree else None)
 
 
+@pytest.mark.parametrize("dt,D,N", [("bf16", 128, 1), ("fp16", 64, 15), ("fp32", 64, 3), ("fp32", 128, 1)])
+def test_units_in_many_parts(dt, D, N):
+    # one long sequence beside a short one and an empty one: more than 40 parts of a unit
+    lens = [12000 + N] if dt != "fp32" else [11000, 0]
+    t = make(lens, N, 768, 16, 4, 2, D, dt, seed=D + N)
+    run(*t[:3], lens, t[3], f"{dt} D={D} N={N}")
+
+
+@pytest.mark.parametrize("dt,D", [("bf16", 128), ("fp16", 64), ("bf16", 32)])
+@pytest.mark.parametrize("tree", [False, True])
+def test_wide_units_of_short_sequences(dt, D, tree):
+    N, lens = 64, [64, 300, 299, 65, 0, 128, 192, 256, 257, 31, 100, 320, 270, 64, 127, 129]
+    t = make(lens, N, 20, 16, 32, 8, D, dt, seed=D)
+    par = [po.draw_tree(po.rng("short", b), N) for b in range(len(lens))] if tree else None
+    run(*t[:3], lens, t[3], f"{dt} D={D} tree={tree}", par)
+
+
 def test_many_sequences():
     rng = po.rng("many")
     lens = [rng.randint(0, 700) for _ in range(150)]
