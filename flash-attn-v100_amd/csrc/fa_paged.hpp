@@ -384,6 +384,21 @@ __device__ FA_INLINE inline void reads_ahead() {
     }
 }
 
+// STEPS times a read of LDS and the products that take it, read AHEAD steps ahead
+template <int STEPS, int AHEAD, typename V, typename R, typename M>
+__device__ FA_INLINE inline void read_ahead(R&& read, M&& products) {
+    V v[STEPS];
+#pragma unroll
+    for (int i = 0; i < (AHEAD < STEPS ? AHEAD : STEPS); ++i) v[i] = read(i);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        if (i + AHEAD < STEPS) v[i + AHEAD] = read(i + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);  // (else they are read where they are used)
+        products(i, v[i]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 // Scores of one block of 32 keys (D / 16 products) beside the exponentials of another, then
 // that one's values (D / 16 products, two reads each) beside the maximum of the scores
 template <int D>
@@ -419,17 +434,19 @@ __device__ FA_INLINE inline void tile_scores(f32x16 (&s)[NB], const T* Ks, const
 #pragma unroll
     for (int x = 0; x < NB; ++x) s[x] = f32x16{};
     if constexpr (C::F32) {
+        static_assert(NB == 1, "float32 takes one block");
+        auto go = [&](auto steps) FA_INLINE {
+            read_ahead<decltype(steps)::value, 2, f32x4>([&](int kk) FA_INLINE { return lds_at<f32x4>(at ^ (kk << 5)); },
+                                                         [&](int kk, const f32x4& a) FA_INLINE {
+                                                             const f32x4 b = __builtin_bit_cast(f32x4, q[kk]);
 #pragma unroll
-        for (int kk = 0; kk < D / 8; ++kk) {
-            if (kk >= D / 16 && 8 * kk >= cols) break;
-#pragma unroll
-            for (int x = 0; x < NB; ++x) {
-                const f32x4 a = lds_at<f32x4>((at ^ (kk << 5)) + x * 32 * C::ROWB);
-                const f32x4 b = __builtin_bit_cast(f32x4, q[kk]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[x] = mfma_f32(a[e], b[e], s[x]);
-            }
-        }
+                                                             for (int e = 0; e < 4; ++e) s[0] = mfma_f32(a[e], b[e], s[0]);
+                                                         });
+        };
+        if (cols > 3 * D / 4)
+            go(template_int<D / 8>{});
+        else
+            go(template_int<3 * D / 32>{});
     } else {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
@@ -448,15 +465,28 @@ __device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16 (&s)[NB],
     if constexpr (C::F32) {
         // rows 8 (x / 4) + 4 hi + x % 4: their swizzles differ from that of row 4 hi by x alone
         const uint32_t at = lds_place(Vs, 4 * hi * C::ROWB + (((l32 >> 2) ^ row_swizzle<C::CW>(4 * hi)) << 4) + 4 * (l32 & 3));
+        auto go = [&](auto blocks) FA_INLINE {
+            constexpr int N = decltype(blocks)::value;
+            struct Row {
+                float v[N];
+            };
+            read_ahead<16, 2, Row>(
+                [&](int x) FA_INLINE {
+                    const int r = 8 * (x >> 2) + (x & 3);
+                    Row row;
 #pragma unroll
-        for (int x = 0; x < 16 * NB; ++x) {
-            const int r = 8 * (x >> 2) + (x & 3);
+                    for (int n = 0; n < N; ++n) row.v[n] = lds_at<float>((at ^ (((8 * n) ^ row_swizzle<C::CW>(r)) << 4)) + r * C::ROWB);
+                    return row;
+                },
+                [&](int x, const Row& row) FA_INLINE {
 #pragma unroll
-            for (int n = 0; n < D / 32; ++n) {
-                if (n > 0 && 32 * n >= cols) break;
-                o[n] = mfma_f32(lds_at<float>((at ^ (((8 * n) ^ row_swizzle<C::CW>(r)) << 4)) + r * C::ROWB), s[x >> 4][x & 15], o[n]);
-            }
-        }
+                    for (int n = 0; n < N; ++n) o[n] = mfma_f32(row.v[n], s[0][x], o[n]);
+                });
+        };
+        if (D <= 64 || cols > 96)
+            go(template_int<D / 32>{});
+        else
+            go(template_int<(D > 32 ? D / 32 - 1 : 1)>{});
     } else {
         const int r0 = 4 * hi + ((lane & 15) >> 2);
         const int chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
