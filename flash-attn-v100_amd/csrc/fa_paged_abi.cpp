@@ -116,17 +116,22 @@ void plan(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared
     int64_t groups = slots / units;
     if (groups * units * 7 < slots * 6) groups = 2 * slots / units;
     p.groups = (int)std::max<int64_t>(groups, 1);
-    // Where no sequence has room for more than 4 steps, units are not shared: the join would
-    // cost more than it saves (one token of 8 heads over 512 keys 8.4 us, with a join 11.0).
-    // Where it is launched, all of more than `alone` steps are, down to `least` a workgroup.  us
-    // with units of 4 steps whole / shared: trees of 12 over up to 1000 21.7 / 16.3; least of 1, 2
-    // and 4: of 24 over up to 4000 21.0, 18.5, 20.6; one token over 8192 16.2, 15.3, 16.6.
+    // Units are shared where a sequence has room for more than join_from steps: below, the join
+    // costs more than it saves, the more so the more units there are beside it.  us of one token
+    // of each of B sequences on 8 and 4 heads, shared / whole: B x up to 600 keys (5 steps), 16 x 8
+    // heads 17.6 / 15.3, 64 x 8 37 / 26; 1000 keys (8 steps), 64 x 4 21 / 16.7, 16 x 8 24.7 / 18.5, the
+    // other way 16 x 4 13.8 / 14.6; 2000 (16 steps), 64 x 8 83 / 74, the other way 16 x 4 20 / 23.
+    // Where the join is launched all the same (tables with room for more than the sequences hold),
+    // what is found to be of `alone` steps at most stays whole: 64 sequences of 150 to 600 of 4096
+    // keys, 8 heads, 36 us shared, 31 whole.  Others are shared down to `least` a workgroup.  us with units of 4 steps whole / shared: trees of 12 over up to 1000 21.7 / 16.3;
+    // least of 1, 2 and 4: of 24 over up to 4000 21.0, 18.5, 20.6; one token over 8192 16.2, 15.3, 16.6.
     // float32, whose steps take longer, from the third step on (64 tokens over up to 250 keys, 16 on 8
     // heads of 128: 51 us shared from the second on, 46 so); wide units, whose parts are large,
     // from the ninth (16 trees of 64 over up to 300 keys 37 us shared, 24 whole; 16 trees of 48 over
-    // up to 600, head dim 64, 29 and, were they whole, 33).
-    const int join_from = f32 ? 2 : p.wide == 1 ? 4 : 8;
-    p.alone = p.wide == 1 ? (most > join_from ? 1 : 4) : 8;
+    // up to 600, head dim 64, 29 and, were they whole, 33; 4 chunks of 500 of 600, head dim 64, 37 / 33).
+    const int64_t all = units * c.batch;
+    const int64_t join_from = f32 ? 2 : p.wide == 1 ? 5 + all / 32 : std::max<int64_t>(8, 4 + all / 64);
+    p.alone = (int)std::min<int64_t>(p.wide == 1 ? std::max<int64_t>(all / 32, 1) : join_from, INT32_MAX);
     p.least = f32 || (p.wide == 1 && most <= 16) ? 1 : p.wide == 1 ? 2 : 4;
     // a wide unit's tree, rows and parts take about as long as 3 of its steps: 16 x 8192, trees of
     // 64: 166 us without, 158 with them in the balance

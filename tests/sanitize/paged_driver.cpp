@@ -62,7 +62,7 @@ hipError_t launch_paged(const PagedParams& p, int D, hipStream_t) {
         }
         CHECK(steps < (1LL << 31));
         int64_t W = std::min<int64_t>(p.groups, (steps + p.least - 1) / p.least);
-        const bool whole = W <= 1 || most - p.extra <= std::max<int64_t>(p.alone, (steps + W - 1) / W);
+        const bool whole = !p.part || W <= 1 || most - p.extra <= std::max<int64_t>(p.alone, (steps + W - 1) / W);
         if (whole) W = p.B;
         CHECK(W * units <= p.o_wgs);
         if (!whole) {
