@@ -109,6 +109,15 @@ def test_wide_units_of_short_sequences(dt, D, tree):
     run(*t[:3], lens, t[3], f"{dt} D={D} tree={tree}", par)
 
 
+@pytest.mark.parametrize("dt,D,tree", [("bf16", 128, True), ("fp16", 96, False)])
+def test_units_of_256_rows(dt, D, tree):
+    # room that makes the units the widest, in sequences of all lengths
+    N, lens = 64, [8192, 100, 0, 4000, 64, 65, 700, 2500, 1, 3000]
+    t = make(lens, N, 512, 16, 32, 8, D, dt, seed=D)
+    par = [po.draw_tree(po.rng("wide", b), N) for b in range(len(lens))] if tree else None
+    run(*t[:3], lens, t[3], f"{dt} D={D} tree={tree}", par)
+
+
 def test_many_sequences():
     rng = po.rng("many")
     lens = [rng.randint(0, 700) for _ in range(150)]
@@ -117,6 +126,17 @@ def test_many_sequences():
     run(*t[:3], lens, t[3], "150 sequences")
     t = make(lens, 4, 44, 16, 4, 1, 64, "bf16", seed=7)
     run(*t[:3], lens, t[3], "150 trees", [po.draw_tree(rng, 4) for _ in lens])
+
+
+@pytest.mark.parametrize("B,N,dt,D,room", [(150, 1, "bf16", 64, 4800), (130, 4, "fp32", 32, 1600), (70, 64, "fp16", 128, 1152)])
+def test_many_sequences_share_units(B, N, dt, D, room):
+    # more sequences than lanes, some much longer than the others
+    rng = po.rng("share", B)
+    lens = [rng.randint(0, 300) for _ in range(B)]
+    for b in (3, 64, B - 1):
+        lens[b] = rng.randint(room * 3 // 4, room)
+    t = make(lens, N, room // 16, 16, 4, 1, D, dt, seed=B)
+    run(*t[:3], lens, t[3], f"{B} sequences", [po.draw_tree(rng, N) for _ in lens] if N > 1 else None)
 
 
 @pytest.mark.parametrize("N", [1, 2, 31, 32, 33, 64, 65, 128, 256])
