@@ -130,6 +130,7 @@ struct PagedParams : RowsParams {
     int unit_tiles, groups;
     int alone, least;      // steps of sequences that are not shared; those of a group, at least
     int many;              // a sequence may be in many parts
+    int2* spans;           // (B) for the join: first and last group
     int extra;             // steps that a unit counts beside its keys'
     int wide;              // waves of a unit of 32 rows each that share its tiles; 1: of 32 rows, whose waves share its keys
 };

@@ -289,22 +289,15 @@ struct PagedWork {
             before += __builtin_amdgcn_readlane(inc, 63);
         }
     }
-    // the first step of sequence b, and its steps
+    // for the join: the first and the last group of every sequence (the same one where it is whole)
     template <int STEP>
-    __device__ FA_INLINE inline void sequence(PagedArgs& p, int b, int lane, int& start, int& len) const {
-        if (!p.lens) {
-            len = steps<STEP>(p, 0);
-            start = b * len;
-        } else if (b < 64) {
-            len = __builtin_amdgcn_readlane(st0, b);
-            start = __builtin_amdgcn_readlane(inc0, b) - len;
-        } else {
-            int sum = st0;
-            for (int b0 = 64; b0 < b; b0 += 64) sum += b0 + lane < b ? steps<STEP>(p, b0 + lane) : 0;
-#pragma unroll
-            for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
-            len = __builtin_amdgcn_readfirstlane(steps<STEP>(p, b));
-            start = __builtin_amdgcn_readfirstlane(sum);
+    __device__ FA_INLINE inline void spans(PagedArgs& p, int lane) const {
+        int before = 0;
+        for (int b0 = 0; b0 < p.B; b0 += 64) {
+            const int b = b0 + lane, st = b0 || whole || !p.lens ? steps<STEP>(p, b) : st0;
+            const int inc = scan(st, lane), start = before + inc - st;
+            if (b < p.B) p.spans[b] = whole ? make_int2(0, 0) : make_int2(whose(start), whose(start + st - p.extra - 1));
+            before += __builtin_amdgcn_readlane(inc, 63);
         }
     }
 };
@@ -1063,6 +1056,7 @@ __global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 * Pag
     const int tid = threadIdx.x, lane = tid & 63;
     PagedWork wk;
     wk.init<S::STEP>(p, lane);
+    if (p.part && blockIdx.x == gridDim.x - 1 && tid < 64) wk.spans<S::STEP>(p, lane);
     const int units = p.Hkv * p.unit_tiles, extra = p.extra;
     if ((int64_t)blockIdx.x >= (int64_t)wk.W * units) return;
     const int g = xcd_remap((int)blockIdx.x, wk.W * units), group = g / units, u = g - group * units;
@@ -1116,12 +1110,9 @@ __global__ __launch_bounds__((64 * JoinShape<D, NW, MANY>::G * JoinShape<D, NW, 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, hi = lane >> 5, b = blockIdx.z;
     const int w = wave % G, block = wave / G, n = blockIdx.y * J::BLOCKS + block;
-    PagedWork wk;
-    wk.init<S::STEP>(p, lane);
-    if (wk.whole) return;
-    int start, len;
-    wk.sequence<S::STEP>(p, b, lane, start, len);
-    const int g0 = wk.whose(start), g1 = wk.whose(start + len - p.extra - 1);
+    // (found again from the lengths, it took half a microsecond of a join's 5)
+    const int2 span = p.spans[b];
+    const int g0 = __builtin_amdgcn_readfirstlane(span.x), g1 = __builtin_amdgcn_readfirstlane(span.y);
     if (g0 == g1) return;
     const int units = p.Hkv * p.unit_tiles, u = blockIdx.x / NW, r0 = 32 * (blockIdx.x % NW);
     const PagedRow row(p, S::ROWS * (u % p.unit_tiles) + r0 + l32, u / p.unit_tiles);

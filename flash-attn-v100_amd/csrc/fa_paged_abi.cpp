@@ -146,7 +146,8 @@ void plan(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared
 size_t part_rows(const PagedParams& p, int64_t shared) { return (size_t)(2 * shared * unit_rows(p)); }
 size_t paged_bytes(const PagedParams& p, int64_t shared) {
     if (!shared) return 0;
-    return up256(part_rows(p, shared) * sizeof(float2)) + up256(part_rows(p, shared) * compiled_dim(p.cols) * sizeof(float));
+    return up256(part_rows(p, shared) * sizeof(float2)) + up256(p.B * sizeof(int2)) +
+           up256(part_rows(p, shared) * compiled_dim(p.cols) * sizeof(float));
 }
 
 void put_paged(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared) {
@@ -230,7 +231,8 @@ int32_t fa_paged_fwd(const fa_paged_args* a, void* workspace, size_t bytes, void
     if (need && (!workspace || bytes < need || !aligned(workspace, 16))) return FA_ERR_WORKSPACE;
     if (need) {
         p.stat = (float2*)workspace;
-        p.part = (float*)((char*)workspace + up256(part_rows(p, shared) * sizeof(float2)));
+        p.spans = (int2*)((char*)workspace + up256(part_rows(p, shared) * sizeof(float2)));
+        p.part = (float*)((char*)p.spans + up256(p.B * sizeof(int2)));
     }
     const int D = compiled_dim(p.cols);
     hipStream_t s = (hipStream_t)stream;

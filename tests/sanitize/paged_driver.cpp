@@ -69,7 +69,7 @@ hipError_t launch_paged(const PagedParams& p, int D, hipStream_t) {
             CHECK(p.part && p.stat);
             const double parts = 2.0 * W * units * unit;
             CHECK(inside(p.stat, 8 * parts) && inside(p.part, 4 * parts * D));
-            CHECK((double)((char*)p.part - (char*)p.stat) >= 8 * parts);
+            CHECK((double)((char*)p.spans - (char*)p.stat) >= 8 * parts && (char*)p.part - (char*)p.spans >= 8LL * p.B);
             CHECK(grid((double)units * p.wide, 512, 4, p.B));
         }
     }
