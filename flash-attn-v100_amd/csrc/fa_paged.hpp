@@ -1110,7 +1110,7 @@ __global__ __launch_bounds__((64 * JoinShape<D, NW, MANY>::G * JoinShape<D, NW, 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l32 = lane & 31, hi = lane >> 5, b = blockIdx.z;
     const int w = wave % G, block = wave / G, n = blockIdx.y * J::BLOCKS + block;
-    // (found again from the lengths, it took half a microsecond of a join's 5)
+    // (found again from the lengths, it took 1.3 us of the 6.2 of a join of 32 tokens' parts)
     const int2 span = p.spans[b];
     const int g0 = __builtin_amdgcn_readfirstlane(span.x), g1 = __builtin_amdgcn_readfirstlane(span.y);
     if (g0 == g1) return;
