@@ -416,24 +416,22 @@ __device__ FA_INLINE inline void block_order() {
     }
 }
 
-// the products of a wave's 32 rows with NB blocks of 32 keys (K tile), log2 units before
+// the products of a wave's 32 rows with 32 keys (K tile), log2 units before
 // the rules (float32, whose products bound it: only over columns that exist)
 // (ORDERED: its place among other instructions is the caller's to say)
-template <typename T, int D, int NB, bool ORDERED = false>
-__device__ FA_INLINE inline void tile_scores(f32x16 (&s)[NB], const T* Ks, const uint4 (&q)[Elem<T>::kF32 ? D / 8 : D / 16], int cols,
+template <typename T, int D, bool ORDERED = false>
+__device__ FA_INLINE inline void tile_scores(f32x16& s, const T* Ks, const uint4 (&q)[Elem<T>::kF32 ? D / 8 : D / 16], int cols,
                                             int l32, int hi) {
     using C = PagedCfg<T, D>;
     const uint32_t at = lds_place(Ks, l32 * C::ROWB + ((hi ^ row_swizzle<C::CW>(l32)) << 4));
-#pragma unroll
-    for (int x = 0; x < NB; ++x) s[x] = f32x16{};
+    s = f32x16{};
     if constexpr (C::F32) {
-        static_assert(NB == 1, "float32 takes one block");
         auto go = [&](auto steps) FA_INLINE {
             read_ahead<decltype(steps)::value, 2, f32x4>([&](int kk) FA_INLINE { return lds_at<f32x4>(at ^ (kk << 5)); },
                                                          [&](int kk, const f32x4& a) FA_INLINE {
                                                              const f32x4 b = __builtin_bit_cast(f32x4, q[kk]);
 #pragma unroll
-                                                             for (int e = 0; e < 4; ++e) s[0] = mfma_f32(a[e], b[e], s[0]);
+                                                             for (int e = 0; e < 4; ++e) s = mfma_f32(a[e], b[e], s);
                                                          });
         };
         if (cols > 3 * D / 4)
@@ -443,16 +441,14 @@ __device__ FA_INLINE inline void tile_scores(f32x16 (&s)[NB], const T* Ks, const
     } else {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-#pragma unroll
-            for (int x = 0; x < NB; ++x)
-                s[x] = Elem<T>::mfma(lds_at<s16x8>((at ^ (kk << 5)) + x * 32 * C::ROWB), __builtin_bit_cast(s16x8, q[kk]), s[x]);
-        if constexpr (!ORDERED) reads_ahead<NB * D / 16, 1, NB * D / 16 < 6 ? NB * D / 16 : 6>();
+            s = Elem<T>::mfma(lds_at<s16x8>(at ^ (kk << 5)), __builtin_bit_cast(s16x8, q[kk]), s);
+        if constexpr (!ORDERED) reads_ahead<D / 16, 1, D / 16 < 6 ? D / 16 : 6>();
     }
 }
 
-// O^T += V^T P^T over NB blocks of 32 keys
-template <typename T, int D, int NB, bool ORDERED = false>
-__device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16 (&s)[NB], f32x16 (&o)[D / 32], int cols, int lane) {
+// O^T += V^T P^T over 32 keys
+template <typename T, int D, bool ORDERED = false>
+__device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16& s, f32x16 (&o)[D / 32], int cols, int lane) {
     using C = PagedCfg<T, D>;
     const int l32 = lane & 31, hi = lane >> 5;
     if constexpr (C::F32) {
@@ -473,7 +469,7 @@ __device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16 (&s)[NB],
                 },
                 [&](int x, const Row& row) FA_INLINE {
 #pragma unroll
-                    for (int n = 0; n < N; ++n) o[n] = mfma_f32(row.v[n], s[0][x], o[n]);
+                    for (int n = 0; n < N; ++n) o[n] = mfma_f32(row.v[n], s[x], o[n]);
                 });
         };
         if (D <= 64 || cols > 96)
@@ -484,23 +480,23 @@ __device__ FA_INLINE inline void tile_values(const T* Vs, const f32x16 (&s)[NB],
         const int r0 = 4 * hi + ((lane & 15) >> 2);
         const int chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
         const uint32_t at = lds_place(Vs, r0 * C::ROWB + ((chunk ^ row_swizzle<C::CW>(r0)) << 4) + 8 * (lane & 1));
-        s16x8 pk[2 * NB];
+        s16x8 pk[2];
 #pragma unroll
-        for (int ks = 0; ks < 2 * NB; ++ks) {
+        for (int ks = 0; ks < 2; ++ks) {
             float tmp[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) tmp[e] = s[ks >> 1][8 * (ks & 1) + e];
+            for (int e = 0; e < 8; ++e) tmp[e] = s[8 * ks + e];
             pk[ks] = pack8<T>(tmp);
         }
 #pragma unroll
-        for (int ks = 0; ks < 2 * NB; ++ks)
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
             for (int n = 0; n < D / 32; ++n) {
                 const s16x8 a = cat4(lds_tr16_at((at ^ (n << 6)) + 16 * ks * C::ROWB),
                                      lds_tr16_at((at ^ ((n << 6) ^ (row_swizzle<C::CW>(8) << 4))) + (16 * ks + 8) * C::ROWB));
                 o[n] = Elem<T>::mfma(a, pk[ks], o[n]);
             }
-        if constexpr (!ORDERED) reads_ahead<2 * NB * D / 32, 2, 2 * NB * D / 32 < 4 ? 4 * NB * D / 32 : 8>();
+        if constexpr (!ORDERED) reads_ahead<D / 16, 2, D / 16 < 4 ? D / 8 : 8>();
     }
 }
 
@@ -636,16 +632,14 @@ __device__ FA_INLINE inline void tile_rules(f32x16& s, TileRules<EXACT>& u, cons
     }
 }
 
-// The running maximum and sum of a row over NB more blocks of scores, which become
+// The running maximum and sum of a row over 32 more scores, which become
 // probabilities: e^(s - m) with an m that is at most 8 (of log2) behind the largest, so
 // that O is rescaled when a maximum grows by more
-template <int D, int NB>
-__device__ FA_INLINE inline void soft_max(const f32x16 (&s)[NB], float unit, float& m_run, float& l_run, f32x16 (&o)[D / 32]) {
+template <int D>
+__device__ FA_INLINE inline void soft_max(const f32x16& s, float unit, float& m_run, float& l_run, f32x16 (&o)[D / 32]) {
     float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int x = 0; x < NB; ++x)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) m4[e & 3] = fmaxf(m4[e & 3], s[x][e]);
+    for (int e = 0; e < 16; ++e) m4[e & 3] = fmaxf(m4[e & 3], s[e]);
     const float m_new = fmaxf(m_run, unit * pair_max(fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]))));
     if (__ballot(m_new > m_run + 8.0f) != 0ull) {
         const float alpha = fast_exp2(m_run - m_new);
@@ -657,16 +651,13 @@ __device__ FA_INLINE inline void soft_max(const f32x16 (&s)[NB], float unit, flo
         m_run = m_new;
     }
 }
-template <int NB>
-__device__ FA_INLINE inline void soft_exp(f32x16 (&s)[NB], float unit, float m_run, float& l_run) {
+__device__ FA_INLINE inline void soft_exp(f32x16& s, float unit, float m_run, float& l_run) {
     float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int x = 0; x < NB; ++x)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            s[x][e] = fast_exp2(__builtin_fmaf(s[x][e], unit, -m_run));
-            ps[e & 3] += s[x][e];
-        }
+    for (int e = 0; e < 16; ++e) {
+        s[e] = fast_exp2(__builtin_fmaf(s[e], unit, -m_run));
+        ps[e & 3] += s[e];
+    }
     l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
 }
 
@@ -750,24 +741,24 @@ __device__ FA_INLINE inline void paged_unit32(T* smem, float (*stat)[2][32], Tre
         constexpr bool HIDDEN = decltype(hidden)::value;
         wait_vmem_below<2 * C::NI16>();  // K(t); only V(t) may be in flight
         asm volatile("" ::: "memory");
-        f32x16 s[1];
-        tile_scores<T, D, 1>(s, Ks, q, kc.cols, l32, hi);
+        f32x16 s;
+        tile_scores<T, D>(s, Ks, q, kc.cols, l32, hi);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K(t) read before it is overwritten
         copy(kc, t + NW, bx, by, Ks);
 
         unsigned have = ~0u, seen = ~0u;
         if (HIDDEN && holes) have = (unsigned)table.template have<2>(2 * t);
-        tile_rules<EXACT, HIDDEN>(s[0], rules, row, tree, 32 * t, c, seen, have, hi);
-        soft_max<D, 1>(s, rules.unit, m_run, l_run, o);
-        soft_exp<1>(s, rules.unit, m_run, l_run);
+        tile_rules<EXACT, HIDDEN>(s, rules, row, tree, 32 * t, c, seen, have, hi);
+        soft_max<D>(s, rules.unit, m_run, l_run, o);
+        soft_exp(s, rules.unit, m_run, l_run);
 
         wait_vmem_below<2 * C::NI16>();  // V(t); only K(t + 4) may be in flight
         asm volatile("" ::: "memory");
         if (HIDDEN && uneven && tile_odd<T, D>(Vs, lane)) {
             stay_branch();
-            tile_values_seen<T, D>(Vs, s[0], seen, o, lane);
+            tile_values_seen<T, D>(Vs, s, seen, o, lane);
         } else {
-            tile_values<T, D, 1>(Vs, s, o, vc.cols, lane);
+            tile_values<T, D>(Vs, s, o, vc.cols, lane);
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V(t) read before it is overwritten
         copy(vc, t + NW, bx, by, Vs);
@@ -961,36 +952,36 @@ __device__ FA_INLINE inline void paged_unit_wide(T* smem, TreeBits* tree, bool n
         // the second block's scores beside the first one's exponentials, the first one's values
         // beside the second one's maximum
         unsigned seen;
-        f32x16 sa[1], sb[1];
-        tile_scores<T, D, 1>(sa, Ks, q, D, l32, hi);
-        tile_rules<EXACT, false>(sa[0], rules, row, tree, 64 * t, c, seen, ~0u, hi);
-        soft_max<D, 1>(sa, rules.unit, m_run, l_run, o);
-        tile_scores<T, D, 1, true>(sb, Ks + 32 * D, q, D, l32, hi);
-        soft_exp<1>(sa, rules.unit, m_run, l_run);
-        tile_values<T, D, 1, true>(Vs, sa, o, D, lane);
+        f32x16 sa, sb;
+        tile_scores<T, D>(sa, Ks, q, D, l32, hi);
+        tile_rules<EXACT, false>(sa, rules, row, tree, 64 * t, c, seen, ~0u, hi);
+        soft_max<D>(sa, rules.unit, m_run, l_run, o);
+        tile_scores<T, D, true>(sb, Ks + 32 * D, q, D, l32, hi);
+        soft_exp(sa, rules.unit, m_run, l_run);
+        tile_values<T, D, true>(Vs, sa, o, D, lane);
         block_order<D>();
-        tile_rules<EXACT, false>(sb[0], rules, row, tree, 64 * t + 32, c, seen, ~0u, hi);
-        soft_max<D, 1>(sb, rules.unit, m_run, l_run, o);
-        soft_exp<1>(sb, rules.unit, m_run, l_run);
-        tile_values<T, D, 1>(Vs + 32 * D, sb, o, D, lane);
+        tile_rules<EXACT, false>(sb, rules, row, tree, 64 * t + 32, c, seen, ~0u, hi);
+        soft_max<D>(sb, rules.unit, m_run, l_run, o);
+        soft_exp(sb, rules.unit, m_run, l_run);
+        tile_values<T, D>(Vs + 32 * D, sb, o, D, lane);
     }
     for (; t < t1; ++t) {
         const T* const Ks = next_tile(t);
 #pragma unroll 1
         for (int x = 0; x < 2; ++x) {
             const T* const Vs = Ks + X::TILE + x * 32 * D;
-            f32x16 s[1];
-            tile_scores<T, D, 1>(s, Ks + x * 32 * D, q, D, l32, hi);
+            f32x16 s;
+            tile_scores<T, D>(s, Ks + x * 32 * D, q, D, l32, hi);
             unsigned have = ~0u, seen;
             if (holes) have = (unsigned)table.template have<2>(4 * t + 2 * x);
-            tile_rules<EXACT, true>(s[0], rules, row, tree, 64 * t + 32 * x, c, seen, have, hi);
-            soft_max<D, 1>(s, rules.unit, m_run, l_run, o);
-            soft_exp<1>(s, rules.unit, m_run, l_run);
+            tile_rules<EXACT, true>(s, rules, row, tree, 64 * t + 32 * x, c, seen, have, hi);
+            soft_max<D>(s, rules.unit, m_run, l_run, o);
+            soft_exp(s, rules.unit, m_run, l_run);
             if (uneven && tile_odd<T, D>(Vs, lane)) {
                 stay_branch();
-                tile_values_seen<T, D>(Vs, s[0], seen, o, lane);
+                tile_values_seen<T, D>(Vs, s, seen, o, lane);
             } else {
-                tile_values<T, D, 1>(Vs, s, o, D, lane);
+                tile_values<T, D>(Vs, s, o, D, lane);
             }
         }
     }
