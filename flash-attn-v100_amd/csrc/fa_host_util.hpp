@@ -31,6 +31,14 @@ inline void put_strides(int64_t (&dst)[4], const at::Tensor& t) {
     for (int d = 0; d < 4; ++d) dst[d] = t.stride(d);
 }
 
+// t has been written, as far as autograd's saved tensors are concerned too.  A tensor made in
+// inference mode has no version (and autograd saves none): bump() would raise for it outside of
+// that mode, after the kernels have been enqueued.
+inline void written(const at::Tensor& t) {
+    c10::TensorImpl* const x = t.unsafeGetTensorImpl();
+    if (x->version_counter().enabled()) x->bump_version();
+}
+
 extern PyMethodDef ops_methods[];    // fa_ops_host.cpp
 extern PyMethodDef paged_methods[];  // fa_paged_host.cpp
 

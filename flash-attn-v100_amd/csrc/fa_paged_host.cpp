@@ -246,10 +246,9 @@ PyObject* paged_fwd(PyObject*, PyObject* const* x, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// pools have changed, as far as autograd's saved tensors are concerned too
 void changed(const at::Tensor& k, const at::Tensor& v) {
-    k.unsafeGetTensorImpl()->bump_version();
-    v.unsafeGetTensorImpl()->bump_version();
+    fa_host::written(k);
+    fa_host::written(v);
 }
 
 // cache_write(k_new, v_new, k, v, lengths, table (or None each), stream) -> status

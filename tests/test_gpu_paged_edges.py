@@ -1,0 +1,46 @@
+"""The paged cache's entry points at their edges: pools and tensors made in inference
+mode."""
+import pytest
+import torch
+
+import flash_attention_v100 as fa
+import paged_oracle as po
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def ints(x, dtype=torch.int32):
+    return torch.tensor(x, dtype=dtype, device=DEV)
+
+
+def randn(*shape, seed=0, dt=torch.float16):
+    return torch.randn(*shape, generator=torch.Generator("cpu").manual_seed(seed)).to(dt).to(DEV)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_pools_of_inference_mode_used_outside_of_it(grad):
+    # such pools have no version that autograd could look at: they are written as others are
+    L, P, size, Hkv, D, N = 2, 12, 16, 2, 64, 5
+    lens, table = [20, 9, 0], [[3, 7, -1], [1, -1, -1], [-1, -1, -1]]
+    with torch.inference_mode():
+        kc, vc = randn(L, P, size, Hkv, D, seed=1), randn(L, P, size, Hkv, D, seed=2)
+        k, v = randn(L, 3, N, Hkv, D, seed=3), randn(L, 3, N, Hkv, D, seed=4)
+    assert kc.is_inference()
+    with torch.set_grad_enabled(grad):
+        want = po.write(kc, vc, k, v, lens, table)
+        fa.paged_cache_write_v100(k, v, kc, vc, ints(lens), ints(table))
+        assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+        path = [[1, 4, -1], [0, 2, 3], [0, -1, -1]]
+        want = po.accept(kc, vc, lens, path, N, table)
+        got = fa.paged_cache_accept_v100(kc, vc, ints(lens), ints(path), N, ints(table))
+        assert torch.equal(kc, want[0]) and torch.equal(vc, want[1]) and got.tolist() == want[2]
+        sources, lens = [0, 0, 1, -1], want[2]
+        want = po.fork(kc, vc, table, lens, sources, [2] * 4)
+        new, filled = fa.paged_cache_fork_v100(kc, vc, ints(table), ints(lens), ints(sources), 2)
+        assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+        assert new.tolist() == want[2] and filled.tolist() == want[3]
+        want = po.compact(kc, vc, want[2], want[3])
+        new, used = fa.paged_cache_compact_v100(kc, vc, new, filled)
+        assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+        assert new.tolist() == want[2] and int(used) == want[3]
