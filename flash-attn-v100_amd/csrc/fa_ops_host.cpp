@@ -401,9 +401,9 @@ PyObject* rotary(PyObject*, PyObject* const* x, Py_ssize_t n) {
         pybind11::gil_scoped_release no_gil;
         st = p_rotary(&a, stream);
     }
-    if (inplace && !st) {  // the inputs have changed, as far as autograd's saved tensors are concerned too
-        q.unsafeGetTensorImpl()->bump_version();
-        if (k.defined()) k.unsafeGetTensorImpl()->bump_version();
+    if (inplace && !st) {
+        fa_host::written(q);
+        if (k.defined()) fa_host::written(k);
     }
     return Py_BuildValue("(iNN)", (int)st, THPVariable_Wrap(qo), wrap_or_none(ko));
     END_HANDLE_TH_ERRORS

@@ -1,5 +1,5 @@
 """The paged cache's entry points at their edges: pools and tensors made in inference
-mode."""
+mode, also rotated in place."""
 import pytest
 import torch
 
@@ -44,3 +44,13 @@ def test_pools_of_inference_mode_used_outside_of_it(grad):
         new, used = fa.paged_cache_compact_v100(kc, vc, new, filled)
         assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])
         assert new.tolist() == want[2] and int(used) == want[3]
+
+
+def test_rotation_in_place_of_tensors_of_inference_mode():
+    table = fa.rotary_table_v100(32, 64)
+    with torch.inference_mode():
+        q, k = randn(2, 8, 4, 64, seed=5), randn(2, 8, 2, 64, seed=6)
+    want = fa.rotary_embedding_v100(q, k, table)
+    with torch.no_grad():
+        got = fa.rotary_embedding_v100(q, k, table, inplace=True)
+    assert got[0].data_ptr() == q.data_ptr() and torch.equal(q, want[0]) and torch.equal(k, want[1])
