@@ -288,9 +288,11 @@ class EnhancedMultiHeadAttention(nn.Module):
         (N, B, E) as ``batch_first`` says, whose keys and values it writes into the cache
         (:func:`paged_cache_write_v100`) and then attends over
         (:func:`flash_attention_v100_paged`): causal, or through the tree of
-        ``parents``.  ``key_lengths`` count the new tokens.  ``positions``: their rotary
-        positions, (B, N) or (N,): their places in the sequence by default, to be given
-        with ``parents`` (a tree's tokens stand at the context's length and their depth).
+        ``parents``.  ``key_lengths`` count the new tokens; one past the cache's room counts as
+        the room, so that the new tokens take the last places of a full cache.
+        ``positions``: their rotary positions, (B, N) or (N,): their places in the sequence
+        by default, to be given with ``parents`` (a tree's tokens stand at the context's
+        length and their depth).
         With ``softcap`` and ``distance_bias``; no dropout, no gradients."""
         if self.training and self.dropout > 0.0:
             raise ValueError("decode has no attention dropout: call eval() or use dropout=0.0")
@@ -302,11 +304,13 @@ class EnhancedMultiHeadAttention(nn.Module):
             if positions is None:
                 if parents is not None:
                     raise ValueError("a tree's rotary positions must be given")
+                room = k_cache.shape[-3] * (1 if page_table is None else page_table.shape[1])
                 n = key_lengths
                 if n is None:
-                    room = k_cache.shape[-3] * (1 if page_table is None else page_table.shape[1])
                     n = torch.full((B,), room, dtype=torch.int32, device=q.device)
-                positions = n[:, None] - N + torch.arange(N, dtype=n.dtype, device=q.device)
+                else:
+                    n = n.clamp(max=room)  # as the cache's operators count them
+                positions = n[:, None] + torch.arange(-N, 0, dtype=n.dtype, device=q.device)
             q, k = rotary_embedding_v100(q, k, self._rotary_table(q.device), positions, interleaved=self.rotary_interleaved)
         elif positions is not None:
             raise ValueError("positions need rotary_dim > 0")

@@ -67,7 +67,7 @@ def flash_attention_v100_paged(
     is no page holds no keys.  Without a table (B, S, Hkv, D): a row of tokens a
     sequence.  They are read as they are, never copied.
     ``key_lengths``: (B,) filled tokens, the new ones among them; all there is room
-    for without it.  Token i lies at place ``key_lengths[b] - N + i``; at a negative
+    for without it, and where they are more than that (M pages, or S).  Token i lies at place ``key_lengths[b] - N + i``; at a negative
     one (a free slot of the batch has length 0) it sees nothing: zero output, LSE
     -inf.
     ``parents``: (N,) or (B, N): the token that each one follows, an index below its

@@ -5,7 +5,11 @@ A cache is a pool of pages, ``k_cache`` and ``v_cache`` (pages, page_size, Hkv, 
 (layers, pages, page_size, Hkv, D) where one table serves several layers, with a
 ``page_table`` (B, M) and ``key_lengths`` (B,).  A page is in use while it is among
 the first ``ceil(key_lengths[b] / page_size)`` columns of a sequence: freeing one is
-setting its length to 0.  Everything is read and decided on the GPU (no host
+setting its length to 0.  A length counts as 0 where it is negative, and as the room, M
+pages, where it is more: a sequence that is told to grow past it stays full, and the new
+tokens that are written take its last places, over the rows that were there (a caller that
+may reach the end asks :func:`paged_cache_fork_v100` for room, which has none to give, or
+counts).  Everything is read and decided on the GPU (no host
 synchronisation), and every call may be captured into a HIP graph.  A number that is
 no page holds nothing: nothing is written to it or moved from it.
 """
@@ -27,8 +31,8 @@ def paged_cache_write_v100(
     page_table: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Writes k, v (B, N, Hkv, D), the newest N tokens of each sequence, into the cache:
-    token i at place ``key_lengths[b] - N + i`` (the lengths count them), a negative
-    place is left out.  With a leading dimension of layers on the cache, k and v have
+    token i at place ``key_lengths[b] - N + i`` (the lengths count them, up to the room), a
+    negative place is left out.  With a leading dimension of layers on the cache, k and v have
     it too.  Without ``page_table`` the cache is (B, S, Hkv, D), a row of tokens a
     sequence.  Returns (k_cache, v_cache), which are written in place; two sequences
     that share a page must not write the same place of it.
