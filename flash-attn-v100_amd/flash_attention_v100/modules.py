@@ -292,7 +292,10 @@ class EnhancedMultiHeadAttention(nn.Module):
         the room, so that the new tokens take the last places of a full cache.
         ``positions``: their rotary positions, (B, N) or (N,): their places in the sequence
         by default, to be given with ``parents`` (a tree's tokens stand at the context's
-        length and their depth).
+        length and their depth).  A token at ``max_positions`` or past it becomes NaN, in the
+        output and in the row of its key, which only tokens behind it see; nothing is raised
+        for it where the positions are on the GPU only (without lengths, where they are known,
+        ``ValueError``).
         With ``softcap`` and ``distance_bias``; no dropout, no gradients."""
         if self.training and self.dropout > 0.0:
             raise ValueError("decode has no attention dropout: call eval() or use dropout=0.0")
@@ -307,6 +310,8 @@ class EnhancedMultiHeadAttention(nn.Module):
                 room = k_cache.shape[-3] * (1 if page_table is None else page_table.shape[1])
                 n = key_lengths
                 if n is None:
+                    if room > self.max_positions:
+                        raise ValueError(f"{room} tokens exceed max_positions={self.max_positions}")
                     n = torch.full((B,), room, dtype=torch.int32, device=q.device)
                 else:
                     n = n.clamp(max=room)  # as the cache's operators count them

@@ -1,4 +1,5 @@
-"""The layer's decode() over a paged cache: lengths past the cache's room."""
+"""The layer's decode() over a paged cache: lengths past the cache's room, positions
+past the rotary table."""
 import pytest
 import torch
 
@@ -36,3 +37,24 @@ def test_lengths_past_the_room_count_as_the_room(paged, dtype):
         outs.append((m.decode(x, kc, vc, ints(lens, dtype), table), kc, vc))
     for a, b in zip(*outs):
         assert torch.equal(a, b)
+
+
+def test_positions_past_the_table():
+    # known on the host: a full cache of more room than the table; else NaN, of such tokens alone
+    m = layer(torch.float32, rotary_dim=64, max_positions=40)
+    far = layer(torch.float32, rotary_dim=64, max_positions=100)
+    far.load_state_dict(m.state_dict())
+    table = ints([[2, 0, 4], [5, 1, 3]])
+    start = randn(6, 16, 4, 64, seed=3), randn(6, 16, 4, 64, seed=4)
+    x = randn(2, 3, 256, seed=5)
+    with pytest.raises(ValueError, match="max_positions"):
+        m.decode(x, *start, None, table)
+    pools = [tuple(t.clone() for t in start) for _ in range(2)]
+    # places 38, 39 | 40 of the first sequence and all of the second one
+    o, want = (a.decode(x, *p, ints([41, 20]), table) for a, p in zip((m, far), pools))
+    assert o[0, 2].isnan().all()
+    assert torch.equal(o[0, :2], want[0, :2]) and torch.equal(o[1], want[1])
+    # a sequence that is cut back to where it ended is what it was
+    y = randn(2, 1, 256, seed=6)
+    o, want = (a.decode(y, *p, ints([40, 21]), table) for a, p in zip((m, far), pools))
+    assert torch.equal(o, want)
