@@ -249,7 +249,8 @@ int32_t fa_cache_write_check(const fa_cache_write_args* a) {
     int32_t st = check_pool(c, false);
     if (st) return st;
     if (a->tokens < 0) return FA_ERR_SHAPE;
-    if ((int64_t)c.batch * a->tokens >= (1LL << 28)) return FA_ERR_TOO_LARGE;
+    // 16 rows a workgroup of 256 threads, which are fewer than 2^32 in a grid
+    if ((int64_t)c.batch * a->tokens > (1LL << 28) - 16) return FA_ERR_TOO_LARGE;
     if (c.batch == 0 || a->tokens == 0 || empty_pool(c)) return FA_OK;
     const int es = elem_size(c.dtype);
     if ((st = check_tensor(a->k, a->k_stride, 5, a->tokens, c.head_dim, es)) ||
