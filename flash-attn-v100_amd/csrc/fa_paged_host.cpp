@@ -11,6 +11,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+
 #include "fa_host_util.hpp"
 #include "fa_paged.h"
 
@@ -102,6 +104,59 @@ bool dual(const at::Tensor& t) {
 }
 bool wants_grad(const at::Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
 
+// Whether two tensors share an element.  One of a and one of b are the same if, counted from
+// the first of a, sum s_i x_i = (last of b) - sum t_j y_j with 0 <= x_i < n_i, 0 <= y_j < m_j: a
+// sum of non-negative terms (those of one stride are one), tried from the longest stride
+// down, whose rest must be within the reach of the shorter ones.  A tensor's strides mostly
+// hold what is inside them, so that few multiples of each are left to try; where it takes
+// too many, false: what the caller has to see to.
+struct Terms {
+    struct Term {
+        int64_t stride, n;  // bytes; the largest multiple
+    } at[16];
+    int64_t reach[17];  // of terms from i on
+    int count = 0, work = 10000;
+    void add(const at::Tensor& t) {
+        for (int64_t d = 0; d < t.dim(); ++d)
+            if (t.size(d) > 1 && t.stride(d) != 0) at[count++] = {t.stride(d) * t.element_size(), t.size(d) - 1};
+    }
+    void order() {
+        std::sort(at, at + count, [](const Term& a, const Term& b) { return a.stride > b.stride; });
+        int m = 0;
+        for (int i = 0; i < count; ++i)
+            if (m && at[m - 1].stride == at[i].stride)
+                at[m - 1].n += at[i].n;
+            else
+                at[m++] = at[i];
+        count = m;
+        reach[m] = 0;
+        for (int i = m; i-- > 0;) reach[i] = reach[i + 1] + at[i].stride * at[i].n;
+    }
+    bool meets(int i, int64_t rest) {
+        if (rest < 0 || rest > reach[i] || --work < 0) return false;
+        if (rest == 0) return true;
+        const int64_t low = rest - reach[i + 1];
+        for (int64_t x = std::min(at[i].n, rest / at[i].stride); x >= 0 && x * at[i].stride >= low; --x)
+            if (meets(i + 1, rest - x * at[i].stride)) return true;
+        return false;
+    }
+};
+bool share(const at::Tensor& a, const at::Tensor& b) {
+    if (a.numel() == 0 || b.numel() == 0 || a.dim() > 8 || b.dim() > 8 || a.device() != b.device()) return false;
+    auto last = [](const at::Tensor& t) {  // (torch has no negative strides)
+        intptr_t x = (intptr_t)t.data_ptr();
+        for (int64_t d = 0; d < t.dim(); ++d) x += (t.size(d) - 1) * t.stride(d) * t.element_size();
+        return x;
+    };
+    const intptr_t a0 = (intptr_t)a.data_ptr(), a1 = last(a), b0 = (intptr_t)b.data_ptr(), b1 = last(b);
+    if (a1 < b0 || b1 < a0) return false;
+    Terms t;
+    t.add(a);
+    t.add(b);
+    t.order();
+    return t.meets(0, b1 - a0);
+}
+
 // What the Python entry points look at before every call, in one: False sends them to
 // their own checks, which name what is wrong.
 bool integer(PyObject* o, const at::Tensor& k, int64_t dim) {
@@ -125,7 +180,7 @@ bool cache_ok(PyObject* ok, PyObject* ov, PyObject* table, PyObject* lens, int64
             if (t->stride(i) < 0 || t->stride(i) * es % 16 != 0) return false;
         if (written && !t->is_contiguous()) return false;
     }
-    if (written && k.numel() && k.data_ptr() == v.data_ptr()) return false;
+    if (written && share(k, v)) return false;
     if (!none(table)) {
         if (!integer(table, k, 2) || k.size(d - 3) % 16 != 0 || k.size(d - 3) == 0) return false;
         const int64_t n = THPVariable_Unpack(table).size(0);
@@ -149,6 +204,17 @@ bool check_count(Py_ssize_t n, Py_ssize_t want) {
     return false;
 }
 
+// shares(a, b): whether two tensors share an element
+PyObject* shares(PyObject*, PyObject* const* x, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (!check_count(n, 2)) return nullptr;
+    if (!THPVariable_Check(x[0]) || !THPVariable_Check(x[1])) {
+        PyErr_SetString(PyExc_TypeError, "expected a tensor");
+        return nullptr;
+    }
+    return PyBool_FromLong(share(THPVariable_Unpack(x[0]), THPVariable_Unpack(x[1])));
+    END_HANDLE_TH_ERRORS
+}
 // pool_ok(k, v, table or None, lengths or None, batch or None, written)
 PyObject* pool_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -177,8 +243,13 @@ PyObject* write_ok(PyObject*, PyObject* const* x, Py_ssize_t n) {
     const at::Tensor &kn = THPVariable_Unpack(x[0]), &k = THPVariable_Unpack(x[2]);
     const int64_t d = kn.dim();
     if (d != k.dim() || d < 4 || !cache_ok(x[2], x[3], x[5], x[4], kn.size(d - 4), true)) Py_RETURN_FALSE;
-    return PyBool_FromLong(rows_ok(x[0], k, d) && rows_ok(x[1], k, d) && kn.sizes() == THPVariable_Unpack(x[1]).sizes() &&
-                           kn.size(d - 2) == k.size(d - 2) && (d == 4 || kn.size(0) == k.size(0)));
+    if (!rows_ok(x[0], k, d) || !rows_ok(x[1], k, d) || kn.sizes() != THPVariable_Unpack(x[1]).sizes() ||
+        kn.size(d - 2) != k.size(d - 2) || (d == 5 && kn.size(0) != k.size(0)))
+        Py_RETURN_FALSE;
+    for (int i = 0; i < 2; ++i)
+        for (int j = 2; j < 4; ++j)
+            if (share(THPVariable_Unpack(x[i]), THPVariable_Unpack(x[j]))) Py_RETURN_FALSE;
+    Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
 }
 // accept_ok(k, v, path, lengths, table (or None each))
@@ -419,6 +490,7 @@ PyObject* bind_paged(PyObject*, PyObject* const* x, Py_ssize_t n) {
 
 PyMethodDef fa_host::paged_methods[] = {
     {"bind_paged", (PyCFunction)(void*)bind_paged, METH_FASTCALL, nullptr},
+    {"shares", (PyCFunction)(void*)shares, METH_FASTCALL, nullptr},
     {"pool_ok", (PyCFunction)(void*)pool_ok, METH_FASTCALL, nullptr},
     {"paged_ok", (PyCFunction)(void*)paged_ok, METH_FASTCALL, nullptr},
     {"write_ok", (PyCFunction)(void*)write_ok, METH_FASTCALL, nullptr},

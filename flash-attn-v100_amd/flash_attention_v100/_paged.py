@@ -206,8 +206,8 @@ def check_cache(what: str, k_cache, v_cache, table, lens, batch: Optional[int], 
             raise ValueError(f"{name} needs rows of unit stride that start at multiples of 16 bytes (it is not copied)")
         if written and _overlaps(t):
             raise ValueError(f"{name} has overlapping elements")
-    if written and k_cache.numel() and k_cache.data_ptr() == v_cache.data_ptr():
-        raise ValueError("k_cache and v_cache must not be the same memory")
+    if written and host().shares(k_cache, v_cache):
+        raise ValueError("k_cache and v_cache must not lie in the same memory")
     if table is not None:
         if not isinstance(table, torch.Tensor):
             raise TypeError("page_table must be a torch.Tensor")

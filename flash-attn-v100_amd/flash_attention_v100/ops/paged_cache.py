@@ -11,7 +11,8 @@ tokens that are written take its last places, over the rows that were there (a c
 may reach the end asks :func:`paged_cache_fork_v100` for room, which has none to give, or
 counts).  Everything is read and decided on the GPU (no host
 synchronisation), and every call may be captured into a HIP graph.  A number that is
-no page holds nothing: nothing is written to it or moved from it.
+no page holds nothing: nothing is written to it or moved from it.  k_cache and v_cache,
+which every operator here writes, must not share memory (``ValueError``).
 """
 from __future__ import annotations
 
@@ -35,7 +36,8 @@ def paged_cache_write_v100(
     negative place is left out.  With a leading dimension of layers on the cache, k and v have
     it too.  Without ``page_table`` the cache is (B, S, Hkv, D), a row of tokens a
     sequence.  Returns (k_cache, v_cache), which are written in place; two sequences
-    that share a page must not write the same place of it.
+    that share a page must not write the same place of it.  k and v must not lie in the
+    caches' memory (``ValueError``).
     """
     if not _paged.host().write_ok(k, v, k_cache, v_cache, key_lengths, page_table):
         _check_write(k, v, k_cache, v_cache, key_lengths, page_table)
@@ -58,6 +60,8 @@ def _check_write(k, v, k_cache, v_cache, key_lengths, page_table) -> None:
     for name, t in (("k", k), ("v", v)):
         if t.dtype != k_cache.dtype or t.device != k_cache.device:
             raise ValueError(f"{name} must have the dtype and device of the cache")
+        if any(_paged.host().shares(t, x) for x in (k_cache, v_cache)):
+            raise ValueError(f"{name} must not lie in the cache's memory")
     _ops.check_dual(what, k, v)
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
         raise NotImplementedError(f"{what} has no backward: call it under torch.no_grad()")

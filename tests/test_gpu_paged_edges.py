@@ -1,5 +1,5 @@
 """The paged cache's entry points at their edges: pools and tensors made in inference
-mode, also rotated in place."""
+mode, also rotated in place; memory that caches share with each other or with new rows."""
 import pytest
 import torch
 
@@ -54,3 +54,34 @@ def test_rotation_in_place_of_tensors_of_inference_mode():
     with torch.no_grad():
         got = fa.rotary_embedding_v100(q, k, table, inplace=True)
     assert got[0].data_ptr() == q.data_ptr() and torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+def test_memory_that_is_written_and_read():
+    L, P, size, Hkv, D, N = 2, 8, 16, 2, 64, 3
+    lens, table = [20, 9], [[3, 7], [1, -1]]
+    args = ints(lens), ints(table)
+    k, v = randn(2, N, Hkv, D, seed=1), randn(2, N, Hkv, D, seed=2)
+    pool = randn(2 * P, size, Hkv, D, seed=3)
+    calls = (lambda kc, vc: fa.paged_cache_write_v100(k, v, kc, vc, *args),
+             lambda kc, vc: fa.paged_cache_accept_v100(kc, vc, args[0], ints([[1], [0]]), N, args[1]),
+             lambda kc, vc: fa.paged_cache_fork_v100(kc, vc, args[1], args[0], ints([0, 0]), 1),
+             lambda kc, vc: fa.paged_cache_compact_v100(kc, vc, args[1], args[0]))
+    before = pool.clone()
+    wide = randn(P, size, Hkv + 1, D, seed=4)
+    for call in calls:
+        for kc, vc in ((pool[:P], pool[:P]), (pool[:P], pool[P - 1:-1]), (wide[:, :, 1:], wide[:, :, :-1])):
+            with pytest.raises(ValueError, match="same memory"):
+                call(kc, vc)
+    kc, vc = pool[:P], pool[P:]
+    for bad in ((kc[:2, :N], v), (k, vc[2:4, 5:5 + N]), (k, kc[-2:, -N:]), (kc[:N, 4:6].transpose(0, 1), v)):
+        with pytest.raises(ValueError, match="cache's memory"):
+            fa.paged_cache_write_v100(*bad, kc, vc, *args)
+    assert torch.equal(pool, before)
+    # K and V of a page side by side; a layer's rows from another layer of the same pages
+    both = randn(P, 2, L, size, Hkv, D, seed=5)
+    kc, vc = both[:, 0, 0], both[:, 1, 0]
+    new = both[:2, 0, 1, :N], both[:2, 1, 1, :N]
+    rest = both[:, :, 1].clone()
+    want = po.write(kc[None], vc[None], new[0][None], new[1][None], lens, table)
+    fa.paged_cache_write_v100(*new, kc, vc, *args)
+    assert torch.equal(kc, want[0][0]) and torch.equal(vc, want[1][0]) and torch.equal(both[:, :, 1], rest)
