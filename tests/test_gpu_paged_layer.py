@@ -1,9 +1,10 @@
 """The layer's decode() over a paged cache: lengths past the cache's room, positions
-past the rotary table."""
+past the rotary table, trees of drafted tokens."""
 import pytest
 import torch
 
 import flash_attention_v100 as fa
+import paged_oracle as po
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -58,3 +59,37 @@ def test_positions_past_the_table():
     y = randn(2, 1, 256, seed=6)
     o, want = (a.decode(y, *p, ints([40, 21]), table) for a, p in zip((m, far), pools))
     assert torch.equal(o, want)
+
+
+@pytest.mark.parametrize("dt,tol", [(torch.float32, 2e-5), (torch.bfloat16, 3e-2)])
+@pytest.mark.parametrize("kw", [{}, {"rotary_dim": 32}, {"rotary_dim": 64, "rotary_interleaved": True, "softcap": 5.0},
+                                {"rotary_dim": 64, "distance_bias": True}])
+@pytest.mark.parametrize("batch_first", [True, False])
+def test_layer_decodes_a_tree(dt, tol, kw, batch_first):
+    # each node is what the causal layer computes at the end of the context and the node's
+    # ancestors: the same sums in another order.  float32: outputs near 1 of 256 products, 2^-24
+    # each way a few times; bf16: projections rounded to 2^-8 of values near 1, in both.
+    m = layer(dt, batch_first=batch_first, **kw)
+    turn = lambda t: t if batch_first else t.transpose(0, 1)  # noqa: E731
+    N, start = 40, [30, 0, 77]
+    par = [po.draw_tree(po.rng("layer", b), N) for b in range(3)]
+    sees = [po.ancestors(r) for r in par]
+    text = randn(3, 77, 256, seed=7, dt=dt)
+    x = randn(3, N, 256, seed=8, dt=dt)
+    table = ints(po.draw_table(po.rng("layer"), [n + N for n in start], 16, 8, 24))
+    kc, vc = (torch.full((24, 16, 4, 64), float("nan"), dtype=dt, device=DEV) for _ in range(2))
+    left = torch.zeros_like(text)  # the contexts, each the newest tokens of its row
+    for b, n in enumerate(start):
+        left[b, 77 - n:] = text[b, :n]
+    m.decode(turn(left), kc, vc, ints(start), table)
+    pos = ints([[n + len(s) - 1 for s in sees[b]] for b, n in enumerate(start)])
+    got = turn(m.decode(turn(x), kc, vc, ints([n + N for n in start]), table, parents=ints(par),
+                        positions=pos if m.rotary_dim else None))
+    worst = 0.0
+    with torch.no_grad():
+        for b, n in enumerate(start):
+            for i in (0, 1, 7, 20, N - 1):
+                want = turn(m(turn(torch.cat([text[b:b + 1, :n], x[b:b + 1, sees[b][i]]], 1)), is_causal=True)[0])[0, -1]
+                worst = max(worst, (got[b, i].float() - want.float()).abs().max().item())
+    print(f"{dt} {kw}: off by at most {worst:.2e}", flush=True)
+    assert worst <= tol
