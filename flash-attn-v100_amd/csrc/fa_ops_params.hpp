@@ -114,8 +114,8 @@ struct RowsParams {
 template <typename T>
 hipError_t launch_rows(const RowsParams& p, int D, hipStream_t s);
 
-// Tokens, or trees of drafted tokens, over a cache of pages (fa_paged.hpp): the rows'
-// own keys only (P = 0, tail = 1), k and v a pool of pages
+// Tokens, or trees of drafted tokens, over a cache of pages (fa_paged.hpp): k and v a pool
+// of pages; nothing of a prefix, offsets or their plans is read
 struct PagedParams : RowsParams {
     const int* table;      // (B, table_cols) pages, null: sequence b is page b
     int64_t table_sb;

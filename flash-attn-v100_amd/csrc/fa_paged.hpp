@@ -18,10 +18,11 @@
 // to 70, for the quarter of the addresses that one channel group serves answers later.
 // Units of 128 or 256 rows (trees of many rows a KV head, chunks of prompts): the waves, on 32
 // rows each, share tiles of 64 keys, which are read once for all of them.  16 trees of 64 on
-// 32 and 8 heads of 128 over up to 8192 keys: 124 us, 610 TFLOP/s of the products of what is
-// seen; the matrix units are busy for 30% of it, and each product of 32 x 32 x 16 has
-// 9 vector instructions beside it (exponentials at a quarter of their rate), with one
-// workgroup of two waves a SIMD (O and q take the registers of more).
+// 32 and 8 heads of 128 over up to 8192 keys: 120 us back to back (140 on a device idle between
+// calls), 630 TFLOP/s of the products of what is seen; the matrix units are busy for 31% of it:
+// each product of 32 x 32 x 16 has 9 vector instructions beside it (exponentials at a
+// quarter of their rate), and all waves go through both behind one barrier a tile, so that they
+// mostly follow one another; one workgroup of two waves a SIMD (O and q take the registers of more).
 //
 // Keys come in blocks of 16 tokens, which never leave a page: one lookup and one
 // buffer descriptor a block, whose range ends with the sequence, so that what lies
@@ -114,7 +115,10 @@ struct PageTable {
         for (int i = 0; i < BLOCKS; ++i) w |= block(blk + i).page < 0 ? 0ull : 0xFFFFull << (16 * i);
         return w;
     }
-    // whether one of blocks [b0, b1) has no page
+    // Whether one of blocks [b0, b1) has no page.  Callers round b1 up to whole tiles: where
+    // pages are smaller than those, a column behind the last key's that holds none counts too, and
+    // the part takes the loop of hidden keys throughout, with the same results (trees of 64 over up
+    // to 8192 keys: 132 us with pages of 64, 190 with pages of 16).
     __device__ FA_INLINE inline bool holes(int b0, int b1, int lane) const {
         if (!row || b0 >= b1) return false;
         bool none = false;
@@ -1081,12 +1085,14 @@ __global__ __launch_bounds__((PagedShape<T, D, NW>::THREADS), (NW == 8 ? 2 * Pag
 
 // The parts of 32 rows (blockIdx.x: KV head, unit, its rows) of a unit that several
 // workgroups shared: for 32 columns G waves, each of which takes every G-th part, two at
-// a time, and whose sums meet in LDS.  Units of 32 rows are few and in up to 64 parts: four
-// waves (16 where a sequence may be in more than 40 parts: one token over 8192 keys in 32
-// parts 16.9 us with four, 17.8 with 16; 15 tokens of 2 heads in 54 parts 20.2 and 18.3; one over
-// 65536 in 64 parts 40.5 and 39.1), 32 columns a workgroup (one token over 65536 keys: 39 us a call, 45 with two and all
-// columns); wide units are in two or three, and what a workgroup finds out about its unit
-// serves all columns (16 trees of 64 over up to 8192: 13 us, 18 with 32 columns).
+// a time, and whose sums meet in LDS.  Units of 32 rows are few, in as many parts as there are
+// workgroups for each: 64 with 8 KV heads, up to 512 with one.  Four waves, 16 where a
+// sequence may be in more than 40 parts (us with 4 and 16: one token of 8 heads over 8192 keys, 32
+// parts, 15.7 and 16.4; 15 tokens of 2 heads in 54 parts 16.9 and 16.4; one of 8 heads over 65536 in 64 parts
+// 39.6 and 38.5; one of one head over 131072 in 512 31.7 and 24.6), 32 columns a workgroup (one token over
+// 65536 keys: 39 us a call, 45 with two and all columns); wide units are in two or three, and
+// what a workgroup finds out about its unit serves all columns (16 trees of 64 over up to 8192:
+// 13 us, 18 with 32 columns).
 template <int D, int NW, bool MANY>
 struct JoinShape {
     static constexpr int G = NW > 1 ? 2 : MANY ? 16 : 4, BLOCKS = NW == 1 ? 1 : D / 32;  // of 32 columns

@@ -86,20 +86,21 @@ void plan(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared
     const int64_t rows = (int64_t)a->seqlen_q * (a->num_heads / c.num_heads_kv);
     // Waves that share tiles read K and V once for 128 or 256 rows, but leave larger parts and
     // fewer units: worth it where a workgroup gets enough steps of units that are full enough.
-    // us of trees of N on 32 and 8 heads of 128, units of 32, 128 and 256 rows (sequences of up
-    // to, N): 16 x 8192, 64: 269, 168, 156; 24 x 4096, 64: 197, 135, 129; 16 x 4000, 64: 151, 125,
-    // 141; 2 x 16000, 48: 73, 64, 68; 8 x 4000, 24: 42, 39, 65; the other way 2 x 1000, 64: 25,
-    // 34, 39; 16 x 4000, 12: 61, 77, 134; 4 x 16000, 12: 40, 49, 84.  Head dims up to 64 have three
-    // workgroups of 128 rows a CU: 16 x 8192, 64: 169, 104, 103 (64 on 8 heads 300, 174, 178); chunks
-    // of 189 in 28 x 546, 96 on 12 heads: 290, 178, 232
+    // us of trees of N on 32 and 8 heads of 128 in units of 32, 128 and 256 rows, pages of 64
+    // (sequences x room, N): 16 x 8192, 64: 263, 143, 132; 24 x 4096, 64: 176, 117, 111; 16 x 4000, 64: 125,
+    // 82, 80; 2 x 16000, 48: 52, 48, 47; 8 x 4000, 24: 36, 34, 42; the other way 2 x 1000, 64: 17, 23,
+    // 26; 16 x 4000, 12: 53, 53, 66; 4 x 16000, 12: 43, 46, 54.  Pages of 16 (which cost wide units more:
+    // PageTable::holes): 16 x 8192, 64: 304, 187, 190; 16 x 4000, 64: 142, 101, 106; 16 x 4000, 12: 55, 60, 86.
+    // Head dims up to 64 have three workgroups of 128 rows a CU, in units of 32 and 128: 16 x 8192, 64:
+    // 161, 86 (64 on 8 heads 287, 148); chunks of 189 in 28 x 546, 96 on 12 heads, pages of 48: 237, 108
     auto busy = [&](int64_t unit, int64_t keys, int64_t workgroups) {
         const int64_t tiles = ceil_div<int64_t>(rows, unit);
         return (double)c.batch * c.num_heads_kv * ceil_div<int64_t>(p.Sk, keys) * tiles / workgroups;
     };
     auto full = [&](int64_t unit) { return (double)rows / (double)(unit * ceil_div<int64_t>(rows, unit)); };
-    // Short sequences, whose units cost their beginnings and ends (trees of 64 over up to 300: 32
-    // sequences 57 -> 33, 16 31 -> 24, 8 17 -> 22; of 12: 32 sequences 18 -> 25): where units alone
-    // fill the device and are filled by their rows.
+    // Short sequences, whose units cost their beginnings and ends (trees of 64 over up to 300, in
+    // units of 32 and 128 rows: 32 sequences 51 and 27, 16 29 and 22, the other way 8 16 and 19; of 12: 32
+    // sequences 16 and 20): where units alone fill the device and are filled by their rows.
     const double units128 = (double)c.batch * c.num_heads_kv * ceil_div<int64_t>(rows, 128);
     if (f32 || rows <= 32 || (busy(32, 128, 512) * full(128) < 8 && units128 * full(128) * full(128) < 140))
         p.wide = 1;
@@ -118,23 +119,26 @@ void plan(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& shared
     p.groups = (int)std::max<int64_t>(groups, 1);
     // Units are shared where a sequence has room for more than join_from steps: below, the join
     // costs more than it saves, the more so the more units there are beside it.  us of one token
-    // of each of B sequences on 8 and 4 heads, shared / whole: B x up to 600 keys (5 steps), 16 x 8
-    // heads 17.6 / 15.3, 64 x 8 37 / 26; 1000 keys (8 steps), 64 x 4 21 / 16.7, 16 x 8 24.7 / 18.5, the
-    // other way 16 x 4 13.8 / 14.6; 2000 (16 steps), 64 x 8 83 / 74, the other way 16 x 4 20 / 23.
+    // of each of B sequences on 8 and 4 heads of 128, shared / whole: B x up to 600 keys (5 steps), 16 x
+    // 8 heads 16.6 / 14.9, 64 x 8 29 / 26; 1000 keys (8 steps), 64 x 4 25.5 / 22.7, 16 x 8 23.8 / 18.0, the
+    // other way 16 x 4 16.5 / 17.5; 2000 (16 steps), 64 x 8 77 / 74, the other way 16 x 4 23.4 / 26.8,
+    // 128 with one head 28.5 / 31.4.
     // Where the join is launched all the same (tables with room for more than the sequences hold),
     // what is found to be of `alone` steps at most stays whole: 64 sequences of 150 to 600 of 4096
-    // keys, 8 heads, 36 us shared, 31 whole.  Others are shared down to `least` a workgroup.  us with units of 4 steps whole / shared: trees of 12 over up to 1000 21.7 / 16.3;
-    // least of 1, 2 and 4: of 24 over up to 4000 21.0, 18.5, 20.6; one token over 8192 16.2, 15.3, 16.6.
-    // float32, whose steps take longer, from the third step on (64 tokens over up to 250 keys, 16 on 8
-    // heads of 128: 51 us shared from the second on, 46 so); wide units, whose parts are large,
-    // from the ninth (16 trees of 64 over up to 300 keys 37 us shared, 24 whole; 16 trees of 48 over
-    // up to 600, head dim 64, 29 and, were they whole, 33; 4 chunks of 500 of 600, head dim 64, 37 / 33).
+    // keys, 8 heads, 35 us shared, 30 whole.  Others are shared down to `least` a workgroup: 4 trees of
+    // 12 over up to 1000, us with 1, 2 and 4: 15.5, 21.4, 23.3 (16.6 whole); 2 of 24 over up to 4000 23.3,
+    // 23.4, 26.2; one token over 8192 16.9, 15.8, 16.8.
+    // float32, whose steps take longer, from the third step on (one token of each of 64 sequences
+    // over up to 250 keys, 16 on 8 heads of 128: 43 us shared from the second on, 39 so); wide units, whose
+    // parts are large, from the ninth (16 trees of 64 over up to 300 keys 26 us shared, 24 whole; 16
+    // trees of 48 over up to 600, head dim 64, 28 and, were they whole, 32; 4 chunks of 500 of 600, head
+    // dim 64, 35 / 32).
     const int64_t all = units * c.batch;
     const int64_t join_from = f32 ? 2 : p.wide == 1 ? 5 + all / 32 : std::max<int64_t>(8, 4 + all / 64);
     p.alone = (int)std::min<int64_t>(p.wide == 1 ? std::max<int64_t>(all / 32, 1) : join_from, INT32_MAX);
     p.least = f32 || (p.wide == 1 && most <= 16) ? 1 : p.wide == 1 ? 2 : 4;
     // a wide unit's tree, rows and parts take about as long as 3 of its steps: 16 x 8192, trees of
-    // 64: 166 us without, 158 with them in the balance
+    // 64: 136 us without, 131 to 135 with 1 to 6 of them in the balance
     p.extra = p.wide == 1 ? 0 : 3;
     // workgroups that may share sequences: none where none is that long or, with all of them
     // full, longer than an even share
@@ -158,14 +162,13 @@ void put_paged(const fa_paged_args* a, PagedParams& p, int64_t& grid, int64_t& s
     p.o_sb = a->o_stride[0]; p.o_ss = a->o_stride[1]; p.o_sh = a->o_stride[2];
     p.k_sp = c.k_stride[1]; p.k_ss = c.k_stride[2]; p.k_sh = c.k_stride[3];
     p.v_sp = c.v_stride[1]; p.v_ss = c.v_stride[2]; p.v_sh = c.v_stride[3];
-    p.B = c.batch; p.Sq = a->seqlen_q; p.P = 0;
+    p.B = c.batch; p.Sq = a->seqlen_q;
     p.Sk = empty_pool(c) ? 0 : (int)room_of(c);
     p.H = a->num_heads; p.Hkv = c.num_heads_kv; p.group = a->num_heads / c.num_heads_kv;
     p.cols = c.head_dim;
     put_cap(p, a->scale, a->softcap);
     p.slopes = a->slopes; p.slopes_sb = a->slopes_batch_stride;
     p.lens = c.key_lengths;
-    p.tail = p.causal = p.masked_neg = 1;
     p.table = p.Sk ? c.page_table : nullptr;
     p.table_sb = c.table_stride;
     p.table_cols = c.table_cols;

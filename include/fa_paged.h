@@ -33,7 +33,7 @@ extern "C" {
 
 /* Rows of head_dim elements, whole 16-byte chunks, up to 128 columns; strides in
  * elements in the order (layer, page, row, head, d), the d stride 1, the others
- * multiples of 16 bytes. */
+ * multiples of 16 bytes.  k and v of a pool that is written share no memory. */
 typedef struct fa_page_pool {
     void* k;
     void* v;
