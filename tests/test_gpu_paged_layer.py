@@ -1,5 +1,5 @@
 """The layer's decode() over a paged cache: lengths past the cache's room, positions
-past the rotary table, trees of drafted tokens."""
+past the rotary table, trees of drafted tokens, steps captured and replayed."""
 import pytest
 import torch
 
@@ -93,3 +93,41 @@ def test_layer_decodes_a_tree(dt, tol, kw, batch_first):
                 worst = max(worst, (got[b, i].float() - want.float()).abs().max().item())
     print(f"{dt} {kw}: off by at most {worst:.2e}", flush=True)
     assert worst <= tol
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_captured_steps(tree):
+    # replays on other lengths, tables and inputs, with eager steps between them, equal the eager step
+    N = 5
+    m = layer(torch.bfloat16, rotary_dim=64, distance_bias=True)
+
+    def state(seed):
+        rng = po.rng("captured", seed)
+        lens = [rng.randint(0, 90) for _ in range(3)] + [100]  # the last one past the room
+        s = {"x": randn(4, N, 256, seed=seed, dt=torch.bfloat16), "kc": randn(24, 16, 4, 64, seed=seed + 10, dt=torch.bfloat16),
+             "vc": randn(24, 16, 4, 64, seed=seed + 20, dt=torch.bfloat16), "lens": ints(lens),
+             "table": ints(po.draw_table(rng, [96] * 4, 16, 6, 24))}
+        if tree:
+            par = [po.draw_tree(rng, N) for _ in range(4)]
+            s["par"] = ints(par)
+            s["pos"] = ints([[min(n, 96) - N + len(a) - 1 for a in po.ancestors(r)] for n, r in zip(lens, par)])
+        return s
+
+    def step(s):
+        return m.decode(s["x"], s["kc"], s["vc"], s["lens"], s["table"], parents=s.get("par"), positions=s.get("pos"))
+
+    st = state(1)
+    step(state(1))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(st)
+    for seed in (1, 2, 3, 2):
+        fresh = state(seed)
+        for name in st:
+            st[name].copy_(fresh[name])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (out, st["kc"], st["vc"])]
+        want = (step(fresh), fresh["kc"], fresh["vc"])
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), seed
